@@ -380,6 +380,72 @@ int32_t wick_cuda_decode_batch_steps(wick_cuda_model* m, const uint32_t* first_t
 int32_t wick_cuda_decode_batch_logits(wick_cuda_model* m, const uint32_t* tokens_host, const uint32_t* seq_ids_host,
                                       uint32_t bs, float* logits_host);
 
+/* ---- operators of a serving step beside the model's own path (extension) ----
+ * Attention of packed prompts, a K / V cache in 4 bits with the attention of single tokens over it, and log probabilities.  They
+ * agree with the formulas within rounding (f32 sums), they do not repeat the CPU path's order of operations.  Like the operators
+ * above they take device pointers and are asynchronous on `stream`; none allocates, synchronises or keeps anything from one call for the
+ * next, so that they can be captured.  The device of the buffers has to be the current one.  `dtype` is a ggml type id. */
+#define WICK_DTYPE_F32 0
+#define WICK_DTYPE_F16 1
+#define WICK_DTYPE_BF16 30
+
+/* Log probability of one given token per row of logits [n][vocab] (rows row_stride elements apart, f32 / f16 / bf16), the entropy of
+ * the row's distribution in nats, and its top_n (0 .. WICK_CUDA_LOGPROBS_MAX_TOP, at most vocab) likeliest tokens with their log
+ * probabilities, descending, equal logits by ascending id; top_ids_dev / top_logprobs_dev [n][top_n] may be NULL when top_n is 0.
+ * NaN counts as -inf (as in cpu_argmax, sampler.rs:8-19); logits beyond +-1e30 count as +-inf, and several +inf share the row.  A token
+ * outside the vocabulary, or with a logit of -inf, has log probability -inf; a row of -inf alone has entropy 0. */
+#define WICK_CUDA_LOGPROBS_MAX_TOP 64
+int32_t wick_cuda_token_logprobs(const void* logits_dev, int32_t dtype, uint64_t row_stride, uint32_t n, uint32_t vocab,
+                                 const int32_t* tokens_dev, uint32_t top_n, float* logprob_dev, float* entropy_dev, int32_t* top_ids_dev,
+                                 float* top_logprobs_dev, void* stream);
+
+/* A K / V cache in 4 bits: for every (slot, KV head) max_seq rows of head_dim / 32 Q4_0 blocks (quant.rs:13-20: an f16 scale d and 32
+ * four-bit numbers q, value d * (q - 8); byte i of a block holds number i in its low and number i + 16 in its high half), in two planes
+ * per side: quants [n_slots][n_kv_heads][max_seq][head_dim / 2], 16-byte aligned, and f16 scales [..][max_seq][head_dim / 32],
+ * 16-byte aligned.  max_seq is a multiple of 64, head_dim of 32 and at most 128. */
+typedef struct wick_cuda_kv_q4 {
+    uint8_t* k_quants;
+    uint16_t* k_scales;
+    uint8_t* v_quants;
+    uint16_t* v_scales;
+    uint32_t n_slots, n_kv_heads, max_seq, head_dim;
+} wick_cuda_kv_q4;
+/* Rounds row j of k and v [n][n_kv_heads*head_dim] (rows k_stride / v_stride elements apart) to Q4_0 and writes them to row
+ * positions_dev[j] of slot slots_dev[j].  A row whose slot or position the cache does not have (a padding row: -1) is skipped.  The
+ * pairs (slot, position) of a call differ from one another: of two rows with the same pair every block is one row's or the other's.
+ * Values are finite and below 524032 in magnitude (the f16 scale). */
+int32_t wick_cuda_kv_append_q4(const wick_cuda_kv_q4* cache, const void* k_dev, uint64_t k_stride, const void* v_dev, uint64_t v_stride,
+                               int32_t dtype, uint32_t n, const int32_t* slots_dev, const int32_t* positions_dev, void* stream);
+/* The values of row positions_dev[j] of slot slots_dev[j] in f32, k and v [n][n_kv_heads*head_dim] (16-byte aligned); zeros for a row
+ * that the cache does not have.  Any row may be asked for any number of times. */
+int32_t wick_cuda_kv_read_q4(const wick_cuda_kv_q4* cache, uint32_t n, const int32_t* slots_dev, const int32_t* positions_dev, float* k_dev,
+                             float* v_dev, void* stream);
+/* Attention of single tokens over the cache: row j of q [n][n_heads*head_dim] (rows q_stride elements apart) attends the first
+ * lengths_dev[j] rows (at most max_seq) of slot slots_dev[j], scores scaled by 1 / sqrt(head_dim); several rows may name the same slot.
+ * out [n][n_heads*head_dim] has q's type.  Length 0 (or less) gives zeros; a row whose slot the cache does not have (a padding row: -1)
+ * is left as it was.  What the cache holds behind a row's length is never used, whatever it is.  workspace_dev: 16-byte aligned, as many
+ * bytes as wick_cuda_attention_q4_workspace says, with any content; of this call alone until it has finished. */
+int32_t wick_cuda_attention_q4_workspace(const wick_cuda_kv_q4* cache, uint32_t n, uint32_t n_heads, uint64_t* bytes);
+int32_t wick_cuda_attention_q4(const wick_cuda_kv_q4* cache, const void* q_dev, uint64_t q_stride, int32_t dtype, uint32_t n, uint32_t n_heads,
+                               const int32_t* slots_dev, const int32_t* lengths_dev, void* out_dev, void* workspace_dev,
+                               uint64_t workspace_bytes, void* stream);
+
+/* Causal attention of packed prompts: sequence s has the tokens [starts[s], starts[s+1]) of q [n_tokens][n_heads*head_dim] and the keys
+ * [key_starts[s], key_starts[s+1]) of k and v [n_keys][n_kv_heads*head_dim]; its last key belongs to its last token, so that token j of
+ * nq attends its keys t <= j + nk - nq.  starts_dev / key_starts_dev hold n_seqs + 1 ascending offsets; key_starts_dev NULL: the same as
+ * starts_dev.  A token without keys gets zeros.  Rows of q and out that belong to no sequence (behind the last one) are not used and left as
+ * they were; so are rows of k and v.  Scores are scaled by 1 / sqrt(head_dim).  All of q, k, v, out have the type `dtype`; rows of q, k,
+ * v are q_stride / k_stride / v_stride elements apart; out rows are dense.  head_dim is a multiple of 8 and at most 128;
+ * pointers and row strides are multiples of 16 bytes (out: of its elements).  A key or value that is infinite or NaN reaches the tokens
+ * that attend it and no others.  workspace_dev: 128-byte aligned, as many bytes as
+ * wick_cuda_attention_prompts_workspace says, with any content; of this call alone until it has finished. */
+int32_t wick_cuda_attention_prompts_workspace(int32_t dtype, uint32_t n_seqs, uint32_t n_tokens, uint32_t n_keys, uint32_t n_heads,
+                                              uint32_t n_kv_heads, uint32_t head_dim, uint64_t* bytes);
+int32_t wick_cuda_attention_prompts(const void* q_dev, uint64_t q_stride, const void* k_dev, uint64_t k_stride, const void* v_dev,
+                                    uint64_t v_stride, int32_t dtype, const int32_t* starts_dev, const int32_t* key_starts_dev,
+                                    uint32_t n_seqs, uint32_t n_tokens, uint32_t n_keys, uint32_t n_heads, uint32_t n_kv_heads,
+                                    uint32_t head_dim, void* out_dev, void* workspace_dev, uint64_t workspace_bytes, void* stream);
+
 /* ---- tensor-parallel all-reduce over peer memory (extension) -----------------
  * wick runs on one device; there is no counterpart in its tree.  For a tensor-parallel split of the LFM2 layers over
  * the GPUs of one NVLink node (one process per GPU): after every row-split mat-vec (attention output, short-conv

@@ -35,6 +35,12 @@ class Config(C.Structure):
                 ("rms_norm_eps", C.c_float)]
 
 
+class KvQ4(C.Structure):
+    """wick_cuda_kv_q4: the planes and sizes of a 4-bit K / V cache."""
+    _fields_ = [("k_quants", C.c_void_p), ("k_scales", C.c_void_p), ("v_quants", C.c_void_p), ("v_scales", C.c_void_p),
+                ("n_slots", C.c_uint32), ("n_kv_heads", C.c_uint32), ("max_seq", C.c_uint32), ("head_dim", C.c_uint32)]
+
+
 _vp, _u32, _i32, _u64, _f = C.c_void_p, C.c_uint32, C.c_int32, C.c_uint64, C.c_float
 
 # name -> argtypes; every function returns int32 except the three noted below
@@ -109,6 +115,13 @@ SIGNATURES = {
     "wick_cuda_attention_prefill": [_vp, _vp, _vp, _vp, _u32, _u32, _u32, _u32, _u32, _i32, _vp],
     "wick_cuda_shortconv": [_vp, _vp, _vp, _vp, _u32, _u32, _u32, _vp],
     "wick_cuda_argmax": [_vp, _u32, _vp, _vp],
+    "wick_cuda_token_logprobs": [_vp, _i32, _u64, _u32, _u32, _vp, _u32, _vp, _vp, _vp, _vp, _vp],
+    "wick_cuda_kv_append_q4": [C.POINTER(KvQ4), _vp, _u64, _vp, _u64, _i32, _u32, _vp, _vp, _vp],
+    "wick_cuda_kv_read_q4": [C.POINTER(KvQ4), _u32, _vp, _vp, _vp, _vp, _vp],
+    "wick_cuda_attention_q4_workspace": [C.POINTER(KvQ4), _u32, _u32, C.POINTER(_u64)],
+    "wick_cuda_attention_q4": [C.POINTER(KvQ4), _vp, _u64, _i32, _u32, _u32, _vp, _vp, _vp, _vp, _u64, _vp],
+    "wick_cuda_attention_prompts_workspace": [_i32, _u32, _u32, _u32, _u32, _u32, _u32, C.POINTER(_u64)],
+    "wick_cuda_attention_prompts": [_vp, _u64, _vp, _u64, _vp, _u64, _i32, _vp, _vp, _u32, _u32, _u32, _u32, _u32, _u32, _vp, _vp, _u64, _vp],
     "wick_cuda_argmax_noalloc": [_vp, _u32, _vp, _vp],
 }
 VOID_FUNCS = {"wick_cuda_model_destroy": [_vp], "wick_cuda_weight_destroy": [_vp], "wick_cuda_tp_comm_destroy": [_vp]}

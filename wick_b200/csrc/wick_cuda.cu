@@ -21,6 +21,7 @@
 #include "gemm_mma.cuh"
 #include "gemm_tc.cuh"
 #include "kernels.cuh"
+#include "serving.cuh"
 #include "word_pool.hpp"
 
 using namespace wick;
@@ -2467,6 +2468,142 @@ int32_t wick_cuda_argmax(const float* logits_dev, uint32_t count, uint32_t* out_
     CU_TRY(cudaMemsetAsync(scratch, 0, 8, st));
     launch_argmax(st, logits_dev, (int)count, scratch, out_dev);
     CU_TRY(cudaFreeAsync(scratch, st));
+    OP_END();
+}
+
+// ── operators of a serving step ─────────────────────────────────────────────
+static int32_t check_dtype(int32_t dtype) {
+    return dtype_bytes(dtype) ? WICK_CUDA_OK : fail(WICK_CUDA_ERR_UNSUPPORTED_DTYPE, "dtype must be f32, f16 or bf16");
+}
+static bool misaligned(const void* p, size_t bytes) { return ((uintptr_t)p & (bytes - 1)) != 0; }
+
+int32_t wick_cuda_token_logprobs(const void* logits_dev, int32_t dtype, uint64_t row_stride, uint32_t n, uint32_t vocab, const int32_t* tokens_dev,
+                                 uint32_t top_n, float* logprob_dev, float* entropy_dev, int32_t* top_ids_dev, float* top_logprobs_dev,
+                                 void* stream) {
+    W_TRY(check_dtype(dtype));
+    if (n == 0) return WICK_CUDA_OK;
+    if (!logits_dev || !tokens_dev || !logprob_dev || !entropy_dev || (top_n && (!top_ids_dev || !top_logprobs_dev)))
+        return fail(WICK_CUDA_ERR_BAD_ARG, "NULL argument");
+    if (vocab == 0 || vocab > 0x7FFFFFF0u || row_stride < vocab) return fail(WICK_CUDA_ERR_BAD_ARG, "token_logprobs: rows of 1 to 2^31 logits that do not overlap");
+    if (top_n > vocab || top_n > WICK_CUDA_LOGPROBS_MAX_TOP) return fail(WICK_CUDA_ERR_BAD_ARG, "token_logprobs: top_n is at most 64 and at most vocab");
+    if (n > 0x7FFFFFFu) return fail(WICK_CUDA_ERR_BAD_ARG, "token_logprobs: too many rows");
+    if (misaligned(logits_dev, dtype_bytes(dtype))) return fail(WICK_CUDA_ERR_BAD_ARG, "token_logprobs: misaligned logits");
+    CU_TRY(launch_token_logprobs((cudaStream_t)stream, logits_dev, dtype, row_stride, (int)n, (int)vocab, tokens_dev, (int)top_n, logprob_dev,
+                                 entropy_dev, top_ids_dev, top_logprobs_dev));
+    OP_END();
+}
+
+static int32_t check_kv_q4(const wick_cuda_kv_q4* cache, KvQ4* out) {
+    if (!cache || !cache->k_quants || !cache->k_scales || !cache->v_quants || !cache->v_scales) return fail(WICK_CUDA_ERR_BAD_ARG, "NULL argument");
+    if (!cache->n_slots || !cache->n_kv_heads || !cache->max_seq || cache->max_seq % KV_Q4_TILE || !cache->head_dim || cache->head_dim % QK ||
+        cache->head_dim > KV_Q4_MAX_HEAD)
+        return fail(WICK_CUDA_ERR_BAD_ARG, "4-bit cache: max_seq must be a multiple of 64, head_dim a multiple of 32 and at most 128");
+    if (cache->n_slots > 0x7FFFFFFFu || cache->n_kv_heads > 65535u || cache->max_seq > 0x7FFFFFFFu) return fail(WICK_CUDA_ERR_BAD_ARG, "4-bit cache: too large");
+    if (misaligned(cache->k_quants, 16) || misaligned(cache->v_quants, 16) || misaligned(cache->k_scales, 16) || misaligned(cache->v_scales, 16))
+        return fail(WICK_CUDA_ERR_BAD_ARG, "4-bit cache: planes must be 16-byte aligned");
+    *out = KvQ4{{cache->k_quants, cache->v_quants}, {(__half*)cache->k_scales, (__half*)cache->v_scales}, (int)cache->n_slots, (int)cache->n_kv_heads,
+                (int)cache->max_seq, (int)cache->head_dim};
+    return WICK_CUDA_OK;
+}
+
+int32_t wick_cuda_kv_append_q4(const wick_cuda_kv_q4* cache, const void* k_dev, uint64_t k_stride, const void* v_dev, uint64_t v_stride, int32_t dtype,
+                               uint32_t n, const int32_t* slots_dev, const int32_t* positions_dev, void* stream) {
+    KvQ4 c;
+    W_TRY(check_kv_q4(cache, &c));
+    W_TRY(check_dtype(dtype));
+    if (n == 0) return WICK_CUDA_OK;
+    if (!k_dev || !v_dev || !slots_dev || !positions_dev) return fail(WICK_CUDA_ERR_BAD_ARG, "NULL argument");
+    const uint64_t dim = (uint64_t)c.n_kv * c.head_dim;
+    if (k_stride < dim || v_stride < dim) return fail(WICK_CUDA_ERR_BAD_ARG, "kv_append_q4: rows overlap");
+    if (n * dim > (1ull << 38)) return fail(WICK_CUDA_ERR_BAD_ARG, "kv_append_q4: too many rows");
+    if (misaligned(k_dev, dtype_bytes(dtype)) || misaligned(v_dev, dtype_bytes(dtype))) return fail(WICK_CUDA_ERR_BAD_ARG, "kv_append_q4: misaligned rows");
+    CU_TRY(launch_kv_append_q4((cudaStream_t)stream, c, k_dev, k_stride, v_dev, v_stride, dtype, (int)n, slots_dev, positions_dev));
+    OP_END();
+}
+
+int32_t wick_cuda_kv_read_q4(const wick_cuda_kv_q4* cache, uint32_t n, const int32_t* slots_dev, const int32_t* positions_dev, float* k_dev, float* v_dev,
+                             void* stream) {
+    KvQ4 c;
+    W_TRY(check_kv_q4(cache, &c));
+    if (n == 0) return WICK_CUDA_OK;
+    if (!k_dev || !v_dev || !slots_dev || !positions_dev) return fail(WICK_CUDA_ERR_BAD_ARG, "NULL argument");
+    if (misaligned(k_dev, 16) || misaligned(v_dev, 16)) return fail(WICK_CUDA_ERR_BAD_ARG, "kv_read_q4: k and v must be 16-byte aligned");
+    if (n * ((uint64_t)c.n_kv * c.head_dim) > (1ull << 38)) return fail(WICK_CUDA_ERR_BAD_ARG, "kv_read_q4: too many rows");
+    CU_TRY(launch_kv_read_q4((cudaStream_t)stream, c, (int)n, slots_dev, positions_dev, k_dev, v_dev));
+    OP_END();
+}
+
+static int32_t check_attention_q4(const wick_cuda_kv_q4* cache, uint32_t n, uint32_t n_heads, KvQ4* c) {
+    W_TRY(check_kv_q4(cache, c));
+    if (!n_heads || n_heads % c->n_kv) return fail(WICK_CUDA_ERR_BAD_ARG, "n_heads must be a multiple of n_kv_heads");
+    if (n > 65535 || n_heads > 65535) return fail(WICK_CUDA_ERR_BAD_ARG, "attention_q4: at most 65535 rows and heads");
+    return WICK_CUDA_OK;
+}
+
+int32_t wick_cuda_attention_q4_workspace(const wick_cuda_kv_q4* cache, uint32_t n, uint32_t n_heads, uint64_t* bytes) {
+    KvQ4 c;
+    if (!bytes) return fail(WICK_CUDA_ERR_BAD_ARG, "NULL argument");
+    W_TRY(check_attention_q4(cache, n, n_heads, &c));
+    *bytes = attention_q4_workspace((int)n, (int)n_heads, c);
+    return WICK_CUDA_OK;
+}
+
+int32_t wick_cuda_attention_q4(const wick_cuda_kv_q4* cache, const void* q_dev, uint64_t q_stride, int32_t dtype, uint32_t n, uint32_t n_heads,
+                               const int32_t* slots_dev, const int32_t* lengths_dev, void* out_dev, void* workspace_dev, uint64_t workspace_bytes,
+                               void* stream) {
+    KvQ4 c;
+    W_TRY(check_attention_q4(cache, n, n_heads, &c));
+    W_TRY(check_dtype(dtype));
+    if (n == 0) return WICK_CUDA_OK;
+    if (!q_dev || !slots_dev || !lengths_dev || !out_dev) return fail(WICK_CUDA_ERR_BAD_ARG, "NULL argument");
+    if (q_stride < (uint64_t)n_heads * c.head_dim) return fail(WICK_CUDA_ERR_BAD_ARG, "attention_q4: rows of q overlap");
+    if (misaligned(q_dev, dtype_bytes(dtype)) || misaligned(out_dev, dtype_bytes(dtype))) return fail(WICK_CUDA_ERR_BAD_ARG, "attention_q4: misaligned rows");
+    const uint64_t need = attention_q4_workspace((int)n, (int)n_heads, c);
+    if (workspace_bytes < need || (need && (!workspace_dev || misaligned(workspace_dev, 16))))
+        return fail(WICK_CUDA_ERR_BAD_ARG, "attention_q4: workspace missing, misaligned or too small");
+    CU_TRY(launch_attention_q4((cudaStream_t)stream, c, q_dev, q_stride, dtype, (int)n, (int)n_heads, slots_dev, lengths_dev, out_dev, workspace_dev));
+    OP_END();
+}
+
+static int32_t check_prompts(const Prompts& p, uint32_t n_seqs, uint32_t n_tokens, uint32_t n_keys, uint32_t n_heads, uint32_t n_kv_heads, uint32_t head_dim) {
+    W_TRY(check_dtype(p.dtype));
+    if (!n_kv_heads || !n_heads || n_heads % n_kv_heads || n_heads / n_kv_heads > 128 || n_heads > 65535 || !head_dim || head_dim % 8 || head_dim > 128)
+        return fail(WICK_CUDA_ERR_BAD_ARG, "attention_prompts: head_dim must be a multiple of 8 and at most 128, n_heads a multiple of n_kv_heads and at most 128 times it");
+    if (n_seqs > (1u << 24) || n_tokens > (1u << 30) || n_keys > (1u << 30)) return fail(WICK_CUDA_ERR_BAD_ARG, "attention_prompts: too many rows");
+    return WICK_CUDA_OK;
+}
+
+int32_t wick_cuda_attention_prompts_workspace(int32_t dtype, uint32_t n_seqs, uint32_t n_tokens, uint32_t n_keys, uint32_t n_heads, uint32_t n_kv_heads,
+                                              uint32_t head_dim, uint64_t* bytes) {
+    if (!bytes) return fail(WICK_CUDA_ERR_BAD_ARG, "NULL argument");
+    Prompts p{};
+    p.dtype = dtype;
+    W_TRY(check_prompts(p, n_seqs, n_tokens, n_keys, n_heads, n_kv_heads, head_dim));
+    p.n_seqs = (int)n_seqs, p.n_tokens = (int)n_tokens, p.n_keys = (int)n_keys, p.n_heads = (int)n_heads, p.n_kv = (int)n_kv_heads, p.head_dim = (int)head_dim;
+    *bytes = attention_prompts_workspace(p);
+    return WICK_CUDA_OK;
+}
+
+int32_t wick_cuda_attention_prompts(const void* q_dev, uint64_t q_stride, const void* k_dev, uint64_t k_stride, const void* v_dev, uint64_t v_stride,
+                                    int32_t dtype, const int32_t* starts_dev, const int32_t* key_starts_dev, uint32_t n_seqs, uint32_t n_tokens,
+                                    uint32_t n_keys, uint32_t n_heads, uint32_t n_kv_heads, uint32_t head_dim, void* out_dev, void* workspace_dev,
+                                    uint64_t workspace_bytes, void* stream) {
+    Prompts p{q_dev, k_dev, v_dev, q_stride, k_stride, v_stride, dtype, starts_dev, key_starts_dev, (int)n_seqs, (int)n_tokens, (int)n_keys,
+              (int)n_heads, (int)n_kv_heads, (int)head_dim, out_dev};
+    W_TRY(check_prompts(p, n_seqs, n_tokens, n_keys, n_heads, n_kv_heads, head_dim));
+    if (n_seqs == 0 || n_tokens == 0) return WICK_CUDA_OK;
+    if (!q_dev || (n_keys && (!k_dev || !v_dev)) || !starts_dev || !out_dev) return fail(WICK_CUDA_ERR_BAD_ARG, "NULL argument");
+    const size_t b = dtype_bytes(dtype);
+    if (q_stride < (uint64_t)n_heads * head_dim || k_stride < (uint64_t)n_kv_heads * head_dim || v_stride < (uint64_t)n_kv_heads * head_dim)
+        return fail(WICK_CUDA_ERR_BAD_ARG, "attention_prompts: rows overlap");
+    if (misaligned(q_dev, 16) || misaligned(k_dev, 16) || misaligned(v_dev, 16) || q_stride * b % 16 || k_stride * b % 16 || v_stride * b % 16 || misaligned(out_dev, b))
+        return fail(WICK_CUDA_ERR_BAD_ARG, "attention_prompts: q, k, v and their row strides must be multiples of 16 bytes");
+    if (q_stride * b >= (1ull << 40) || k_stride * b >= (1ull << 40) || v_stride * b >= (1ull << 40))
+        return fail(WICK_CUDA_ERR_BAD_ARG, "attention_prompts: row strides too large");
+    const uint64_t need = attention_prompts_workspace(p);
+    if (workspace_bytes < need || (need && (!workspace_dev || misaligned(workspace_dev, 128))))
+        return fail(WICK_CUDA_ERR_BAD_ARG, "attention_prompts: workspace missing, misaligned or too small");
+    CU_TRY(launch_attention_prompts((cudaStream_t)stream, p, workspace_dev));
     OP_END();
 }
 

@@ -196,3 +196,176 @@ def argmax_noalloc(logits: torch.Tensor, out: torch.Tensor) -> torch.Tensor:
     if code != 0:
         raise _lib.WickCudaError(code, lib.wick_cuda_argmax_noalloc_last_error().decode())
     return out
+
+
+# ── operators of a serving step beside the model's own path ────────────────────────────────────────
+# f32, f16 and bf16; rows may be strided views (the last dimension dense).  Misuse raises WickCudaError (BAD_ARG or
+# UNSUPPORTED_DTYPE).  They launch on the current stream of their tensors' device.
+DTYPE_ID = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 30}
+
+
+def _need(ok: bool, message: str) -> None:
+    if not ok:
+        raise _lib.WickCudaError(_lib.ERR_BAD_ARG, message)
+
+
+def _dtype_id(t: torch.Tensor) -> int:
+    if t.dtype not in DTYPE_ID:
+        raise _lib.WickCudaError(_lib.ERR_UNSUPPORTED_DTYPE, f"{t.dtype}: f32, f16 or bf16 is needed")
+    return DTYPE_ID[t.dtype]
+
+
+def _rows(t: torch.Tensor, name: str, device: torch.device) -> torch.Tensor:
+    """t as rows with a dense last dimension that do not overlap."""
+    _need(t.is_cuda and t.device == device, f"{name} must be on {device}")
+    _need(t.dim() == 2, f"{name} must have two dimensions")
+    if (t.shape[1] > 1 and t.stride(1) != 1) or (t.shape[0] > 1 and t.stride(0) < t.shape[1]):
+        return t.contiguous()
+    return t
+
+
+def _stride(t: torch.Tensor) -> int:
+    """Elements from row to row; torch keeps any number there for a single row."""
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+
+
+def _ids(t: torch.Tensor, n: int, name: str, device: torch.device) -> torch.Tensor:
+    _need(t.dtype == torch.int32 and t.device == device, f"{name} must be int32 on {device}")
+    _need(t.dim() == 1 and t.shape[0] == n, f"{name} must hold {n} numbers")
+    return t if t.is_contiguous() else t.contiguous()
+
+
+def _call(name: str, device: torch.device, *args) -> None:
+    """The library's function `name` on the current stream of `device`."""
+    fn = getattr(_lib.load(), name)
+    stream = torch.cuda.current_stream(device).cuda_stream
+    if device.index == torch.cuda.current_device():
+        check(fn(*args, stream))
+    else:
+        with torch.cuda.device(device):
+            check(fn(*args, stream))
+
+
+def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top_n: int = 0):
+    """Log probability of tokens[j] under row j of logits [n, vocab], the rows' entropies (nats) and their top_n (at most 64)
+    likeliest tokens: (logprob [n], entropy [n], top ids [n, top_n] int32, top logprobs [n, top_n]), f32.  Equal logits by
+    ascending id; NaN counts as -inf; a token outside the vocabulary has -inf."""
+    device = logits.device
+    logits = _rows(logits, "logits", device)
+    n, vocab = logits.shape
+    tokens = _ids(tokens, n, "tokens", device)
+    dtype = _dtype_id(logits)
+    _need(0 <= top_n <= 64, "top_n must be 0 to 64")
+    out = torch.empty((2, n), dtype=torch.float32, device=device)
+    ids = torch.empty((n, top_n), dtype=torch.int32, device=device)
+    lps = torch.empty((n, top_n), dtype=torch.float32, device=device)
+    p = out.data_ptr()
+    _call("wick_cuda_token_logprobs", device, logits.data_ptr(), dtype, _stride(logits), n, vocab, tokens.data_ptr(), top_n, p, p + 4 * n,
+          ids.data_ptr() if top_n else None, lps.data_ptr() if top_n else None)
+    return out[0], out[1], ids, lps
+
+
+class KvCacheQ4:
+    """A K / V cache in 4 bits: Q4_0 blocks of 32 values, quants [slots, kv_heads, max_seq, head_dim / 2] uint8 and scales
+    [slots, kv_heads, max_seq, head_dim / 32] f16 for each of the two sides (byte i of a block's 16 holds number i in its low and number
+    i + 16 in its high half; value = scale * (number - 8)).  Holds the given tensors; max_seq is a multiple of 64, head_dim of 32 and at
+    most 128."""
+
+    def __init__(self, k_quants: torch.Tensor, k_scales: torch.Tensor, v_quants: torch.Tensor, v_scales: torch.Tensor):
+        planes = (k_quants, k_scales, v_quants, v_scales)
+        self.device = k_quants.device
+        for t, dtype in zip(planes, (torch.uint8, torch.float16) * 2):
+            _need(t.is_cuda and t.device == self.device and t.dtype == dtype and t.dim() == 4 and t.is_contiguous(),
+                  "planes must be dense tensors of four dimensions on one GPU, quants uint8 and scales f16")
+        slots, heads, rows, half = k_quants.shape
+        _need(v_quants.shape == k_quants.shape and half % 16 == 0 and k_scales.shape == v_scales.shape == (slots, heads, rows, half // 16),
+              "the planes' shapes do not match")
+        self.k_quants, self.k_scales, self.v_quants, self.v_scales = planes
+        self.n_slots, self.n_kv_heads, self.max_seq, self.head_dim = slots, heads, rows, half * 2
+        self._c = _lib.KvQ4(*(t.data_ptr() for t in planes), slots, heads, rows, half * 2)
+
+    @classmethod
+    def empty(cls, n_slots: int, max_seq: int, n_kv_heads: int, head_dim: int, device="cuda") -> "KvCacheQ4":
+        """A cache of zeros for at least max_seq rows per slot."""
+        _need(n_slots > 0 and max_seq > 0 and n_kv_heads > 0 and head_dim > 0 and head_dim % 32 == 0 and head_dim <= 128,
+              "sizes must be positive, head_dim a multiple of 32 and at most 128")
+        rows = -(-max_seq // 64) * 64
+        planes = []
+        for _ in range(2):
+            planes.append(torch.full((n_slots, n_kv_heads, rows, head_dim // 2), 0x88, dtype=torch.uint8, device=device))
+            planes.append(torch.zeros((n_slots, n_kv_heads, rows, head_dim // 32), dtype=torch.float16, device=device))
+        return cls(*planes)
+
+
+def kv_append_q4(cache: KvCacheQ4, k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, positions: torch.Tensor) -> None:
+    """Rounds the rows of k and v [n, kv_heads * head_dim] to Q4_0 and writes row j to row positions[j] of slot slots[j].  Rows whose
+    slot or position the cache does not have (padding: -1) are skipped; the pairs of a call must differ."""
+    device = cache.device
+    k, v = _rows(k, "k", device), _rows(v, "v", device)
+    n, dim = k.shape
+    _need(v.shape == k.shape and v.dtype == k.dtype, "k and v must have the same shape and type")
+    _need(dim == cache.n_kv_heads * cache.head_dim, "k and v must have kv_heads * head_dim columns")
+    slots, positions = _ids(slots, n, "slots", device), _ids(positions, n, "positions", device)
+    _call("wick_cuda_kv_append_q4", device, C.byref(cache._c), k.data_ptr(), _stride(k), v.data_ptr(), _stride(v), _dtype_id(k), n,
+          slots.data_ptr(), positions.data_ptr())
+
+
+def kv_read_q4(cache: KvCacheQ4, slots: torch.Tensor, positions: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
+    """The values of row positions[j] of slot slots[j]: k and v [n, kv_heads * head_dim] f32; zeros where the cache has no such row."""
+    device, n = cache.device, slots.shape[0]
+    slots, positions = _ids(slots, n, "slots", device), _ids(positions, n, "positions", device)
+    k, v = torch.empty((2, n, cache.n_kv_heads * cache.head_dim), dtype=torch.float32, device=device)
+    _call("wick_cuda_kv_read_q4", device, C.byref(cache._c), n, slots.data_ptr(), positions.data_ptr(), k.data_ptr(), v.data_ptr())
+    return k, v
+
+
+def attention_q4(q: torch.Tensor, cache: KvCacheQ4, slots: torch.Tensor, lengths: torch.Tensor, n_heads: int,
+                 out: torch.Tensor | None = None) -> torch.Tensor:
+    """Attention of single tokens over the cache: row j of q [n, n_heads * head_dim] attends the first lengths[j] rows of slot
+    slots[j]; several rows may name one slot.  Length 0 gives zeros; rows whose slot the cache does not have (padding: -1) are left as
+    they are in `out` (a new one starts with zeros)."""
+    device = cache.device
+    q = _rows(q, "q", device)
+    n, dim = q.shape
+    _need(dim == n_heads * cache.head_dim, "q must have n_heads * head_dim columns")
+    slots, lengths = _ids(slots, n, "slots", device), _ids(lengths, n, "lengths", device)
+    dtype = _dtype_id(q)
+    if out is None:
+        out = torch.zeros((n, dim), dtype=q.dtype, device=device)
+    _need(out.shape == q.shape and out.dtype == q.dtype and out.device == device and out.is_contiguous(), "out must be dense, of q's shape and type")
+    size = C.c_uint64(0)
+    check(_lib.load().wick_cuda_attention_q4_workspace(C.byref(cache._c), n, n_heads, C.byref(size)))
+    work = torch.empty(size.value, dtype=torch.uint8, device=device)
+    _call("wick_cuda_attention_q4", device, C.byref(cache._c), q.data_ptr(), _stride(q), dtype, n, n_heads, slots.data_ptr(), lengths.data_ptr(),
+          out.data_ptr(), work.data_ptr(), size.value)
+    return out
+
+
+def attention_prompts(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, starts: torch.Tensor, n_heads: int, n_kv_heads: int, head_dim: int,
+                      key_starts: torch.Tensor | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
+    """Causal attention of packed prompts: sequence s has the tokens starts[s] .. starts[s + 1] of q [tokens, n_heads * head_dim] and the
+    keys key_starts[s] .. key_starts[s + 1] (default: the same) of k and v [keys, n_kv_heads * head_dim]; its last key belongs to its last
+    token.  Tokens without a key get zeros; rows behind the last sequence are left as they are in `out` (a new one starts with zeros)."""
+    device = q.device
+    q, k, v = _rows(q, "q", device), _rows(k, "k", device), _rows(v, "v", device)
+    _need(q.dtype == k.dtype == v.dtype, "q, k and v must have the same type")
+    _need(n_heads > 0 and n_kv_heads > 0 and q.shape[1] == n_heads * head_dim, "q must have n_heads * head_dim columns")
+    _need(k.shape == v.shape and k.shape[1] == n_kv_heads * head_dim, "k and v must have n_kv_heads * head_dim columns")
+    n_seqs = starts.shape[0] - 1
+    _need(n_seqs >= 0, "starts must hold at least one offset")
+    starts = _ids(starts, n_seqs + 1, "starts", device)
+    if key_starts is not None:
+        key_starts = _ids(key_starts, n_seqs + 1, "key_starts", device)
+    dtype = _dtype_id(q)
+    # 16-byte loads: rows that start elsewhere are copied
+    q, k, v = (t if (t.data_ptr() | _stride(t) * t.element_size()) % 16 == 0 else t.clone(memory_format=torch.contiguous_format) for t in (q, k, v))
+    if out is None:
+        out = torch.zeros(q.shape, dtype=q.dtype, device=device)
+    _need(out.shape == q.shape and out.dtype == q.dtype and out.device == device and out.is_contiguous(), "out must be dense, of q's shape and type")
+    size = C.c_uint64(0)
+    check(_lib.load().wick_cuda_attention_prompts_workspace(dtype, n_seqs, q.shape[0], k.shape[0], n_heads, n_kv_heads, head_dim, C.byref(size)))
+    work = torch.empty(size.value, dtype=torch.uint8, device=device)
+    _call("wick_cuda_attention_prompts", device, q.data_ptr(), _stride(q), k.data_ptr(), _stride(k), v.data_ptr(), _stride(v), dtype,
+          starts.data_ptr(), key_starts.data_ptr() if key_starts is not None else None, n_seqs, q.shape[0], k.shape[0], n_heads, n_kv_heads,
+          head_dim, out.data_ptr(), work.data_ptr(), size.value)
+    return out
