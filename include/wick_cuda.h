@@ -433,10 +433,10 @@ int32_t wick_cuda_attention_q4(const wick_cuda_kv_q4* cache, const void* q_dev, 
 /* Causal attention of packed prompts: sequence s has the tokens [starts[s], starts[s+1]) of q [n_tokens][n_heads*head_dim] and the keys
  * [key_starts[s], key_starts[s+1]) of k and v [n_keys][n_kv_heads*head_dim]; its last key belongs to its last token, so that token j of
  * nq attends its keys t <= j + nk - nq.  starts_dev / key_starts_dev hold n_seqs + 1 ascending offsets; key_starts_dev NULL: the same as
- * starts_dev.  A token without keys gets zeros.  Rows of q and out that belong to no sequence (behind the last one) are not used and left as
- * they were; so are rows of k and v.  Scores are scaled by 1 / sqrt(head_dim).  All of q, k, v, out have the type `dtype`; rows of q, k,
+ * starts_dev.  A token without keys gets zeros.  Rows of q, k and v that belong to no sequence (behind the last one) are not used, those of
+ * out are set to zero with zero_rest != 0 and left as they were otherwise.  Scores are scaled by 1 / sqrt(head_dim).  All of q, k, v, out have the type `dtype`; rows of q, k,
  * v are q_stride / k_stride / v_stride elements apart; out rows are dense.  head_dim is a multiple of 8 and at most 128;
- * pointers and row strides are multiples of 16 bytes (out: of its elements).  A key or value that is infinite or NaN reaches the tokens
+ * pointers and row strides are multiples of 16 bytes.  A key or value that is infinite or NaN reaches the tokens
  * that attend it and no others.  workspace_dev: 128-byte aligned, as many bytes as
  * wick_cuda_attention_prompts_workspace says, with any content; of this call alone until it has finished. */
 int32_t wick_cuda_attention_prompts_workspace(int32_t dtype, uint32_t n_seqs, uint32_t n_tokens, uint32_t n_keys, uint32_t n_heads,
@@ -444,7 +444,8 @@ int32_t wick_cuda_attention_prompts_workspace(int32_t dtype, uint32_t n_seqs, ui
 int32_t wick_cuda_attention_prompts(const void* q_dev, uint64_t q_stride, const void* k_dev, uint64_t k_stride, const void* v_dev,
                                     uint64_t v_stride, int32_t dtype, const int32_t* starts_dev, const int32_t* key_starts_dev,
                                     uint32_t n_seqs, uint32_t n_tokens, uint32_t n_keys, uint32_t n_heads, uint32_t n_kv_heads,
-                                    uint32_t head_dim, void* out_dev, void* workspace_dev, uint64_t workspace_bytes, void* stream);
+                                    uint32_t head_dim, void* out_dev, int32_t zero_rest, void* workspace_dev, uint64_t workspace_bytes,
+                                    void* stream);
 
 /* ---- tensor-parallel all-reduce over peer memory (extension) -----------------
  * wick runs on one device; there is no counterpart in its tree.  For a tensor-parallel split of the LFM2 layers over

@@ -67,7 +67,7 @@ def test_attention_prompts(cuda_lib):
     size = C.c_uint64(0)
 
     def call(q=A, qs=256, k=A, ks=128, v=A, vs=128, dtype=0, starts=A, seqs=2, tokens=9, keys=9, heads=4, kv=2, hd=64, out=A, work=A, room=1 << 40):
-        return cuda_lib.wick_cuda_attention_prompts(q, qs, k, ks, v, vs, dtype, starts, None, seqs, tokens, keys, heads, kv, hd, out, work, room, None)
+        return cuda_lib.wick_cuda_attention_prompts(q, qs, k, ks, v, vs, dtype, starts, None, seqs, tokens, keys, heads, kv, hd, out, 0, work, room, None)
 
     for bad in (dict(q=None), dict(k=None), dict(starts=None), dict(out=None), dict(qs=255), dict(ks=64), dict(vs=127), dict(heads=5), dict(heads=0),
                 dict(kv=0), dict(hd=0), dict(hd=4), dict(hd=136), dict(q=A + 8), dict(v=A + 4), dict(ks=129), dict(heads=514, kv=2), dict(tokens=(1 << 30) + 1),

@@ -37,6 +37,7 @@ struct Prompts {
     const int32_t *starts, *key_starts;
     int n_seqs, n_tokens, n_keys, n_heads, n_kv, head_dim;
     void* out;
+    int zero_rest;  // rows of out that belong to no sequence: set to zero (else left alone)
 };
 size_t attention_prompts_workspace(const Prompts& p);
 cudaError_t launch_attention_prompts(cudaStream_t st, const Prompts& p, void* workspace);

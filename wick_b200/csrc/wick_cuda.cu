@@ -2586,18 +2586,18 @@ int32_t wick_cuda_attention_prompts_workspace(int32_t dtype, uint32_t n_seqs, ui
 
 int32_t wick_cuda_attention_prompts(const void* q_dev, uint64_t q_stride, const void* k_dev, uint64_t k_stride, const void* v_dev, uint64_t v_stride,
                                     int32_t dtype, const int32_t* starts_dev, const int32_t* key_starts_dev, uint32_t n_seqs, uint32_t n_tokens,
-                                    uint32_t n_keys, uint32_t n_heads, uint32_t n_kv_heads, uint32_t head_dim, void* out_dev, void* workspace_dev,
-                                    uint64_t workspace_bytes, void* stream) {
+                                    uint32_t n_keys, uint32_t n_heads, uint32_t n_kv_heads, uint32_t head_dim, void* out_dev, int32_t zero_rest,
+                                    void* workspace_dev, uint64_t workspace_bytes, void* stream) {
     Prompts p{q_dev, k_dev, v_dev, q_stride, k_stride, v_stride, dtype, starts_dev, key_starts_dev, (int)n_seqs, (int)n_tokens, (int)n_keys,
-              (int)n_heads, (int)n_kv_heads, (int)head_dim, out_dev};
+              (int)n_heads, (int)n_kv_heads, (int)head_dim, out_dev, zero_rest};
     W_TRY(check_prompts(p, n_seqs, n_tokens, n_keys, n_heads, n_kv_heads, head_dim));
     if (n_seqs == 0 || n_tokens == 0) return WICK_CUDA_OK;
     if (!q_dev || (n_keys && (!k_dev || !v_dev)) || !starts_dev || !out_dev) return fail(WICK_CUDA_ERR_BAD_ARG, "NULL argument");
     const size_t b = dtype_bytes(dtype);
     if (q_stride < (uint64_t)n_heads * head_dim || k_stride < (uint64_t)n_kv_heads * head_dim || v_stride < (uint64_t)n_kv_heads * head_dim)
         return fail(WICK_CUDA_ERR_BAD_ARG, "attention_prompts: rows overlap");
-    if (misaligned(q_dev, 16) || misaligned(k_dev, 16) || misaligned(v_dev, 16) || q_stride * b % 16 || k_stride * b % 16 || v_stride * b % 16 || misaligned(out_dev, b))
-        return fail(WICK_CUDA_ERR_BAD_ARG, "attention_prompts: q, k, v and their row strides must be multiples of 16 bytes");
+    if (misaligned(q_dev, 16) || misaligned(k_dev, 16) || misaligned(v_dev, 16) || q_stride * b % 16 || k_stride * b % 16 || v_stride * b % 16 || misaligned(out_dev, 16))
+        return fail(WICK_CUDA_ERR_BAD_ARG, "attention_prompts: q, k, v, out and the row strides must be multiples of 16 bytes");
     if (q_stride * b >= (1ull << 40) || k_stride * b >= (1ull << 40) || v_stride * b >= (1ull << 40))
         return fail(WICK_CUDA_ERR_BAD_ARG, "attention_prompts: row strides too large");
     const uint64_t need = attention_prompts_workspace(p);

@@ -359,13 +359,17 @@ def attention_prompts(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, starts:
     dtype = _dtype_id(q)
     # 16-byte loads: rows that start elsewhere are copied
     q, k, v = (t if (t.data_ptr() | _stride(t) * t.element_size()) % 16 == 0 else t.clone(memory_format=torch.contiguous_format) for t in (q, k, v))
-    if out is None:
-        out = torch.zeros(q.shape, dtype=q.dtype, device=device)
-    _need(out.shape == q.shape and out.dtype == q.dtype and out.device == device and out.is_contiguous(), "out must be dense, of q's shape and type")
+    fresh = out is None
+    if fresh:
+        out = torch.empty(q.shape, dtype=q.dtype, device=device)
+    _need(out.shape == q.shape and out.dtype == q.dtype and out.device == device and out.is_contiguous() and out.data_ptr() % 16 == 0,
+          "out must be dense, of q's shape and type and start on a 16-byte boundary")
     size = C.c_uint64(0)
     check(_lib.load().wick_cuda_attention_prompts_workspace(dtype, n_seqs, q.shape[0], k.shape[0], n_heads, n_kv_heads, head_dim, C.byref(size)))
     work = torch.empty(size.value, dtype=torch.uint8, device=device)
+    if n_seqs == 0:
+        return out.zero_() if fresh else out
     _call("wick_cuda_attention_prompts", device, q.data_ptr(), _stride(q), k.data_ptr(), _stride(k), v.data_ptr(), _stride(v), dtype,
           starts.data_ptr(), key_starts.data_ptr() if key_starts is not None else None, n_seqs, q.shape[0], k.shape[0], n_heads, n_kv_heads,
-          head_dim, out.data_ptr(), work.data_ptr(), size.value)
+          head_dim, out.data_ptr(), fresh, work.data_ptr(), size.value)
     return out
