@@ -24,7 +24,7 @@ def test_caches_that_do_not_fit(cuda_lib, bad):
     assert cuda_lib.wick_cuda_kv_append_q4(C.byref(c), A, 128, A, 128, 0, 1, A, A, None) == _lib.ERR_BAD_ARG
     assert cuda_lib.wick_cuda_kv_read_q4(C.byref(c), 1, A, A, A, A, None) == _lib.ERR_BAD_ARG
     assert cuda_lib.wick_cuda_attention_q4_workspace(C.byref(c), 1, 4, C.byref(size)) == _lib.ERR_BAD_ARG
-    assert cuda_lib.wick_cuda_attention_q4(C.byref(c), A, 256, 0, 1, 4, A, A, A, A, 1 << 30, None) == _lib.ERR_BAD_ARG
+    assert cuda_lib.wick_cuda_attention_q4(C.byref(c), A, 256, 0, 1, 4, A, A, A, 0, A, 1 << 30, None) == _lib.ERR_BAD_ARG
 
 
 def test_append_and_read(cuda_lib):
@@ -51,15 +51,15 @@ def test_attention_q4(cuda_lib):
     assert cuda_lib.wick_cuda_attention_q4_workspace(c, 70000, 4, C.byref(size)) == _lib.ERR_BAD_ARG
     assert cuda_lib.wick_cuda_attention_q4_workspace(c, 3, 4, C.byref(size)) == _lib.OK
     big = 1 << 30
-    assert f(c, A, 255, 0, 3, 4, A, A, A, A, big, None) == _lib.ERR_BAD_ARG
-    assert f(c, A, 256, 5, 3, 4, A, A, A, A, big, None) == _lib.ERR_UNSUPPORTED_DTYPE
-    assert f(c, A + 2, 256, 0, 3, 4, A, A, A, A, big, None) == _lib.ERR_BAD_ARG
-    assert f(c, A, 256, 0, 3, 4, None, A, A, A, big, None) == _lib.ERR_BAD_ARG
-    assert f(c, A, 256, 0, 0, 4, None, None, None, None, 0, None) == _lib.OK
+    assert f(c, A, 255, 0, 3, 4, A, A, A, 0, A, big, None) == _lib.ERR_BAD_ARG
+    assert f(c, A, 256, 5, 3, 4, A, A, A, 0, A, big, None) == _lib.ERR_UNSUPPORTED_DTYPE
+    assert f(c, A + 2, 256, 0, 3, 4, A, A, A, 0, A, big, None) == _lib.ERR_BAD_ARG
+    assert f(c, A, 256, 0, 3, 4, None, A, A, 0, A, big, None) == _lib.ERR_BAD_ARG
+    assert f(c, A, 256, 0, 0, 4, None, None, None, 0, None, 0, None) == _lib.OK
     if size.value:
-        assert f(c, A, 256, 0, 3, 4, A, A, A, A, size.value - 1, None) == _lib.ERR_BAD_ARG
-        assert f(c, A, 256, 0, 3, 4, A, A, A, A + 8, size.value, None) == _lib.ERR_BAD_ARG
-        assert f(c, A, 256, 0, 3, 4, A, A, A, None, size.value, None) == _lib.ERR_BAD_ARG
+        assert f(c, A, 256, 0, 3, 4, A, A, A, 0, A, size.value - 1, None) == _lib.ERR_BAD_ARG
+        assert f(c, A, 256, 0, 3, 4, A, A, A, 0, A + 8, size.value, None) == _lib.ERR_BAD_ARG
+        assert f(c, A, 256, 0, 3, 4, A, A, A, 0, None, size.value, None) == _lib.ERR_BAD_ARG
 
 
 def test_attention_prompts(cuda_lib):

@@ -1,0 +1,564 @@
+// Attention of single tokens over the 4-bit cache:  o = sum_t p_t V_t / sum_t p_t,  p_t = 2^(x_t - m),
+// x_t = log2(e) / sqrt(d) q . K_t, with K_t and V_t blocks d (n - 8) of four-bit numbers n.
+//
+// Bound: HBM, 18 bytes per 32 keys' or values' elements.  f32 arithmetic on the CUDA cores could not keep up with it (4 query heads to a KV head need
+// 14 f32 operations per byte, four times what the SMs have beside unpacking), and an M = 128 tile of tcgen05 would hold 4 to 8 useful rows: the products are
+// mma.sync m16n8k16 with the numbers n - 8, exact in f16, as one operand.  The other one, q or the weights, is f32 and is held as two
+// f16 parts (22 bits): rows 0 .. 7 of a tile are the high parts of up to 8 query heads, rows 8 .. 15 their low parts, so that both
+// come out of one instruction and are added in the lane that holds them.
+//   scores:  S = sum over blocks of d_K (q . (n - 8));  the blocks' integers are products of their own, scaled and added in f32;
+//   values:  the weight of a key is p d_V, per block; sums over the 64 keys of a tile in the tensor core, over tiles in registers
+//            (with the running maximum's factor), since the tensor core's additions truncate.
+// High and low parts need a common exponent: q is scaled by a power of two per head, weights by one per tile, the largest |d_V| of
+// the keys so far.
+//
+// Work: tiles of 64 keys of every (row, group of up to 8 query heads of a KV head), as one list that is cut into equal parts, first over the
+// CTAs, then over their warps: any mix of lengths keeps every SM busy.  A warp streams its tiles through a ring of its own (four
+// bulk copies per tile).  A (row, group) that lies within a warp's part is finished there, parts of one are joined within the CTA, and
+// what reaches over CTAs goes to the workspace, where k_attention_q4_join adds it up in order: results do not depend on timing.
+//
+// What lies behind a row's length is read (the tile is there) but not used: its scores are masked, its scales count as 0.
+// Waits are bounded: on expiry the warp's outputs become NaN.
+#include "serving.cuh"
+
+namespace wick {
+
+namespace {
+
+constexpr int A4_TILE = KV_Q4_TILE, A4_HEADS = 8;
+constexpr uint32_t A4_SPIN_LIMIT = 1u << 18;
+
+template <int NB>  // 32-element blocks of a head
+struct Q4Cfg {
+    static constexpr int HD = 32 * NB;
+    static constexpr int QUANTS = A4_TILE * 16 * NB, SCALES = A4_TILE * 2 * NB;  // bytes of a tile
+    static constexpr int STAGE = 2 * (QUANTS + SCALES);
+    static constexpr int PART = A4_HEADS * HD + 2 * A4_HEADS;                    // floats of a partial result: o, m, l
+    static constexpr int STAGES = NB > 2 ? 2 : 3;
+    static constexpr int FIT = (216 * 1024) / (STAGES * STAGE + 2 * PART * 4), WARPS = FIT < 12 ? FIT : 12;
+    static constexpr int THREADS = 32 * WARPS;
+    static constexpr size_t SMEM = (size_t)WARPS * (STAGES * STAGE + 2 * PART * 4);
+};
+
+struct Q4Args {
+    KvQ4 c;
+    const void* q;
+    size_t q_stride;
+    const int32_t *slots, *lengths;
+    void* out;
+    int n, n_heads, group, sub, n_hg;  // query heads per KV head, head groups per KV head and in all
+    int zero_rest;
+    float scale_log2;
+    float* parts;   // [ctas][2][PART]: a CTA's part of what began before it, and of what goes on behind it
+    int4* descs;    // [ctas][2]: row, head group, whether it holds its begin (1) and its end (2), whether there is one
+};
+
+__device__ __forceinline__ uint32_t s_u32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
+__device__ __forceinline__ void bulk_copy(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src), "r"(bytes), "r"(bar)
+                 : "memory");
+}
+__device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity) {
+    for (uint32_t i = 0; i < A4_SPIN_LIMIT; i++) {
+        uint32_t ok;
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t"
+            "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+            "selp.u32 %0, 1, 0, p;\n\t}"
+            : "=r"(ok)
+            : "r"(bar), "r"(parity)
+            : "memory");
+        if (ok) return true;
+    }
+    return false;
+}
+__device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t pack_f16(float a, float b) {  // a in the low half
+    uint32_t r;
+    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(b), "f"(a));
+    return r;
+}
+__device__ __forceinline__ float exp2_approx(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+// Four-bit numbers at bits 0 and 16, or 4 and 20, of w as n - 8 in f16: 1024 + n is a number's bits behind f16's 1024.
+__device__ __forceinline__ uint32_t low_pair(uint32_t w) {
+    uint32_t r;
+    asm("add.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"((w & 0x000F000Fu) | 0x64006400u), "r"(0xE408E408u));  // - 1032
+    return r;
+}
+__device__ __forceinline__ uint32_t high_pair(uint32_t w) {
+    uint32_t r;
+    asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(r) : "r"((w & 0x00F000F0u) | 0x64006400u), "r"(0x2C002C00u), "r"(0xD480D480u));  // / 16 - 72
+    return r;
+}
+// The high part of x, 11 bits.
+__device__ __forceinline__ float high_part(float x) { return __uint_as_float(__float_as_uint(x) & 0xFFFFE000u); }
+__device__ __forceinline__ float pow2(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }  // -126 <= e <= 127
+
+// The scales of a key's blocks in shared memory, as f32.
+template <int NB>
+__device__ __forceinline__ void load_scales(const __half* p, float (&d)[NB]) {
+    if constexpr (NB == 2 || NB == 4) {
+#pragma unroll
+        for (int i = 0; i < NB; i += 2) {
+            const float2 f = __half22float2(reinterpret_cast<const __half2*>(p)[i / 2]);
+            d[i] = f.x, d[i + 1] = f.y;
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < NB; i++) d[i] = __half2float(p[i]);
+    }
+}
+
+struct Cursor {  // a tile of the list
+    int j, hg, t, tiles, len, slot;
+};
+__device__ __forceinline__ int row_tiles(const Q4Args& a, int j) {
+    const int slot = a.slots[j];
+    return slot < 0 || slot >= a.c.n_slots ? 0 : (max(0, min(a.lengths[j], a.c.max_seq)) + A4_TILE - 1) / A4_TILE;
+}
+__device__ __forceinline__ void enter_row(const Q4Args& a, Cursor& c) {
+    c.slot = a.slots[c.j];
+    c.len = max(0, min(a.lengths[c.j], a.c.max_seq));
+    c.tiles = (c.len + A4_TILE - 1) / A4_TILE;
+}
+__device__ __forceinline__ void advance(const Q4Args& a, Cursor& c) {  // (the caller knows that there is another tile)
+    if (++c.t < c.tiles) return;
+    c.t = 0;
+    if (++c.hg < a.n_hg) return;
+    c.hg = 0;
+    do c.j++;
+    while (c.j < a.n - 1 && row_tiles(a, c.j) == 0);
+    enter_row(a, c);
+}
+
+template <int NB>
+__device__ __forceinline__ void fetch(const Q4Args& a, const Cursor& c, uint32_t stage, uint32_t bar) {
+    using C = Q4Cfg<NB>;
+    const size_t row = a.c.row(c.slot, c.hg / a.sub, c.t * A4_TILE);
+    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(C::STAGE) : "memory");
+    bulk_copy(stage, a.c.q[0] + row * (16 * NB), C::QUANTS, bar);
+    bulk_copy(stage + C::QUANTS, a.c.q[1] + row * (16 * NB), C::QUANTS, bar);
+    bulk_copy(stage + 2 * C::QUANTS, a.c.d[0] + row * NB, C::SCALES, bar);
+    bulk_copy(stage + 2 * C::QUANTS + C::SCALES, a.c.d[1] + row * NB, C::SCALES, bar);
+}
+
+// Dim of column n (0 .. 7) of value tile i of a block: the four numbers of bytes 2n, 2n + 1.
+__device__ __forceinline__ int value_dim(int i, int n) { return 16 * (i & 1) + 2 * n + (i >> 1); }
+
+// One head of a chain of parts, added up in order by a warp (lane: the dims lane, lane + 32, ..): its result, or, keep not null, the part
+// that all of them are.  `next` gives the parts one after the other, NULL behind the last, and starts anew when called with true.
+template <class T, int NB, class Next>
+__device__ __forceinline__ void join_head(const Q4Args& a, int row, int hg, int g, Next&& next, float* keep) {
+    using C = Q4Cfg<NB>;
+    const int lane = threadIdx.x & 31, head = hg / a.sub * a.group + hg % a.sub * A4_HEADS + g;
+    float m = __int_as_float(0xFF800000);
+    for (const float* p = next(true); p; p = next(false)) m = fmaxf(m, p[A4_HEADS * C::HD + g]);
+    float l = 0.0f, o[NB] = {};
+    for (const float* p = next(true); p; p = next(false)) {
+        const float mi = p[A4_HEADS * C::HD + g], f = mi == m ? 1.0f : exp2_approx(mi - m);
+        l = fmaf(p[A4_HEADS * C::HD + A4_HEADS + g], f, l);
+#pragma unroll
+        for (int b = 0; b < NB; b++) o[b] = fmaf(p[g * C::HD + 32 * b + lane], f, o[b]);
+    }
+    if (keep) {
+#pragma unroll
+        for (int b = 0; b < NB; b++) keep[g * C::HD + 32 * b + lane] = o[b];
+        if (lane == 0) keep[A4_HEADS * C::HD + g] = m, keep[A4_HEADS * C::HD + A4_HEADS + g] = l;
+    } else {
+        const float inv = __fdiv_rn(1.0f, l);
+        T* out = static_cast<T*>(a.out) + ((size_t)row * a.n_heads + head) * C::HD;
+#pragma unroll
+        for (int b = 0; b < NB; b++) out[32 * b + lane] = from_f32<T>(__fmul_rn(o[b], inv));
+    }
+}
+
+template <class T, int NB>
+__global__ void __launch_bounds__(Q4Cfg<NB>::THREADS, 1) k_attention_q4(const __grid_constant__ Q4Args a) {
+    using C = Q4Cfg<NB>;
+    extern __shared__ __align__(128) uint8_t sm[];
+    __shared__ __align__(8) unsigned long long bars[C::WARPS][C::STAGES];
+    __shared__ unsigned long long pre[C::THREADS + 1];  // tiles of the rows before a thread's
+    __shared__ unsigned long long warp_sum[C::WARPS];
+    __shared__ int4 desc[C::WARPS][2];
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t4 = lane & 3;
+    if (lane < C::STAGES) asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(s_u32(&bars[warp][lane])) : "memory");
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    if (lane < 2) desc[warp][lane] = make_int4(0, 0, 0, 0);
+    pdl_trigger();
+    pdl_wait();
+
+    // ── where this CTA's and this warp's part of the list begins ──
+    const int chunk = (a.n + C::THREADS - 1) / C::THREADS;
+    unsigned long long mine = 0;
+    for (int i = 0; i < chunk; i++) {
+        const int j = tid * chunk + i;
+        if (j < a.n) mine += row_tiles(a, j);
+    }
+    unsigned long long scan = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const unsigned long long v = __shfl_up_sync(0xffffffffu, scan, o);
+        if (lane >= o) scan += v;
+    }
+    if (lane == 31) warp_sum[warp] = scan;
+    __syncthreads();
+    unsigned long long before = 0, total = 0;
+#pragma unroll
+    for (int w = 0; w < C::WARPS; w++) {
+        if (w < warp) before += warp_sum[w];
+        total += warp_sum[w];
+    }
+    pre[tid] = before + scan - mine;
+    __syncthreads();
+    total *= (unsigned)a.n_hg;
+    const unsigned long long ctas = total < gridDim.x ? total : gridDim.x;  // (a short list: one tile to a CTA)
+    unsigned long long p0 = 0, p1 = 0;
+    if (blockIdx.x < ctas) {
+        const unsigned long long c0 = total * blockIdx.x / ctas, c1 = total * (blockIdx.x + 1) / ctas;
+        p0 = c0 + (c1 - c0) * warp / C::WARPS, p1 = c0 + (c1 - c0) * (warp + 1) / C::WARPS;
+    }
+    // rows without a tile: zeros where the row is one of the cache (or zero_rest asks for it)
+    for (int j = blockIdx.x; j < a.n; j += gridDim.x)
+        if (row_tiles(a, j) == 0 && (a.zero_rest || (a.slots[j] >= 0 && a.slots[j] < a.c.n_slots)))
+            for (int i = tid; i < a.n_heads * C::HD; i += C::THREADS) static_cast<T*>(a.out)[(size_t)j * a.n_heads * C::HD + i] = from_f32<T>(0.0f);
+
+    float* parts = reinterpret_cast<float*>(sm + (size_t)C::WARPS * C::STAGES * C::STAGE);  // [warps][2][PART]
+    bool ok = true;
+    if (p0 < p1) {
+        Cursor cur;
+        {
+            const unsigned long long row_at = p0 / (unsigned)a.n_hg;
+            int lo = 0, hi = C::THREADS - 1;
+            while (lo < hi) {  // the last thread whose rows begin at or before it
+                const int mid = (lo + hi + 1) / 2;
+                if (pre[mid] <= row_at) lo = mid;
+                else hi = mid - 1;
+            }
+            unsigned long long acc = pre[lo];
+            cur.j = lo * chunk;
+            for (; cur.j < a.n - 1; cur.j++) {
+                const int n = row_tiles(a, cur.j);
+                if (acc + n > row_at) break;
+                acc += n;
+            }
+            enter_row(a, cur);
+            const unsigned long long r = p0 - acc * (unsigned)a.n_hg;
+            cur.hg = (int)(r / (unsigned)cur.tiles), cur.t = (int)(r % (unsigned)cur.tiles);
+        }
+        const unsigned n_mine = (unsigned)(p1 - p0);
+        uint8_t* ring = sm + (size_t)warp * C::STAGES * C::STAGE;
+        Cursor ahead = cur;
+        unsigned fetched = 0;
+        for (; fetched < C::STAGES && fetched < n_mine; fetched++) {
+            if (fetched) advance(a, ahead);
+            if (lane == 0) fetch<NB>(a, ahead, s_u32(ring + fetched * C::STAGE), s_u32(&bars[warp][fetched]));
+        }
+        uint32_t qa[NB][2][4];  // q of heads g (rows g: high, g + 8: low parts)
+        float q_inv = 0.0f, m = 0.0f, l = 0.0f, o[NB][4][2];
+        int vexp = -100;        // weights are scaled by 2^(12 - vexp)
+        bool begins = false, fresh = true;
+        for (unsigned i = 0; i < n_mine; i++) {
+            if (fresh) {  // another row or head group
+                fresh = false;
+                begins = cur.t == 0;
+                m = __int_as_float(0xFF800000), l = 0.0f, vexp = -100;
+#pragma unroll
+                for (int b = 0; b < NB; b++)
+#pragma unroll
+                    for (int c = 0; c < 4; c++) o[b][c][0] = o[b][c][1] = 0.0f;
+                const int h0 = cur.hg % a.sub * A4_HEADS;
+                const bool real = h0 + g < a.group;
+                const T* q = static_cast<const T*>(a.q) + (size_t)cur.j * a.q_stride + (size_t)((cur.hg / a.sub) * a.group + h0 + (real ? g : 0)) * C::HD;
+                float x[NB][2][4], top = 0.0f;
+#pragma unroll
+                for (int b = 0; b < NB; b++)
+#pragma unroll
+                    for (int h = 0; h < 2; h++)
+#pragma unroll
+                        for (int e = 0; e < 4; e++) {
+                            x[b][h][e] = real ? __fmul_rn(to_f32(q[32 * b + 16 * h + 4 * t4 + e]), a.scale_log2) : 0.0f;
+                            top = fmaxf(top, fabsf(x[b][h][e]));
+                        }
+                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+                const int e = max(-100, min(100, (int)((__float_as_uint(top) >> 23) & 255u) - 127));
+                const float f = pow2(12 - e);
+                q_inv = pow2(e - 12);
+#pragma unroll
+                for (int b = 0; b < NB; b++)
+#pragma unroll
+                    for (int s = 0; s < 2; s++)
+#pragma unroll
+                        for (int h = 0; h < 2; h++) {
+                            const float x0 = __fmul_rn(x[b][h][s], f), x1 = __fmul_rn(x[b][h][2 + s], f), h0v = high_part(x0), h1v = high_part(x1);
+                            qa[b][s][2 * h] = pack_f16(h0v, h1v);
+                            qa[b][s][2 * h + 1] = pack_f16(__fsub_rn(x0, h0v), __fsub_rn(x1, h1v));
+                        }
+            }
+            const unsigned st = i % C::STAGES;
+            if (ok) ok = __all_sync(0xffffffffu, bar_wait(s_u32(&bars[warp][st]), (i / C::STAGES) & 1));
+            const uint8_t* stage = ring + st * C::STAGE;
+            const uint32_t* kw = reinterpret_cast<const uint32_t*>(stage);
+            const uint32_t* vw = reinterpret_cast<const uint32_t*>(stage + C::QUANTS);
+            const __half* kd = reinterpret_cast<const __half*>(stage + 2 * C::QUANTS);
+            const __half* vd = reinterpret_cast<const __half*>(stage + 2 * C::QUANTS + C::SCALES);
+            const int seen = cur.len - cur.t * A4_TILE;
+            // scores: columns 2 t4, 2 t4 + 1 of the 8-key tiles (block of 16 keys b16, e) are the keys 16 b16 + t4 + 8 e (+ 4)
+            float s[4][2][2];
+#pragma unroll
+            for (int b16 = 0; b16 < 4; b16++)
+#pragma unroll
+                for (int e = 0; e < 2; e++) {
+                    const int key = 16 * b16 + (g >> 1) + 8 * e + 4 * (g & 1), col = 16 * b16 + t4 + 8 * e;
+                    float d0[NB], d1[NB];
+                    load_scales<NB>(kd + col * NB, d0);
+                    load_scales<NB>(kd + (col + 4) * NB, d1);
+                    float s0 = 0.0f, s1 = 0.0f;
+#pragma unroll
+                    for (int b = 0; b < NB; b++) {
+                        const uint32_t w = kw[key * 4 * NB + 4 * b + t4];
+                        float c[4] = {0.f, 0.f, 0.f, 0.f};
+                        mma16816(c, qa[b][0], low_pair(w), high_pair(w));
+                        mma16816(c, qa[b][1], low_pair(w >> 8), high_pair(w >> 8));
+                        s0 = fmaf(__fadd_rn(c[0], c[2]), d0[b], s0);
+                        s1 = fmaf(__fadd_rn(c[1], c[3]), d1[b], s1);
+                    }
+                    s[b16][e][0] = __fmul_rn(s0, q_inv), s[b16][e][1] = __fmul_rn(s1, q_inv);
+                }
+            float dv[4][2][2][NB], vtop = 0.0f;
+#pragma unroll
+            for (int b16 = 0; b16 < 4; b16++)
+#pragma unroll
+                for (int e = 0; e < 2; e++)
+#pragma unroll
+                    for (int f = 0; f < 2; f++) {
+                        const int key = 16 * b16 + t4 + 8 * e + 4 * f;
+                        load_scales<NB>(vd + key * NB, dv[b16][e][f]);
+                        if (key >= seen) {
+                            s[b16][e][f] = __int_as_float(0xFF800000);
+#pragma unroll
+                            for (int b = 0; b < NB; b++) dv[b16][e][f][b] = 0.0f;
+                        }
+#pragma unroll
+                        for (int b = 0; b < NB; b++) vtop = fmaxf(vtop, fabsf(dv[b16][e][f][b]));
+                    }
+            float top = m;
+#pragma unroll
+            for (int b16 = 0; b16 < 4; b16++) top = fmaxf(top, fmaxf(fmaxf(s[b16][0][0], s[b16][0][1]), fmaxf(s[b16][1][0], s[b16][1][1])));
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+            vtop = fmaxf(vtop, __shfl_xor_sync(0xffffffffu, vtop, 1));
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+            vtop = fmaxf(vtop, __shfl_xor_sync(0xffffffffu, vtop, 2));
+            const int old = vexp;
+            vexp = max(vexp, (int)((__float_as_uint(vtop) >> 23) & 255u) - 127);  // (f16 scales: at most 15, NaN and infinity 128)
+            vexp = min(vexp, 100);
+            const float alpha = m == top ? 1.0f : exp2_approx(m - top), keep = __fmul_rn(alpha, pow2(max(old - vexp, -126)));
+            m = top;
+            const float base = m == __int_as_float(0xFF800000) ? 0.0f : m, up = pow2(12 - vexp);
+            float sum = 0.0f;
+#pragma unroll
+            for (int b16 = 0; b16 < 4; b16++)
+#pragma unroll
+                for (int e = 0; e < 2; e++)
+#pragma unroll
+                    for (int f = 0; f < 2; f++) {
+                        const float p = exp2_approx(__fsub_rn(s[b16][e][f], base));
+                        sum += p;
+                        s[b16][e][f] = __fmul_rn(p, up);
+                    }
+            l = fmaf(l, alpha, sum);
+            const uint32_t half_sel = (g & 1) ? 0x7632u : 0x5410u;
+#pragma unroll
+            for (int b = 0; b < NB; b++) {
+                float acc[4][4];
+#pragma unroll
+                for (int c = 0; c < 4; c++) acc[c][0] = acc[c][1] = acc[c][2] = acc[c][3] = 0.0f;
+#pragma unroll
+                for (int b16 = 0; b16 < 4; b16++) {
+                    uint32_t pa[4], r[2];
+#pragma unroll
+                    for (int e = 0; e < 2; e++) {
+                        const float x0 = __fmul_rn(s[b16][e][0], dv[b16][e][0][b]), x1 = __fmul_rn(s[b16][e][1], dv[b16][e][1][b]);
+                        const float h0 = high_part(x0), h1 = high_part(x1);
+                        pa[2 * e] = pack_f16(h0, h1);
+                        pa[2 * e + 1] = pack_f16(__fsub_rn(x0, h0), __fsub_rn(x1, h1));
+                        const int key = 16 * b16 + t4 + 8 * e;
+                        r[e] = __byte_perm(vw[key * 4 * NB + 4 * b + (g >> 1)], vw[(key + 4) * 4 * NB + 4 * b + (g >> 1)], half_sel);
+                    }
+                    mma16816(acc[0], pa, low_pair(r[0]), low_pair(r[1]));
+                    mma16816(acc[1], pa, high_pair(r[0]), high_pair(r[1]));
+                    mma16816(acc[2], pa, low_pair(r[0] >> 8), low_pair(r[1] >> 8));
+                    mma16816(acc[3], pa, high_pair(r[0] >> 8), high_pair(r[1] >> 8));
+                }
+#pragma unroll
+                for (int c = 0; c < 4; c++) {
+                    o[b][c][0] = fmaf(o[b][c][0], keep, __fadd_rn(acc[c][0], acc[c][2]));
+                    o[b][c][1] = fmaf(o[b][c][1], keep, __fadd_rn(acc[c][1], acc[c][3]));
+                }
+            }
+            __syncwarp();  // every lane has read the stage
+            if (fetched < n_mine) {
+                advance(a, ahead);
+                if (lane == 0 && ok) fetch<NB>(a, ahead, s_u32(ring + st * C::STAGE), s_u32(&bars[warp][st]));
+                fetched++;
+            }
+            const bool ends = cur.t + 1 == cur.tiles;
+            if (ends || i + 1 == n_mine) {
+                l += __shfl_xor_sync(0xffffffffu, l, 1);
+                l += __shfl_xor_sync(0xffffffffu, l, 2);
+                if (!ok) l = __int_as_float(0x7FC00000);
+                const float down = pow2(vexp - 12);
+                const int h0 = cur.hg % a.sub * A4_HEADS;
+                if (begins && ends) {
+                    if (h0 + g < a.group) {
+                        const float inv = __fdiv_rn(down, l);
+                        T* out = static_cast<T*>(a.out) + ((size_t)cur.j * a.n_heads + (cur.hg / a.sub) * a.group + h0 + g) * C::HD;
+#pragma unroll
+                        for (int b = 0; b < NB; b++)
+#pragma unroll
+                            for (int c = 0; c < 4; c++)
+#pragma unroll
+                                for (int x = 0; x < 2; x++) out[32 * b + value_dim(c, 2 * t4 + x)] = from_f32<T>(__fmul_rn(o[b][c][x], inv));
+                    }
+                } else {
+                    const int place = begins ? 1 : 0;
+                    float* part = parts + (warp * 2 + place) * C::PART;
+#pragma unroll
+                    for (int b = 0; b < NB; b++)
+#pragma unroll
+                        for (int c = 0; c < 4; c++)
+#pragma unroll
+                            for (int x = 0; x < 2; x++) part[g * C::HD + 32 * b + value_dim(c, 2 * t4 + x)] = __fmul_rn(o[b][c][x], down);
+                    if (t4 == 0) part[A4_HEADS * C::HD + g] = m, part[A4_HEADS * C::HD + A4_HEADS + g] = l;
+                    if (lane == 0) desc[warp][place] = make_int4(cur.j, cur.hg, (begins ? 1 : 0) | (ends ? 2 : 0), 1);
+                }
+                fresh = true;
+            }
+            if (i + 1 < n_mine) advance(a, cur);
+        }
+    }
+    if (tid < 2) a.descs[(size_t)blockIdx.x * 2 + tid] = make_int4(0, 0, 0, 0);
+    if (!ok)
+        for (int i = 0; i < 64; i++) __nanosleep(1000);  // copies may still be landing
+    __syncthreads();
+
+    // ── parts within the CTA.  A chain starts with the part that begins in a warp (place 1) or with the first part of all, if that began
+    //    before the CTA, and goes on with the parts that began before (place 0) of the warps behind. ──
+    for (int item = warp; item < (C::WARPS + 1) * A4_HEADS; item += C::WARPS) {
+        const int g8 = item % A4_HEADS, place = item / A4_HEADS < C::WARPS ? 1 : 0;
+        int first = item / A4_HEADS;
+        if (place == 0) {
+            first = 0;
+            while (first < C::WARPS && !desc[first][0].w && !desc[first][1].w) first++;
+        }
+        if (first == C::WARPS || !desc[first][place].w) continue;
+        const int4 d = desc[first][place];
+        if (d.y % a.sub * A4_HEADS + g8 >= a.group) continue;
+        uint32_t chain = 0;  // the warps behind
+        int flags = d.z;
+        for (int w = first + 1; w < C::WARPS && !(flags & 2); w++)
+            if (desc[w][0].w) chain |= 1u << w, flags |= desc[w][0].z;
+        uint32_t left = 0;
+        auto next = [&](bool anew) -> const float* {
+            if (anew) {
+                left = chain;
+                return parts + (first * 2 + place) * C::PART;
+            }
+            if (!left) return nullptr;
+            const int w = __ffs(left) - 1;
+            left &= left - 1;
+            return parts + w * 2 * C::PART;
+        };
+        const bool whole = flags == 3;
+        const size_t to = (size_t)blockIdx.x * 2 + place;
+        join_head<T, NB>(a, d.x, d.y, g8, next, whole ? nullptr : a.parts + to * C::PART);
+        if (!whole && g8 == 0 && lane == 0) a.descs[to] = make_int4(d.x, d.y, flags, 1);
+    }
+}
+
+// What reaches over CTAs: CTA b joins what begins in CTA b of the kernel above and goes on, a warp per head.
+template <class T, int NB>
+__global__ void __launch_bounds__(32 * A4_HEADS) k_attention_q4_join(const __grid_constant__ Q4Args a) {
+    using C = Q4Cfg<NB>;
+    pdl_trigger();
+    pdl_wait();
+    const int4 d = a.descs[(size_t)blockIdx.x * 2 + 1];
+    const int g = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    if (!d.w || d.y % a.sub * A4_HEADS + g >= a.group) return;
+    int last = blockIdx.x;  // the CTA that holds the end
+    for (int b = blockIdx.x + 1;; b += 32) {
+        const bool in = b + lane < (int)gridDim.x;
+        const uint32_t end = __ballot_sync(0xffffffffu, in && (a.descs[(size_t)(b + lane) * 2].z & 2));
+        if (end) {
+            last = b + __ffs(end) - 1;
+            break;
+        }
+        if (b + 32 >= (int)gridDim.x) return;  // (cannot be)
+    }
+    int at = 0;
+    auto next = [&](bool anew) -> const float* {
+        if (anew) {
+            at = blockIdx.x;
+            return a.parts + ((size_t)at * 2 + 1) * C::PART;
+        }
+        return ++at <= last ? a.parts + (size_t)at * 2 * C::PART : nullptr;
+    };
+    join_head<T, NB>(a, d.x, d.y, g, next, nullptr);
+}
+
+constexpr int A4_MAX_CTAS = 256;
+size_t part_bytes(const KvQ4& c) { return (size_t)A4_MAX_CTAS * 2 * (A4_HEADS * c.head_dim + 2 * A4_HEADS) * sizeof(float); }
+
+template <class T, int NB>
+cudaError_t launch_typed(cudaStream_t st, Q4Args& a) {
+    using C = Q4Cfg<NB>;
+    static RaisedPerDevice limit;
+    int dev = 0, sms = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    if ((e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev)) != cudaSuccess) return e;
+    if ((e = raise_dynamic_smem(limit, (const void*)k_attention_q4<T, NB>, C::SMEM)) != cudaSuccess) return e;
+    const dim3 grid((unsigned)(sms < A4_MAX_CTAS ? sms : A4_MAX_CTAS));
+    g_kernel_launches += 2;
+    if ((e = launch_pdl(st, k_attention_q4<T, NB>, grid, dim3(C::THREADS), C::SMEM, a)) != cudaSuccess) return e;
+    return launch_pdl(st, k_attention_q4_join<T, NB>, grid, dim3(32 * A4_HEADS), 0, a);
+}
+template <class T>
+cudaError_t launch_head(cudaStream_t st, Q4Args& a) {
+    switch (a.c.head_dim / QK) {
+        case 1: return launch_typed<T, 1>(st, a);
+        case 2: return launch_typed<T, 2>(st, a);
+        case 3: return launch_typed<T, 3>(st, a);
+        default: return launch_typed<T, 4>(st, a);
+    }
+}
+
+}  // namespace
+
+size_t attention_q4_workspace(const KvQ4& c) { return part_bytes(c) + A4_MAX_CTAS * 2 * sizeof(int4); }
+
+cudaError_t launch_attention_q4(cudaStream_t st, const KvQ4& c, const void* q, size_t q_stride, int dtype, int n, int n_heads, const int32_t* slots,
+                                const int32_t* lengths, void* out, int zero_rest, void* workspace) {
+    Q4Args a{};
+    a.c = c;
+    a.q = q, a.q_stride = q_stride;
+    a.slots = slots, a.lengths = lengths;
+    a.out = out;
+    a.n = n, a.n_heads = n_heads, a.group = n_heads / c.n_kv, a.sub = (a.group + A4_HEADS - 1) / A4_HEADS, a.n_hg = c.n_kv * a.sub;
+    a.zero_rest = zero_rest;
+    a.scale_log2 = 1.4426950408889634f / sqrtf((float)c.head_dim);
+    a.parts = static_cast<float*>(workspace);
+    a.descs = reinterpret_cast<int4*>(static_cast<uint8_t*>(workspace) + part_bytes(c));
+    return dtype == DT_F32 ? launch_head<float>(st, a) : dtype == DT_F16 ? launch_head<__half>(st, a) : launch_head<__nv_bfloat16>(st, a);
+}
+
+}  // namespace wick

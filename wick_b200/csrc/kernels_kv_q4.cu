@@ -1,4 +1,4 @@
-// The 4-bit K / V cache: append (Q4_0 rounding), read back, and the attention of single tokens over it.
+// The 4-bit K / V cache: append (Q4_0 rounding) and read back; the attention over it is attn_q4.cu.
 //
 // A block is 32 values: d = m / -8 with m the value of largest magnitude (the first of equal ones), q = min(15, trunc(x / d + 8.5)) as
 // x * (1 / d), d kept in f16; the value it stands for is f16(d) * (q - 8).  Byte i of a block's 16 holds value i in its low and value
@@ -63,12 +63,6 @@ __global__ void __launch_bounds__(KV_THREADS) k_kv_append_q4(KvQ4 c, const T* __
     if (e == 0) c.d[val][row * per_head + blk] = __float2half_rn(d);
 }
 
-__device__ __forceinline__ float q4_value(const KvQ4& c, int val, size_t row, int dim) {
-    const int blk = dim / QK, i = dim % QK;
-    const uint8_t b = c.q[val][row * (c.head_dim / 2) + blk * 16 + (i & 15)];
-    return __fmul_rn(__half2float(c.d[val][row * (c.head_dim / QK) + blk]), (float)((i < 16 ? b & 15 : b >> 4) - 8));
-}
-
 // One thread per four bytes of quants: eight values.  A row that the cache does not have reads as zeros.
 __global__ void __launch_bounds__(KV_THREADS) k_kv_read_q4(KvQ4 c, int n, const int32_t* __restrict__ slots, const int32_t* __restrict__ positions,
                                                            float* __restrict__ k, float* __restrict__ v) {
@@ -94,44 +88,6 @@ __global__ void __launch_bounds__(KV_THREADS) k_kv_read_q4(KvQ4 c, int n, const 
     *reinterpret_cast<float4*>(out + 16) = hi;
 }
 
-// One CTA per (row, query head): runs of 128 keys, a running maximum and sum.
-constexpr int Q4_THREADS = 128;
-template <class T>
-__global__ void __launch_bounds__(Q4_THREADS) k_attention_q4(KvQ4 c, const T* __restrict__ q, size_t q_stride, int n_heads,
-                                                             const int32_t* __restrict__ slots, const int32_t* __restrict__ lengths, T* __restrict__ out) {
-    __shared__ float qs[KV_Q4_MAX_HEAD], p[Q4_THREADS], red[4];
-    const int h = blockIdx.x, j = blockIdx.y, hd = c.head_dim, tid = threadIdx.x, kvh = h / (n_heads / c.n_kv);
-    const int slot = slots[j], len = max(0, min(lengths[j], c.max_seq));
-    if (slot < 0 || slot >= c.n_slots) return;
-    const float scale = __fdiv_rn(1.0f, sqrtf((float)hd));
-    for (int d = tid; d < hd; d += Q4_THREADS) qs[d] = __fmul_rn(to_f32(q[(size_t)j * q_stride + h * hd + d]), scale);
-    float m = __int_as_float(0xFF800000), l = 0.0f, acc = 0.0f;
-    for (int t0 = 0; t0 < len; t0 += Q4_THREADS) {
-        const int t = t0 + tid, nt = min(Q4_THREADS, len - t0);
-        __syncthreads();
-        float s = __int_as_float(0xFF800000);
-        if (t < len) {
-            s = 0.0f;
-            for (int d = 0; d < hd; d++) s = fmaf(qs[d], q4_value(c, 0, c.row(slot, kvh, t), d), s);
-        }
-        float top = s;
-        for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-        if ((tid & 31) == 0) red[tid >> 5] = top;
-        __syncthreads();
-        const float m2 = fmaxf(m, fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3])));
-        const float a = expf(m - m2);
-        p[tid] = t < len ? expf(s - m2) : 0.0f;
-        m = m2;
-        __syncthreads();
-        l *= a, acc *= a;
-        for (int i = 0; i < nt; i++) {
-            l += p[i];
-            if (tid < hd) acc = fmaf(p[i], q4_value(c, 1, c.row(slot, kvh, t0 + i), tid), acc);
-        }
-    }
-    if (tid < hd) out[((size_t)j * n_heads + h) * hd + tid] = from_f32<T>(len ? acc / l : 0.0f);
-}
-
 }  // namespace
 
 cudaError_t launch_kv_append_q4(cudaStream_t st, const KvQ4& c, const void* k, size_t k_stride, const void* v, size_t v_stride, int dtype, int n,
@@ -153,21 +109,6 @@ cudaError_t launch_kv_read_q4(cudaStream_t st, const KvQ4& c, int n, const int32
     const size_t threads = (size_t)n * c.n_kv * c.head_dim / 4;
     g_kernel_launches++;
     return launch_pdl(st, k_kv_read_q4, dim3((unsigned)((threads + KV_THREADS - 1) / KV_THREADS)), dim3(KV_THREADS), 0, c, n, slots, positions, k, v);
-}
-
-size_t attention_q4_workspace(int, int, const KvQ4&) { return 0; }
-
-cudaError_t launch_attention_q4(cudaStream_t st, const KvQ4& c, const void* q, size_t q_stride, int dtype, int n, int n_heads, const int32_t* slots,
-                                const int32_t* lengths, void* out, void*) {
-    const dim3 grid((unsigned)n_heads, (unsigned)n);
-    g_kernel_launches++;
-    if (dtype == DT_F32)
-        k_attention_q4<<<grid, Q4_THREADS, 0, st>>>(c, (const float*)q, q_stride, n_heads, slots, lengths, (float*)out);
-    else if (dtype == DT_F16)
-        k_attention_q4<<<grid, Q4_THREADS, 0, st>>>(c, (const __half*)q, q_stride, n_heads, slots, lengths, (__half*)out);
-    else
-        k_attention_q4<<<grid, Q4_THREADS, 0, st>>>(c, (const __nv_bfloat16*)q, q_stride, n_heads, slots, lengths, (__nv_bfloat16*)out);
-    return cudaGetLastError();
 }
 
 }  // namespace wick

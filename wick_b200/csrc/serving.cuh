@@ -24,9 +24,9 @@ constexpr int KV_Q4_MAX_HEAD = 128;
 cudaError_t launch_kv_append_q4(cudaStream_t st, const KvQ4& c, const void* k, size_t k_stride, const void* v, size_t v_stride, int dtype, int n,
                                 const int32_t* slots, const int32_t* positions);
 cudaError_t launch_kv_read_q4(cudaStream_t st, const KvQ4& c, int n, const int32_t* slots, const int32_t* positions, float* k, float* v);
-size_t attention_q4_workspace(int n, int n_heads, const KvQ4& c);
+size_t attention_q4_workspace(const KvQ4& c);
 cudaError_t launch_attention_q4(cudaStream_t st, const KvQ4& c, const void* q, size_t q_stride, int dtype, int n, int n_heads, const int32_t* slots,
-                                const int32_t* lengths, void* out, void* workspace);
+                                const int32_t* lengths, void* out, int zero_rest, void* workspace);
 
 // Packed prompts.  Rows of q / k / v are q_stride / k_stride / v_stride elements apart; starts (and key_starts, NULL: the same)
 // hold n_seqs + 1 offsets.

@@ -2544,13 +2544,13 @@ int32_t wick_cuda_attention_q4_workspace(const wick_cuda_kv_q4* cache, uint32_t 
     KvQ4 c;
     if (!bytes) return fail(WICK_CUDA_ERR_BAD_ARG, "NULL argument");
     W_TRY(check_attention_q4(cache, n, n_heads, &c));
-    *bytes = attention_q4_workspace((int)n, (int)n_heads, c);
+    *bytes = attention_q4_workspace(c);
     return WICK_CUDA_OK;
 }
 
 int32_t wick_cuda_attention_q4(const wick_cuda_kv_q4* cache, const void* q_dev, uint64_t q_stride, int32_t dtype, uint32_t n, uint32_t n_heads,
-                               const int32_t* slots_dev, const int32_t* lengths_dev, void* out_dev, void* workspace_dev, uint64_t workspace_bytes,
-                               void* stream) {
+                               const int32_t* slots_dev, const int32_t* lengths_dev, void* out_dev, int32_t zero_rest, void* workspace_dev,
+                               uint64_t workspace_bytes, void* stream) {
     KvQ4 c;
     W_TRY(check_attention_q4(cache, n, n_heads, &c));
     W_TRY(check_dtype(dtype));
@@ -2558,10 +2558,10 @@ int32_t wick_cuda_attention_q4(const wick_cuda_kv_q4* cache, const void* q_dev, 
     if (!q_dev || !slots_dev || !lengths_dev || !out_dev) return fail(WICK_CUDA_ERR_BAD_ARG, "NULL argument");
     if (q_stride < (uint64_t)n_heads * c.head_dim) return fail(WICK_CUDA_ERR_BAD_ARG, "attention_q4: rows of q overlap");
     if (misaligned(q_dev, dtype_bytes(dtype)) || misaligned(out_dev, dtype_bytes(dtype))) return fail(WICK_CUDA_ERR_BAD_ARG, "attention_q4: misaligned rows");
-    const uint64_t need = attention_q4_workspace((int)n, (int)n_heads, c);
+    const uint64_t need = attention_q4_workspace(c);
     if (workspace_bytes < need || (need && (!workspace_dev || misaligned(workspace_dev, 16))))
         return fail(WICK_CUDA_ERR_BAD_ARG, "attention_q4: workspace missing, misaligned or too small");
-    CU_TRY(launch_attention_q4((cudaStream_t)stream, c, q_dev, q_stride, dtype, (int)n, (int)n_heads, slots_dev, lengths_dev, out_dev, workspace_dev));
+    CU_TRY(launch_attention_q4((cudaStream_t)stream, c, q_dev, q_stride, dtype, (int)n, (int)n_heads, slots_dev, lengths_dev, out_dev, zero_rest, workspace_dev));
     OP_END();
 }
 

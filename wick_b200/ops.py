@@ -330,14 +330,15 @@ def attention_q4(q: torch.Tensor, cache: KvCacheQ4, slots: torch.Tensor, lengths
     _need(dim == n_heads * cache.head_dim, "q must have n_heads * head_dim columns")
     slots, lengths = _ids(slots, n, "slots", device), _ids(lengths, n, "lengths", device)
     dtype = _dtype_id(q)
-    if out is None:
-        out = torch.zeros((n, dim), dtype=q.dtype, device=device)
+    fresh = out is None
+    if fresh:
+        out = torch.empty((n, dim), dtype=q.dtype, device=device)
     _need(out.shape == q.shape and out.dtype == q.dtype and out.device == device and out.is_contiguous(), "out must be dense, of q's shape and type")
     size = C.c_uint64(0)
     check(_lib.load().wick_cuda_attention_q4_workspace(C.byref(cache._c), n, n_heads, C.byref(size)))
     work = torch.empty(size.value, dtype=torch.uint8, device=device)
     _call("wick_cuda_attention_q4", device, C.byref(cache._c), q.data_ptr(), _stride(q), dtype, n, n_heads, slots.data_ptr(), lengths.data_ptr(),
-          out.data_ptr(), work.data_ptr(), size.value)
+          out.data_ptr(), fresh, work.data_ptr(), size.value)
     return out
 
 

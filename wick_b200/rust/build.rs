@@ -12,7 +12,7 @@ const SOURCES: &[&str] = &[
     "kernels_attn.cu",
     "kernels_q6k.cu",
     "kernels_batch.cu",
-    "kernels_sample.cu", "kernels_logprobs.cu", "kernels_kv_q4.cu", "attn_prompts.cu",
+    "kernels_sample.cu", "kernels_logprobs.cu", "kernels_kv_q4.cu", "attn_q4.cu", "attn_prompts.cu",
     "tp_comm.cu",
     "decode_mega.cu",
     "gemm_tc.cu",
