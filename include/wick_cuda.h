@@ -425,7 +425,7 @@ int32_t wick_cuda_kv_read_q4(const wick_cuda_kv_q4* cache, uint32_t n, const int
  * out [n][n_heads*head_dim] has q's type.  Length 0 (or less) gives zeros; a row whose slot the cache does not have (a padding row: -1)
  * is set to zero with zero_rest != 0 and left as it was otherwise.  What the cache holds behind a row's length is never used, whatever it is.  workspace_dev: 16-byte aligned, as many
  * bytes as wick_cuda_attention_q4_workspace says, with any content; of this call alone until it has finished. */
-int32_t wick_cuda_attention_q4_workspace(const wick_cuda_kv_q4* cache, uint32_t n, uint32_t n_heads, uint64_t* bytes);
+int32_t wick_cuda_attention_q4_workspace(uint32_t head_dim, uint64_t* bytes);
 int32_t wick_cuda_attention_q4(const wick_cuda_kv_q4* cache, const void* q_dev, uint64_t q_stride, int32_t dtype, uint32_t n, uint32_t n_heads,
                                const int32_t* slots_dev, const int32_t* lengths_dev, void* out_dev, int32_t zero_rest, void* workspace_dev,
                                uint64_t workspace_bytes, void* stream);

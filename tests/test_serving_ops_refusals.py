@@ -20,10 +20,9 @@ BAD_CACHES = [dict(k_quants=None), dict(v_scales=None), dict(n_slots=0), dict(n_
 @pytest.mark.parametrize("bad", BAD_CACHES, ids=[str(b) for b in BAD_CACHES])
 def test_caches_that_do_not_fit(cuda_lib, bad):
     from wick_b200 import _lib
-    c, size = _cache(**bad), C.c_uint64(0)
+    c = _cache(**bad)
     assert cuda_lib.wick_cuda_kv_append_q4(C.byref(c), A, 128, A, 128, 0, 1, A, A, None) == _lib.ERR_BAD_ARG
     assert cuda_lib.wick_cuda_kv_read_q4(C.byref(c), 1, A, A, A, A, None) == _lib.ERR_BAD_ARG
-    assert cuda_lib.wick_cuda_attention_q4_workspace(C.byref(c), 1, 4, C.byref(size)) == _lib.ERR_BAD_ARG
     assert cuda_lib.wick_cuda_attention_q4(C.byref(c), A, 256, 0, 1, 4, A, A, A, 0, A, 1 << 30, None) == _lib.ERR_BAD_ARG
 
 
@@ -46,11 +45,14 @@ def test_attention_q4(cuda_lib):
     from wick_b200 import _lib
     c, size = C.byref(_cache()), C.c_uint64(0)
     f = cuda_lib.wick_cuda_attention_q4
-    assert cuda_lib.wick_cuda_attention_q4_workspace(c, 3, 4, None) == _lib.ERR_BAD_ARG
-    assert cuda_lib.wick_cuda_attention_q4_workspace(c, 3, 3, C.byref(size)) == _lib.ERR_BAD_ARG  # 3 heads over 2 KV heads
-    assert cuda_lib.wick_cuda_attention_q4_workspace(c, 70000, 4, C.byref(size)) == _lib.ERR_BAD_ARG
-    assert cuda_lib.wick_cuda_attention_q4_workspace(c, 3, 4, C.byref(size)) == _lib.OK
+    query = cuda_lib.wick_cuda_attention_q4_workspace
+    assert query(64, None) == _lib.ERR_BAD_ARG
+    for head_dim in (0, 40, 160):
+        assert query(head_dim, C.byref(size)) == _lib.ERR_BAD_ARG
+    assert query(64, C.byref(size)) == _lib.OK
     big = 1 << 30
+    assert f(c, A, 256, 0, 3, 3, A, A, A, 0, A, big, None) == _lib.ERR_BAD_ARG  # 3 heads over 2 KV heads
+    assert f(c, A, 256, 0, 70000, 4, A, A, A, 0, A, big, None) == _lib.ERR_BAD_ARG
     assert f(c, A, 255, 0, 3, 4, A, A, A, 0, A, big, None) == _lib.ERR_BAD_ARG
     assert f(c, A, 256, 5, 3, 4, A, A, A, 0, A, big, None) == _lib.ERR_UNSUPPORTED_DTYPE
     assert f(c, A + 2, 256, 0, 3, 4, A, A, A, 0, A, big, None) == _lib.ERR_BAD_ARG

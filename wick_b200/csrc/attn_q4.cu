@@ -3,10 +3,11 @@
 //
 // Bound: HBM, 18 bytes per 32 keys' or values' elements.  f32 arithmetic on the CUDA cores could not keep up with it (4 query heads to a KV head need
 // 14 f32 operations per byte, four times what the SMs have beside unpacking), and an M = 128 tile of tcgen05 would hold 4 to 8 useful rows: the products are
-// mma.sync m16n8k16 with the numbers n - 8, exact in f16, as one operand.  The other one, q or the weights, is f32 and is held as two
+// mma.sync m16n8k16 with the numbers, exact in f16, as one operand.  The other one, q or the weights, is f32 and is held as two
 // f16 parts (22 bits): rows 0 .. 7 of a tile are the high parts of up to 8 query heads, rows 8 .. 15 their low parts, so that both
 // come out of one instruction and are added in the lane that holds them.
-//   scores:  S = sum over blocks of d_K (q . (n - 8));  the blocks' integers are products of their own, scaled and added in f32;
+//   scores:  S = sum over blocks of d_K (q . (n - 8));  a block is two products, scaled and added in f32.  (Numbers as they are stored are
+//            f16's n 2^-24, and a sum could start at -8 sum q: fewer instructions, the same time, and 1.1e-6 off instead of 2.4e-7.)
 //   values:  the weight of a key is p d_V, per block; sums over the 64 keys of a tile in the tensor core, over tiles in registers
 //            (with the running maximum's factor), since the tensor core's additions truncate.
 // High and low parts need a common exponent: q is scaled by a power of two per head, weights by one per tile, the largest |d_V| of
@@ -27,6 +28,7 @@ namespace {
 
 constexpr int A4_TILE = KV_Q4_TILE, A4_HEADS = 8;
 constexpr uint32_t A4_SPIN_LIMIT = 1u << 18;
+constexpr int A4_MIN_EXP = -24;  // of f16's smallest number
 
 template <int NB>  // 32-element blocks of a head
 struct Q4Cfg {
@@ -34,8 +36,8 @@ struct Q4Cfg {
     static constexpr int QUANTS = A4_TILE * 16 * NB, SCALES = A4_TILE * 2 * NB;  // bytes of a tile
     static constexpr int STAGE = 2 * (QUANTS + SCALES);
     static constexpr int PART = A4_HEADS * HD + 2 * A4_HEADS;                    // floats of a partial result: o, m, l
-    static constexpr int STAGES = NB > 2 ? 2 : 3;
-    static constexpr int FIT = (216 * 1024) / (STAGES * STAGE + 2 * PART * 4), WARPS = FIT < 12 ? FIT : 12;
+    static constexpr int STAGES = 2;
+    static constexpr int FIT = (218 * 1024) / (STAGES * STAGE + 2 * PART * 4), WARPS = FIT < 16 ? FIT : 16;
     static constexpr int THREADS = 32 * WARPS;
     static constexpr size_t SMEM = (size_t)WARPS * (STAGES * STAGE + 2 * PART * 4);
 };
@@ -77,6 +79,11 @@ __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], 
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
+__device__ __forceinline__ void mma16816_zero(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {  // (a zero operand is no register)
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
+                 : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.0f));
+}
 __device__ __forceinline__ uint32_t pack_f16(float a, float b) {  // a in the low half
     uint32_t r;
     asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(b), "f"(a));
@@ -88,14 +95,19 @@ __device__ __forceinline__ float exp2_approx(float x) {
     return y;
 }
 // Four-bit numbers at bits 0 and 16, or 4 and 20, of w as n - 8 in f16: 1024 + n is a number's bits behind f16's 1024.
+__device__ __forceinline__ uint32_t behind_1024(uint32_t w, uint32_t mask) {
+    uint32_t r;
+    asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(r) : "r"(w), "r"(mask), "r"(0x64006400u));  // (w & mask) | 1024s, in one
+    return r;
+}
 __device__ __forceinline__ uint32_t low_pair(uint32_t w) {
     uint32_t r;
-    asm("add.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"((w & 0x000F000Fu) | 0x64006400u), "r"(0xE408E408u));  // - 1032
+    asm("add.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(behind_1024(w, 0x000F000Fu)), "r"(0xE408E408u));  // - 1032
     return r;
 }
 __device__ __forceinline__ uint32_t high_pair(uint32_t w) {
     uint32_t r;
-    asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(r) : "r"((w & 0x00F000F0u) | 0x64006400u), "r"(0x2C002C00u), "r"(0xD480D480u));  // / 16 - 72
+    asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(behind_1024(w, 0x00F000F0u)), "r"(0x2C002C00u), "r"(0xD480D480u));  // / 16 - 72
     return r;
 }
 // The high part of x, 11 bits.
@@ -121,8 +133,8 @@ struct Cursor {  // a tile of the list
     int j, hg, t, tiles, len, slot;
 };
 __device__ __forceinline__ int row_tiles(const Q4Args& a, int j) {
-    const int slot = a.slots[j];
-    return slot < 0 || slot >= a.c.n_slots ? 0 : (max(0, min(a.lengths[j], a.c.max_seq)) + A4_TILE - 1) / A4_TILE;
+    const int slot = a.slots[j], len = a.lengths[j];
+    return slot < 0 || slot >= a.c.n_slots ? 0 : (max(0, min(len, a.c.max_seq)) + A4_TILE - 1) / A4_TILE;
 }
 __device__ __forceinline__ void enter_row(const Q4Args& a, Cursor& c) {
     c.slot = a.slots[c.j];
@@ -139,35 +151,78 @@ __device__ __forceinline__ void advance(const Q4Args& a, Cursor& c) {  // (the c
     enter_row(a, c);
 }
 
+// The tiles ahead of the cursor, as running pointers: a tile costs four additions, another (row, head group) a look at the lists.
 template <int NB>
-__device__ __forceinline__ void fetch(const Q4Args& a, const Cursor& c, uint32_t stage, uint32_t bar) {
+struct Stream {
     using C = Q4Cfg<NB>;
-    const size_t row = a.c.row(c.slot, c.hg / a.sub, c.t * A4_TILE);
-    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(C::STAGE) : "memory");
-    bulk_copy(stage, a.c.q[0] + row * (16 * NB), C::QUANTS, bar);
-    bulk_copy(stage + C::QUANTS, a.c.q[1] + row * (16 * NB), C::QUANTS, bar);
-    bulk_copy(stage + 2 * C::QUANTS, a.c.d[0] + row * NB, C::SCALES, bar);
-    bulk_copy(stage + 2 * C::QUANTS + C::SCALES, a.c.d[1] + row * NB, C::SCALES, bar);
-}
+    Cursor at;
+    const uint8_t *kq, *vq;
+    const __half *kd, *vd;
+    __device__ __forceinline__ void place(const Q4Args& a) {
+        const size_t row = a.c.row(at.slot, at.hg / a.sub, at.t * A4_TILE);
+        kq = a.c.q[0] + row * (16 * NB), vq = a.c.q[1] + row * (16 * NB);
+        kd = a.c.d[0] + row * NB, vd = a.c.d[1] + row * NB;
+    }
+    __device__ __forceinline__ void step(const Q4Args& a) {
+        if (at.t + 1 < at.tiles) {
+            at.t++;
+            kq += C::QUANTS, vq += C::QUANTS, kd += C::SCALES / 2, vd += C::SCALES / 2;
+        } else {
+            advance(a, at);
+            place(a);
+        }
+    }
+    __device__ __forceinline__ void fetch(uint32_t stage, uint32_t bar) const {
+        asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(C::STAGE) : "memory");
+        bulk_copy(stage, kq, C::QUANTS, bar);
+        bulk_copy(stage + C::QUANTS, vq, C::QUANTS, bar);
+        bulk_copy(stage + 2 * C::QUANTS, kd, C::SCALES, bar);
+        bulk_copy(stage + 2 * C::QUANTS + C::SCALES, vd, C::SCALES, bar);
+    }
+};
 
 // Dim of column n (0 .. 7) of value tile i of a block: the four numbers of bytes 2n, 2n + 1.
 __device__ __forceinline__ int value_dim(int i, int n) { return 16 * (i & 1) + 2 * n + (i >> 1); }
 
-// One head of a chain of parts, added up in order by a warp (lane: the dims lane, lane + 32, ..): its result, or, keep not null, the part
-// that all of them are.  `next` gives the parts one after the other, NULL behind the last, and starts anew when called with true.
-template <class T, int NB, class Next>
-__device__ __forceinline__ void join_head(const Q4Args& a, int row, int hg, int g, Next&& next, float* keep) {
+// One head of a chain of n parts, added up in order by a warp: its result, or, keep not null, the part that all of them are.  The maxima
+// and sums are read by a lane per part, the weighted values eight parts at a time: a chain of dependent loads per part took 0.6 us each.
+template <class T, int NB, class Part>
+__device__ __forceinline__ void join_head(const Q4Args& a, int row, int hg, int g, int n, Part&& part, float* keep) {
     using C = Q4Cfg<NB>;
     const int lane = threadIdx.x & 31, head = hg / a.sub * a.group + hg % a.sub * A4_HEADS + g;
     float m = __int_as_float(0xFF800000);
-    for (const float* p = next(true); p; p = next(false)) m = fmaxf(m, p[A4_HEADS * C::HD + g]);
-    float l = 0.0f, o[NB] = {};
-    for (const float* p = next(true); p; p = next(false)) {
-        const float mi = p[A4_HEADS * C::HD + g], f = mi == m ? 1.0f : exp2_approx(mi - m);
-        l = fmaf(p[A4_HEADS * C::HD + A4_HEADS + g], f, l);
+    for (int k = lane; k < n; k += 32) m = fmaxf(m, part(k)[A4_HEADS * C::HD + g]);
 #pragma unroll
-        for (int b = 0; b < NB; b++) o[b] = fmaf(p[g * C::HD + 32 * b + lane], f, o[b]);
+    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+    float l = 0.0f, o[NB] = {};
+    for (int k0 = 0; k0 < n; k0 += 32) {
+        float f = 0.0f;
+        if (k0 + lane < n) {
+            const float* p = part(k0 + lane);
+            const float mi = p[A4_HEADS * C::HD + g];
+            f = mi == m ? 1.0f : exp2_approx(mi - m);
+            l = fmaf(p[A4_HEADS * C::HD + A4_HEADS + g], f, l);
+        }
+        for (int k = k0; k < min(n, k0 + 32); k += 8) {
+            float x[8][NB];
+#pragma unroll
+            for (int u = 0; u < 8; u++) {
+                const float* p = part(min(k + u, n - 1)) + g * C::HD + lane;
+#pragma unroll
+                for (int b = 0; b < NB; b++) x[u][b] = p[32 * b];
+            }
+#pragma unroll
+            for (int u = 0; u < 8; u++) {
+                const float w = __shfl_sync(0xffffffffu, f, (k - k0 + u) & 31);
+                if (k + u < n) {
+#pragma unroll
+                    for (int b = 0; b < NB; b++) o[b] = fmaf(x[u][b], w, o[b]);
+                }
+            }
+        }
     }
+#pragma unroll
+    for (int x = 16; x > 0; x >>= 1) l += __shfl_xor_sync(0xffffffffu, l, x);
     if (keep) {
 #pragma unroll
         for (int b = 0; b < NB; b++) keep[g * C::HD + 32 * b + lane] = o[b];
@@ -222,15 +277,13 @@ __global__ void __launch_bounds__(Q4Cfg<NB>::THREADS, 1) k_attention_q4(const __
     total *= (unsigned)a.n_hg;
     const unsigned long long ctas = total < gridDim.x ? total : gridDim.x;  // (a short list: one tile to a CTA)
     unsigned long long p0 = 0, p1 = 0;
+    int working = 0;
     if (blockIdx.x < ctas) {
         const unsigned long long c0 = total * blockIdx.x / ctas, c1 = total * (blockIdx.x + 1) / ctas;
-        p0 = c0 + (c1 - c0) * warp / C::WARPS, p1 = c0 + (c1 - c0) * (warp + 1) / C::WARPS;
+        const unsigned long long share = c1 - c0 < C::WARPS ? c1 - c0 : C::WARPS;  // (the first warps, where there are fewer tiles)
+        working = (int)share;
+        if (warp < working) p0 = c0 + (c1 - c0) * warp / share, p1 = c0 + (c1 - c0) * (warp + 1) / share;
     }
-    // rows without a tile: zeros where the row is one of the cache (or zero_rest asks for it)
-    for (int j = blockIdx.x; j < a.n; j += gridDim.x)
-        if (row_tiles(a, j) == 0 && (a.zero_rest || (a.slots[j] >= 0 && a.slots[j] < a.c.n_slots)))
-            for (int i = tid; i < a.n_heads * C::HD; i += C::THREADS) static_cast<T*>(a.out)[(size_t)j * a.n_heads * C::HD + i] = from_f32<T>(0.0f);
-
     float* parts = reinterpret_cast<float*>(sm + (size_t)C::WARPS * C::STAGES * C::STAGE);  // [warps][2][PART]
     bool ok = true;
     if (p0 < p1) {
@@ -256,21 +309,24 @@ __global__ void __launch_bounds__(Q4Cfg<NB>::THREADS, 1) k_attention_q4(const __
         }
         const unsigned n_mine = (unsigned)(p1 - p0);
         uint8_t* ring = sm + (size_t)warp * C::STAGES * C::STAGE;
-        Cursor ahead = cur;
+        const uint32_t ring_at = s_u32(ring), bars_at = s_u32(bars[warp]);
+        Stream<NB> ahead;
+        ahead.at = cur;
+        ahead.place(a);
         unsigned fetched = 0;
         for (; fetched < C::STAGES && fetched < n_mine; fetched++) {
-            if (fetched) advance(a, ahead);
-            if (lane == 0) fetch<NB>(a, ahead, s_u32(ring + fetched * C::STAGE), s_u32(&bars[warp][fetched]));
+            if (fetched) ahead.step(a);
+            if (lane == 0) ahead.fetch(ring_at + fetched * C::STAGE, bars_at + fetched * 8);
         }
         uint32_t qa[NB][2][4];  // q of heads g (rows g: high, g + 8: low parts)
         float q_inv = 0.0f, m = 0.0f, l = 0.0f, o[NB][4][2];
-        int vexp = -100;        // weights are scaled by 2^(12 - vexp)
+        int vexp = A4_MIN_EXP;   // l and o are scaled by 2^(12 - vexp)
         bool begins = false, fresh = true;
         for (unsigned i = 0; i < n_mine; i++) {
             if (fresh) {  // another row or head group
                 fresh = false;
                 begins = cur.t == 0;
-                m = __int_as_float(0xFF800000), l = 0.0f, vexp = -100;
+                m = __int_as_float(0xFF800000), l = 0.0f, vexp = A4_MIN_EXP;
 #pragma unroll
                 for (int b = 0; b < NB; b++)
 #pragma unroll
@@ -305,7 +361,7 @@ __global__ void __launch_bounds__(Q4Cfg<NB>::THREADS, 1) k_attention_q4(const __
                         }
             }
             const unsigned st = i % C::STAGES;
-            if (ok) ok = __all_sync(0xffffffffu, bar_wait(s_u32(&bars[warp][st]), (i / C::STAGES) & 1));
+            ok = ok && bar_wait(bars_at + st * 8, (i / C::STAGES) & 1);
             const uint8_t* stage = ring + st * C::STAGE;
             const uint32_t* kw = reinterpret_cast<const uint32_t*>(stage);
             const uint32_t* vw = reinterpret_cast<const uint32_t*>(stage + C::QUANTS);
@@ -322,17 +378,16 @@ __global__ void __launch_bounds__(Q4Cfg<NB>::THREADS, 1) k_attention_q4(const __
                     float d0[NB], d1[NB];
                     load_scales<NB>(kd + col * NB, d0);
                     load_scales<NB>(kd + (col + 4) * NB, d1);
-                    float s0 = 0.0f, s1 = 0.0f;
+                    f32x2 sum = pack2(0.0f, 0.0f);
 #pragma unroll
                     for (int b = 0; b < NB; b++) {
-                        const uint32_t w = kw[key * 4 * NB + 4 * b + t4];
-                        float c[4] = {0.f, 0.f, 0.f, 0.f};
-                        mma16816(c, qa[b][0], low_pair(w), high_pair(w));
-                        mma16816(c, qa[b][1], low_pair(w >> 8), high_pair(w >> 8));
-                        s0 = fmaf(__fadd_rn(c[0], c[2]), d0[b], s0);
-                        s1 = fmaf(__fadd_rn(c[1], c[3]), d1[b], s1);
+                        const uint32_t w = kw[key * 4 * NB + 4 * b + t4], w8 = w >> 8;
+                        float c[4];
+                        mma16816_zero(c, qa[b][0], low_pair(w), high_pair(w));
+                        mma16816(c, qa[b][1], low_pair(w8), high_pair(w8));
+                        sum = fma2(add2(pack2(c[0], c[1]), pack2(c[2], c[3])), pack2(d0[b], d1[b]), sum);
                     }
-                    s[b16][e][0] = __fmul_rn(s0, q_inv), s[b16][e][1] = __fmul_rn(s1, q_inv);
+                    unpack2(sum, s[b16][e][0], s[b16][e][1]);
                 }
             float dv[4][2][2][NB], vtop = 0.0f;
 #pragma unroll
@@ -340,75 +395,91 @@ __global__ void __launch_bounds__(Q4Cfg<NB>::THREADS, 1) k_attention_q4(const __
 #pragma unroll
                 for (int e = 0; e < 2; e++)
 #pragma unroll
-                    for (int f = 0; f < 2; f++) {
-                        const int key = 16 * b16 + t4 + 8 * e + 4 * f;
-                        load_scales<NB>(vd + key * NB, dv[b16][e][f]);
-                        if (key >= seen) {
-                            s[b16][e][f] = __int_as_float(0xFF800000);
+                    for (int f = 0; f < 2; f++) load_scales<NB>(vd + (16 * b16 + t4 + 8 * e + 4 * f) * NB, dv[b16][e][f]);
+            if (seen < A4_TILE) {  // the row's last tile
 #pragma unroll
-                            for (int b = 0; b < NB; b++) dv[b16][e][f][b] = 0.0f;
-                        }
+                for (int b16 = 0; b16 < 4; b16++)
 #pragma unroll
-                        for (int b = 0; b < NB; b++) vtop = fmaxf(vtop, fabsf(dv[b16][e][f][b]));
-                    }
-            float top = m;
+                    for (int e = 0; e < 2; e++)
 #pragma unroll
-            for (int b16 = 0; b16 < 4; b16++) top = fmaxf(top, fmaxf(fmaxf(s[b16][0][0], s[b16][0][1]), fmaxf(s[b16][1][0], s[b16][1][1])));
+                        for (int f = 0; f < 2; f++)
+                            if (16 * b16 + t4 + 8 * e + 4 * f >= seen) {
+                                s[b16][e][f] = __int_as_float(0xFF800000);
+#pragma unroll
+                                for (int b = 0; b < NB; b++) dv[b16][e][f][b] = 0.0f;
+                            }
+            }
+            float top = s[0][0][0];
+#pragma unroll
+            for (int b16 = 0; b16 < 4; b16++)
+#pragma unroll
+                for (int e = 0; e < 2; e++) {
+                    top = fmaxf(top, fmaxf(s[b16][e][0], s[b16][e][1]));
+#pragma unroll
+                    for (int b = 0; b < NB; b++) vtop = fmaxf(vtop, fmaxf(fabsf(dv[b16][e][0][b]), fabsf(dv[b16][e][1][b])));
+                }
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
             vtop = fmaxf(vtop, __shfl_xor_sync(0xffffffffu, vtop, 1));
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
             vtop = fmaxf(vtop, __shfl_xor_sync(0xffffffffu, vtop, 2));
+            top = fmaxf(m, __fmul_rn(top, q_inv));
             const int old = vexp;
-            vexp = max(vexp, (int)((__float_as_uint(vtop) >> 23) & 255u) - 127);  // (f16 scales: at most 15, NaN and infinity 128)
-            vexp = min(vexp, 100);
-            const float alpha = m == top ? 1.0f : exp2_approx(m - top), keep = __fmul_rn(alpha, pow2(max(old - vexp, -126)));
+            vexp = max(vexp, min((int)((__float_as_uint(vtop) >> 23) & 255u) - 127, 16));  // (not finite: 16)
+            const float keep = __fmul_rn(m == top ? 1.0f : exp2_approx(m - top), pow2(old - vexp));
             m = top;
-            const float base = m == __int_as_float(0xFF800000) ? 0.0f : m, up = pow2(12 - vexp);
-            float sum = 0.0f;
+            const float base = (m == __int_as_float(0xFF800000) ? 0.0f : -m) + (float)(12 - vexp);
+            const f32x2 q_inv2 = pack2(q_inv, q_inv), base2 = pack2(base, base);
+            f32x2 p2[4][2], sum = pack2(0.0f, 0.0f);  // weights of the keys t4, t4 + 4 of (b16, e)
 #pragma unroll
             for (int b16 = 0; b16 < 4; b16++)
 #pragma unroll
-                for (int e = 0; e < 2; e++)
-#pragma unroll
-                    for (int f = 0; f < 2; f++) {
-                        const float p = exp2_approx(__fsub_rn(s[b16][e][f], base));
-                        sum += p;
-                        s[b16][e][f] = __fmul_rn(p, up);
-                    }
-            l = fmaf(l, alpha, sum);
+                for (int e = 0; e < 2; e++) {
+                    float x0, x1;
+                    unpack2(fma2(pack2(s[b16][e][0], s[b16][e][1]), q_inv2, base2), x0, x1);
+                    p2[b16][e] = pack2(exp2_approx(x0), exp2_approx(x1));
+                    sum = add2(sum, p2[b16][e]);
+                }
+            {
+                float s0, s1;
+                unpack2(sum, s0, s1);
+                l = fmaf(l, keep, __fadd_rn(s0, s1));
+            }
+            const f32x2 keep2 = pack2(keep, keep), minus = pack2(-1.0f, -1.0f);
             const uint32_t half_sel = (g & 1) ? 0x7632u : 0x5410u;
 #pragma unroll
             for (int b = 0; b < NB; b++) {
                 float acc[4][4];
 #pragma unroll
-                for (int c = 0; c < 4; c++) acc[c][0] = acc[c][1] = acc[c][2] = acc[c][3] = 0.0f;
-#pragma unroll
                 for (int b16 = 0; b16 < 4; b16++) {
                     uint32_t pa[4], r[2];
 #pragma unroll
                     for (int e = 0; e < 2; e++) {
-                        const float x0 = __fmul_rn(s[b16][e][0], dv[b16][e][0][b]), x1 = __fmul_rn(s[b16][e][1], dv[b16][e][1][b]);
+                        const f32x2 x = mul2(p2[b16][e], pack2(dv[b16][e][0][b], dv[b16][e][1][b]));
+                        float x0, x1, l0, l1;
+                        unpack2(x, x0, x1);
                         const float h0 = high_part(x0), h1 = high_part(x1);
+                        unpack2(fma2(pack2(h0, h1), minus, x), l0, l1);
                         pa[2 * e] = pack_f16(h0, h1);
-                        pa[2 * e + 1] = pack_f16(__fsub_rn(x0, h0), __fsub_rn(x1, h1));
+                        pa[2 * e + 1] = pack_f16(l0, l1);
                         const int key = 16 * b16 + t4 + 8 * e;
                         r[e] = __byte_perm(vw[key * 4 * NB + 4 * b + (g >> 1)], vw[(key + 4) * 4 * NB + 4 * b + (g >> 1)], half_sel);
                     }
-                    mma16816(acc[0], pa, low_pair(r[0]), low_pair(r[1]));
-                    mma16816(acc[1], pa, high_pair(r[0]), high_pair(r[1]));
-                    mma16816(acc[2], pa, low_pair(r[0] >> 8), low_pair(r[1] >> 8));
-                    mma16816(acc[3], pa, high_pair(r[0] >> 8), high_pair(r[1] >> 8));
+                    const uint32_t v0[4] = {low_pair(r[0]), high_pair(r[0]), low_pair(r[0] >> 8), high_pair(r[0] >> 8)};
+                    const uint32_t v1[4] = {low_pair(r[1]), high_pair(r[1]), low_pair(r[1] >> 8), high_pair(r[1] >> 8)};
+#pragma unroll
+                    for (int c = 0; c < 4; c++) {
+                        if (b16 == 0) mma16816_zero(acc[c], pa, v0[c], v1[c]);
+                        else mma16816(acc[c], pa, v0[c], v1[c]);
+                    }
                 }
 #pragma unroll
-                for (int c = 0; c < 4; c++) {
-                    o[b][c][0] = fmaf(o[b][c][0], keep, __fadd_rn(acc[c][0], acc[c][2]));
-                    o[b][c][1] = fmaf(o[b][c][1], keep, __fadd_rn(acc[c][1], acc[c][3]));
-                }
+                for (int c = 0; c < 4; c++)
+                    unpack2(fma2(pack2(o[b][c][0], o[b][c][1]), keep2, add2(pack2(acc[c][0], acc[c][1]), pack2(acc[c][2], acc[c][3]))), o[b][c][0], o[b][c][1]);
             }
             __syncwarp();  // every lane has read the stage
             if (fetched < n_mine) {
-                advance(a, ahead);
-                if (lane == 0 && ok) fetch<NB>(a, ahead, s_u32(ring + st * C::STAGE), s_u32(&bars[warp][st]));
+                ahead.step(a);
+                if (lane == 0 && ok) ahead.fetch(ring_at + st * C::STAGE, bars_at + st * 8);
                 fetched++;
             }
             const bool ends = cur.t + 1 == cur.tiles;
@@ -420,7 +491,7 @@ __global__ void __launch_bounds__(Q4Cfg<NB>::THREADS, 1) k_attention_q4(const __
                 const int h0 = cur.hg % a.sub * A4_HEADS;
                 if (begins && ends) {
                     if (h0 + g < a.group) {
-                        const float inv = __fdiv_rn(down, l);
+                        const float inv = __fdiv_rn(1.0f, l);
                         T* out = static_cast<T*>(a.out) + ((size_t)cur.j * a.n_heads + (cur.hg / a.sub) * a.group + h0 + g) * C::HD;
 #pragma unroll
                         for (int b = 0; b < NB; b++)
@@ -438,7 +509,7 @@ __global__ void __launch_bounds__(Q4Cfg<NB>::THREADS, 1) k_attention_q4(const __
                         for (int c = 0; c < 4; c++)
 #pragma unroll
                             for (int x = 0; x < 2; x++) part[g * C::HD + 32 * b + value_dim(c, 2 * t4 + x)] = __fmul_rn(o[b][c][x], down);
-                    if (t4 == 0) part[A4_HEADS * C::HD + g] = m, part[A4_HEADS * C::HD + A4_HEADS + g] = l;
+                    if (t4 == 0) part[A4_HEADS * C::HD + g] = m, part[A4_HEADS * C::HD + A4_HEADS + g] = __fmul_rn(l, down);
                     if (lane == 0) desc[warp][place] = make_int4(cur.j, cur.hg, (begins ? 1 : 0) | (ends ? 2 : 0), 1);
                 }
                 fresh = true;
@@ -446,42 +517,35 @@ __global__ void __launch_bounds__(Q4Cfg<NB>::THREADS, 1) k_attention_q4(const __
             if (i + 1 < n_mine) advance(a, cur);
         }
     }
+    // rows without a tile: zeros where the row is one of the cache (or zero_rest asks for it)
+    for (int j = blockIdx.x; j < a.n; j += gridDim.x)
+        if (row_tiles(a, j) == 0 && (a.zero_rest || (a.slots[j] >= 0 && a.slots[j] < a.c.n_slots)))
+            for (int i = tid; i < a.n_heads * C::HD; i += C::THREADS) static_cast<T*>(a.out)[(size_t)j * a.n_heads * C::HD + i] = from_f32<T>(0.0f);
     if (tid < 2) a.descs[(size_t)blockIdx.x * 2 + tid] = make_int4(0, 0, 0, 0);
     if (!ok)
         for (int i = 0; i < 64; i++) __nanosleep(1000);  // copies may still be landing
     __syncthreads();
 
     // ── parts within the CTA.  A chain starts with the part that begins in a warp (place 1) or with the first part of all, if that began
-    //    before the CTA, and goes on with the parts that began before (place 0) of the warps behind. ──
-    for (int item = warp; item < (C::WARPS + 1) * A4_HEADS; item += C::WARPS) {
-        const int g8 = item % A4_HEADS, place = item / A4_HEADS < C::WARPS ? 1 : 0;
-        int first = item / A4_HEADS;
-        if (place == 0) {
-            first = 0;
-            while (first < C::WARPS && !desc[first][0].w && !desc[first][1].w) first++;
-        }
-        if (first == C::WARPS || !desc[first][place].w) continue;
+    //    before the CTA, and goes on with the parts that began before (place 0) of the warps behind, up to the one that holds the end. ──
+    const bool has0 = lane < C::WARPS && desc[lane < C::WARPS ? lane : 0][0].w, has1 = lane < C::WARPS && desc[lane < C::WARPS ? lane : 0][1].w;
+    const uint32_t valid0 = __ballot_sync(0xffffffffu, has0), valid1 = __ballot_sync(0xffffffffu, has1);
+    const uint32_t end0 = __ballot_sync(0xffffffffu, has0 && (desc[lane < C::WARPS ? lane : 0][0].z & 2));
+    const int opening = valid0 ? __ffs(valid0) - 1 : C::WARPS;  // the warp whose part began before the CTA
+    const bool opens = valid0 && !(valid1 & ((1u << opening) - 1));
+    const int chains = __popc(valid1) + (opens ? 1 : 0);
+    for (int item = warp; item < chains * A4_HEADS; item += C::WARPS) {
+        const int g8 = item % A4_HEADS, c = item / A4_HEADS - (opens ? 1 : 0), place = c < 0 ? 0 : 1;
+        const int first = c < 0 ? opening : __fns(valid1, 0, c + 1);
         const int4 d = desc[first][place];
         if (d.y % a.sub * A4_HEADS + g8 >= a.group) continue;
-        uint32_t chain = 0;  // the warps behind
-        int flags = d.z;
-        for (int w = first + 1; w < C::WARPS && !(flags & 2); w++)
-            if (desc[w][0].w) chain |= 1u << w, flags |= desc[w][0].z;
-        uint32_t left = 0;
-        auto next = [&](bool anew) -> const float* {
-            if (anew) {
-                left = chain;
-                return parts + (first * 2 + place) * C::PART;
-            }
-            if (!left) return nullptr;
-            const int w = __ffs(left) - 1;
-            left &= left - 1;
-            return parts + w * 2 * C::PART;
-        };
-        const bool whole = flags == 3;
+        const uint32_t ends = place == 0 ? end0 >> first << first : first == 31 ? 0 : end0 >> (first + 1) << (first + 1);
+        const int last = ends ? __ffs(ends) - 1 : working - 1;
+        const int flags = (place ? 1 : 0) | (ends ? 2 : 0);
         const size_t to = (size_t)blockIdx.x * 2 + place;
-        join_head<T, NB>(a, d.x, d.y, g8, next, whole ? nullptr : a.parts + to * C::PART);
-        if (!whole && g8 == 0 && lane == 0) a.descs[to] = make_int4(d.x, d.y, flags, 1);
+        join_head<T, NB>(a, d.x, d.y, g8, last - first + 1, [&](int k) { return parts + ((first + k) * 2 + (k == 0 ? place : 0)) * C::PART; },
+                         flags == 3 ? nullptr : a.parts + to * C::PART);
+        if (flags != 3 && g8 == 0 && lane == 0) a.descs[to] = make_int4(d.x, d.y, flags, 1);
     }
 }
 
@@ -504,19 +568,12 @@ __global__ void __launch_bounds__(32 * A4_HEADS) k_attention_q4_join(const __gri
         }
         if (b + 32 >= (int)gridDim.x) return;  // (cannot be)
     }
-    int at = 0;
-    auto next = [&](bool anew) -> const float* {
-        if (anew) {
-            at = blockIdx.x;
-            return a.parts + ((size_t)at * 2 + 1) * C::PART;
-        }
-        return ++at <= last ? a.parts + (size_t)at * 2 * C::PART : nullptr;
-    };
-    join_head<T, NB>(a, d.x, d.y, g, next, nullptr);
+    const float* first = a.parts + ((size_t)blockIdx.x * 2 + 1) * C::PART;
+    join_head<T, NB>(a, d.x, d.y, g, last - (int)blockIdx.x + 1, [&](int k) { return first + (k == 0 ? 0 : (k * 2 - 1) * C::PART); }, nullptr);
 }
 
 constexpr int A4_MAX_CTAS = 256;
-size_t part_bytes(const KvQ4& c) { return (size_t)A4_MAX_CTAS * 2 * (A4_HEADS * c.head_dim + 2 * A4_HEADS) * sizeof(float); }
+size_t part_bytes(int head_dim) { return (size_t)A4_MAX_CTAS * 2 * (A4_HEADS * head_dim + 2 * A4_HEADS) * sizeof(float); }
 
 template <class T, int NB>
 cudaError_t launch_typed(cudaStream_t st, Q4Args& a) {
@@ -544,7 +601,7 @@ cudaError_t launch_head(cudaStream_t st, Q4Args& a) {
 
 }  // namespace
 
-size_t attention_q4_workspace(const KvQ4& c) { return part_bytes(c) + A4_MAX_CTAS * 2 * sizeof(int4); }
+size_t attention_q4_workspace(int head_dim) { return part_bytes(head_dim) + A4_MAX_CTAS * 2 * sizeof(int4); }
 
 cudaError_t launch_attention_q4(cudaStream_t st, const KvQ4& c, const void* q, size_t q_stride, int dtype, int n, int n_heads, const int32_t* slots,
                                 const int32_t* lengths, void* out, int zero_rest, void* workspace) {
@@ -557,7 +614,7 @@ cudaError_t launch_attention_q4(cudaStream_t st, const KvQ4& c, const void* q, s
     a.zero_rest = zero_rest;
     a.scale_log2 = 1.4426950408889634f / sqrtf((float)c.head_dim);
     a.parts = static_cast<float*>(workspace);
-    a.descs = reinterpret_cast<int4*>(static_cast<uint8_t*>(workspace) + part_bytes(c));
+    a.descs = reinterpret_cast<int4*>(static_cast<uint8_t*>(workspace) + part_bytes(c.head_dim));
     return dtype == DT_F32 ? launch_head<float>(st, a) : dtype == DT_F16 ? launch_head<__half>(st, a) : launch_head<__nv_bfloat16>(st, a);
 }
 

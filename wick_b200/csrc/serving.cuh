@@ -24,7 +24,7 @@ constexpr int KV_Q4_MAX_HEAD = 128;
 cudaError_t launch_kv_append_q4(cudaStream_t st, const KvQ4& c, const void* k, size_t k_stride, const void* v, size_t v_stride, int dtype, int n,
                                 const int32_t* slots, const int32_t* positions);
 cudaError_t launch_kv_read_q4(cudaStream_t st, const KvQ4& c, int n, const int32_t* slots, const int32_t* positions, float* k, float* v);
-size_t attention_q4_workspace(const KvQ4& c);
+size_t attention_q4_workspace(int head_dim);
 cudaError_t launch_attention_q4(cudaStream_t st, const KvQ4& c, const void* q, size_t q_stride, int dtype, int n, int n_heads, const int32_t* slots,
                                 const int32_t* lengths, void* out, int zero_rest, void* workspace);
 

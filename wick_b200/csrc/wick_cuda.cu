@@ -2540,11 +2540,10 @@ static int32_t check_attention_q4(const wick_cuda_kv_q4* cache, uint32_t n, uint
     return WICK_CUDA_OK;
 }
 
-int32_t wick_cuda_attention_q4_workspace(const wick_cuda_kv_q4* cache, uint32_t n, uint32_t n_heads, uint64_t* bytes) {
-    KvQ4 c;
+int32_t wick_cuda_attention_q4_workspace(uint32_t head_dim, uint64_t* bytes) {
     if (!bytes) return fail(WICK_CUDA_ERR_BAD_ARG, "NULL argument");
-    W_TRY(check_attention_q4(cache, n, n_heads, &c));
-    *bytes = attention_q4_workspace(c);
+    if (!head_dim || head_dim % QK || head_dim > KV_Q4_MAX_HEAD) return fail(WICK_CUDA_ERR_BAD_ARG, "4-bit cache: head_dim must be a multiple of 32 and at most 128");
+    *bytes = attention_q4_workspace((int)head_dim);
     return WICK_CUDA_OK;
 }
 
@@ -2558,7 +2557,7 @@ int32_t wick_cuda_attention_q4(const wick_cuda_kv_q4* cache, const void* q_dev, 
     if (!q_dev || !slots_dev || !lengths_dev || !out_dev) return fail(WICK_CUDA_ERR_BAD_ARG, "NULL argument");
     if (q_stride < (uint64_t)n_heads * c.head_dim) return fail(WICK_CUDA_ERR_BAD_ARG, "attention_q4: rows of q overlap");
     if (misaligned(q_dev, dtype_bytes(dtype)) || misaligned(out_dev, dtype_bytes(dtype))) return fail(WICK_CUDA_ERR_BAD_ARG, "attention_q4: misaligned rows");
-    const uint64_t need = attention_q4_workspace(c);
+    const uint64_t need = attention_q4_workspace(c.head_dim);
     if (workspace_bytes < need || (need && (!workspace_dev || misaligned(workspace_dev, 16))))
         return fail(WICK_CUDA_ERR_BAD_ARG, "attention_q4: workspace missing, misaligned or too small");
     CU_TRY(launch_attention_q4((cudaStream_t)stream, c, q_dev, q_stride, dtype, (int)n, (int)n_heads, slots_dev, lengths_dev, out_dev, zero_rest, workspace_dev));

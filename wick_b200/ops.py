@@ -7,6 +7,7 @@ in for (wick/src/backend/simd.rs, cpu.rs).
 from __future__ import annotations
 
 import ctypes as C
+import functools
 from typing import Tuple
 
 import numpy as np
@@ -200,69 +201,82 @@ def argmax_noalloc(logits: torch.Tensor, out: torch.Tensor) -> torch.Tensor:
 
 # ── operators of a serving step beside the model's own path ────────────────────────────────────────
 # f32, f16 and bf16; rows may be strided views (the last dimension dense).  Misuse raises WickCudaError (BAD_ARG or
-# UNSUPPORTED_DTYPE).  They launch on the current stream of their tensors' device.
+# UNSUPPORTED_DTYPE).  They launch on the current stream of their tensors' device.  A decode step calls them between kernels of a
+# few microseconds: checks compare plain numbers, and devices go by index.
 DTYPE_ID = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 30}
 
 
-def _need(ok: bool, message: str) -> None:
-    if not ok:
-        raise _lib.WickCudaError(_lib.ERR_BAD_ARG, message)
+def _bad(message: str):
+    raise _lib.WickCudaError(_lib.ERR_BAD_ARG, message)
 
 
 def _dtype_id(t: torch.Tensor) -> int:
-    if t.dtype not in DTYPE_ID:
+    i = DTYPE_ID.get(t.dtype)
+    if i is None:
         raise _lib.WickCudaError(_lib.ERR_UNSUPPORTED_DTYPE, f"{t.dtype}: f32, f16 or bf16 is needed")
-    return DTYPE_ID[t.dtype]
+    return i
 
 
-def _rows(t: torch.Tensor, name: str, device: torch.device) -> torch.Tensor:
-    """t as rows with a dense last dimension that do not overlap."""
-    _need(t.is_cuda and t.device == device, f"{name} must be on {device}")
-    _need(t.dim() == 2, f"{name} must have two dimensions")
-    if (t.shape[1] > 1 and t.stride(1) != 1) or (t.shape[0] > 1 and t.stride(0) < t.shape[1]):
-        return t.contiguous()
-    return t
+def _rows(t: torch.Tensor, name: str, dev: int) -> Tuple[torch.Tensor, int, int, int]:
+    """(t with a dense last dimension and rows that do not overlap, rows, columns, elements from row to row)."""
+    if dev < 0 or t.get_device() != dev:
+        _bad(f"{name} must be on the same GPU as the other tensors")
+    if t.dim() != 2:
+        _bad(f"{name} must have two dimensions")
+    n, m = t.shape
+    stride, dense = t.stride()
+    if (m > 1 and dense != 1) or (n > 1 and stride < m):
+        t, stride = t.contiguous(), m
+    return t, n, m, stride if n > 1 else m  # (torch keeps any stride for a single row)
 
 
-def _stride(t: torch.Tensor) -> int:
-    """Elements from row to row; torch keeps any number there for a single row."""
-    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
-
-
-def _ids(t: torch.Tensor, n: int, name: str, device: torch.device) -> torch.Tensor:
-    _need(t.dtype == torch.int32 and t.device == device, f"{name} must be int32 on {device}")
-    _need(t.dim() == 1 and t.shape[0] == n, f"{name} must hold {n} numbers")
+def _ids(t: torch.Tensor, n: int, name: str, dev: int) -> torch.Tensor:
+    if t.dtype is not torch.int32 or t.get_device() != dev or t.dim() != 1 or t.shape[0] != n:
+        _bad(f"{name} must hold {n} int32 numbers on the tensors' GPU")
     return t if t.is_contiguous() else t.contiguous()
 
 
-def _call(name: str, device: torch.device, *args) -> None:
-    """The library's function `name` on the current stream of `device`."""
-    fn = getattr(_lib.load(), name)
-    stream = torch.cuda.current_stream(device).cuda_stream
-    if device.index == torch.cuda.current_device():
-        check(fn(*args, stream))
+def _out(out: torch.Tensor, like: torch.Tensor, shape: tuple, dev: int) -> None:
+    if out.shape != shape or out.dtype is not like.dtype or out.get_device() != dev or not out.is_contiguous() or out.data_ptr() % 16:
+        _bad("out must be dense, of q's shape and type and start on a 16-byte boundary")
+
+
+def _call(fn, dev: int, *args) -> None:
+    """A function of the library on the current stream of device `dev`."""
+    if dev == torch.cuda.current_device():
+        code = fn(*args, torch.cuda.current_stream(dev).cuda_stream)
     else:
-        with torch.cuda.device(device):
-            check(fn(*args, stream))
+        with torch.cuda.device(dev):
+            code = fn(*args, torch.cuda.current_stream(dev).cuda_stream)
+    if code:
+        check(code)
+
+
+@functools.lru_cache(maxsize=1024)
+def _workspace(name: str, *sizes) -> int:
+    """What a workspace function of the library says for these sizes."""
+    size = C.c_uint64(0)
+    check(getattr(_lib.load(), name)(*sizes, C.byref(size)))
+    return size.value
 
 
 def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top_n: int = 0):
     """Log probability of tokens[j] under row j of logits [n, vocab], the rows' entropies (nats) and their top_n (at most 64)
     likeliest tokens: (logprob [n], entropy [n], top ids [n, top_n] int32, top logprobs [n, top_n]), f32.  Equal logits by
     ascending id; NaN counts as -inf; a token outside the vocabulary has -inf."""
+    dev = logits.get_device()
+    logits, n, vocab, stride = _rows(logits, "logits", dev)
+    tokens = _ids(tokens, n, "tokens", dev)
+    if not 0 <= top_n <= 64:
+        _bad("top_n must be 0 to 64")
     device = logits.device
-    logits = _rows(logits, "logits", device)
-    n, vocab = logits.shape
-    tokens = _ids(tokens, n, "tokens", device)
-    dtype = _dtype_id(logits)
-    _need(0 <= top_n <= 64, "top_n must be 0 to 64")
-    out = torch.empty((2, n), dtype=torch.float32, device=device)
+    logprob = torch.empty(n, dtype=torch.float32, device=device)
+    entropy = torch.empty(n, dtype=torch.float32, device=device)
     ids = torch.empty((n, top_n), dtype=torch.int32, device=device)
     lps = torch.empty((n, top_n), dtype=torch.float32, device=device)
-    p = out.data_ptr()
-    _call("wick_cuda_token_logprobs", device, logits.data_ptr(), dtype, _stride(logits), n, vocab, tokens.data_ptr(), top_n, p, p + 4 * n,
-          ids.data_ptr() if top_n else None, lps.data_ptr() if top_n else None)
-    return out[0], out[1], ids, lps
+    _call(_lib.load().wick_cuda_token_logprobs, dev, logits.data_ptr(), _dtype_id(logits), stride, n, vocab, tokens.data_ptr(), top_n,
+          logprob.data_ptr(), entropy.data_ptr(), ids.data_ptr(), lps.data_ptr())
+    return logprob, entropy, ids, lps
 
 
 class KvCacheQ4:
@@ -272,23 +286,22 @@ class KvCacheQ4:
     most 128."""
 
     def __init__(self, k_quants: torch.Tensor, k_scales: torch.Tensor, v_quants: torch.Tensor, v_scales: torch.Tensor):
-        planes = (k_quants, k_scales, v_quants, v_scales)
-        self.device = k_quants.device
-        for t, dtype in zip(planes, (torch.uint8, torch.float16) * 2):
-            _need(t.is_cuda and t.device == self.device and t.dtype == dtype and t.dim() == 4 and t.is_contiguous(),
-                  "planes must be dense tensors of four dimensions on one GPU, quants uint8 and scales f16")
-        slots, heads, rows, half = k_quants.shape
-        _need(v_quants.shape == k_quants.shape and half % 16 == 0 and k_scales.shape == v_scales.shape == (slots, heads, rows, half // 16),
-              "the planes' shapes do not match")
-        self.k_quants, self.k_scales, self.v_quants, self.v_scales = planes
-        self.n_slots, self.n_kv_heads, self.max_seq, self.head_dim = slots, heads, rows, half * 2
-        self._c = _lib.KvQ4(*(t.data_ptr() for t in planes), slots, heads, rows, half * 2)
+        dev = k_quants.get_device()
+        for t, dtype in ((k_quants, torch.uint8), (k_scales, torch.float16), (v_quants, torch.uint8), (v_scales, torch.float16)):
+            if dev < 0 or t.get_device() != dev or t.dtype is not dtype or t.dim() != 4 or not t.is_contiguous():
+                _bad("planes must be dense tensors of four dimensions on one GPU, quants uint8 and scales f16")
+        slots, heads, rows, half = shape = k_quants.shape
+        if v_quants.shape != shape or half % 16 or k_scales.shape != (slots, heads, rows, half // 16) or v_scales.shape != k_scales.shape:
+            _bad("the planes' shapes do not match")
+        self.k_quants, self.k_scales, self.v_quants, self.v_scales = k_quants, k_scales, v_quants, v_scales
+        self.n_slots, self.n_kv_heads, self.max_seq, self.head_dim, self.dev = slots, heads, rows, half * 2, dev
+        self._c = _lib.KvQ4(k_quants.data_ptr(), k_scales.data_ptr(), v_quants.data_ptr(), v_scales.data_ptr(), slots, heads, rows, half * 2)
 
     @classmethod
     def empty(cls, n_slots: int, max_seq: int, n_kv_heads: int, head_dim: int, device="cuda") -> "KvCacheQ4":
         """A cache of zeros for at least max_seq rows per slot."""
-        _need(n_slots > 0 and max_seq > 0 and n_kv_heads > 0 and head_dim > 0 and head_dim % 32 == 0 and head_dim <= 128,
-              "sizes must be positive, head_dim a multiple of 32 and at most 128")
+        if not (n_slots > 0 and max_seq > 0 and n_kv_heads > 0 and 0 < head_dim <= 128) or head_dim % 32:
+            _bad("sizes must be positive, head_dim a multiple of 32 and at most 128")
         rows = -(-max_seq // 64) * 64
         planes = []
         for _ in range(2):
@@ -300,22 +313,23 @@ class KvCacheQ4:
 def kv_append_q4(cache: KvCacheQ4, k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, positions: torch.Tensor) -> None:
     """Rounds the rows of k and v [n, kv_heads * head_dim] to Q4_0 and writes row j to row positions[j] of slot slots[j].  Rows whose
     slot or position the cache does not have (padding: -1) are skipped; the pairs of a call must differ."""
-    device = cache.device
-    k, v = _rows(k, "k", device), _rows(v, "v", device)
-    n, dim = k.shape
-    _need(v.shape == k.shape and v.dtype == k.dtype, "k and v must have the same shape and type")
-    _need(dim == cache.n_kv_heads * cache.head_dim, "k and v must have kv_heads * head_dim columns")
-    slots, positions = _ids(slots, n, "slots", device), _ids(positions, n, "positions", device)
-    _call("wick_cuda_kv_append_q4", device, C.byref(cache._c), k.data_ptr(), _stride(k), v.data_ptr(), _stride(v), _dtype_id(k), n,
-          slots.data_ptr(), positions.data_ptr())
+    dev = cache.dev
+    k, n, dim, k_stride = _rows(k, "k", dev)
+    v, n_v, dim_v, v_stride = _rows(v, "v", dev)
+    if n_v != n or dim_v != dim or v.dtype is not k.dtype or dim != cache.n_kv_heads * cache.head_dim:
+        _bad("k and v must have the same type and kv_heads * head_dim columns")
+    slots, positions = _ids(slots, n, "slots", dev), _ids(positions, n, "positions", dev)
+    _call(_lib.load().wick_cuda_kv_append_q4, dev, cache._c, k.data_ptr(), k_stride, v.data_ptr(), v_stride, _dtype_id(k), n, slots.data_ptr(),
+          positions.data_ptr())
 
 
 def kv_read_q4(cache: KvCacheQ4, slots: torch.Tensor, positions: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
     """The values of row positions[j] of slot slots[j]: k and v [n, kv_heads * head_dim] f32; zeros where the cache has no such row."""
-    device, n = cache.device, slots.shape[0]
-    slots, positions = _ids(slots, n, "slots", device), _ids(positions, n, "positions", device)
-    k, v = torch.empty((2, n, cache.n_kv_heads * cache.head_dim), dtype=torch.float32, device=device)
-    _call("wick_cuda_kv_read_q4", device, C.byref(cache._c), n, slots.data_ptr(), positions.data_ptr(), k.data_ptr(), v.data_ptr())
+    dev, n = cache.dev, slots.shape[0]
+    slots, positions = _ids(slots, n, "slots", dev), _ids(positions, n, "positions", dev)
+    k = torch.empty((n, cache.n_kv_heads * cache.head_dim), dtype=torch.float32, device=slots.device)
+    v = torch.empty_like(k)
+    _call(_lib.load().wick_cuda_kv_read_q4, dev, cache._c, n, slots.data_ptr(), positions.data_ptr(), k.data_ptr(), v.data_ptr())
     return k, v
 
 
@@ -323,22 +337,21 @@ def attention_q4(q: torch.Tensor, cache: KvCacheQ4, slots: torch.Tensor, lengths
                  out: torch.Tensor | None = None) -> torch.Tensor:
     """Attention of single tokens over the cache: row j of q [n, n_heads * head_dim] attends the first lengths[j] rows of slot
     slots[j]; several rows may name one slot.  Length 0 gives zeros; rows whose slot the cache does not have (padding: -1) are left as
-    they are in `out` (a new one starts with zeros)."""
-    device = cache.device
-    q = _rows(q, "q", device)
-    n, dim = q.shape
-    _need(dim == n_heads * cache.head_dim, "q must have n_heads * head_dim columns")
-    slots, lengths = _ids(slots, n, "slots", device), _ids(lengths, n, "lengths", device)
-    dtype = _dtype_id(q)
-    fresh = out is None
+    they are in `out` (a new one has zeros there)."""
+    dev = cache.dev
+    q, n, dim, stride = _rows(q, "q", dev)
+    if dim != n_heads * cache.head_dim:
+        _bad("q must have n_heads * head_dim columns")
+    slots, lengths = _ids(slots, n, "slots", dev), _ids(lengths, n, "lengths", dev)
+    dtype, fresh = _dtype_id(q), out is None
     if fresh:
-        out = torch.empty((n, dim), dtype=q.dtype, device=device)
-    _need(out.shape == q.shape and out.dtype == q.dtype and out.device == device and out.is_contiguous(), "out must be dense, of q's shape and type")
-    size = C.c_uint64(0)
-    check(_lib.load().wick_cuda_attention_q4_workspace(C.byref(cache._c), n, n_heads, C.byref(size)))
-    work = torch.empty(size.value, dtype=torch.uint8, device=device)
-    _call("wick_cuda_attention_q4", device, C.byref(cache._c), q.data_ptr(), _stride(q), dtype, n, n_heads, slots.data_ptr(), lengths.data_ptr(),
-          out.data_ptr(), fresh, work.data_ptr(), size.value)
+        out = torch.empty((n, dim), dtype=q.dtype, device=q.device)
+    else:
+        _out(out, q, (n, dim), dev)
+    size = _workspace("wick_cuda_attention_q4_workspace", cache.head_dim)
+    work = torch.empty(size, dtype=torch.uint8, device=q.device)
+    _call(_lib.load().wick_cuda_attention_q4, dev, cache._c, q.data_ptr(), stride, dtype, n, n_heads, slots.data_ptr(), lengths.data_ptr(),
+          out.data_ptr(), fresh, work.data_ptr(), size)
     return out
 
 
@@ -346,31 +359,38 @@ def attention_prompts(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, starts:
                       key_starts: torch.Tensor | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
     """Causal attention of packed prompts: sequence s has the tokens starts[s] .. starts[s + 1] of q [tokens, n_heads * head_dim] and the
     keys key_starts[s] .. key_starts[s + 1] (default: the same) of k and v [keys, n_kv_heads * head_dim]; its last key belongs to its last
-    token.  Tokens without a key get zeros; rows behind the last sequence are left as they are in `out` (a new one starts with zeros)."""
-    device = q.device
-    q, k, v = _rows(q, "q", device), _rows(k, "k", device), _rows(v, "v", device)
-    _need(q.dtype == k.dtype == v.dtype, "q, k and v must have the same type")
-    _need(n_heads > 0 and n_kv_heads > 0 and q.shape[1] == n_heads * head_dim, "q must have n_heads * head_dim columns")
-    _need(k.shape == v.shape and k.shape[1] == n_kv_heads * head_dim, "k and v must have n_kv_heads * head_dim columns")
+    token.  Tokens without a key get zeros; rows behind the last sequence are left as they are in `out` (a new one has zeros there)."""
+    dev = q.get_device()
+    q, n, dim, q_stride = _rows(q, "q", dev)
+    k, n_keys, dim_k, k_stride = _rows(k, "k", dev)
+    v, n_values, dim_v, v_stride = _rows(v, "v", dev)
+    if q.dtype is not k.dtype or q.dtype is not v.dtype:
+        _bad("q, k and v must have the same type")
+    if n_heads <= 0 or n_kv_heads <= 0 or head_dim <= 0 or dim != n_heads * head_dim or n_values != n_keys or dim_k != n_kv_heads * head_dim or dim_v != dim_k:
+        _bad("q must have n_heads * head_dim columns, k and v n_kv_heads * head_dim columns and the same rows")
     n_seqs = starts.shape[0] - 1
-    _need(n_seqs >= 0, "starts must hold at least one offset")
-    starts = _ids(starts, n_seqs + 1, "starts", device)
+    if n_seqs < 0:
+        _bad("starts must hold at least one offset")
+    starts = _ids(starts, n_seqs + 1, "starts", dev)
     if key_starts is not None:
-        key_starts = _ids(key_starts, n_seqs + 1, "key_starts", device)
-    dtype = _dtype_id(q)
+        key_starts = _ids(key_starts, n_seqs + 1, "key_starts", dev)
+    dtype, size, fresh = _dtype_id(q), q.element_size(), out is None
     # 16-byte loads: rows that start elsewhere are copied
-    q, k, v = (t if (t.data_ptr() | _stride(t) * t.element_size()) % 16 == 0 else t.clone(memory_format=torch.contiguous_format) for t in (q, k, v))
-    fresh = out is None
+    if (q.data_ptr() | q_stride * size) % 16:
+        q, q_stride = q.clone(memory_format=torch.contiguous_format), dim
+    if (k.data_ptr() | k_stride * size) % 16:
+        k, k_stride = k.clone(memory_format=torch.contiguous_format), dim_k
+    if (v.data_ptr() | v_stride * size) % 16:
+        v, v_stride = v.clone(memory_format=torch.contiguous_format), dim_k
     if fresh:
-        out = torch.empty(q.shape, dtype=q.dtype, device=device)
-    _need(out.shape == q.shape and out.dtype == q.dtype and out.device == device and out.is_contiguous() and out.data_ptr() % 16 == 0,
-          "out must be dense, of q's shape and type and start on a 16-byte boundary")
-    size = C.c_uint64(0)
-    check(_lib.load().wick_cuda_attention_prompts_workspace(dtype, n_seqs, q.shape[0], k.shape[0], n_heads, n_kv_heads, head_dim, C.byref(size)))
-    work = torch.empty(size.value, dtype=torch.uint8, device=device)
+        out = torch.empty((n, dim), dtype=q.dtype, device=q.device)
+    else:
+        _out(out, q, (n, dim), dev)
     if n_seqs == 0:
         return out.zero_() if fresh else out
-    _call("wick_cuda_attention_prompts", device, q.data_ptr(), _stride(q), k.data_ptr(), _stride(k), v.data_ptr(), _stride(v), dtype,
-          starts.data_ptr(), key_starts.data_ptr() if key_starts is not None else None, n_seqs, q.shape[0], k.shape[0], n_heads, n_kv_heads,
-          head_dim, out.data_ptr(), fresh, work.data_ptr(), size.value)
+    room = _workspace("wick_cuda_attention_prompts_workspace", dtype, n_seqs, n, n_keys, n_heads, n_kv_heads, head_dim)
+    work = torch.empty(room, dtype=torch.uint8, device=q.device) if room else None
+    _call(_lib.load().wick_cuda_attention_prompts, dev, q.data_ptr(), q_stride, k.data_ptr(), k_stride, v.data_ptr(), v_stride, dtype,
+          starts.data_ptr(), key_starts.data_ptr() if key_starts is not None else None, n_seqs, n, n_keys, n_heads, n_kv_heads, head_dim,
+          out.data_ptr(), fresh, work.data_ptr() if room else None, room)
     return out
