@@ -1,15 +1,16 @@
 // Attention of single tokens over the 4-bit cache:  o = sum_t p_t V_t / sum_t p_t,  p_t = 2^(x_t - m),
 // x_t = log2(e) / sqrt(d) q . K_t, with K_t and V_t blocks d (n - 8) of four-bit numbers n.
 //
-// Bound: HBM, 18 bytes per 32 keys' or values' elements.  f32 arithmetic on the CUDA cores could not keep up with it (4 query heads to a KV head need
-// 14 f32 operations per byte, four times what the SMs have beside unpacking), and an M = 128 tile of tcgen05 would hold 4 to 8 useful rows: the products are
-// mma.sync m16n8k16 with the numbers, exact in f16, as one operand.  The other one, q or the weights, is f32 and is held as two
-// f16 parts (22 bits): rows 0 .. 7 of a tile are the high parts of up to 8 query heads, rows 8 .. 15 their low parts, so that both
-// come out of one instruction and are added in the lane that holds them.
-//   scores:  S = sum over blocks of d_K (q . (n - 8));  a block is two products, scaled and added in f32.  (Numbers as they are stored are
-//            f16's n 2^-24, and a sum could start at -8 sum q: fewer instructions, the same time, and 1.1e-6 off instead of 2.4e-7.)
-//   values:  the weight of a key is p d_V, per block; sums over the 64 keys of a tile in the tensor core, over tiles in registers
-//            (with the running maximum's factor), since the tensor core's additions truncate.
+// Bound by HBM it would be 18 bytes per 32 elements of keys or values; it is bound by instructions, most of them the unpacking (per 8 numbers one
+// shift, four bit operations and four f16 ones), and mma.sync holds the issue port for 8 cycles.  f32 arithmetic on the CUDA cores would need 14
+// operations per byte for 4 query heads, and an M = 128 tile of tcgen05 operands in shared memory that the CUDA cores would have to write.  So the
+// products are mma.sync m16n8k16 with the numbers n - 8, exact in f16, as the 16-row operand.  The 8 columns of the other are 4 query
+// heads: q, or the weights, is f32 and is held as two f16 parts (22 bits), the high one in an even column, the low one in the odd column behind it,
+// so that the lane that gets both adds them.  (As rows of the 16-row operand, 4 heads left half of it empty: 1550 instead of 910 cycles per tile.)
+//   scores:  S^T = sum over blocks of d_K ((n - 8) . q);  a block is two products, scaled and added in f32.
+//   values:  O^T += (n - 8)^T (p d_V), per block; the weights' parts change from a lane per (key, head) to the operand's order by
+//            movmatrix.  Sums over the 64 keys of a tile in the tensor core, over tiles in registers (with the running maximum's factor), since
+//            the tensor core's additions truncate.
 // High and low parts need a common exponent: q is scaled by a power of two per head, weights by one per tile, the largest |d_V| of
 // the keys so far.
 //
@@ -129,6 +130,20 @@ __device__ __forceinline__ void load_scales(const __half* p, float (&d)[NB]) {
     }
 }
 
+// The same, kept as they are: two to a register.
+template <int NB>
+__device__ __forceinline__ void load_packed(const __half* p, uint32_t (&w)[(NB + 1) / 2]) {
+    if constexpr (NB % 2 == 0) {
+#pragma unroll
+        for (int i = 0; i < NB / 2; i++) w[i] = reinterpret_cast<const uint32_t*>(p)[i];
+    } else {
+        const uint16_t* u = reinterpret_cast<const uint16_t*>(p);
+#pragma unroll
+        for (int i = 0; i < NB; i += 2) w[i / 2] = u[i] | (i + 1 < NB ? (uint32_t)u[i + 1 < NB ? i + 1 : 0] << 16 : 0u);
+    }
+}
+__device__ __forceinline__ float half_of(uint32_t w, int i) { return __half2float(__ushort_as_half((unsigned short)(i & 1 ? w >> 16 : w & 0xFFFFu))); }
+
 struct Cursor {  // a tile of the list
     int j, hg, t, tiles, len, slot;
 };
@@ -181,8 +196,12 @@ struct Stream {
     }
 };
 
-// Dim of column n (0 .. 7) of value tile i of a block: the four numbers of bytes 2n, 2n + 1.
-__device__ __forceinline__ int value_dim(int i, int n) { return 16 * (i & 1) + 2 * n + (i >> 1); }
+// An 8 x 8 matrix of 16-bit numbers, two of a row to a lane, transposed.
+__device__ __forceinline__ uint32_t transposed(uint32_t v) {
+    uint32_t r;
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+    return r;
+}
 
 // One head of a chain of n parts, added up in order by a warp: its result, or, keep not null, the part that all of them are.  The maxima
 // and sums are read by a lane per part, the weighted values eight parts at a time: a chain of dependent loads per part took 0.6 us each.
@@ -235,7 +254,8 @@ __device__ __forceinline__ void join_head(const Q4Args& a, int row, int hg, int 
     }
 }
 
-template <class T, int NB>
+// HQ: quads of query heads (1, or 2 for groups of 5 to 8).
+template <class T, int NB, int HQ>
 __global__ void __launch_bounds__(Q4Cfg<NB>::THREADS, 1) k_attention_q4(const __grid_constant__ Q4Args a) {
     using C = Q4Cfg<NB>;
     extern __shared__ __align__(128) uint8_t sm[];
@@ -318,47 +338,49 @@ __global__ void __launch_bounds__(Q4Cfg<NB>::THREADS, 1) k_attention_q4(const __
             if (fetched) ahead.step(a);
             if (lane == 0) ahead.fetch(ring_at + fetched * C::STAGE, bars_at + fetched * 8);
         }
-        uint32_t qa[NB][2][4];  // q of heads g (rows g: high, g + 8: low parts)
-        float q_inv = 0.0f, m = 0.0f, l = 0.0f, o[NB][4][2];
+        uint32_t qb[HQ][NB][2][2];  // column g: head g / 2 of the quad, its high (g even) or low part
+        float q_inv[HQ], m[HQ], l[HQ], o[HQ][NB][2][2];  // of head t4 of the quad; o: dims 16 h + 2 g + e of a block as [h][e]
         int vexp = A4_MIN_EXP;   // l and o are scaled by 2^(12 - vexp)
         bool begins = false, fresh = true;
         for (unsigned i = 0; i < n_mine; i++) {
             if (fresh) {  // another row or head group
                 fresh = false;
                 begins = cur.t == 0;
-                m = __int_as_float(0xFF800000), l = 0.0f, vexp = A4_MIN_EXP;
-#pragma unroll
-                for (int b = 0; b < NB; b++)
-#pragma unroll
-                    for (int c = 0; c < 4; c++) o[b][c][0] = o[b][c][1] = 0.0f;
+                vexp = A4_MIN_EXP;
                 const int h0 = cur.hg % a.sub * A4_HEADS;
-                const bool real = h0 + g < a.group;
-                const T* q = static_cast<const T*>(a.q) + (size_t)cur.j * a.q_stride + (size_t)((cur.hg / a.sub) * a.group + h0 + (real ? g : 0)) * C::HD;
-                float x[NB][2][4], top = 0.0f;
 #pragma unroll
-                for (int b = 0; b < NB; b++)
+                for (int u = 0; u < HQ; u++) {
+                    m[u] = __int_as_float(0xFF800000), l[u] = 0.0f;
 #pragma unroll
-                    for (int h = 0; h < 2; h++)
+                    for (int b = 0; b < NB; b++) o[u][b][0][0] = o[u][b][0][1] = o[u][b][1][0] = o[u][b][1][1] = 0.0f;
+                    const int h = h0 + 4 * u + (g >> 1);
+                    const bool real = h < a.group;
+                    const T* q = static_cast<const T*>(a.q) + (size_t)cur.j * a.q_stride + (size_t)((cur.hg / a.sub) * a.group + (real ? h : 0)) * C::HD;
+                    float x[NB][2][4], top = 0.0f;
 #pragma unroll
-                        for (int e = 0; e < 4; e++) {
-                            x[b][h][e] = real ? __fmul_rn(to_f32(q[32 * b + 16 * h + 4 * t4 + e]), a.scale_log2) : 0.0f;
-                            top = fmaxf(top, fabsf(x[b][h][e]));
-                        }
-                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-                const int e = max(-100, min(100, (int)((__float_as_uint(top) >> 23) & 255u) - 127));
-                const float f = pow2(12 - e);
-                q_inv = pow2(e - 12);
+                    for (int b = 0; b < NB; b++)
 #pragma unroll
-                for (int b = 0; b < NB; b++)
+                        for (int k = 0; k < 2; k++)
 #pragma unroll
-                    for (int s = 0; s < 2; s++)
+                            for (int e = 0; e < 4; e++) {
+                                x[b][k][e] = real ? __fmul_rn(to_f32(q[32 * b + 16 * k + 4 * t4 + e]), a.scale_log2) : 0.0f;
+                                top = fmaxf(top, fabsf(x[b][k][e]));
+                            }
+                    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+                    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+                    const int e = max(-100, min(100, (int)((__float_as_uint(top) >> 23) & 255u) - 127));
+                    const float f = pow2(12 - e);
+                    q_inv[u] = __shfl_sync(0xffffffffu, pow2(e - 12), 8 * t4);  // (from the lanes of column 2 t4)
 #pragma unroll
-                        for (int h = 0; h < 2; h++) {
-                            const float x0 = __fmul_rn(x[b][h][s], f), x1 = __fmul_rn(x[b][h][2 + s], f), h0v = high_part(x0), h1v = high_part(x1);
-                            qa[b][s][2 * h] = pack_f16(h0v, h1v);
-                            qa[b][s][2 * h + 1] = pack_f16(__fsub_rn(x0, h0v), __fsub_rn(x1, h1v));
-                        }
+                    for (int b = 0; b < NB; b++)
+#pragma unroll
+                        for (int s = 0; s < 2; s++)
+#pragma unroll
+                            for (int k = 0; k < 2; k++) {
+                                const float x0 = __fmul_rn(x[b][k][s], f), x1 = __fmul_rn(x[b][k][2 + s], f), y0 = high_part(x0), y1 = high_part(x1);
+                                qb[u][b][s][k] = (g & 1) ? pack_f16(__fsub_rn(x0, y0), __fsub_rn(x1, y1)) : pack_f16(y0, y1);
+                            }
+                }
             }
             const unsigned st = i % C::STAGES;
             ok = ok && bar_wait(bars_at + st * 8, (i / C::STAGES) & 1);
@@ -368,113 +390,124 @@ __global__ void __launch_bounds__(Q4Cfg<NB>::THREADS, 1) k_attention_q4(const __
             const __half* kd = reinterpret_cast<const __half*>(stage + 2 * C::QUANTS);
             const __half* vd = reinterpret_cast<const __half*>(stage + 2 * C::QUANTS + C::SCALES);
             const int seen = cur.len - cur.t * A4_TILE;
-            // scores: columns 2 t4, 2 t4 + 1 of the 8-key tiles (block of 16 keys b16, e) are the keys 16 b16 + t4 + 8 e (+ 4)
-            float s[4][2][2];
+            // Row g of the 8-key half e of a block of 16 keys is its key g / 2 + 4 (g & 1) + 8 e: a lane then reads the values of rows 2 t4 and
+            // 2 t4 + 1 without bank conflicts.
+            const int key_g = (g >> 1) + 4 * (g & 1);
+            float s[HQ][4][2];
+            constexpr int NW = (NB + 1) / 2;
+            uint32_t dv[4][2][NW];
 #pragma unroll
-            for (int b16 = 0; b16 < 4; b16++)
+            for (int b16 = 0; b16 < 4; b16++) {
+                float d0[NB], d1[NB], sum[HQ][2];
+                const int key = 16 * b16 + key_g;
+                load_scales<NB>(kd + key * NB, d0);
+                load_scales<NB>(kd + (key + 8) * NB, d1);
+                load_packed<NB>(vd + key * NB, dv[b16][0]);
+                load_packed<NB>(vd + (key + 8) * NB, dv[b16][1]);
 #pragma unroll
-                for (int e = 0; e < 2; e++) {
-                    const int key = 16 * b16 + (g >> 1) + 8 * e + 4 * (g & 1), col = 16 * b16 + t4 + 8 * e;
-                    float d0[NB], d1[NB];
-                    load_scales<NB>(kd + col * NB, d0);
-                    load_scales<NB>(kd + (col + 4) * NB, d1);
-                    f32x2 sum = pack2(0.0f, 0.0f);
+                for (int u = 0; u < HQ; u++) sum[u][0] = sum[u][1] = 0.0f;
 #pragma unroll
-                    for (int b = 0; b < NB; b++) {
-                        const uint32_t w = kw[key * 4 * NB + 4 * b + t4], w8 = w >> 8;
+                for (int b = 0; b < NB; b++) {
+                    const uint32_t w0 = kw[key * 4 * NB + 4 * b + t4], w1 = kw[(key + 8) * 4 * NB + 4 * b + t4];
+                    const uint32_t k0[4] = {low_pair(w0), low_pair(w1), high_pair(w0), high_pair(w1)};
+                    const uint32_t k1[4] = {low_pair(w0 >> 8), low_pair(w1 >> 8), high_pair(w0 >> 8), high_pair(w1 >> 8)};
+#pragma unroll
+                    for (int u = 0; u < HQ; u++) {
                         float c[4];
-                        mma16816_zero(c, qa[b][0], low_pair(w), high_pair(w));
-                        mma16816(c, qa[b][1], low_pair(w8), high_pair(w8));
-                        sum = fma2(add2(pack2(c[0], c[1]), pack2(c[2], c[3])), pack2(d0[b], d1[b]), sum);
+                        mma16816_zero(c, k0, qb[u][b][0][0], qb[u][b][0][1]);
+                        mma16816(c, k1, qb[u][b][1][0], qb[u][b][1][1]);
+                        sum[u][0] = fmaf(__fadd_rn(c[0], c[1]), d0[b], sum[u][0]);
+                        sum[u][1] = fmaf(__fadd_rn(c[2], c[3]), d1[b], sum[u][1]);
                     }
-                    unpack2(sum, s[b16][e][0], s[b16][e][1]);
                 }
-            float dv[4][2][2][NB], vtop = 0.0f;
 #pragma unroll
-            for (int b16 = 0; b16 < 4; b16++)
-#pragma unroll
-                for (int e = 0; e < 2; e++)
-#pragma unroll
-                    for (int f = 0; f < 2; f++) load_scales<NB>(vd + (16 * b16 + t4 + 8 * e + 4 * f) * NB, dv[b16][e][f]);
+                for (int u = 0; u < HQ; u++) s[u][b16][0] = sum[u][0], s[u][b16][1] = sum[u][1];
+            }
             if (seen < A4_TILE) {  // the row's last tile
 #pragma unroll
                 for (int b16 = 0; b16 < 4; b16++)
 #pragma unroll
                     for (int e = 0; e < 2; e++)
+                        if (16 * b16 + 8 * e + key_g >= seen) {
 #pragma unroll
-                        for (int f = 0; f < 2; f++)
-                            if (16 * b16 + t4 + 8 * e + 4 * f >= seen) {
-                                s[b16][e][f] = __int_as_float(0xFF800000);
+                            for (int u = 0; u < HQ; u++) s[u][b16][e] = __int_as_float(0xFF800000);
 #pragma unroll
-                                for (int b = 0; b < NB; b++) dv[b16][e][f][b] = 0.0f;
-                            }
+                            for (int b = 0; b < NW; b++) dv[b16][e][b] = 0;
+                        }
             }
-            float top = s[0][0][0];
+            __half2 vmax = __float2half2_rn(0.0f);
 #pragma unroll
             for (int b16 = 0; b16 < 4; b16++)
 #pragma unroll
-                for (int e = 0; e < 2; e++) {
-                    top = fmaxf(top, fmaxf(s[b16][e][0], s[b16][e][1]));
+                for (int e = 0; e < 2; e++)
 #pragma unroll
-                    for (int b = 0; b < NB; b++) vtop = fmaxf(vtop, fmaxf(fabsf(dv[b16][e][0][b]), fabsf(dv[b16][e][1][b])));
-                }
-            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-            vtop = fmaxf(vtop, __shfl_xor_sync(0xffffffffu, vtop, 1));
-            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-            vtop = fmaxf(vtop, __shfl_xor_sync(0xffffffffu, vtop, 2));
-            top = fmaxf(m, __fmul_rn(top, q_inv));
+                    for (int b = 0; b < NW; b++) vmax = __hmax2(vmax, __habs2(*reinterpret_cast<__half2*>(&dv[b16][e][b])));
+            float vtop = fmaxf(__low2float(vmax), __high2float(vmax));
+#pragma unroll
+            for (int x = 4; x < 32; x <<= 1) vtop = fmaxf(vtop, __shfl_xor_sync(0xffffffffu, vtop, x));
             const int old = vexp;
             vexp = max(vexp, min((int)((__float_as_uint(vtop) >> 23) & 255u) - 127, 16));  // (not finite: 16)
-            const float keep = __fmul_rn(m == top ? 1.0f : exp2_approx(m - top), pow2(old - vexp));
-            m = top;
-            const float base = (m == __int_as_float(0xFF800000) ? 0.0f : -m) + (float)(12 - vexp);
-            const f32x2 q_inv2 = pack2(q_inv, q_inv), base2 = pack2(base, base);
-            f32x2 p2[4][2], sum = pack2(0.0f, 0.0f);  // weights of the keys t4, t4 + 4 of (b16, e)
+            const float moved = pow2(old - vexp);
+            float keep[HQ];
 #pragma unroll
-            for (int b16 = 0; b16 < 4; b16++)
+            for (int u = 0; u < HQ; u++) {
+                float top = fmaxf(s[u][0][0], s[u][0][1]);
 #pragma unroll
-                for (int e = 0; e < 2; e++) {
-                    float x0, x1;
-                    unpack2(fma2(pack2(s[b16][e][0], s[b16][e][1]), q_inv2, base2), x0, x1);
-                    p2[b16][e] = pack2(exp2_approx(x0), exp2_approx(x1));
-                    sum = add2(sum, p2[b16][e]);
-                }
-            {
-                float s0, s1;
-                unpack2(sum, s0, s1);
-                l = fmaf(l, keep, __fadd_rn(s0, s1));
+                for (int b16 = 1; b16 < 4; b16++) top = fmaxf(top, fmaxf(s[u][b16][0], s[u][b16][1]));
+#pragma unroll
+                for (int x = 4; x < 32; x <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
+                top = fmaxf(m[u], __fmul_rn(top, q_inv[u]));
+                keep[u] = __fmul_rn(m[u] == top ? 1.0f : exp2_approx(m[u] - top), moved);
+                m[u] = top;
+                const float base = (top == __int_as_float(0xFF800000) ? 0.0f : -top) + (float)(12 - vexp);
+                float sum = 0.0f;
+#pragma unroll
+                for (int b16 = 0; b16 < 4; b16++)
+#pragma unroll
+                    for (int e = 0; e < 2; e++) {
+                        s[u][b16][e] = exp2_approx(fmaf(s[u][b16][e], q_inv[u], base));
+                        sum = __fadd_rn(sum, s[u][b16][e]);
+                    }
+                l[u] = fmaf(l[u], keep[u], sum);
             }
-            const f32x2 keep2 = pack2(keep, keep), minus = pack2(-1.0f, -1.0f);
             const uint32_t half_sel = (g & 1) ? 0x7632u : 0x5410u;
 #pragma unroll
             for (int b = 0; b < NB; b++) {
-                float acc[4][4];
+                float acc[HQ][2][4];
 #pragma unroll
                 for (int b16 = 0; b16 < 4; b16++) {
-                    uint32_t pa[4], r[2];
+                    uint32_t r[2];
 #pragma unroll
                     for (int e = 0; e < 2; e++) {
-                        const f32x2 x = mul2(p2[b16][e], pack2(dv[b16][e][0][b], dv[b16][e][1][b]));
-                        float x0, x1, l0, l1;
-                        unpack2(x, x0, x1);
-                        const float h0 = high_part(x0), h1 = high_part(x1);
-                        unpack2(fma2(pack2(h0, h1), minus, x), l0, l1);
-                        pa[2 * e] = pack_f16(h0, h1);
-                        pa[2 * e + 1] = pack_f16(l0, l1);
-                        const int key = 16 * b16 + t4 + 8 * e;
+                        const int key = 16 * b16 + 8 * e + t4;
                         r[e] = __byte_perm(vw[key * 4 * NB + 4 * b + (g >> 1)], vw[(key + 4) * 4 * NB + 4 * b + (g >> 1)], half_sel);
                     }
-                    const uint32_t v0[4] = {low_pair(r[0]), high_pair(r[0]), low_pair(r[0] >> 8), high_pair(r[0] >> 8)};
-                    const uint32_t v1[4] = {low_pair(r[1]), high_pair(r[1]), low_pair(r[1] >> 8), high_pair(r[1] >> 8)};
+                    const uint32_t v0[4] = {low_pair(r[0]), high_pair(r[0]), low_pair(r[1]), high_pair(r[1])};                          // dims 2 g, 16 + 2 g
+                    const uint32_t v1[4] = {low_pair(r[0] >> 8), high_pair(r[0] >> 8), low_pair(r[1] >> 8), high_pair(r[1] >> 8)};  // and the next ones
 #pragma unroll
-                    for (int c = 0; c < 4; c++) {
-                        if (b16 == 0) mma16816_zero(acc[c], pa, v0[c], v1[c]);
-                        else mma16816(acc[c], pa, v0[c], v1[c]);
+                    for (int u = 0; u < HQ; u++) {
+                        uint32_t pb[2];
+#pragma unroll
+                        for (int e = 0; e < 2; e++) {
+                            const float x = __fmul_rn(s[u][b16][e], half_of(dv[b16][e][b / 2], b)), y = high_part(x);
+                            pb[e] = transposed(pack_f16(y, __fsub_rn(x, y)));
+                        }
+                        if (b16 == 0) {
+                            mma16816_zero(acc[u][0], v0, pb[0], pb[1]);
+                            mma16816_zero(acc[u][1], v1, pb[0], pb[1]);
+                        } else {
+                            mma16816(acc[u][0], v0, pb[0], pb[1]);
+                            mma16816(acc[u][1], v1, pb[0], pb[1]);
+                        }
                     }
                 }
 #pragma unroll
-                for (int c = 0; c < 4; c++)
-                    unpack2(fma2(pack2(o[b][c][0], o[b][c][1]), keep2, add2(pack2(acc[c][0], acc[c][1]), pack2(acc[c][2], acc[c][3]))), o[b][c][0], o[b][c][1]);
+                for (int u = 0; u < HQ; u++)
+#pragma unroll
+                    for (int e = 0; e < 2; e++) {
+                        o[u][b][0][e] = fmaf(o[u][b][0][e], keep[u], __fadd_rn(acc[u][e][0], acc[u][e][1]));
+                        o[u][b][1][e] = fmaf(o[u][b][1][e], keep[u], __fadd_rn(acc[u][e][2], acc[u][e][3]));
+                    }
             }
             __syncwarp();  // every lane has read the stage
             if (fetched < n_mine) {
@@ -484,34 +517,41 @@ __global__ void __launch_bounds__(Q4Cfg<NB>::THREADS, 1) k_attention_q4(const __
             }
             const bool ends = cur.t + 1 == cur.tiles;
             if (ends || i + 1 == n_mine) {
-                l += __shfl_xor_sync(0xffffffffu, l, 1);
-                l += __shfl_xor_sync(0xffffffffu, l, 2);
-                if (!ok) l = __int_as_float(0x7FC00000);
                 const float down = pow2(vexp - 12);
                 const int h0 = cur.hg % a.sub * A4_HEADS;
-                if (begins && ends) {
-                    if (h0 + g < a.group) {
-                        const float inv = __fdiv_rn(1.0f, l);
-                        T* out = static_cast<T*>(a.out) + ((size_t)cur.j * a.n_heads + (cur.hg / a.sub) * a.group + h0 + g) * C::HD;
+                const bool whole = begins && ends;
+                const int place = begins ? 1 : 0;
+                float* part = parts + (warp * 2 + place) * C::PART;
+#pragma unroll
+                for (int u = 0; u < HQ; u++) {
+                    const int h = 4 * u + t4;
+#pragma unroll
+                    for (int x = 4; x < 32; x <<= 1) l[u] += __shfl_xor_sync(0xffffffffu, l[u], x);
+                    if (!ok) l[u] = __int_as_float(0x7FC00000);
+                    if (whole) {
+                        if (h0 + h < a.group) {
+                            const float inv = __fdiv_rn(1.0f, l[u]);
+                            T* out = static_cast<T*>(a.out) + ((size_t)cur.j * a.n_heads + (cur.hg / a.sub) * a.group + h0 + h) * C::HD + 2 * g;
+#pragma unroll
+                            for (int b = 0; b < NB; b++)
+#pragma unroll
+                                for (int k = 0; k < 2; k++) {
+                                    out[32 * b + 16 * k] = from_f32<T>(__fmul_rn(o[u][b][k][0], inv));
+                                    out[32 * b + 16 * k + 1] = from_f32<T>(__fmul_rn(o[u][b][k][1], inv));
+                                }
+                        }
+                    } else {
 #pragma unroll
                         for (int b = 0; b < NB; b++)
 #pragma unroll
-                            for (int c = 0; c < 4; c++)
-#pragma unroll
-                                for (int x = 0; x < 2; x++) out[32 * b + value_dim(c, 2 * t4 + x)] = from_f32<T>(__fmul_rn(o[b][c][x], inv));
+                            for (int k = 0; k < 2; k++) {
+                                part[h * C::HD + 32 * b + 16 * k + 2 * g] = __fmul_rn(o[u][b][k][0], down);
+                                part[h * C::HD + 32 * b + 16 * k + 2 * g + 1] = __fmul_rn(o[u][b][k][1], down);
+                            }
+                        if (g == 0) part[A4_HEADS * C::HD + h] = m[u], part[A4_HEADS * C::HD + A4_HEADS + h] = __fmul_rn(l[u], down);
                     }
-                } else {
-                    const int place = begins ? 1 : 0;
-                    float* part = parts + (warp * 2 + place) * C::PART;
-#pragma unroll
-                    for (int b = 0; b < NB; b++)
-#pragma unroll
-                        for (int c = 0; c < 4; c++)
-#pragma unroll
-                            for (int x = 0; x < 2; x++) part[g * C::HD + 32 * b + value_dim(c, 2 * t4 + x)] = __fmul_rn(o[b][c][x], down);
-                    if (t4 == 0) part[A4_HEADS * C::HD + g] = m, part[A4_HEADS * C::HD + A4_HEADS + g] = __fmul_rn(l, down);
-                    if (lane == 0) desc[warp][place] = make_int4(cur.j, cur.hg, (begins ? 1 : 0) | (ends ? 2 : 0), 1);
                 }
+                if (!whole && lane == 0) desc[warp][place] = make_int4(cur.j, cur.hg, (begins ? 1 : 0) | (ends ? 2 : 0), 1);
                 fresh = true;
             }
             if (i + 1 < n_mine) advance(a, cur);
@@ -575,19 +615,23 @@ __global__ void __launch_bounds__(32 * A4_HEADS) k_attention_q4_join(const __gri
 constexpr int A4_MAX_CTAS = 256;
 size_t part_bytes(int head_dim) { return (size_t)A4_MAX_CTAS * 2 * (A4_HEADS * head_dim + 2 * A4_HEADS) * sizeof(float); }
 
-template <class T, int NB>
-cudaError_t launch_typed(cudaStream_t st, Q4Args& a) {
+template <class T, int NB, int HQ>
+cudaError_t launch_quads(cudaStream_t st, Q4Args& a) {
     using C = Q4Cfg<NB>;
     static RaisedPerDevice limit;
     int dev = 0, sms = 0;
     cudaError_t e = cudaGetDevice(&dev);
     if (e != cudaSuccess) return e;
     if ((e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev)) != cudaSuccess) return e;
-    if ((e = raise_dynamic_smem(limit, (const void*)k_attention_q4<T, NB>, C::SMEM)) != cudaSuccess) return e;
+    if ((e = raise_dynamic_smem(limit, (const void*)k_attention_q4<T, NB, HQ>, C::SMEM)) != cudaSuccess) return e;
     const dim3 grid((unsigned)(sms < A4_MAX_CTAS ? sms : A4_MAX_CTAS));
     g_kernel_launches += 2;
-    if ((e = launch_pdl(st, k_attention_q4<T, NB>, grid, dim3(C::THREADS), C::SMEM, a)) != cudaSuccess) return e;
+    if ((e = launch_pdl(st, k_attention_q4<T, NB, HQ>, grid, dim3(C::THREADS), C::SMEM, a)) != cudaSuccess) return e;
     return launch_pdl(st, k_attention_q4_join<T, NB>, grid, dim3(32 * A4_HEADS), 0, a);
+}
+template <class T, int NB>
+cudaError_t launch_typed(cudaStream_t st, Q4Args& a) {
+    return a.group <= 4 ? launch_quads<T, NB, 1>(st, a) : launch_quads<T, NB, 2>(st, a);
 }
 template <class T>
 cudaError_t launch_head(cudaStream_t st, Q4Args& a) {
