@@ -38,7 +38,7 @@ struct Q4Cfg {
     static constexpr int STAGE = 2 * (QUANTS + SCALES);
     static constexpr int PART = A4_HEADS * HD + 2 * A4_HEADS;                    // floats of a partial result: o, m, l
     static constexpr int STAGES = 2;
-    static constexpr int FIT = (218 * 1024) / (STAGES * STAGE + 2 * PART * 4), WARPS = FIT < 16 ? FIT : 16;
+    static constexpr int FIT = (218 * 1024) / (STAGES * STAGE + 2 * PART * 4), WARPS = FIT < 12 ? FIT : 12;  // (10, 13, 14: 40, 40, 37 us where 12 and 16 take 36: whole warps per scheduler)
     static constexpr int THREADS = 32 * WARPS;
     static constexpr size_t SMEM = (size_t)WARPS * (STAGES * STAGE + 2 * PART * 4);
 };
