@@ -3,22 +3,22 @@
 // Token j of a sequence with nq tokens and nk keys attends its keys t <= j + nk - nq:  o_j = sum_t p_t v_t / sum_t p_t with
 // p_t = 2^(x_t - m), x_t = log2(e) / sqrt(d) q_j . k_t, m a running maximum.
 //
-// A CTA takes 2 x 128 rows of one KV head: a row is a (token, query head of the group) pair, 128 / group tokens to a tile, so that a K / V tile
-// that lies in shared memory serves every head of its group and short prompts fill the rows.  K and V tiles of NK keys go through one ring
-// of TMA slots (K0 V0 K1 V1 ..).  Per row tile: S = Q K^T (tcgen05, S in tensor memory) -> the tile's four softmax warps, one row per
-// thread -> P over S in tensor memory -> P V with P as the A operand from there.  The two row tiles alternate: while one is in the
-// tensor core the other is in its softmax.
+// A CTA per SM walks over items: 2 x 128 rows of one KV head.  A row is a (token, query head of the group) pair, 128 / group tokens to a row tile, so
+// that a K / V tile that lies in shared memory serves every head of its group and short prompts fill the rows.  K and V tiles of NK keys go through
+// one ring of TMA slots (K0 V0 K1 V1 ..), which runs on from item to item.  Per row tile: S = Q K^T (tcgen05, S in tensor memory) -> the tile's four
+// softmax warps, one row per thread -> P in tensor memory -> P V with P as the A operand from there.  The two row tiles alternate: while one is
+// in the tensor core the other is in its softmax; and an item's last rows are written while the next one's first scores are computed.
 //
 // f16, bf16: one product each; O stays in tensor memory, and is rescaled only where a row's maximum has grown by more than 2^8 (a weight is at
 //   most 2^8 then; the last maximum that was used cancels in the quotient).
 // f32: every operand is split into two f16 parts, x = 2^e (hi + lo), 22 bits, with one power of two per row of Q and per tile of K and V
-//   (k_split), and a product is hi hi + hi lo + lo hi (lo lo is 2^-22 of it).  The tensor core adds with truncation, so that a sum over
+//   (K and V by k_split; a row of Q where it lies in shared memory, by the thread that owns it), and a product is hi hi + hi lo + lo hi (lo lo is 2^-22 of it).  The tensor core adds with truncation, so that a sum over
 //   thousands of keys would drift by 1e-5: O is taken out after every tile and added up in registers.
 //
 // Masked places may hold anything.  Scores are masked after the product; V is different, 0 * NaN is NaN: a warp looks at every V
 // tile that some row sees in part, zeroes what is not finite, and notes the keys; rows that attend such a key add its values at the end.
 //
-// Every wait is bounded: on expiry all roles leave their loops and the rows of the CTA become NaN.
+// Every wait is bounded: on expiry all roles leave their loops and all rows of the CTA's items become NaN.
 #include <cuda.h>
 #include <algorithm>
 #include <mutex>
@@ -30,9 +30,9 @@ namespace wick {
 namespace {
 
 constexpr int PR_ROWS = 128;      // rows of a tile == lanes of tensor memory
-constexpr int PR_THREADS = 384;   // TMA, MMA, V check, idle; 2 x 4 softmax warps
+constexpr int PR_THREADS = 384;   // TMA, MMA, V check, items; 2 x 4 softmax warps
+constexpr int PR_ITEMS = 3;       // items that are known ahead
 constexpr int PR_MASKED = 8;      // tiles that some row of a CTA sees in part: at most 256 / 64 + 2
-constexpr int PR_ZERO_CTAS = 32;
 constexpr uint32_t PR_SPIN_LIMIT = 1u << 18;  // try_wait suspends for a while: of the order of a second
 constexpr float PR_LAZY = 8.0f;
 
@@ -46,25 +46,42 @@ struct Cfg {
     static constexpr int FIT = (225 * 1024 - 2 * PLANES * QBYTES) / SLOT, NS = FIT < 6 ? FIT : 6;
     static constexpr bool O_IN_TMEM = PLANES == 1;
     static constexpr int O_BUFS = PLANES == 2 && HDP == 64 ? 2 : 1;
-    static constexpr int S_COL = 0, O_COL = NK;                      // columns of a row tile's 256
-    static_assert(NK + O_BUFS * HDP <= 256 && NS >= 3, "tensor or shared memory");
+    // columns of a row tile's 256: S, O, and P over S or, where there is room, beside it (the next S need not wait for P V then)
+    static constexpr bool P_APART = PLANES == 1 && HDP == 64;
+    static constexpr int S_COL = 0, P_COL = P_APART ? NK : 0, O_COL = NK + (P_APART ? NK / 2 : 0);
+    static_assert(O_COL + O_BUFS * HDP <= 256 && NS >= 3, "tensor or shared memory");
     static constexpr size_t SMEM = 1024 + (size_t)2 * PLANES * QBYTES + (size_t)NS * SLOT + 1024;
 };
 
-struct Barriers {
-    unsigned long long q_full, full[6], empty[6], ready[6], s_full[2], p_ready[2], checked[PR_MASKED];
-    uint32_t mask[PR_MASKED][4];
+struct Item {
+    int token0, tokens;   // first token (a row of q), tokens
+    int key0, keys;       // first key (a row of k), keys of the sequence
+    int first_visible;    // keys that the first token attends (may be negative)
+    int key_slot0, kvh;   // place of the sequence's first key tile; KV head (-1: no more items)
+    int n_tiles[2];       // tiles of keys that the two row tiles see
+    uint32_t mask[PR_MASKED][4];  // keys of the tiles from first_masked() on whose values are not finite
+    __device__ __forceinline__ int visible(int j) const { return max(0, min(first_visible + j, keys)); }
+    __device__ __forceinline__ int nt() const { return max(n_tiles[0], n_tiles[1]); }
+    template <int NK>
+    __device__ __forceinline__ int first_masked() const { return max(0, first_visible) / NK; }  // tiles from here on are seen in part by some row
+};
+struct Shared {
+    unsigned long long q_full[2], q_raw[2], q_empty, full[6], empty[6], ready[6], s_full[2], s_read[2], p_ready[2], o_full[2];
+    unsigned long long item_full[PR_ITEMS], item_empty[PR_ITEMS], checked[PR_ITEMS];
+    Item item[PR_ITEMS];
     uint32_t tmem_base;
     volatile uint32_t abort;
 };
+static_assert(sizeof(Shared) <= 1024, "room behind the ring");
 
 // What the kernels read besides the tensor maps.
 struct PromptArgs {
     Prompts p;
-    const float *q_inv, *k_inv, *v_inv;  // f32: the powers of two taken out of q rows and K / V tiles
+    const float *k_inv, *v_inv;          // f32: the powers of two taken out of K / V tiles
     int group, tile_tokens;              // query heads per KV head, tokens of a row tile
     int slots;                           // places for (sequence, block of 2 * tile_tokens tokens)
     int zero_rest;
+    int wide_rows;                       // rows of out start on 32-byte boundaries
     float scale_log2;
 };
 
@@ -90,7 +107,7 @@ __device__ __forceinline__ bool bar_try(void* bar, uint32_t parity) {
     return ok != 0;
 }
 // false: the limit, or another role has given up
-__device__ __forceinline__ bool bar_wait(Barriers* b, void* bar, uint32_t parity) {
+__device__ __forceinline__ bool bar_wait(Shared* b, void* bar, uint32_t parity) {
     for (uint32_t i = 0; i < PR_SPIN_LIMIT; i++) {
         if (bar_try(bar, parity)) return true;
         if ((i & 255u) == 255u && b->abort) return false;
@@ -198,437 +215,6 @@ __device__ __forceinline__ int find_seq(const int32_t* starts, int n_seqs, int n
     }
 }
 
-struct Block {  // the rows of a CTA
-    int token0, tokens;  // first token (a row of q), tokens of the block
-    int key0, keys;      // first key (a row of k), keys of the sequence
-    int first_visible;   // keys that the block's first token attends (may be negative)
-    __device__ __forceinline__ int visible(int j) const { return max(0, min(first_visible + j, keys)); }
-};
-
-template <class T, int PLANES, int HDP>
-__global__ void __launch_bounds__(PR_THREADS, 1)
-k_attention_prompts(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
-                    const __grid_constant__ PromptArgs a) {
-    using C = Cfg<PLANES, HDP>;
-    using T16 = typename std::conditional<PLANES == 2, __half, T>::type;
-    constexpr int NK = C::NK, NS = C::NS;
-    extern __shared__ uint8_t smem_raw[];
-    uint8_t* sm = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
-    Barriers* bar = reinterpret_cast<Barriers*>(sm + 2 * PLANES * C::QBYTES + NS * C::SLOT);
-    const uint32_t q_smem = smem_u32(sm), ring = q_smem + 2 * PLANES * C::QBYTES;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, hd = a.p.head_dim;
-    pdl_trigger();
-    pdl_wait();
-
-    if ((int)blockIdx.x >= a.slots * a.p.n_kv) {  // rows of no sequence
-        const int first = max(0, min(a.p.starts[0], a.p.n_tokens)), last = max(first, min(a.p.starts[a.p.n_seqs], a.p.n_tokens));
-        const size_t row = (size_t)a.p.n_heads * hd * sizeof(T) / 16, n = (size_t)(a.p.n_tokens - last + first) * row;
-        for (size_t i = (size_t)(blockIdx.x - a.slots * a.p.n_kv) * PR_THREADS + threadIdx.x; i < n; i += (size_t)PR_ZERO_CTAS * PR_THREADS)
-            reinterpret_cast<uint4*>(a.p.out)[i < first * row ? i : i + (size_t)(last - first) * row] = make_uint4(0, 0, 0, 0);
-        return;
-    }
-    // The last places first: a sequence's last blocks have the most keys, and the launch then ends with short ones.
-    const int slot = a.slots - 1 - (int)blockIdx.x / a.p.n_kv, kvh = (int)blockIdx.x % a.p.n_kv;
-    const int seq = find_seq(a.p.starts, a.p.n_seqs, a.p.n_tokens, 2 * a.tile_tokens, slot);
-    if (seq < 0) return;
-    Block blk;
-    int key_slot0;
-    {
-        const int32_t* ks = a.p.key_starts ? a.p.key_starts : a.p.starts;
-        const int q0 = max(0, min(a.p.starts[seq], a.p.n_tokens)), q1 = max(q0, min(a.p.starts[seq + 1], a.p.n_tokens));
-        const int k0 = max(0, min(ks[seq], a.p.n_keys)), k1 = max(k0, min(ks[seq + 1], a.p.n_keys));
-        const int at = (slot - (q0 / (2 * a.tile_tokens) + seq)) * 2 * a.tile_tokens;
-        if (at >= q1 - q0) return;
-        blk.token0 = q0 + at;
-        blk.tokens = min(2 * a.tile_tokens, q1 - blk.token0);
-        blk.key0 = k0, blk.keys = k1 - k0;
-        blk.first_visible = at + 1 + blk.keys - (q1 - q0);
-        key_slot0 = k0 / NK + seq;
-    }
-    // tiles of keys that the two row tiles see
-    int n_tiles[2];
-#pragma unroll
-    for (int m = 0; m < 2; m++) {
-        const int rows = min(a.tile_tokens, blk.tokens - m * a.tile_tokens);
-        n_tiles[m] = rows > 0 ? (blk.visible(m * a.tile_tokens + rows - 1) + NK - 1) / NK : 0;
-    }
-    const int nt = max(n_tiles[0], n_tiles[1]);
-    const int first_masked = max(0, blk.first_visible) / NK;  // tiles from here on are seen in part by some row
-
-    if (threadIdx.x == 0) {
-        bar_init(&bar->q_full, 1);
-        for (int s = 0; s < NS; s++) bar_init(&bar->full[s], 1), bar_init(&bar->empty[s], 1), bar_init(&bar->ready[s], 1);
-        for (int m = 0; m < 2; m++) bar_init(&bar->s_full[m], 1), bar_init(&bar->p_ready[m], 4);
-        for (int i = 0; i < PR_MASKED; i++) bar_init(&bar->checked[i], 1);
-        bar->abort = 0;
-        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-    }
-    if (warp == 1) {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&bar->tmem_base)), "r"(512u) : "memory");
-        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
-    }
-    tc_fence_before();
-    __syncthreads();
-    tc_fence_after();
-    const uint32_t tmem = bar->tmem_base;
-
-    if (warp == 0) {
-        // ── TMA ──────────────────────────────────────────────────────────────
-        if (lane == 0 && nt > 0) {
-            const int tiles_q = n_tiles[1] > 0 ? 2 : 1;
-            bar_expect(&bar->q_full, (uint32_t)(tiles_q * PLANES * C::CH * a.group * a.tile_tokens * 128));
-            for (int m = 0; m < tiles_q; m++)
-                for (int p = 0; p < PLANES; p++)
-                    for (int c = 0; c < C::CH; c++)
-                        tma_4d(q_smem + (m * PLANES + p) * C::QBYTES + c * PR_ROWS * 128, &map_q, &bar->q_full, c * 64, kvh * a.group,
-                               blk.token0 + m * a.tile_tokens, p);
-            for (int g = 0; g < 2 * nt; g++) {
-                const int s = g % NS, u = g / NS;
-                if (!bar_wait(bar, &bar->empty[s], (u & 1) ^ 1)) break;
-                bar_expect(&bar->full[s], C::SLOT);
-                for (int p = 0; p < PLANES; p++)
-                    for (int c = 0; c < C::CH; c++)
-                        tma_4d(ring + s * C::SLOT + p * C::KBYTES + c * NK * 128, (g & 1) ? &map_v : &map_k, &bar->full[s], c * 64, kvh,
-                               blk.key0 + (g >> 1) * NK, p);
-            }
-        }
-    } else if (warp == 1) {
-        // ── MMA ──────────────────────────────────────────────────────────────
-        const uint32_t leader = elect_one();
-        constexpr uint32_t type = std::is_same<T16, __nv_bfloat16>::value ? 1u : 0u;
-        constexpr uint32_t idesc_s = (1u << 4) | (type << 7) | (type << 10) | ((uint32_t)(NK >> 3) << 17) | ((uint32_t)(PR_ROWS >> 4) << 24);
-        constexpr uint32_t idesc_o = (1u << 4) | (type << 7) | (type << 10) | (1u << 16) | ((uint32_t)(HDP >> 3) << 17) | ((uint32_t)(PR_ROWS >> 4) << 24);
-        auto scores = [&](int m, uint32_t k_tile) {  // the small products first
-            const uint32_t d = tmem + m * 256 + C::S_COL, q = q_smem + m * PLANES * C::QBYTES;
-            uint32_t add = 0;
-#pragma unroll
-            for (int part = PLANES == 2 ? 0 : 2; part < 3; part++) {
-                const uint32_t qa = q + (part == 1 ? C::QBYTES : 0), ka = k_tile + (part == 0 ? C::KBYTES : 0);
-#pragma unroll
-                for (int ks = 0; ks < HDP / 16; ks++) {
-                    umma_ss(d, umma_desc(qa + (ks / 4) * PR_ROWS * 128 + (ks % 4) * 32, 16), umma_desc(ka + (ks / 4) * NK * 128 + (ks % 4) * 32, 16), idesc_s, add);
-                    add = 1;
-                }
-            }
-        };
-        auto weighted = [&](int m, int i, uint32_t v_tile) {
-            const uint32_t d = tmem + m * 256 + C::O_COL + (C::O_BUFS == 2 ? (i & 1) * HDP : 0), p = tmem + m * 256 + C::S_COL;
-            uint32_t add = C::O_IN_TMEM && i > 0;
-#pragma unroll
-            for (int part = PLANES == 2 ? 0 : 2; part < 3; part++) {
-#pragma unroll
-                for (int ks = 0; ks < NK / 16; ks++) {
-                    // P of 32 keys: 16 columns, of f32 followed by the 16 of its low parts
-                    const uint32_t pa = PLANES == 1 ? p + ks * 8 : p + (ks / 2) * 32 + (ks % 2) * 8 + (part == 1 ? 16 : 0);
-                    umma_ts(d, pa, umma_desc(v_tile + (part == 0 ? C::KBYTES : 0) + ks * 2048, NK * 128), idesc_o, add);
-                    add = 1;
-                }
-            }
-        };
-        bool ok = true;
-        if (nt > 0) ok = bar_wait(bar, &bar->q_full, 0) && bar_wait(bar, &bar->full[0], 0);
-        ok = __all_sync(0xffffffffu, ok);
-        if (ok && nt > 0) {
-            tc_fence_after();
-            if (leader) {
-                for (int m = 0; m < 2; m++)
-                    if (n_tiles[m] > 0) {
-                        scores(m, ring);
-                        umma_commit(&bar->s_full[m]);
-                    }
-                umma_commit(&bar->empty[0]);
-            }
-            __syncwarp();
-        }
-        for (int i = 0; i < nt && ok; i++) {
-            const int gv = 2 * i + 1, gk = gv + 1, sv = gv % NS, uv = gv / NS, sk = gk % NS, uk = gk / NS;
-            ok = bar_wait(bar, &bar->ready[sv], ((NS & 1) ? uv >> 1 : uv) & 1);
-            for (int m = 0; m < 2 && ok; m++) {
-                if (i >= n_tiles[m]) continue;
-                ok = bar_wait(bar, &bar->p_ready[m], i & 1);
-                ok = __all_sync(0xffffffffu, ok);
-                if (!ok) break;
-                tc_fence_after();
-                if (leader) weighted(m, i, ring + sv * C::SLOT);
-                __syncwarp();
-                if (i + 1 < n_tiles[m]) {
-                    ok = __all_sync(0xffffffffu, bar_wait(bar, &bar->full[sk], uk & 1));
-                    if (!ok) break;
-                    tc_fence_after();
-                    if (leader) scores(m, ring + sk * C::SLOT);
-                }
-                if (leader) umma_commit(&bar->s_full[m]);  // P V of this tile and S of the next
-                __syncwarp();
-            }
-            ok = __all_sync(0xffffffffu, ok);
-            if (ok && leader) {
-                umma_commit(&bar->empty[sv]);
-                if (i + 1 < nt) umma_commit(&bar->empty[sk]);
-            }
-            __syncwarp();
-        }
-    } else if (warp == 2) {
-        // ── V check ──────────────────────────────────────────────────────────
-        constexpr uint32_t EXP = std::is_same<T16, __nv_bfloat16>::value ? 0x7F807F80u : 0x7C007C00u;  // exponent bits, and
-        constexpr uint32_t ONE = std::is_same<T16, __nv_bfloat16>::value ? 0x00800080u : 0x04000400u;  // their lowest one
-        for (int i = 0; i < nt; i++) {
-            const int g = 2 * i + 1, s = g % NS;
-            if (!__all_sync(0xffffffffu, bar_wait(bar, &bar->full[s], (g / NS) & 1))) break;
-            if (i >= first_masked) {
-                uint8_t* tile = sm + 2 * PLANES * C::QBYTES + s * C::SLOT;
-                uint32_t found[4] = {0, 0, 0, 0};
-                for (int r = 0; r < NK; r += 4) {  // 8 lanes to a row of 128 bytes
-                    bool odd = false;
-#pragma unroll
-                    for (int c = 0; c < PLANES * C::CH; c++) {
-                        uint4* at = reinterpret_cast<uint4*>(tile + c * NK * 128 + (r + lane / 8) * 128) + lane % 8;
-                        uint4 w = *at;
-                        uint32_t* u = reinterpret_cast<uint32_t*>(&w);
-                        uint32_t hit = 0;
-#pragma unroll
-                        for (int x = 0; x < 4; x++) hit |= (u[x] & EXP) + ONE;
-                        if (hit & 0x80008000u) {
-                            odd = true;
-#pragma unroll
-                            for (int x = 0; x < 4; x++) {
-                                const uint32_t h = (u[x] & EXP) + ONE;
-                                if (h & 0x8000u) u[x] &= 0xFFFF0000u;
-                                if (h & 0x80000000u) u[x] &= 0x0000FFFFu;
-                            }
-                            *at = w;
-                        }
-                    }
-                    const uint32_t votes = __ballot_sync(0xffffffffu, odd);
-                    if (votes) {
-                        uint32_t rows = 0;
-#pragma unroll
-                        for (int x = 0; x < 4; x++) rows |= ((votes >> (8 * x)) & 255u) ? 1u << x : 0u;
-#pragma unroll
-                        for (int x = 0; x < 4; x++)
-                            if (r / 32 == x) found[x] |= rows << (r % 32);
-                    }
-                }
-                if (lane < 4) bar->mask[i - first_masked][lane] = lane == 0 ? found[0] : lane == 1 ? found[1] : lane == 2 ? found[2] : found[3];
-                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                __syncwarp();
-                if (lane == 0) bar_arrive(&bar->checked[i - first_masked]);
-            }
-            __syncwarp();
-            if (lane == 0) bar_arrive(&bar->ready[s]);
-        }
-    } else if (warp >= 4) {
-        // ── softmax: one row per thread ──────────────────────────────────────
-        const int m = (warp - 4) >> 2, r = (warp & 3) * 32 + lane, n = n_tiles[m];
-        const int j = m * a.tile_tokens + r / a.group, head = kvh * a.group + r % a.group;
-        const bool real = r < a.tile_tokens * a.group && j < blk.tokens;
-        const int limit = real ? blk.visible(j) : 0;
-        const uint32_t t_s = tmem + m * 256 + C::S_COL + ((uint32_t)((warp & 3) * 32) << 16), t_o = t_s + C::O_COL;
-        const float NEG = __int_as_float(0xFF800000);
-        float row_max = NEG, row_sum = 0.0f;
-        float o[C::O_IN_TMEM ? 1 : HDP];
-        bool ok = true;
-        if constexpr (C::O_IN_TMEM) {
-            for (int i = 0; i < n; i++) {
-                if (!(ok = __all_sync(0xffffffffu, bar_wait(bar, &bar->s_full[m], i & 1)))) break;
-                tc_fence_after();
-                float s[NK];
-#pragma unroll
-                for (int c = 0; c < NK / 32; c++) tmem_ld32(t_s + 32 * c, s + 32 * c);
-                tmem_ld_wait();
-                const int seen = limit - i * NK;
-                if (__any_sync(0xffffffffu, seen < NK)) {
-#pragma unroll
-                    for (int c = 0; c < NK; c++)
-                        if (c >= seen) s[c] = NEG;
-                }
-                float top[4] = {s[0], s[1], s[2], s[3]};
-#pragma unroll
-                for (int c = 4; c < NK; c++) top[c & 3] = fmaxf(top[c & 3], s[c]);
-                const float tile_max = __fmul_rn(fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])), a.scale_log2);
-                const bool grown = tile_max > row_max + PR_LAZY || (row_max == NEG && tile_max > NEG);
-                if (__any_sync(0xffffffffu, grown)) {
-                    float f = 1.0f;
-                    if (grown) {
-                        f = exp2_approx(row_max - tile_max);
-                        row_max = tile_max;
-                        row_sum = __fmul_rn(row_sum, f);
-                    }
-                    if (i > 0) {
-#pragma unroll 1
-                        for (int c = 0; c < HDP; c += 32) {
-                            float x[32];
-                            tmem_ld32(t_o + c, x);
-                            tmem_ld_wait();
-#pragma unroll
-                            for (int d = 0; d < 32; d++) x[d] = __fmul_rn(x[d], f);
-                            tmem_st32(t_o + c, x);
-                        }
-                    }
-                }
-                const float base = row_max == NEG ? 0.0f : -row_max;
-                float sum[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                for (int c = 0; c < NK / 32; c++) {
-                    uint32_t p[16];
-#pragma unroll
-                    for (int x = 0; x < 16; x++) {
-                        const float p0 = exp2_approx(fmaf(s[32 * c + 2 * x], a.scale_log2, base)), p1 = exp2_approx(fmaf(s[32 * c + 2 * x + 1], a.scale_log2, base));
-                        sum[(2 * x) & 3] += p0, sum[(2 * x + 1) & 3] += p1;
-                        p[x] = pack16<T16>(p0, p1);
-                    }
-                    tmem_st16(t_s + 16 * c, p);
-                }
-                row_sum += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-                tmem_st_wait();
-                tc_fence_before();
-                __syncwarp();
-                if (lane == 0) bar_arrive(&bar->p_ready[m]);
-            }
-            if (n > 0 && ok) ok = __all_sync(0xffffffffu, bar_wait(bar, &bar->s_full[m], n & 1));
-            tc_fence_after();
-        } else {
-#pragma unroll
-            for (int d = 0; d < HDP; d++) o[d] = 0.0f;
-            const float row_scale = real ? __fmul_rn(a.q_inv[(size_t)(blk.token0 + j) * a.p.n_heads + head], a.scale_log2) : 0.0f;
-            const float* k_inv = a.k_inv + (size_t)key_slot0 * a.p.n_kv + kvh;
-            const float* v_inv = a.v_inv + (size_t)key_slot0 * a.p.n_kv + kvh;
-            float rescale = 0.0f;  // of what `o` holds, for the tile whose P V is still in tensor memory
-            auto take_o = [&](int i) {
-                const float f = v_inv[(size_t)i * a.p.n_kv];
-#pragma unroll
-                for (int c = 0; c < HDP; c += 32) {
-                    float x[32];
-                    tmem_ld32(t_o + (C::O_BUFS == 2 ? (i & 1) * HDP : 0) + c, x);
-                    tmem_ld_wait();
-#pragma unroll
-                    for (int d = 0; d < 32; d++) o[c + d] = fmaf(x[d], f, __fmul_rn(o[c + d], rescale));
-                }
-            };
-            for (int i = 0; i < n; i++) {
-                const float scale = __fmul_rn(row_scale, k_inv[(size_t)i * a.p.n_kv]);
-                if (!(ok = __all_sync(0xffffffffu, bar_wait(bar, &bar->s_full[m], i & 1)))) break;
-                tc_fence_after();
-                const int seen = limit - i * NK;
-                const bool masked = __any_sync(0xffffffffu, seen < NK);
-                float top = NEG;
-#pragma unroll
-                for (int c = 0; c < NK / 32; c++) {
-                    float s[32];
-                    tmem_ld32(t_s + 32 * c, s);
-                    tmem_ld_wait();
-                    if (masked) {
-#pragma unroll
-                        for (int x = 0; x < 32; x++)
-                            if (32 * c + x >= seen) s[x] = NEG;
-                    }
-#pragma unroll
-                    for (int x = 0; x < 32; x++) top = fmaxf(top, s[x]);
-                }
-                if (C::O_BUFS == 1 && i > 0) take_o(i - 1);
-                const float new_max = fmaxf(row_max, __fmul_rn(top, scale));
-                const float f = row_max == NEG ? 0.0f : exp2_approx(row_max - new_max);
-                // weights up to 2^8, so that the low parts of small ones stay in f16's range
-                const float base = new_max == NEG ? 0.0f : PR_LAZY - new_max;
-                row_max = new_max;
-                float sum[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                for (int c = 0; c < NK / 32; c++) {
-                    float s[32];
-                    tmem_ld32(t_s + 32 * c, s);
-                    tmem_ld_wait();
-                    uint32_t hi[16], lo[16];
-#pragma unroll
-                    for (int x = 0; x < 32; x += 2) {
-                        float p[2], h[2];
-#pragma unroll
-                        for (int y = 0; y < 2; y++) {
-                            float v = fmaf(s[x + y], scale, base);
-                            if (masked && 32 * c + x + y >= seen) v = NEG;
-                            p[y] = exp2_approx(v);
-                            h[y] = __uint_as_float(__float_as_uint(p[y]) & 0xFFFFE000u);  // 11 bits: exact in f16
-                            sum[(x + y) & 3] += p[y];
-                        }
-                        hi[x / 2] = pack16<T16>(h[0], h[1]);
-                        lo[x / 2] = pack16<T16>(__fsub_rn(p[0], h[0]), __fsub_rn(p[1], h[1]));
-                    }
-                    tmem_st16(t_s + 32 * c, hi);
-                    tmem_st16(t_s + 32 * c + 16, lo);
-                }
-                row_sum = fmaf(row_sum, f, (sum[0] + sum[1]) + (sum[2] + sum[3]));
-                tmem_st_wait();
-                tc_fence_before();
-                __syncwarp();
-                if (lane == 0) bar_arrive(&bar->p_ready[m]);
-                if (C::O_BUFS == 2 && i > 0) take_o(i - 1);
-                rescale = f;
-            }
-            if (n > 0 && ok) ok = __all_sync(0xffffffffu, bar_wait(bar, &bar->s_full[m], n & 1));
-            tc_fence_after();
-            if (n > 0 && ok) take_o(n - 1);
-        }
-        for (int i = first_masked; i < nt && ok; i++) ok = __all_sync(0xffffffffu, bar_wait(bar, &bar->checked[i - first_masked], 0));
-
-        // ── the rows: quotient, values that are not finite, rounding ─────────
-        const float inv = limit > 0 ? __fdiv_rn(1.0f, row_sum) : 0.0f;
-        T* out = reinterpret_cast<T*>(a.p.out) + ((size_t)(blk.token0 + j) * a.p.n_heads + head) * hd;
-#pragma unroll
-        for (int c = 0; c < HDP; c += 32) {
-            float x[32];
-            if (C::O_IN_TMEM) {
-                if (n > 0) {  // (uniform in the warp)
-                    tmem_ld32(t_o + c, x);
-                    tmem_ld_wait();
-                }
-            } else {
-#pragma unroll
-                for (int d = 0; d < 32; d++) x[d] = o[C::O_IN_TMEM ? 0 : c + d];
-            }
-#pragma unroll
-            for (int d = 0; d < 32; d++) x[d] = limit > 0 ? __fmul_rn(x[d], inv) : 0.0f;
-            if (!ok) {
-#pragma unroll
-                for (int d = 0; d < 32; d++) x[d] = __int_as_float(0x7FC00000);
-            }
-            for (int i = first_masked; i < nt; i++)
-                for (int w = 0; w < NK / 32; w++)
-                    for (uint32_t bits = bar->mask[i - first_masked][w]; bits; bits &= bits - 1) {
-                        const int t = i * NK + w * 32 + __ffs(bits) - 1;
-                        if (t >= limit) continue;
-                        const T* v = reinterpret_cast<const T*>(a.p.v) + (size_t)(blk.key0 + t) * a.p.v_stride + (size_t)kvh * hd;
-#pragma unroll
-                        for (int d = 0; d < 32; d++)
-                            if (c + d < hd) {
-                                const float y = to_f32(v[c + d]);
-                                if (!(fabsf(y) <= 3.402823466e38f)) x[d] += y;
-                            }
-                    }
-            if (real) {
-                constexpr int V = 16 / (int)sizeof(T);
-#pragma unroll
-                for (int d = 0; d < 32; d += V)
-                    if (c + d < hd) {
-                        uint4 w;
-                        if constexpr (sizeof(T) == 4)
-                            w = make_uint4(__float_as_uint(x[d]), __float_as_uint(x[d + 1]), __float_as_uint(x[d + 2]), __float_as_uint(x[d + 3]));
-                        else
-                            w = make_uint4(pack16<T>(x[d], x[d + 1]), pack16<T>(x[d + 2], x[d + 3]), pack16<T>(x[d + 4], x[d + 5]), pack16<T>(x[d + 6], x[d + 7]));
-                        *reinterpret_cast<uint4*>(out + c + d) = w;
-                    }
-            }
-        }
-    }
-
-    tc_fence_before();
-    __syncthreads();
-    if (warp == 1) {
-        if (bar->abort)
-            for (int i = 0; i < 64; i++) __nanosleep(1000);  // copies issued before the failure may still be landing
-        tc_fence_after();
-        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
-    }
-}
-
 // ── f32: two f16 parts and a power of two ───────────────────────────────────
 // The power of two that takes a largest magnitude into [2^13, 2^14); 1 where there is none.
 __device__ __forceinline__ float to_range(float top) {
@@ -642,8 +228,8 @@ __device__ __forceinline__ void split4(float4 v, float f, uint2& hi, uint2& lo) 
 #pragma unroll
     for (int i = 0; i < 4; i++) {
         const float y = __fmul_rn(x[i], f);
-        h[i] = __half2float(__float2half_rn(y));
-        l[i] = fabsf(y) <= 65504.0f ? __fsub_rn(y, h[i]) : 0.0f;
+        h[i] = __uint_as_float(__float_as_uint(y) & 0xFFFFE000u);  // 11 bits: exact in f16
+        l[i] = fabsf(y) <= 65504.0f ? __fsub_rn(y, h[i]) : 0.0f;   // (an infinity's or NaN's high part says it)
     }
     hi = make_uint2(pack16<__half>(h[0], h[1]), pack16<__half>(h[2], h[3]));
     lo = make_uint2(pack16<__half>(l[0], l[1]), pack16<__half>(l[2], l[3]));
@@ -651,69 +237,687 @@ __device__ __forceinline__ void split4(float4 v, float f, uint2& hi, uint2& lo) 
 __device__ __forceinline__ float finite_abs(float x) { return fabsf(x) <= 3.402823466e38f ? fabsf(x) : 0.0f; }
 __device__ __forceinline__ float finite_max(float4 v) { return fmaxf(fmaxf(finite_abs(v.x), finite_abs(v.y)), fmaxf(finite_abs(v.z), finite_abs(v.w))); }
 
+// Place idx of the list, by a whole warp; false: there is nothing there.  The last places come first, since a sequence's last blocks have the
+// most keys and the launch then ends with short ones.
+template <int NK>
+__device__ __forceinline__ bool make_item(const PromptArgs& a, int idx, Item& it) {
+    const int block = 2 * a.tile_tokens, slot = a.slots - 1 - idx / a.p.n_kv;
+    const int seq = find_seq(a.p.starts, a.p.n_seqs, a.p.n_tokens, block, slot);
+    if (seq < 0) return false;
+    const int32_t* ks = a.p.key_starts ? a.p.key_starts : a.p.starts;
+    const int s0 = a.p.starts[seq], s1 = a.p.starts[seq + 1], t0 = ks[seq], t1 = ks[seq + 1];
+    const int q0 = max(0, min(s0, a.p.n_tokens)), q1 = max(q0, min(s1, a.p.n_tokens));
+    const int k0 = max(0, min(t0, a.p.n_keys)), k1 = max(k0, min(t1, a.p.n_keys));
+    const int at = (slot - (q0 / block + seq)) * block;
+    if (at >= q1 - q0) return false;
+    it.kvh = idx % a.p.n_kv;
+    it.token0 = q0 + at;
+    it.tokens = min(block, q1 - it.token0);
+    it.key0 = k0, it.keys = k1 - k0;
+    it.first_visible = at + 1 + it.keys - (q1 - q0);
+    it.key_slot0 = k0 / NK + seq;
+#pragma unroll
+    for (int m = 0; m < 2; m++) {
+        const int rows = min(a.tile_tokens, it.tokens - m * a.tile_tokens);
+        it.n_tiles[m] = rows > 0 ? (it.visible(m * a.tile_tokens + rows - 1) + NK - 1) / NK : 0;
+    }
+    return true;
+}
+
+template <class T, int PLANES, int HDP>
+__global__ void __launch_bounds__(PR_THREADS, 1)
+k_attention_prompts(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
+                    const __grid_constant__ PromptArgs a) {
+    using C = Cfg<PLANES, HDP>;
+    using T16 = typename std::conditional<PLANES == 2, __half, T>::type;
+    constexpr int NK = C::NK, NS = C::NS;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* sm = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+    Shared* sh = reinterpret_cast<Shared*>(sm + 2 * PLANES * C::QBYTES + NS * C::SLOT);
+    const uint32_t q_smem = smem_u32(sm), ring = q_smem + 2 * PLANES * C::QBYTES;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, hd = a.p.head_dim;
+
+    if (threadIdx.x == 0) {
+        for (int m = 0; m < 2; m++) {
+            bar_init(&sh->q_full[m], PLANES == 2 ? 4 : 1), bar_init(&sh->q_raw[m], 1);
+            bar_init(&sh->s_full[m], 1), bar_init(&sh->s_read[m], 4), bar_init(&sh->p_ready[m], 4), bar_init(&sh->o_full[m], 1);
+        }
+        bar_init(&sh->q_empty, 1);
+        for (int s = 0; s < NS; s++) bar_init(&sh->full[s], 1), bar_init(&sh->empty[s], 1), bar_init(&sh->ready[s], 1);
+        for (int i = 0; i < PR_ITEMS; i++) bar_init(&sh->item_full[i], 1), bar_init(&sh->item_empty[i], 11), bar_init(&sh->checked[i], 1);
+        sh->abort = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    }
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sh->tmem_base)), "r"(512u) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    pdl_trigger();
+    pdl_wait();
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = sh->tmem_base;
+
+    // Registers: the launch has 12 warps of 168; four give up 80 each, eight take 40 more (4 x 88 + 8 x 208 = 12 x 168).  One instruction for the
+    // four, in front of their branches: a warpgroup executes it together.
+    // An item of the list, for a role: waits until it is known.  false: no more items (or a wait ran out).
+    auto next_item = [&](uint32_t k) -> const Item* {
+        if (!__all_sync(0xffffffffu, bar_wait(sh, &sh->item_full[k % PR_ITEMS], (k / PR_ITEMS) & 1))) return nullptr;
+        const Item* it = &sh->item[k % PR_ITEMS];
+        return it->kvh < 0 ? nullptr : it;
+    };
+    auto leave_item = [&](uint32_t k) {
+        __syncwarp();
+        if (lane == 0) bar_arrive(&sh->item_empty[k % PR_ITEMS]);
+    };
+
+    if (warp < 4) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+        if (warp == 3) {
+        // ── items ────────────────────────────────────────────────────────────
+        const int total = a.slots * a.p.n_kv;
+        uint32_t k = 0;
+        for (int idx = blockIdx.x;; idx += gridDim.x) {
+            Item it;
+            it.kvh = -1;
+            if (idx < total && !make_item<NK>(a, idx, it)) continue;
+            if (!__all_sync(0xffffffffu, bar_wait(sh, &sh->item_empty[k % PR_ITEMS], ((k / PR_ITEMS) & 1) ^ 1))) break;
+            if (lane == 0) {
+                Item* to = &sh->item[k % PR_ITEMS];
+                to->token0 = it.token0, to->tokens = it.tokens, to->key0 = it.key0, to->keys = it.keys, to->first_visible = it.first_visible;
+                to->key_slot0 = it.key_slot0, to->kvh = it.kvh, to->n_tiles[0] = it.n_tiles[0], to->n_tiles[1] = it.n_tiles[1];
+                bar_arrive(&sh->item_full[k % PR_ITEMS]);
+            }
+            __syncwarp();
+            k++;
+            if (it.kvh < 0) break;
+        }
+        if (a.zero_rest) {  // rows of no sequence
+            const int first = max(0, min(a.p.starts[0], a.p.n_tokens)), last = max(first, min(a.p.starts[a.p.n_seqs], a.p.n_tokens));
+            const size_t row = (size_t)a.p.n_heads * hd * sizeof(T) / 16, n = (size_t)(a.p.n_tokens - last + first) * row;
+            for (size_t i = (size_t)blockIdx.x * 32 + lane; i < n; i += (size_t)gridDim.x * 32)
+                reinterpret_cast<uint4*>(a.p.out)[i < first * row ? i : i + (size_t)(last - first) * row] = make_uint4(0, 0, 0, 0);
+        }
+    } else if (warp == 0) {
+        // ── TMA ──────────────────────────────────────────────────────────────
+        uint32_t g = 0, qn = 0;  // ring positions; items with keys
+        bool ok = true;
+        for (uint32_t k = 0; ok; k++) {
+            const Item* it = next_item(k);
+            if (!it) break;
+            const int nt = it->nt();
+            if (nt > 0) {
+                if (lane == 0) {
+                    // Q: 128-byte columns, 64 elements of 16 bits or 32 of f32 (which its owners turn into two parts where they lie)
+                    constexpr int COLS = PLANES * C::CH, WIDTH = 64 / PLANES;
+                    ok = bar_wait(sh, &sh->q_empty, (qn & 1) ^ 1);
+                    for (int m = 0; m < 2 && ok; m++) {
+                        if (it->n_tiles[m] == 0) continue;
+                        unsigned long long* bar = PLANES == 2 ? &sh->q_raw[m] : &sh->q_full[m];
+                        bar_expect(bar, (uint32_t)(COLS * a.group * a.tile_tokens * 128));
+                        for (int c = 0; c < COLS; c++)
+                            tma_4d(q_smem + m * PLANES * C::QBYTES + c * PR_ROWS * 128, &map_q, bar, c * WIDTH, it->kvh * a.group,
+                                   it->token0 + m * a.tile_tokens, 0);
+                    }
+                    for (int i = 0; i < 2 * nt && ok; i++) {
+                        const uint32_t s = (g + i) % NS, u = (g + i) / NS;
+                        ok = bar_wait(sh, &sh->empty[s], (u & 1) ^ 1);
+                        if (!ok) break;
+                        bar_expect(&sh->full[s], C::SLOT);
+                        for (int p = 0; p < PLANES; p++)
+                            for (int c = 0; c < C::CH; c++)
+                                tma_4d(ring + s * C::SLOT + p * C::KBYTES + c * NK * 128, (i & 1) ? &map_v : &map_k, &sh->full[s], c * 64, it->kvh,
+                                       it->key0 + (i >> 1) * NK, p);
+                    }
+                }
+                ok = __all_sync(0xffffffffu, ok);
+                g += 2 * nt, qn++;
+            }
+            leave_item(k);
+        }
+    } else if (warp == 1) {
+        // ── MMA ──────────────────────────────────────────────────────────────
+        const uint32_t leader = elect_one();
+        constexpr uint32_t type = std::is_same<T16, __nv_bfloat16>::value ? 1u : 0u;
+        constexpr uint32_t idesc_s = (1u << 4) | (type << 7) | (type << 10) | ((uint32_t)(NK >> 3) << 17) | ((uint32_t)(PR_ROWS >> 4) << 24);
+        constexpr uint32_t idesc_o = (1u << 4) | (type << 7) | (type << 10) | (1u << 16) | ((uint32_t)(HDP >> 3) << 17) | ((uint32_t)(PR_ROWS >> 4) << 24);
+        auto scores = [&](int m, uint32_t k_tile) {  // the small products first
+            const uint32_t d = tmem + m * 256 + C::S_COL, q = q_smem + m * PLANES * C::QBYTES;
+            uint32_t add = 0;
+#pragma unroll
+            for (int part = PLANES == 2 ? 0 : 2; part < 3; part++) {
+                const uint32_t qa = q + (part == 1 ? PR_ROWS * 128 : 0), ka = k_tile + (part == 0 ? C::KBYTES : 0);
+#pragma unroll
+                for (int ks = 0; ks < HDP / 16; ks++) {
+                    umma_ss(d, umma_desc(qa + (ks / 4) * PLANES * PR_ROWS * 128 + (ks % 4) * 32, 16), umma_desc(ka + (ks / 4) * NK * 128 + (ks % 4) * 32, 16), idesc_s, add);
+                    add = 1;
+                }
+            }
+        };
+        auto weighted = [&](int m, int i, uint32_t buf, uint32_t v_tile) {
+            const uint32_t d = tmem + m * 256 + C::O_COL + (C::O_BUFS == 2 ? buf * HDP : 0), p = tmem + m * 256 + C::P_COL;
+            uint32_t add = C::O_IN_TMEM && i > 0;
+#pragma unroll
+            for (int part = PLANES == 2 ? 0 : 2; part < 3; part++) {
+#pragma unroll
+                for (int ks = 0; ks < NK / 16; ks++) {
+                    // P of 32 keys: 16 columns, of f32 followed by the 16 of its low parts
+                    const uint32_t pa = PLANES == 1 ? p + ks * 8 : p + (ks / 2) * 32 + (ks % 2) * 8 + (part == 1 ? 16 : 0);
+                    umma_ts(d, pa, umma_desc(v_tile + (part == 0 ? C::KBYTES : 0) + ks * 2048, NK * 128), idesc_o, add);
+                    add = 1;
+                }
+            }
+        };
+        uint32_t g = 0, done[2] = {0, 0}, qn[2] = {0, 0};  // ring positions; tiles and items of each row tile so far
+        bool ok = true;
+        for (uint32_t k = 0; ok; k++) {
+            const Item* it = next_item(k);
+            if (!it) break;
+            const int n0 = it->n_tiles[0], n1 = it->n_tiles[1], nt = max(n0, n1);
+            // S of tile i of a row tile, in whose place (P_APART: behind whose reading) the one before has been
+            auto issue_scores = [&](int m, uint32_t slot, int i) -> bool {
+                if (C::P_APART && done[m] + i > 0 && !__all_sync(0xffffffffu, bar_wait(sh, &sh->s_read[m], (done[m] + i - 1) & 1))) return false;
+                tc_fence_after();
+                if (leader) {
+                    scores(m, ring + slot * C::SLOT);
+                    umma_commit(&sh->s_full[m]);
+                }
+                __syncwarp();
+                return true;
+            };
+            if (nt > 0) {
+                ok = __all_sync(0xffffffffu, bar_wait(sh, &sh->full[g % NS], (g / NS) & 1));
+                for (int m = 0; m < 2 && ok; m++)
+                    if (it->n_tiles[m] > 0) {
+                        ok = __all_sync(0xffffffffu, bar_wait(sh, &sh->q_full[m], qn[m] & 1));
+                        if (ok) ok = issue_scores(m, g % NS, 0);
+                        qn[m]++;
+                    }
+                if (ok && leader) {
+                    umma_commit(&sh->empty[g % NS]);
+                    if (nt == 1) umma_commit(&sh->q_empty);
+                }
+                __syncwarp();
+            }
+            for (int i = 0; i < nt && ok; i++) {
+                const uint32_t gv = g + 2 * i + 1, gk = gv + 1, sv = gv % NS, uv = gv / NS, sk = gk % NS, uk = gk / NS;
+                const bool more = i + 1 < nt;
+                if (C::P_APART && more) {  // the next scores first
+                    ok = __all_sync(0xffffffffu, bar_wait(sh, &sh->full[sk], uk & 1));
+                    for (int m = 0; m < 2 && ok; m++)
+                        if (i + 1 < it->n_tiles[m]) ok = issue_scores(m, sk, i + 1);
+                    if (!ok) break;
+                    if (leader) {
+                        umma_commit(&sh->empty[sk]);
+                        if (i + 2 == nt) umma_commit(&sh->q_empty);
+                    }
+                    __syncwarp();
+                }
+                ok = __all_sync(0xffffffffu, bar_wait(sh, &sh->ready[sv], ((NS & 1) ? uv >> 1 : uv) & 1));
+                for (int m = 0; m < 2 && ok; m++) {
+                    const int n = m ? n1 : n0;
+                    if (i >= n) continue;
+                    ok = __all_sync(0xffffffffu, bar_wait(sh, &sh->p_ready[m], (done[m] + i) & 1));
+                    if (!ok) break;
+                    tc_fence_after();
+                    if (leader) {
+                        weighted(m, i, (done[m] + i) & 1, ring + sv * C::SLOT);
+                        if (C::P_APART || i + 1 == n) umma_commit(&sh->o_full[m]);
+                    }
+                    __syncwarp();
+                    if (!C::P_APART && i + 1 < n) {
+                        ok = __all_sync(0xffffffffu, bar_wait(sh, &sh->full[sk], uk & 1));
+                        if (ok) ok = issue_scores(m, sk, i + 1);
+                    }
+                }
+                if (ok && leader) {
+                    umma_commit(&sh->empty[sv]);
+                    if (!C::P_APART && more) {
+                        umma_commit(&sh->empty[sk]);
+                        if (i + 2 == nt) umma_commit(&sh->q_empty);
+                    }
+                }
+                __syncwarp();
+            }
+            g += 2 * nt, done[0] += n0, done[1] += n1;
+            leave_item(k);
+        }
+    } else if (warp == 2) {
+        // ── V check ──────────────────────────────────────────────────────────
+        constexpr uint32_t EXP = std::is_same<T16, __nv_bfloat16>::value ? 0x7F807F80u : 0x7C007C00u;  // exponent bits, and
+        constexpr uint32_t ONE = std::is_same<T16, __nv_bfloat16>::value ? 0x00800080u : 0x04000400u;  // their lowest one
+        uint32_t g0 = 0;
+        bool ok = true;
+        for (uint32_t k = 0; ok; k++) {
+            const Item* it = next_item(k);
+            if (!it) break;
+            Item* notes = &sh->item[k % PR_ITEMS];
+            const int nt = it->nt(), first_masked = it->template first_masked<NK>();
+            for (int i = 0; i < nt; i++) {
+                const uint32_t g = g0 + 2 * i + 1, s = g % NS;
+                if (!(ok = __all_sync(0xffffffffu, bar_wait(sh, &sh->full[s], (g / NS) & 1)))) break;
+                if (i >= first_masked) {
+                    uint8_t* tile = sm + 2 * PLANES * C::QBYTES + s * C::SLOT;
+                    uint32_t found[4] = {0, 0, 0, 0};
+                    for (int r = 0; r < NK; r += 4) {  // 8 lanes to a row of 128 bytes
+                        bool odd = false;
+#pragma unroll
+                        for (int c = 0; c < PLANES * C::CH; c++) {
+                            uint4* at = reinterpret_cast<uint4*>(tile + c * NK * 128 + (r + lane / 8) * 128) + lane % 8;
+                            uint4 w = *at;
+                            uint32_t* u = reinterpret_cast<uint32_t*>(&w);
+                            uint32_t hit = 0;
+#pragma unroll
+                            for (int x = 0; x < 4; x++) hit |= (u[x] & EXP) + ONE;
+                            if (hit & 0x80008000u) {
+                                odd = true;
+#pragma unroll
+                                for (int x = 0; x < 4; x++) {
+                                    const uint32_t h = (u[x] & EXP) + ONE;
+                                    if (h & 0x8000u) u[x] &= 0xFFFF0000u;
+                                    if (h & 0x80000000u) u[x] &= 0x0000FFFFu;
+                                }
+                                *at = w;
+                            }
+                        }
+                        const uint32_t votes = __ballot_sync(0xffffffffu, odd);
+                        if (votes) {
+                            uint32_t rows = 0;
+#pragma unroll
+                            for (int x = 0; x < 4; x++) rows |= ((votes >> (8 * x)) & 255u) ? 1u << x : 0u;
+#pragma unroll
+                            for (int x = 0; x < 4; x++)
+                                if (r / 32 == x) found[x] |= rows << (r % 32);
+                        }
+                    }
+                    if (lane < 4) notes->mask[i - first_masked][lane] = lane == 0 ? found[0] : lane == 1 ? found[1] : lane == 2 ? found[2] : found[3];
+                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                }
+                __syncwarp();
+                if (lane == 0) bar_arrive(&sh->ready[s]);
+            }
+            g0 += 2 * nt;
+            __syncwarp();
+            if (lane == 0 && ok) bar_arrive(&sh->checked[k % PR_ITEMS]);
+            leave_item(k);
+        }
+    }
+    } else {
+        // ── softmax: one row per thread ──────────────────────────────────────
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
+        const int m = (warp - 4) >> 2, r = (warp & 3) * 32 + lane, j = m * a.tile_tokens + r / a.group;
+        const uint32_t t_s = tmem + m * 256 + C::S_COL + ((uint32_t)((warp & 3) * 32) << 16), t_p = t_s + C::P_COL, t_o = t_s + C::O_COL;
+        const float NEG = __int_as_float(0xFF800000);
+        uint32_t done = 0, items = 0;  // tiles and items with keys of this row tile so far
+        float next_q = 0.0f;           // f32: the power of two taken out of this row of the item that comes next
+        // f32: this thread's row of an item's Q.  It has come as 32 elements to a 128-byte column; columns 2 c and 2 c + 1 become the high and
+        // the low parts of their 64 elements, in the same row of the same columns, so that a thread touches bytes of its own row only.
+        uint32_t raw = 0;  // items whose Q this row tile has taken
+        auto write_q = [&]() -> float {
+            if (!bar_wait(sh, &sh->q_raw[m], raw & 1)) return 0.0f;
+            raw++;
+            uint8_t* row = sm + m * PLANES * C::QBYTES + r * 128;
+            float top = 0.0f;
+            float4 v[16];
+#pragma unroll
+            for (int c = 0; c < C::CH; c++) {
+#pragma unroll
+                for (int x = 0; x < 16; x++) v[x] = *reinterpret_cast<float4*>(row + (2 * c + x / 8) * PR_ROWS * 128 + ((x & 7) ^ (r & 7)) * 16);
+#pragma unroll
+                for (int x = 0; x < 16; x++) top = fmaxf(top, finite_max(v[x]));
+            }
+            const float f = to_range(top);
+#pragma unroll
+            for (int c = 0; c < C::CH; c++) {
+                if (C::CH > 1) {
+#pragma unroll
+                    for (int x = 0; x < 16; x++) v[x] = *reinterpret_cast<float4*>(row + (2 * c + x / 8) * PR_ROWS * 128 + ((x & 7) ^ (r & 7)) * 16);
+                }
+#pragma unroll
+                for (int x = 0; x < 8; x++) {  // eight values, 16 bytes of each part
+                    uint2 h0, l0, h1, l1;
+                    split4(v[2 * x], f, h0, l0);
+                    split4(v[2 * x + 1], f, h1, l1);
+                    uint8_t* to = row + 2 * c * PR_ROWS * 128 + (x ^ (r & 7)) * 16;
+                    *reinterpret_cast<uint4*>(to) = make_uint4(h0.x, h0.y, h1.x, h1.y);
+                    *reinterpret_cast<uint4*>(to + PR_ROWS * 128) = make_uint4(l0.x, l0.y, l1.x, l1.y);
+                }
+            }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) bar_arrive(&sh->q_full[m]);
+            return __fdiv_rn(1.0f, f);
+        };
+        bool ok = true;
+        bool written = false;  // f32: the coming item's Q is in its place
+        for (uint32_t k = 0;; k++) {
+            const Item* it = next_item(k);
+            if (!it) break;
+            const int head = it->kvh * a.group + r % a.group, n = it->n_tiles[m], nt = it->nt(), first_masked = it->template first_masked<NK>();
+            const bool real = r < a.tile_tokens * a.group && j < it->tokens;
+            const int limit = real ? it->visible(j) : 0;
+            float row_max = NEG, row_sum = 0.0f;
+            float o[C::O_IN_TMEM ? 1 : HDP];
+            if constexpr (C::O_IN_TMEM) {
+                for (int i = 0; i < n && ok; i++) {
+                    if (!(ok = __all_sync(0xffffffffu, bar_wait(sh, &sh->s_full[m], (done + i) & 1)))) break;
+                    tc_fence_after();
+                    float s[NK];
+#pragma unroll
+                    for (int c = 0; c < NK / 32; c++) tmem_ld32(t_s + 32 * c, s + 32 * c);
+                    tmem_ld_wait();
+                    if (C::P_APART) {
+                        tc_fence_before();
+                        __syncwarp();
+                        if (lane == 0) bar_arrive(&sh->s_read[m]);
+                    }
+                    const int seen = limit - i * NK;
+                    if (__any_sync(0xffffffffu, seen < NK)) {
+#pragma unroll
+                        for (int c = 0; c < NK; c++)
+                            if (c >= seen) s[c] = NEG;
+                    }
+                    float top[4] = {s[0], s[1], s[2], s[3]};
+#pragma unroll
+                    for (int c = 4; c < NK; c++) top[c & 3] = fmaxf(top[c & 3], s[c]);
+                    const float tile_max = __fmul_rn(fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])), a.scale_log2);
+                    const bool grown = tile_max > row_max + PR_LAZY || (row_max == NEG && tile_max > NEG);
+                    // P V of the tile before is done: with P over S by the order of the tensor core's work, with P apart by this wait
+                    if (C::P_APART && i > 0 && !(ok = __all_sync(0xffffffffu, bar_wait(sh, &sh->o_full[m], (done + i - 1) & 1)))) break;
+                    if (__any_sync(0xffffffffu, grown)) {
+                        float f = 1.0f;
+                        if (grown) {
+                            f = exp2_approx(row_max - tile_max);
+                            row_max = tile_max;
+                            row_sum = __fmul_rn(row_sum, f);
+                        }
+                        if (i > 0) {
+#pragma unroll 1
+                            for (int c = 0; c < HDP; c += 32) {
+                                float x[32];
+                                tmem_ld32(t_o + c, x);
+                                tmem_ld_wait();
+#pragma unroll
+                                for (int d = 0; d < 32; d++) x[d] = __fmul_rn(x[d], f);
+                                tmem_st32(t_o + c, x);
+                            }
+                        }
+                    }
+                    const float base = row_max == NEG ? 0.0f : -row_max;
+                    const f32x2 base2 = pack2(base, base), scale2 = pack2(a.scale_log2, a.scale_log2);
+                    f32x2 sum[2] = {pack2(0.f, 0.f), pack2(0.f, 0.f)};
+#pragma unroll
+                    for (int c = 0; c < NK / 32; c++) {
+                        uint32_t p[16];
+#pragma unroll
+                        for (int x = 0; x < 16; x++) {
+                            float p0, p1;
+                            unpack2(fma2(pack2(s[32 * c + 2 * x], s[32 * c + 2 * x + 1]), scale2, base2), p0, p1);
+                            p0 = exp2_approx(p0), p1 = exp2_approx(p1);
+                            sum[x & 1] = add2(sum[x & 1], pack2(p0, p1));
+                            p[x] = pack16<T16>(p0, p1);
+                        }
+                        tmem_st16(t_p + 16 * c, p);
+                    }
+                    {
+                        float s0, s1;
+                        unpack2(add2(sum[0], sum[1]), s0, s1);
+                        row_sum += s0 + s1;
+                    }
+                    tmem_st_wait();
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) bar_arrive(&sh->p_ready[m]);
+                }
+            } else {
+                if (n > 0 && !written) next_q = write_q();
+                written = false;
+#pragma unroll
+                for (int d = 0; d < HDP; d++) o[d] = 0.0f;
+                const float row_scale = __fmul_rn(next_q, a.scale_log2);
+                const float* k_inv = a.k_inv + (size_t)it->key_slot0 * a.p.n_kv + it->kvh;
+                const float* v_inv = a.v_inv + (size_t)it->key_slot0 * a.p.n_kv + it->kvh;
+                float rescale = 0.0f;  // of what `o` holds, for the tile whose P V is still in tensor memory
+                float k_next = n > 0 ? k_inv[0] : 0.0f, v_now = 0.0f, v_next = n > 0 ? v_inv[0] : 0.0f;  // (a tile ahead)
+                auto take_o = [&](int i, float f) {
+                    const f32x2 f2 = pack2(f, f), rescale2 = pack2(rescale, rescale);
+#pragma unroll
+                    for (int c = 0; c < HDP; c += 32) {
+                        float x[32];
+                        tmem_ld32(t_o + (C::O_BUFS == 2 ? ((done + i) & 1) * HDP : 0) + c, x);
+                        tmem_ld_wait();
+#pragma unroll
+                        for (int d = 0; d < 32; d += 2)
+                            unpack2(fma2(pack2(x[d], x[d + 1]), f2, mul2(pack2(o[c + d], o[c + d + 1]), rescale2)), o[c + d], o[c + d + 1]);
+                    }
+                };
+                for (int i = 0; i < n && ok; i++) {
+                    const float scale = __fmul_rn(row_scale, k_next), v_before = v_now;
+                    v_now = v_next;
+                    if (i + 1 < n) k_next = k_inv[(size_t)(i + 1) * a.p.n_kv], v_next = v_inv[(size_t)(i + 1) * a.p.n_kv];
+                    if (!(ok = __all_sync(0xffffffffu, bar_wait(sh, &sh->s_full[m], (done + i) & 1)))) break;
+                    tc_fence_after();
+                    const int seen = limit - i * NK;
+                    const bool masked = __any_sync(0xffffffffu, seen < NK);
+                    float tops[4] = {NEG, NEG, NEG, NEG};
+#pragma unroll
+                    for (int c = 0; c < NK / 32; c++) {
+                        float s[32];
+                        tmem_ld32(t_s + 32 * c, s);
+                        tmem_ld_wait();
+                        if (masked) {
+#pragma unroll
+                            for (int x = 0; x < 32; x++)
+                                if (32 * c + x >= seen) s[x] = NEG;
+                        }
+#pragma unroll
+                        for (int x = 0; x < 32; x++) tops[x & 3] = fmaxf(tops[x & 3], s[x]);
+                    }
+                    const float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
+                    if (C::O_BUFS == 1 && i > 0) take_o(i - 1, v_before);
+                    const float new_max = fmaxf(row_max, __fmul_rn(top, scale));
+                    const float f = row_max == NEG ? 0.0f : exp2_approx(row_max - new_max);
+                    // weights up to 2^8, so that the low parts of small ones stay in f16's range
+                    const float base = new_max == NEG ? 0.0f : PR_LAZY - new_max;
+                    row_max = new_max;
+                    const f32x2 base2 = pack2(base, base), scale2 = pack2(scale, scale), minus = pack2(-1.0f, -1.0f);
+                    f32x2 sum[2] = {pack2(0.f, 0.f), pack2(0.f, 0.f)};
+#pragma unroll
+                    for (int c = 0; c < NK / 32; c++) {
+                        float s[32];
+                        tmem_ld32(t_s + 32 * c, s);
+                        tmem_ld_wait();
+                        uint32_t hi[16], lo[16];
+#pragma unroll
+                        for (int x = 0; x < 16; x++) {
+                            float p0, p1, l0, l1;
+                            unpack2(fma2(pack2(s[2 * x], s[2 * x + 1]), scale2, base2), p0, p1);
+                            if (masked) {
+                                if (32 * c + 2 * x >= seen) p0 = NEG;
+                                if (32 * c + 2 * x + 1 >= seen) p1 = NEG;
+                            }
+                            const f32x2 p2 = pack2(p0 = exp2_approx(p0), p1 = exp2_approx(p1));
+                            sum[x & 1] = add2(sum[x & 1], p2);
+                            const float h0 = __uint_as_float(__float_as_uint(p0) & 0xFFFFE000u);  // 11 bits: exact in f16
+                            const float h1 = __uint_as_float(__float_as_uint(p1) & 0xFFFFE000u);
+                            unpack2(fma2(pack2(h0, h1), minus, p2), l0, l1);
+                            hi[x] = pack16<T16>(h0, h1);
+                            lo[x] = pack16<T16>(l0, l1);
+                        }
+                        tmem_st16(t_p + 32 * c, hi);
+                        tmem_st16(t_p + 32 * c + 16, lo);
+                    }
+                    {
+                        float s0, s1;
+                        unpack2(add2(sum[0], sum[1]), s0, s1);
+                        row_sum = fmaf(row_sum, f, s0 + s1);
+                    }
+                    tmem_st_wait();
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) bar_arrive(&sh->p_ready[m]);
+                    if (C::O_BUFS == 2 && i > 0) take_o(i - 1, v_before);
+                    rescale = f;
+                }
+                if (n > 0 && ok) {
+                    // the next item's Q while the last P V runs (all of this one's scores have been computed)
+                    const Item* then = next_item(k + 1);
+                    if (then && then->n_tiles[m] > 0) {
+                        next_q = write_q();
+                        written = true;
+                    }
+                    if ((ok = __all_sync(0xffffffffu, bar_wait(sh, &sh->o_full[m], items & 1)))) {
+                        tc_fence_after();
+                        take_o(n - 1, v_now);
+                    }
+                }
+            }
+            if (C::O_IN_TMEM && n > 0 && ok) {
+                ok = __all_sync(0xffffffffu, bar_wait(sh, &sh->o_full[m], (C::P_APART ? done + n - 1 : items) & 1));
+                tc_fence_after();
+            }
+            ok = ok && __all_sync(0xffffffffu, bar_wait(sh, &sh->checked[k % PR_ITEMS], (k / PR_ITEMS) & 1));
+
+            // ── the rows: quotient, values that are not finite, rounding ─────
+            const float inv = limit > 0 ? __fdiv_rn(1.0f, row_sum) : 0.0f;
+            T* out = reinterpret_cast<T*>(a.p.out) + ((size_t)(it->token0 + j) * a.p.n_heads + head) * hd;
+            uint32_t odd = 0;
+            for (int i = first_masked; i < nt; i++)
+                for (int w = 0; w < NK / 32; w++) odd |= it->mask[i - first_masked][w];
+#pragma unroll
+            for (int c = 0; c < HDP; c += 32) {
+                float x[32];
+                if (C::O_IN_TMEM) {
+                    if (n > 0) {  // (uniform in the warp)
+                        tmem_ld32(t_o + c, x);
+                        tmem_ld_wait();
+                    }
+                } else {
+#pragma unroll
+                    for (int d = 0; d < 32; d++) x[d] = o[C::O_IN_TMEM ? 0 : c + d];
+                }
+#pragma unroll
+                for (int d = 0; d < 32; d++) x[d] = limit > 0 ? __fmul_rn(x[d], inv) : 0.0f;
+                if (odd)
+                    for (int i = first_masked; i < nt; i++)
+                        for (int w = 0; w < NK / 32; w++)
+                            for (uint32_t bits = it->mask[i - first_masked][w]; bits; bits &= bits - 1) {
+                                const int t = i * NK + w * 32 + __ffs(bits) - 1;
+                                if (t >= limit) continue;
+                                const T* v = reinterpret_cast<const T*>(a.p.v) + (size_t)(it->key0 + t) * a.p.v_stride + (size_t)it->kvh * hd;
+#pragma unroll
+                                for (int d = 0; d < 32; d++)
+                                    if (c + d < hd) {
+                                        const float y = to_f32(v[c + d]);
+                                        if (!(fabsf(y) <= 3.402823466e38f)) x[d] += y;
+                                    }
+                            }
+                if (real && ok) {
+                    constexpr int V = 16 / (int)sizeof(T);
+#pragma unroll
+                    for (int d = 0; d < 32; d += 2 * V) {
+                        uint32_t w[8];
+#pragma unroll
+                        for (int u = 0; u < 8; u++)
+                            if constexpr (sizeof(T) == 4)
+                                w[u] = __float_as_uint(x[d + u]);
+                            else
+                                w[u] = pack16<T>(x[d + 2 * u], x[d + 2 * u + 1]);
+                        T* to = out + c + d;
+                        // A row is a thread's: 32 bytes at a time are whole sectors (16 at a time took 8000 cycles for 256 rows of 256 bytes)
+                        if (a.wide_rows && c + d + 2 * V <= hd)
+                            asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(to), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]),
+                                         "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
+                                         : "memory");
+                        else {
+                            if (c + d < hd) *reinterpret_cast<uint4*>(to) = make_uint4(w[0], w[1], w[2], w[3]);
+                            if (c + d + V < hd) *reinterpret_cast<uint4*>(to + V) = make_uint4(w[4], w[5], w[6], w[7]);
+                        }
+                    }
+                }
+            }
+            tc_fence_before();  // (tensor memory has been read before the next P V, which waits for p_ready)
+            done += n, items += n > 0 ? 1 : 0;
+            leave_item(k);
+        }
+    }
+
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 1) {
+        if (sh->abort) {
+            for (int i = 0; i < 64; i++) __nanosleep(1000);  // copies issued before the failure may still be landing
+            for (int idx = blockIdx.x; idx < a.slots * a.p.n_kv; idx += gridDim.x) {  // no row is left without a sign of it
+                Item it;
+                if (!make_item<NK>(a, idx, it)) continue;
+                for (int i = lane; i < it.tokens * a.group * hd; i += 32)
+                    reinterpret_cast<T*>(a.p.out)[((size_t)(it.token0 + i / (a.group * hd)) * a.p.n_heads + it.kvh * a.group) * hd + i % (a.group * hd)] =
+                        from_f32<T>(__int_as_float(0x7FC00000));
+            }
+        }
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
+    }
+}
+
 struct SplitArgs {
     Prompts p;
-    __half *q, *k, *v;  // [2][rows][heads * head_dim]
-    float *q_inv, *k_inv, *v_inv;
-    int tile, key_slots;  // keys of a tile; places for (sequence, tile)
+    __half* to[2];  // keys, values: [2][rows][heads * head_dim]
+    float* inv[2];
+    int lanes;      // of a row: head_dim / 4 rounded up to a power of two
 };
 constexpr int SP_THREADS = 256;
 
-// CTAs [0, key_slots * n_kv * 2): a tile of K or V each; the others: rows of q, one (token, head) per warp.  Bound: HBM (4 bytes in, 4 out
+// A tile of K or V per CTA, held in registers between the search for its largest magnitude and its parts.  Bound: HBM (4 bytes in, 4 out
 // per element), the launch for short prompts.
+template <int NK>
 __global__ void __launch_bounds__(SP_THREADS) k_split(const __grid_constant__ SplitArgs a) {
     pdl_trigger();
     pdl_wait();
-    const int hd = a.p.head_dim, pieces = hd / 4, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int tiles = a.key_slots * a.p.n_kv * 2;
-    if ((int)blockIdx.x < tiles) {
-        __shared__ float red[SP_THREADS / 32];
-        const int val = blockIdx.x & 1, kvh = (blockIdx.x >> 1) % a.p.n_kv, slot = (blockIdx.x >> 1) / a.p.n_kv;
-        const int32_t* ks = a.p.key_starts ? a.p.key_starts : a.p.starts;
-        const int seq = find_seq(ks, a.p.n_seqs, a.p.n_keys, a.tile, slot);
-        if (seq < 0) return;
-        const int k0 = max(0, min(ks[seq], a.p.n_keys)), k1 = max(k0, min(ks[seq + 1], a.p.n_keys));
-        const int first = k0 + (slot - (k0 / a.tile + seq)) * a.tile, rows = min(a.tile, k1 - first);
-        if (rows <= 0) return;
-        const float* src = (val ? (const float*)a.p.v + (size_t)first * a.p.v_stride : (const float*)a.p.k + (size_t)first * a.p.k_stride) + (size_t)kvh * hd;
-        const size_t stride = val ? a.p.v_stride : a.p.k_stride, dim = (size_t)a.p.n_kv * hd, plane = (size_t)a.p.n_keys * dim;
-        __half* dst = (val ? a.v : a.k) + (size_t)first * dim + (size_t)kvh * hd;
-        float top = 0.0f;
-        for (int i = threadIdx.x; i < rows * pieces; i += SP_THREADS) top = fmaxf(top, finite_max(reinterpret_cast<const float4*>(src + (i / pieces) * stride)[i % pieces]));
+    __shared__ float red[SP_THREADS / 32];
+    const int hd = a.p.head_dim, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int val = blockIdx.x & 1, kvh = (blockIdx.x >> 1) % a.p.n_kv, slot = (blockIdx.x >> 1) / a.p.n_kv;
+    const int32_t* ks = a.p.key_starts ? a.p.key_starts : a.p.starts;
+    const int seq = find_seq(ks, a.p.n_seqs, a.p.n_keys, NK, slot);
+    if (seq < 0) return;
+    const int k0 = max(0, min(ks[seq], a.p.n_keys)), k1 = max(k0, min(ks[seq + 1], a.p.n_keys));
+    const int first = k0 + (slot - (k0 / NK + seq)) * NK, rows = min(NK, k1 - first);
+    if (rows <= 0) return;
+    const size_t stride = val ? a.p.v_stride : a.p.k_stride, dim = (size_t)a.p.n_kv * hd, plane = (size_t)a.p.n_keys * dim;
+    const int piece = threadIdx.x & (a.lanes - 1), row0 = threadIdx.x / a.lanes, step = SP_THREADS / a.lanes;
+    const float* src = (const float*)(val ? a.p.v : a.p.k) + (size_t)first * stride + (size_t)kvh * hd + 4 * piece;
+    const bool in = 4 * piece < hd;
+    constexpr int MOST = NK * (NK == 128 ? 16 : 32) / SP_THREADS;  // rows of a thread, at most (heads of up to 64 have tiles of 128 keys)
+    float4 x[MOST];
+    float top = 0.0f;
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-        if (lane == 0) red[warp] = top;
-        __syncthreads();
-#pragma unroll
-        for (int w = 0; w < SP_THREADS / 32; w++) top = fmaxf(top, red[w]);
-        const float f = to_range(top);
-        for (int i = threadIdx.x; i < rows * pieces; i += SP_THREADS) {
-            uint2 hi, lo;
-            split4(reinterpret_cast<const float4*>(src + (i / pieces) * stride)[i % pieces], f, hi, lo);
-            uint2* at = reinterpret_cast<uint2*>(dst + (i / pieces) * dim) + i % pieces;
-            *at = hi;
-            *reinterpret_cast<uint2*>(reinterpret_cast<__half*>(at) + plane) = lo;
-        }
-        if (threadIdx.x == 0) (val ? a.v_inv : a.k_inv)[(size_t)slot * a.p.n_kv + kvh] = __fdiv_rn(1.0f, f);
-        return;
+    for (int i = 0; i < MOST; i++) {
+        const int row = row0 + i * step;
+        x[i] = in && row < rows ? *reinterpret_cast<const float4*>(src + row * stride) : make_float4(0.f, 0.f, 0.f, 0.f);
     }
-    const size_t at = (size_t)(blockIdx.x - tiles) * (SP_THREADS / 32) + warp, rows = (size_t)a.p.n_tokens * a.p.n_heads;
-    if (at >= rows) return;
-    const size_t token = at / a.p.n_heads, head = at % a.p.n_heads;
-    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (lane < pieces) v = reinterpret_cast<const float4*>((const float*)a.p.q + token * a.p.q_stride + head * hd)[lane];
-    float top = finite_max(v);
+#pragma unroll
+    for (int i = 0; i < MOST; i++) top = fmaxf(top, finite_max(x[i]));
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    if (lane == 0) red[warp] = top;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < SP_THREADS / 32; w++) top = fmaxf(top, red[w]);
     const float f = to_range(top);
-    uint2 hi, lo;
-    split4(v, f, hi, lo);
-    if (lane < pieces) {
-        uint2* dst = reinterpret_cast<uint2*>(a.q + at * hd) + lane;
-        *dst = hi;
-        *reinterpret_cast<uint2*>(reinterpret_cast<__half*>(dst) + rows * hd) = lo;
+    __half* dst = a.to[val] + (size_t)first * dim + (size_t)kvh * hd + 4 * piece;
+#pragma unroll
+    for (int i = 0; i < MOST; i++) {
+        const int row = row0 + i * step;
+        if (in && row < rows) {
+            uint2 hi, lo;
+            split4(x[i], f, hi, lo);
+            *reinterpret_cast<uint2*>(dst + row * dim) = hi;
+            *reinterpret_cast<uint2*>(dst + row * dim + plane) = lo;
+        }
     }
-    if (lane == 0) a.q_inv[at] = __fdiv_rn(1.0f, f);
+    if (threadIdx.x == 0) a.inv[val][(size_t)slot * a.p.n_kv + kvh] = __fdiv_rn(1.0f, f);
 }
 
 // ── host side ───────────────────────────────────────────────────────────────
@@ -730,14 +934,15 @@ EncodeTiledFn encode_tiled_fn() {
     });
     return fn;
 }
-// 16-bit rows [planes][rows][heads][head_dim]; box: 64 columns (zeros behind head_dim) x box_heads x box_rows, 128-byte swizzle.
-cudaError_t encode_heads(const void* base, bool bf16, int hd, int heads, int rows, int planes, size_t stride, int box_heads, int box_rows, CUtensorMap* out) {
+// Rows [planes][rows][heads][head_dim]; box: 128 bytes of a head (zeros behind head_dim) x box_heads x box_rows, 128-byte swizzle.
+cudaError_t encode_heads(const void* base, int dtype, int hd, int heads, int rows, int planes, size_t stride, int box_heads, int box_rows, CUtensorMap* out) {
     EncodeTiledFn fn = encode_tiled_fn();
     if (!fn) return cudaErrorNotSupported;
-    const cuuint64_t dims[4] = {(cuuint64_t)hd, (cuuint64_t)heads, (cuuint64_t)rows, (cuuint64_t)planes};
-    const cuuint64_t strides[3] = {(cuuint64_t)hd * 2, (cuuint64_t)stride * 2, (cuuint64_t)stride * 2 * (cuuint64_t)rows};
-    const cuuint32_t box[4] = {64, (cuuint32_t)box_heads, (cuuint32_t)box_rows, 1}, step[4] = {1, 1, 1, 1};
-    const CUresult r = fn(out, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, const_cast<void*>(base), dims, strides, box,
+    const cuuint64_t size = (cuuint64_t)dtype_bytes(dtype), dims[4] = {(cuuint64_t)hd, (cuuint64_t)heads, (cuuint64_t)rows, (cuuint64_t)planes};
+    const cuuint64_t strides[3] = {(cuuint64_t)hd * size, (cuuint64_t)stride * size, (cuuint64_t)stride * size * (cuuint64_t)rows};
+    const cuuint32_t box[4] = {(cuuint32_t)(128 / size), (cuuint32_t)box_heads, (cuuint32_t)box_rows, 1}, step[4] = {1, 1, 1, 1};
+    const CUtensorMapDataType type = dtype == DT_F32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : dtype == DT_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+    const CUresult r = fn(out, type, 4, const_cast<void*>(base), dims, strides, box,
                           step, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                           CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     return r == CUDA_SUCCESS ? cudaSuccess : cudaErrorInvalidValue;
@@ -748,7 +953,7 @@ int keys_per_tile(const Prompts& p) { return p.dtype == DT_F32 && p.head_dim > 6
 int places(int rows, int seqs, int block) { return rows / block + seqs + 1; }
 
 struct Workspace {
-    size_t q, k, v, q_inv, k_inv, v_inv, bytes;
+    size_t k, v, k_inv, v_inv, bytes;
     explicit Workspace(const Prompts& p) {
         const size_t key_slots = (size_t)places(p.n_keys, p.n_seqs, keys_per_tile(p));
         size_t at = 0;
@@ -757,10 +962,8 @@ struct Workspace {
             at += up128(n);
             return here;
         };
-        q = take((size_t)p.n_tokens * p.n_heads * p.head_dim * 4);
         k = take((size_t)p.n_keys * p.n_kv * p.head_dim * 4);
         v = take((size_t)p.n_keys * p.n_kv * p.head_dim * 4);
-        q_inv = take((size_t)p.n_tokens * p.n_heads * 4);
         k_inv = take(key_slots * p.n_kv * 4);
         v_inv = take(key_slots * p.n_kv * 4);
         bytes = at;
@@ -779,34 +982,38 @@ cudaError_t launch_typed(cudaStream_t st, const Prompts& p, void* workspace) {
     a.tile_tokens = PR_ROWS / a.group;
     a.slots = places(p.n_tokens, p.n_seqs, 2 * a.tile_tokens);
     a.zero_rest = p.zero_rest;
+    a.wide_rows = (((uintptr_t)p.out | (size_t)p.head_dim * sizeof(T)) & 31) == 0;
     a.scale_log2 = 1.4426950408889634f / sqrtf((float)p.head_dim);
-    const bool bf16 = std::is_same<T, __nv_bfloat16>::value;
-    const void *q = p.q, *k = p.k, *v = p.v;
-    size_t qs = p.q_stride, ks = p.k_stride, vs = p.v_stride;
-    if (PLANES == 2) {
+    const int parts = PLANES == 2 ? DT_F16 : p.dtype;  // what K and V are in
+    const void *k = p.k, *v = p.v;
+    size_t ks = p.k_stride, vs = p.v_stride;
+    if (PLANES == 2 && p.n_keys > 0) {
         const Workspace w(p);
         uint8_t* base = static_cast<uint8_t*>(workspace);
-        SplitArgs s{p, (__half*)(base + w.q), (__half*)(base + w.k), (__half*)(base + w.v), (float*)(base + w.q_inv), (float*)(base + w.k_inv),
-                    (float*)(base + w.v_inv), C::NK, p.n_keys > 0 ? places(p.n_keys, p.n_seqs, C::NK) : 0};
-        const long long ctas = (long long)s.key_slots * p.n_kv * 2 + ((long long)p.n_tokens * p.n_heads + SP_THREADS / 32 - 1) / (SP_THREADS / 32);
+        SplitArgs s{p, {(__half*)(base + w.k), (__half*)(base + w.v)}, {(float*)(base + w.k_inv), (float*)(base + w.v_inv)}, 1};
+        while (s.lanes * 4 < p.head_dim) s.lanes *= 2;
+        const long long ctas = (long long)places(p.n_keys, p.n_seqs, C::NK) * p.n_kv * 2;
         if (ctas > 0x7FFFFFFFll) return cudaErrorInvalidValue;
         g_kernel_launches++;
-        if ((e = launch_pdl(st, k_split, dim3((unsigned)ctas), dim3(SP_THREADS), 0, s)) != cudaSuccess) return e;
-        q = s.q, k = s.k, v = s.v;
-        qs = (size_t)p.n_heads * p.head_dim, ks = vs = (size_t)p.n_kv * p.head_dim;
-        a.q_inv = s.q_inv, a.k_inv = s.k_inv, a.v_inv = s.v_inv;
+        if ((e = launch_pdl(st, k_split<C::NK>, dim3((unsigned)ctas), dim3(SP_THREADS), 0, s)) != cudaSuccess) return e;
+        k = s.to[0], v = s.to[1];
+        ks = vs = (size_t)p.n_kv * p.head_dim;
+        a.k_inv = s.inv[0], a.v_inv = s.inv[1];
     }
-    CUtensorMap mq, mk, mv;
-    if ((e = encode_heads(q, bf16, p.head_dim, p.n_heads, p.n_tokens, PLANES, qs, a.group, a.tile_tokens, &mq)) != cudaSuccess) return e;
-    mk = mv = mq;  // (without any keys: never read)
+    CUtensorMap mq, mk, mv;  // (without any keys none is read)
+    if ((e = encode_heads(p.q, p.dtype, p.head_dim, p.n_heads, p.n_tokens, 1, p.q_stride, a.group, a.tile_tokens, &mq)) != cudaSuccess) return e;
+    mk = mv = mq;
     if (p.n_keys > 0) {
-        if ((e = encode_heads(k, bf16, p.head_dim, p.n_kv, p.n_keys, PLANES, ks, 1, C::NK, &mk)) != cudaSuccess) return e;
-        if ((e = encode_heads(v, bf16, p.head_dim, p.n_kv, p.n_keys, PLANES, vs, 1, C::NK, &mv)) != cudaSuccess) return e;
+        if ((e = encode_heads(k, parts, p.head_dim, p.n_kv, p.n_keys, PLANES, ks, 1, C::NK, &mk)) != cudaSuccess) return e;
+        if ((e = encode_heads(v, parts, p.head_dim, p.n_kv, p.n_keys, PLANES, vs, 1, C::NK, &mv)) != cudaSuccess) return e;
     }
-    const long long grid = (long long)a.slots * p.n_kv + (p.zero_rest ? PR_ZERO_CTAS : 0);
-    if (grid > 0x7FFFFFFFll) return cudaErrorInvalidValue;
+    int dev = 0, sms = 0;
+    if ((e = cudaGetDevice(&dev)) != cudaSuccess) return e;
+    if ((e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev)) != cudaSuccess) return e;
+    const long long items = (long long)a.slots * p.n_kv;
+    if (items > 0x7FFFFFFFll - sms) return cudaErrorInvalidValue;
     g_kernel_launches++;
-    return launch_pdl(st, k_attention_prompts<T, PLANES, HDP>, dim3((unsigned)grid), dim3(PR_THREADS), C::SMEM, mq, mk, mv, a);
+    return launch_pdl(st, k_attention_prompts<T, PLANES, HDP>, dim3((unsigned)std::min<long long>(items, sms)), dim3(PR_THREADS), C::SMEM, mq, mk, mv, a);
 }
 
 }  // namespace
