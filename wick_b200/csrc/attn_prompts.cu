@@ -183,6 +183,13 @@ __device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t* r) {
 }
 __device__ __forceinline__ void tmem_ld_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+// Shared memory by 32-bit address (the aligned buffer's pointer is a generic one to the compiler)
+__device__ __forceinline__ void lds_4(uint32_t at, float* v) {
+    asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]) : "r"(at) : "memory");
+}
+__device__ __forceinline__ void sts_4(uint32_t at, const uint32_t* v) {
+    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]) : "memory");
+}
 __device__ __forceinline__ float exp2_approx(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -388,10 +395,13 @@ k_attention_prompts(const __grid_constant__ CUtensorMap map_q, const __grid_cons
             uint32_t add = 0;
 #pragma unroll
             for (int part = PLANES == 2 ? 0 : 2; part < 3; part++) {
-                const uint32_t qa = q + (part == 1 ? PR_ROWS * 128 : 0), ka = k_tile + (part == 0 ? C::KBYTES : 0);
+                const uint32_t ka = k_tile + (part == 0 ? C::KBYTES : 0);
 #pragma unroll
                 for (int ks = 0; ks < HDP / 16; ks++) {
-                    umma_ss(d, umma_desc(qa + (ks / 4) * PLANES * PR_ROWS * 128 + (ks % 4) * 32, 16), umma_desc(ka + (ks / 4) * NK * 128 + (ks % 4) * 32, 16), idesc_s, add);
+                    // Q: 64 elements to a 128-byte column; of f32 32, the low parts behind the high ones
+                    const uint32_t qa = PLANES == 1 ? q + (ks / 4) * PR_ROWS * 128 + (ks % 4) * 32
+                                                    : q + (ks / 2) * PR_ROWS * 128 + (part == 1 ? 64 : 0) + (ks % 2) * 32;
+                    umma_ss(d, umma_desc(qa, 16), umma_desc(ka + (ks / 4) * NK * 128 + (ks % 4) * 32, 16), idesc_s, add);
                     add = 1;
                 }
             }
@@ -552,37 +562,43 @@ k_attention_prompts(const __grid_constant__ CUtensorMap map_q, const __grid_cons
         const float NEG = __int_as_float(0xFF800000);
         uint32_t done = 0, items = 0;  // tiles and items with keys of this row tile so far
         float next_q = 0.0f;           // f32: the power of two taken out of this row of the item that comes next
-        // f32: this thread's row of an item's Q.  It has come as 32 elements to a 128-byte column; columns 2 c and 2 c + 1 become the high and
-        // the low parts of their 64 elements, in the same row of the same columns, so that a thread touches bytes of its own row only.
+        // f32: this thread's row of an item's Q.  It has come as 32 elements to a 128-byte column, whose bytes become the 32 high and the 32 low
+        // parts.  Loops stay loops here and below: code that runs once per item is fetched anew each time, and unrolled it took longer
+        // to fetch than to run (3000 to 7000 cycles for this).
         uint32_t raw = 0;  // items whose Q this row tile has taken
         auto write_q = [&]() -> float {
             if (!bar_wait(sh, &sh->q_raw[m], raw & 1)) return 0.0f;
             raw++;
-            uint8_t* row = sm + m * PLANES * C::QBYTES + r * 128;
-            float top = 0.0f;
-            float4 v[16];
+            const uint32_t row = q_smem + m * PLANES * C::QBYTES + r * 128;
+            float top = 0.0f;  // (an infinity or NaN makes the row's results NaN in any case)
+            float v[32];
+#pragma unroll 1
+            for (int c = 0; c < 2 * C::CH; c++) {
 #pragma unroll
-            for (int c = 0; c < C::CH; c++) {
+                for (int x = 0; x < 8; x++) lds_4(row + c * PR_ROWS * 128 + (x ^ (r & 7)) * 16, v + 4 * x);
 #pragma unroll
-                for (int x = 0; x < 16; x++) v[x] = *reinterpret_cast<float4*>(row + (2 * c + x / 8) * PR_ROWS * 128 + ((x & 7) ^ (r & 7)) * 16);
-#pragma unroll
-                for (int x = 0; x < 16; x++) top = fmaxf(top, finite_max(v[x]));
+                for (int x = 0; x < 32; x++) top = fmaxf(top, fabsf(v[x]));
             }
             const float f = to_range(top);
+            const f32x2 f2 = pack2(f, f), minus = pack2(-1.0f, -1.0f);
+#pragma unroll 1
+            for (int c = 0; c < 2 * C::CH; c++) {
 #pragma unroll
-            for (int c = 0; c < C::CH; c++) {
-                if (C::CH > 1) {
+                for (int x = 0; x < 8; x++) lds_4(row + c * PR_ROWS * 128 + (x ^ (r & 7)) * 16, v + 4 * x);
 #pragma unroll
-                    for (int x = 0; x < 16; x++) v[x] = *reinterpret_cast<float4*>(row + (2 * c + x / 8) * PR_ROWS * 128 + ((x & 7) ^ (r & 7)) * 16);
-                }
+                for (int x = 0; x < 4; x++) {  // eight values, 16 bytes of each part
+                    uint32_t hi[4], lo[4];
 #pragma unroll
-                for (int x = 0; x < 8; x++) {  // eight values, 16 bytes of each part
-                    uint2 h0, l0, h1, l1;
-                    split4(v[2 * x], f, h0, l0);
-                    split4(v[2 * x + 1], f, h1, l1);
-                    uint8_t* to = row + 2 * c * PR_ROWS * 128 + (x ^ (r & 7)) * 16;
-                    *reinterpret_cast<uint4*>(to) = make_uint4(h0.x, h0.y, h1.x, h1.y);
-                    *reinterpret_cast<uint4*>(to + PR_ROWS * 128) = make_uint4(l0.x, l0.y, l1.x, l1.y);
+                    for (int y = 0; y < 4; y++) {
+                        const f32x2 q2 = mul2(pack2(v[8 * x + 2 * y], v[8 * x + 2 * y + 1]), f2);
+                        float q0, q1, l0, l1;
+                        unpack2(q2, q0, q1);
+                        const float h0 = __uint_as_float(__float_as_uint(q0) & 0xFFFFE000u), h1 = __uint_as_float(__float_as_uint(q1) & 0xFFFFE000u);
+                        unpack2(fma2(pack2(h0, h1), minus, q2), l0, l1);
+                        hi[y] = pack16<T16>(h0, h1), lo[y] = pack16<T16>(l0, l1);
+                    }
+                    sts_4(row + c * PR_ROWS * 128 + (x ^ (r & 7)) * 16, hi);
+                    sts_4(row + c * PR_ROWS * 128 + ((x + 4) ^ (r & 7)) * 16, lo);
                 }
             }
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -702,7 +718,7 @@ k_attention_prompts(const __grid_constant__ CUtensorMap map_q, const __grid_cons
                     const int seen = limit - i * NK;
                     const bool masked = __any_sync(0xffffffffu, seen < NK);
                     float tops[4] = {NEG, NEG, NEG, NEG};
-#pragma unroll
+#pragma unroll 1
                     for (int c = 0; c < NK / 32; c++) {
                         float s[32];
                         tmem_ld32(t_s + 32 * c, s);
@@ -710,7 +726,7 @@ k_attention_prompts(const __grid_constant__ CUtensorMap map_q, const __grid_cons
                         if (masked) {
 #pragma unroll
                             for (int x = 0; x < 32; x++)
-                                if (32 * c + x >= seen) s[x] = NEG;
+                                if (x >= seen - 32 * c) s[x] = NEG;
                         }
 #pragma unroll
                         for (int x = 0; x < 32; x++) tops[x & 3] = fmaxf(tops[x & 3], s[x]);
@@ -724,7 +740,7 @@ k_attention_prompts(const __grid_constant__ CUtensorMap map_q, const __grid_cons
                     row_max = new_max;
                     const f32x2 base2 = pack2(base, base), scale2 = pack2(scale, scale), minus = pack2(-1.0f, -1.0f);
                     f32x2 sum[2] = {pack2(0.f, 0.f), pack2(0.f, 0.f)};
-#pragma unroll
+#pragma unroll 1
                     for (int c = 0; c < NK / 32; c++) {
                         float s[32];
                         tmem_ld32(t_s + 32 * c, s);
@@ -735,8 +751,8 @@ k_attention_prompts(const __grid_constant__ CUtensorMap map_q, const __grid_cons
                             float p0, p1, l0, l1;
                             unpack2(fma2(pack2(s[2 * x], s[2 * x + 1]), scale2, base2), p0, p1);
                             if (masked) {
-                                if (32 * c + 2 * x >= seen) p0 = NEG;
-                                if (32 * c + 2 * x + 1 >= seen) p1 = NEG;
+                                if (2 * x >= seen - 32 * c) p0 = NEG;
+                                if (2 * x + 1 >= seen - 32 * c) p1 = NEG;
                             }
                             const f32x2 p2 = pack2(p0 = exp2_approx(p0), p1 = exp2_approx(p1));
                             sum[x & 1] = add2(sum[x & 1], p2);
@@ -780,64 +796,66 @@ k_attention_prompts(const __grid_constant__ CUtensorMap map_q, const __grid_cons
             }
             ok = ok && __all_sync(0xffffffffu, bar_wait(sh, &sh->checked[k % PR_ITEMS], (k / PR_ITEMS) & 1));
 
-            // ── the rows: quotient, values that are not finite, rounding ─────
+            // ── the rows: quotient, rounding, values that are not finite ─────
             const float inv = limit > 0 ? __fdiv_rn(1.0f, row_sum) : 0.0f;
             T* out = reinterpret_cast<T*>(a.p.out) + ((size_t)(it->token0 + j) * a.p.n_heads + head) * hd;
-            uint32_t odd = 0;
-            for (int i = first_masked; i < nt; i++)
-                for (int w = 0; w < NK / 32; w++) odd |= it->mask[i - first_masked][w];
+            auto write_32 = [&](int c, float (&x)[32]) {
 #pragma unroll
-            for (int c = 0; c < HDP; c += 32) {
-                float x[32];
-                if (C::O_IN_TMEM) {
+                for (int d = 0; d < 32; d++) x[d] = limit > 0 ? __fmul_rn(x[d], inv) : 0.0f;
+                constexpr int V = 16 / (int)sizeof(T);
+#pragma unroll
+                for (int d = 0; d < 32; d += 2 * V) {
+                    uint32_t w[8];
+#pragma unroll
+                    for (int u = 0; u < 8; u++)
+                        if constexpr (sizeof(T) == 4)
+                            w[u] = __float_as_uint(x[d + u]);
+                        else
+                            w[u] = pack16<T>(x[d + 2 * u], x[d + 2 * u + 1]);
+                    T* to = out + c + d;
+                    // A row is a thread's: 32 bytes at a time are whole sectors
+                    if (a.wide_rows && c + d + 2 * V <= hd)
+                        asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(to), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]),
+                                     "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
+                                     : "memory");
+                    else {
+                        if (c + d < hd) *reinterpret_cast<uint4*>(to) = make_uint4(w[0], w[1], w[2], w[3]);
+                        if (c + d + V < hd) *reinterpret_cast<uint4*>(to + V) = make_uint4(w[4], w[5], w[6], w[7]);
+                    }
+                }
+            };
+            if constexpr (C::O_IN_TMEM) {
+#pragma unroll 1
+                for (int c = 0; c < HDP; c += 32) {
+                    float x[32];
                     if (n > 0) {  // (uniform in the warp)
                         tmem_ld32(t_o + c, x);
                         tmem_ld_wait();
                     }
-                } else {
+                    if (real && ok) write_32(c, x);
+                }
+            } else if (real && ok) {
+#pragma unroll
+                for (int c = 0; c < HDP; c += 32) {
+                    float x[32];
 #pragma unroll
                     for (int d = 0; d < 32; d++) x[d] = o[C::O_IN_TMEM ? 0 : c + d];
-                }
-#pragma unroll
-                for (int d = 0; d < 32; d++) x[d] = limit > 0 ? __fmul_rn(x[d], inv) : 0.0f;
-                if (odd)
-                    for (int i = first_masked; i < nt; i++)
-                        for (int w = 0; w < NK / 32; w++)
-                            for (uint32_t bits = it->mask[i - first_masked][w]; bits; bits &= bits - 1) {
-                                const int t = i * NK + w * 32 + __ffs(bits) - 1;
-                                if (t >= limit) continue;
-                                const T* v = reinterpret_cast<const T*>(a.p.v) + (size_t)(it->key0 + t) * a.p.v_stride + (size_t)it->kvh * hd;
-#pragma unroll
-                                for (int d = 0; d < 32; d++)
-                                    if (c + d < hd) {
-                                        const float y = to_f32(v[c + d]);
-                                        if (!(fabsf(y) <= 3.402823466e38f)) x[d] += y;
-                                    }
-                            }
-                if (real && ok) {
-                    constexpr int V = 16 / (int)sizeof(T);
-#pragma unroll
-                    for (int d = 0; d < 32; d += 2 * V) {
-                        uint32_t w[8];
-#pragma unroll
-                        for (int u = 0; u < 8; u++)
-                            if constexpr (sizeof(T) == 4)
-                                w[u] = __float_as_uint(x[d + u]);
-                            else
-                                w[u] = pack16<T>(x[d + 2 * u], x[d + 2 * u + 1]);
-                        T* to = out + c + d;
-                        // A row is a thread's: 32 bytes at a time are whole sectors (16 at a time took 8000 cycles for 256 rows of 256 bytes)
-                        if (a.wide_rows && c + d + 2 * V <= hd)
-                            asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(to), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]),
-                                         "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
-                                         : "memory");
-                        else {
-                            if (c + d < hd) *reinterpret_cast<uint4*>(to) = make_uint4(w[0], w[1], w[2], w[3]);
-                            if (c + d + V < hd) *reinterpret_cast<uint4*>(to + V) = make_uint4(w[4], w[5], w[6], w[7]);
-                        }
-                    }
+                    write_32(c, x);
                 }
             }
+            for (int i = first_masked; i < nt; i++)
+#pragma unroll 1
+                for (int w = 0; w < NK / 32; w++)
+                    for (uint32_t bits = it->mask[i - first_masked][w]; bits; bits &= bits - 1) {
+                        const int t = i * NK + w * 32 + __ffs(bits) - 1;
+                        if (t >= limit || !ok) continue;
+                        const T* v = reinterpret_cast<const T*>(a.p.v) + (size_t)(it->key0 + t) * a.p.v_stride + (size_t)it->kvh * hd;
+#pragma unroll 1
+                        for (int d = 0; d < hd; d++) {
+                            const float y = to_f32(v[d]);
+                            if (!(fabsf(y) <= 3.402823466e38f)) out[d] = from_f32<T>(__fadd_rn(to_f32(out[d]), y));
+                        }
+                    }
             tc_fence_before();  // (tensor memory has been read before the next P V, which waits for p_ready)
             done += n, items += n > 0 ? 1 : 0;
             leave_item(k);
