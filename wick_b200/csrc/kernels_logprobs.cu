@@ -1,14 +1,15 @@
 // Log probabilities of given tokens, with the entropy and the largest alternatives, over rows of logits x:
 //     m = max x,  S = sum exp(x - m),  T = sum exp(x - m) (x - m)
 //     log p(t) = (x_t - m) - log S,    H = -sum p log p = log S - T / S
-// One pass: every thread keeps a running (m, S, T) of its elements and rescales it when its maximum grows (S' = S e,
+// One pass: every thread keeps a running (m, S, T) of its elements, 32 at a time, and rescales it when its maximum grows (S' = S e,
 // T' = (T + S (m - m')) e with e = exp(m - m')); threads, then the CTAs of a row, are joined by the same rule.
 //
 // A cluster of 1 to 8 CTAs takes a row: as many as give every SM work (the rule in launch_token_logprobs), joined through
 // distributed shared memory, so that the call is one launch and needs no workspace.  Bound: the read of the logits.
 //
-// Alternatives: the top_n-th largest of the threads' maxima is a bound that top_n elements reach and few others do.  A second read
-// (the row is in L2 by then) collects what reaches it; candidates are ordered by counting, CTAs' lists are joined the same way.
+// Alternatives: from the threads' maxima follows a value that top_n elements reach and few others do.  What reaches it is collected, from
+// registers where the CTA's part of the row fits them and by a second read otherwise (L2 has it by then); candidates are ordered by counting, the
+// CTAs' lists are joined the same way.
 // Where ties make too many candidates (a vocabulary that is masked but for a few tokens), top_n rounds of "largest key below the
 // last one" follow instead.
 //
@@ -39,37 +40,78 @@ __device__ __forceinline__ uint32_t value_key(float x) {
 __device__ __forceinline__ float key_value(uint32_t k) { return __uint_as_float(k ^ ((k >> 31) ? 0x80000000u : 0xFFFFFFFFu)); }
 __device__ __forceinline__ unsigned long long full_key(float x, uint32_t i) { return ((unsigned long long)value_key(x) << 32) | (0xFFFFFFFFu - i); }
 
+constexpr float LOG2E = 1.44269504088896341f;
+__device__ __forceinline__ float exp2_approx(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ float max_nan(float a, float b, float c) {  // (NaN if one is)
+    float r;
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
+__device__ __forceinline__ float min_nan(float a, float b, float c) {
+    float r;
+    asm("min.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
+
+// A thread's running maximum and sums, and one step of them by N values: half an instruction each for the maximum, the minimum, the difference,
+// its product with log2 e and the two sums, one for the exponential.
 struct Running {
-    float m, s, t;
+    float m = -LP_BOUND;
+    f32x2 s = 0, t = 0;  // (two zeros)
     template <int N>
-    __device__ __forceinline__ void add(const float (&x)[N]) {
-        float top = m;
+    __device__ __forceinline__ void add(float (&x)[N]) {
+        static_assert(N == 1 || N % 2 == 0, "pairs");
+        float top = x[0], low = x[0];
 #pragma unroll
-        for (int i = 0; i < N; i++) top = fmaxf(top, x[i]);
+        for (int i = 1; i + 1 < N; i += 2) top = max_nan(top, x[i], x[i + 1]), low = min_nan(low, x[i], x[i + 1]);
+        if (N % 2 == 0) top = max_nan(top, top, x[N - 1]), low = min_nan(low, low, x[N - 1]);
+        if (!(top <= LP_BOUND && low >= -LP_BOUND)) {  // infinities, NaN
+            top = -LP_BOUND;
+#pragma unroll
+            for (int i = 0; i < N; i++) x[i] = held(x[i]), top = fmaxf(top, x[i]);
+        }
         if (top > m) {
-            const float d = __fsub_rn(m, top), e = expf(d);
-            t = __fmul_rn(fmaf(s, d, t), e);
-            s = __fmul_rn(s, e);
+            const float d = __fsub_rn(m, top), e = exp2_approx(__fmul_rn(d, LOG2E));
+            t = mul2(fma2(s, pack2(d, d), t), pack2(e, e));
+            s = mul2(s, pack2(e, e));
             m = top;
         }
+        if constexpr (N == 1) {
+            const float d = __fsub_rn(x[0], m), e = exp2_approx(__fmul_rn(d, LOG2E));
+            s = add2(s, pack2(e, 0.0f));
+            t = add2(t, pack2(__fmul_rn(e, d), 0.0f));
+        } else {
+            const f32x2 minus = pack2(-m, -m), log2e = pack2(LOG2E, LOG2E);
 #pragma unroll
-        for (int i = 0; i < N; i++) {
-            const float d = __fsub_rn(x[i], m), e = expf(d);
-            s = __fadd_rn(s, e);
-            t = fmaf(e, d, t);
+            for (int i = 0; i < N; i += 2) {
+                const f32x2 d = add2(pack2(x[i], x[i + 1]), minus);
+                float y0, y1;
+                unpack2(mul2(d, log2e), y0, y1);
+                const f32x2 e = pack2(exp2_approx(y0), exp2_approx(y1));
+                s = add2(s, e);
+                t = fma2(e, d, t);
+            }
         }
     }
 };
 struct Joined {
     double s, t;
     float m;
-    __device__ __forceinline__ void join(float m2, double s2, double t2) {
-        const float top = fmaxf(m, m2);
-        const double d1 = (double)m - top, d2 = (double)m2 - top;
-        const double e1 = d1 == 0.0 ? 1.0 : (double)expf((float)d1), e2 = d2 == 0.0 ? 1.0 : (double)expf((float)d2);
-        t = (s > 0.0 ? (t + s * d1) * e1 : 0.0) + (s2 > 0.0 ? (t2 + s2 * d2) * e2 : 0.0);
-        s = s * e1 + s2 * e2;
+    // The join of the 32 lanes' sums, in a fixed order, in every lane.
+    __device__ __forceinline__ void over_lanes() {
+        float top = m;
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+        const double d = (double)m - (double)top, f = m == top ? 1.0 : (double)exp2_approx(__fmul_rn(__fsub_rn(m, top), LOG2E));
+        t = s > 0.0 ? (t + s * d) * f : 0.0;
+        s *= f;
         m = top;
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o), t += __shfl_xor_sync(0xffffffffu, t, o);
     }
 };
 
@@ -88,8 +130,6 @@ struct Slice {  // the part of a row that a CTA reads: 16-byte pieces [v0, v1), 
     __device__ __forceinline__ int index(int vec) const { return head + vec * V; }
     __device__ __forceinline__ void load(int vec, float (&x)[V]) const {
         unpack16(__ldg(reinterpret_cast<const uint4*>(row + head) + vec), x, (const T*)nullptr);
-#pragma unroll
-        for (int i = 0; i < V; i++) x[i] = held(x[i]);
     }
     // The at most one single element of this thread (a head or tail is shorter than 16 elements): its index or -1.
     __device__ __forceinline__ int single() const {
@@ -97,10 +137,12 @@ struct Slice {  // the part of a row that a CTA reads: 16-byte pieces [v0, v1), 
         if (i < head1) return i;
         return i - head1 < tail1 - tail0 ? tail0 + i - head1 : -1;
     }
-    __device__ __forceinline__ float at(int i) const { return held(to_f32(row[i])); }
+    __device__ __forceinline__ float at(int i) const { return to_f32(row[i]); }
 };
 
-template <class T>
+// HELD: the CTA's part of the row stays in registers (at most LP_HELD elements per thread), and is not read a second time for the alternatives.
+constexpr int LP_HELD = 32;
+template <class T, bool HELD>
 __global__ void __launch_bounds__(LP_THREADS) k_token_logprobs(const T* __restrict__ logits, size_t row_stride, int vocab,
                                                                const int32_t* __restrict__ tokens, int top_n, float* __restrict__ logprob,
                                                                float* __restrict__ entropy, int32_t* __restrict__ top_ids,
@@ -111,73 +153,117 @@ __global__ void __launch_bounds__(LP_THREADS) k_token_logprobs(const T* __restri
     __shared__ Joined part;                              // the CTA's, read by the row's first CTA
     __shared__ unsigned long long best[LOGPROBS_MAX_TOP];  // the CTA's top_n keys, descending
     __shared__ unsigned long long cand[LP_CAND];
-    __shared__ uint32_t sh_key[LP_THREADS];
     __shared__ int n_cand;
-    __shared__ uint32_t sh_floor;
+    __shared__ uint32_t sh_floor[LP_WARPS];
     cg::cluster_group cluster = cg::this_cluster();
     const int ctas = (int)cluster.num_blocks(), rank = (int)cluster.block_rank(), row = blockIdx.x / ctas;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const Slice<T> sl(logits + (size_t)row * row_stride, vocab, rank, ctas);
-    constexpr int V = Slice<T>::V;
+    constexpr int V = Slice<T>::V, AT_ONCE = LP_HELD / V;  // elements of a load; loads that are under way together
 
-    Running r{-LP_BOUND, 0.0f, 0.0f};
+    Running r;
     const int one = sl.single();
+    float x_one[1] = {-LP_BOUND};
     if (one >= 0) {
-        const float x[1] = {sl.at(one)};
+        x_one[0] = sl.at(one);
+        r.add(x_one);
+    }
+    float x[LP_HELD];
+    if constexpr (HELD) {
+#pragma unroll
+        for (int u = 0; u < AT_ONCE; u++) {
+            const int v = sl.v0 + tid + u * LP_THREADS;
+            float y[V];
+#pragma unroll
+            for (int i = 0; i < V; i++) y[i] = -LP_BOUND;
+            if (v < sl.v1) sl.load(v, y);
+#pragma unroll
+            for (int i = 0; i < V; i++) x[u * V + i] = y[i];
+        }
         r.add(x);
-    }
-    int v = sl.v0 + tid;
-    for (; v + 3 * LP_THREADS < sl.v1; v += 4 * LP_THREADS) {
-        float x[4][V];
+    } else {
+        int v = sl.v0 + tid;
+        for (; v + (AT_ONCE - 1) * LP_THREADS < sl.v1; v += AT_ONCE * LP_THREADS) {
 #pragma unroll
-        for (int u = 0; u < 4; u++) sl.load(v + u * LP_THREADS, x[u]);
+            for (int u = 0; u < AT_ONCE; u++) {
+                float y[V];
+                sl.load(v + u * LP_THREADS, y);
 #pragma unroll
-        for (int u = 0; u < 4; u++) r.add(x[u]);
+                for (int i = 0; i < V; i++) x[u * V + i] = y[i];
+            }
+            r.add(x);
+        }
+        for (; v < sl.v1; v += LP_THREADS) {
+            float y[V];
+            sl.load(v, y);
+            r.add(y);
+        }
     }
-    for (; v < sl.v1; v += LP_THREADS) {
-        float x[V];
-        sl.load(v, x);
-        r.add(x);
+    const uint32_t mine = value_key(r.m);
+    Joined j;
+    {
+        float s0, s1, t0, t1;
+        unpack2(r.s, s0, s1);
+        unpack2(r.t, t0, t1);
+        j.s = (double)s0 + s1, j.t = (double)t0 + t1, j.m = r.m;
     }
-    const float thread_max = r.m;
-    Joined j{(double)r.s, (double)r.t, r.m};
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-        const float m2 = __shfl_xor_sync(0xffffffffu, j.m, o);
-        const double s2 = __shfl_xor_sync(0xffffffffu, j.s, o), t2 = __shfl_xor_sync(0xffffffffu, j.t, o);
-        j.join(m2, s2, t2);
-    }
+    j.over_lanes();
     if (lane == 0) sh_m[warp] = j.m, sh_s[warp] = j.s, sh_t[warp] = j.t;
     if (tid == 0) n_cand = 0;
-    sh_key[tid] = value_key(thread_max);
+    if (top_n > 0) {
+        // A value that top_n elements of the CTA reach: every warp has k = top_n / 8 (upwards) threads whose maxima do, if it is the smallest
+        // of the warps' k-th largest maxima.
+        uint32_t left = mine;
+        uint32_t kth = 0;
+        for (int k = 0; k < top_n; k += LP_WARPS) {
+            kth = __reduce_max_sync(0xffffffffu, left);
+            const uint32_t at = __ballot_sync(0xffffffffu, left == kth);
+            if (lane == __ffs(at) - 1) left = 0;
+        }
+        if (lane == 0) sh_floor[warp] = kth;
+    }
     __syncthreads();
-    if (tid == 0) {
-        for (int w = 1; w < LP_WARPS; w++) j.join(sh_m[w], sh_s[w], sh_t[w]);
-        part = j;
+    if (warp == 0) {
+        j.m = lane < LP_WARPS ? sh_m[lane] : -LP_BOUND, j.s = lane < LP_WARPS ? sh_s[lane] : 0.0, j.t = lane < LP_WARPS ? sh_t[lane] : 0.0;
+        j.over_lanes();
+        if (lane == 0) part = j;
     }
 
     if (top_n > 0) {
-        // the top_n-th largest of the threads' maxima, equal ones in thread order
-        const uint32_t mine = sh_key[tid];
-        int above = 0;
-        for (int i = 0; i < LP_THREADS; i++) above += sh_key[i] > mine || (sh_key[i] == mine && i < tid);
-        if (above == top_n - 1) sh_floor = mine;
         if (tid < top_n) best[tid] = 0;
-        __syncthreads();
-        const uint32_t floor_key = sh_floor;
+        uint32_t floor_key = 0xFFFFFFFFu;
+#pragma unroll
+        for (int w = 0; w < LP_WARPS; w++) floor_key = min(floor_key, sh_floor[w]);
+        const float floor_value = key_value(floor_key);
         auto offer = [&](float x, int i) {
-            if (value_key(x) >= floor_key) {
+            if (x >= floor_value) {
                 const int at = atomicAdd(&n_cand, 1);
                 if (at < LP_CAND) cand[at] = full_key(x, (uint32_t)i);
             }
         };
         if (mine >= floor_key) {  // (threads whose maximum lies below have nothing to offer)
-            if (one >= 0) offer(sl.at(one), one);
-            for (int u = sl.v0 + tid; u < sl.v1; u += LP_THREADS) {
-                float x[V];
-                sl.load(u, x);
+            if (one >= 0) offer(held(x_one[0]), one);
+            if constexpr (HELD) {
 #pragma unroll
-                for (int i = 0; i < V; i++) offer(x[i], sl.index(u) + i);
+                for (int u = 0; u < AT_ONCE; u++) {
+                    const int v = sl.v0 + tid + u * LP_THREADS;
+                    if (v < sl.v1) {
+#pragma unroll
+                        for (int i = 0; i < V; i++) offer(x[u * V + i], sl.index(v) + i);
+                    }
+                }
+            } else {
+                for (int v = sl.v0 + tid; v < sl.v1; v += 4 * LP_THREADS) {
+                    float y[4][V];
+#pragma unroll
+                    for (int u = 0; u < 4; u++) sl.load(min(v + u * LP_THREADS, sl.v1 - 1), y[u]);
+#pragma unroll
+                    for (int u = 0; u < 4; u++)
+                        if (v + u * LP_THREADS < sl.v1) {
+#pragma unroll
+                            for (int i = 0; i < V; i++) offer(held(y[u][i]), sl.index(v + u * LP_THREADS) + i);
+                        }
+                }
             }
         }
         __syncthreads();
@@ -197,12 +283,12 @@ __global__ void __launch_bounds__(LP_THREADS) k_token_logprobs(const T* __restri
                     const unsigned long long k = full_key(x, (uint32_t)i);
                     if (k < last && k > top) top = k;
                 };
-                if (one >= 0) look(sl.at(one), one);
+                if (one >= 0) look(held(x_one[0]), one);
                 for (int u = sl.v0 + tid; u < sl.v1; u += LP_THREADS) {
-                    float x[V];
-                    sl.load(u, x);
+                    float y[V];
+                    sl.load(u, y);
 #pragma unroll
-                    for (int i = 0; i < V; i++) look(x[i], sl.index(u) + i);
+                    for (int i = 0; i < V; i++) look(held(y[i]), sl.index(u) + i);
                 }
 #pragma unroll
                 for (int o = 16; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
@@ -218,11 +304,12 @@ __global__ void __launch_bounds__(LP_THREADS) k_token_logprobs(const T* __restri
     __syncthreads();
     if (ctas > 1) cluster.sync();
     if (rank == 0) {
-        if (tid == 0) {
-            for (int c = 1; c < ctas; c++) {
-                const Joined* o = cluster.map_shared_rank(&part, c);
-                part.join(o->m, o->s, o->t);
-            }
+        if (ctas > 1 && warp == 0) {
+            const Joined* o = cluster.map_shared_rank(&part, lane < ctas ? lane : 0);
+            j.m = lane < ctas ? o->m : -LP_BOUND, j.s = lane < ctas ? o->s : 0.0, j.t = lane < ctas ? o->t : 0.0;
+            j.over_lanes();
+            __syncwarp();
+            if (lane == 0) part = j;
         }
         if (top_n > 0 && ctas > 1) {
             // lists of keys that differ from one another: the place in the whole is the number of larger ones
@@ -238,7 +325,7 @@ __global__ void __launch_bounds__(LP_THREADS) k_token_logprobs(const T* __restri
         };
         if (tid == 0) {
             const int t = tokens[row];
-            logprob[row] = t >= 0 && t < vocab ? log_p(sl.at(t)) : ninf;
+            logprob[row] = t >= 0 && t < vocab ? log_p(held(sl.at(t))) : ninf;
             entropy[row] = none ? 0.0f : (float)(lse - part.t / part.s);
         }
         if (top_n > 0) {
@@ -280,8 +367,10 @@ cudaError_t launch_typed(cudaStream_t st, const void* logits, size_t row_stride,
     cfg.attrs = attr;
     cfg.numAttrs = 2;
     g_kernel_launches++;
-    return cudaLaunchKernelEx(&cfg, k_token_logprobs<T>, static_cast<const T*>(logits), row_stride, vocab, tokens, top_n, logprob, entropy, top_ids,
-                              top_logprobs);
+    const int loads = vocab / (16 / (int)sizeof(T));
+    const bool held = (loads + ctas - 1) / ctas <= LP_HELD / (16 / (int)sizeof(T)) * LP_THREADS;
+    return cudaLaunchKernelEx(&cfg, held ? k_token_logprobs<T, true> : k_token_logprobs<T, false>, static_cast<const T*>(logits), row_stride, vocab,
+                              tokens, top_n, logprob, entropy, top_ids, top_logprobs);
 }
 
 }  // namespace
