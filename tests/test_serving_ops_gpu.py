@@ -114,6 +114,42 @@ def test_attention_prompts_long(ops, dtype):
     _check(out, ref, tol, v.abs().max().double())
 
 
+SPLIT = [  # few tokens, many keys: the keys of a block are cut into parts
+    (4, 2, 64, [200, 3, 90], [3000, 2500, 4000]),
+    (8, 8, 128, [70, 300], [2000, 3333]),
+    (2, 1, 64, [2600], [0]),
+    (6, 2, 96, [1, 1, 0, 1], [5000, 1, 7, 6001]),
+    (5, 1, 32, [64, 1], [6100, 900]),
+]
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("shape", SPLIT, ids=str)
+def test_attention_prompts_in_parts(ops, dtype, shape):
+    heads, kv, hd, nq, prefix = shape
+    nk = [n + p for n, p in zip(nq, prefix)]
+    g = _gen(sum(nk))
+    q, k, v = _randn(g, sum(nq), heads * hd).to(dtype), _randn(g, sum(nk), kv * hd).to(dtype), (_randn(g, sum(nk), kv * hd) + 0.3).to(dtype)
+    starts, key_starts = _starts(nq), _starts(nk) if any(prefix) else None
+    out = ops.attention_prompts(q, k, v, starts, heads, kv, hd, key_starts=key_starts)
+    ref, tol = _prompts_ref(q, k, v, nq, nk, heads, kv, hd)
+    _check(out, ref, tol, v.abs().max().double())
+    # a value that only the last token of the first sequence attends, one that all of its tokens do, and padding behind the sequences
+    v2 = v.clone()
+    v2[nk[0] - 1, 1] = math.inf
+    v2[0, 2] = math.nan
+    pad = torch.full((9, kv * hd), math.nan, dtype=dtype, device="cuda")
+    out2 = torch.full((sum(nq) + 5, heads * hd), 7.0, dtype=dtype, device="cuda")
+    ops.attention_prompts(torch.cat([q, q[:5].expand(5, -1) if nq[0] > 5 else q[:1].expand(5, -1)]), torch.cat([k, pad]), torch.cat([v2, pad]), starts, heads, kv, hd,
+                          key_starts=key_starts if key_starts is not None else starts, out=out2)
+    hit = torch.zeros_like(out, dtype=torch.bool).view(-1, heads, hd)
+    hit[nq[0] - 1, :heads // kv, 1] = True
+    hit[:nq[0], :heads // kv, 2] = True
+    hit = hit.flatten(1)
+    assert (out2[sum(nq):] == 7).all() and torch.equal(out2[:sum(nq)][~hit], out[~hit])
+    assert not torch.isfinite(out2[:sum(nq)][hit]).any()
+
+
 @pytest.mark.parametrize("dtype", TYPES, ids=str)
 def test_attention_prompts_fewer_keys_than_tokens(ops, dtype):
     """Tokens that have no key get zeros; a sequence without any keys, one without tokens."""

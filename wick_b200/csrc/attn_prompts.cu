@@ -15,12 +15,16 @@
 //   (K and V by k_split; a row of Q where it lies in shared memory, by the thread that owns it), and a product is hi hi + hi lo + lo hi (lo lo is 2^-22 of it).  The tensor core adds with truncation, so that a sum over
 //   thousands of keys would drift by 1e-5: O is taken out after every tile and added up in registers.
 //
+// Few items with many keys (a chunk of tokens behind a long prefix): the keys of an item are cut into `splits` parts, each an item of its own,
+// whose sums go to the workspace in f32 and are joined by k_join.
+//
 // Masked places may hold anything.  Scores are masked after the product; V is different, 0 * NaN is NaN: a warp looks at every V
 // tile that some row sees in part, zeroes what is not finite, and notes the keys; rows that attend such a key add its values at the end.
 //
 // Every wait is bounded: on expiry all roles leave their loops and all rows of the CTA's items become NaN.
 #include <cuda.h>
 #include <algorithm>
+#include <cmath>
 #include <mutex>
 
 #include "serving.cuh"
@@ -33,7 +37,7 @@ constexpr int PR_ROWS = 128;      // rows of a tile == lanes of tensor memory
 constexpr int PR_THREADS = 384;   // TMA, MMA, V check, items; 2 x 4 softmax warps
 constexpr int PR_ITEMS = 3;       // items that are known ahead
 constexpr int PR_MASKED = 8;      // tiles that some row of a CTA sees in part: at most 256 / 64 + 2
-constexpr uint32_t PR_SPIN_LIMIT = 1u << 18;  // try_wait suspends for a while: of the order of a second
+constexpr uint32_t PR_SPIN_LIMIT = 1u << 24;  // about half a second (2^18: 8 ms)
 constexpr float PR_LAZY = 8.0f;
 
 template <int PLANES, int HDP>
@@ -58,6 +62,7 @@ struct Item {
     int key0, keys;       // first key (a row of k), keys of the sequence
     int first_visible;    // keys that the first token attends (may be negative)
     int key_slot0, kvh;   // place of the sequence's first key tile; KV head (-1: no more items)
+    int part;             // of the block's keys
     int n_tiles[2];       // tiles of keys that the two row tiles see
     uint32_t mask[PR_MASKED][4];  // keys of the tiles from first_masked() on whose values are not finite
     __device__ __forceinline__ int visible(int j) const { return max(0, min(first_visible + j, keys)); }
@@ -80,6 +85,8 @@ struct PromptArgs {
     const float *k_inv, *v_inv;          // f32: the powers of two taken out of K / V tiles
     int group, tile_tokens;              // query heads per KV head, tokens of a row tile
     int slots;                           // places for (sequence, block of 2 * tile_tokens tokens)
+    int splits;                          // parts of a block's keys, and where their rows' sums go: [splits][tokens][heads][head_dim], [..][2]
+    float *part_o, *part_ml;
     int zero_rest;
     int wide_rows;                       // rows of out start on 32-byte boundaries
     float scale_log2;
@@ -244,20 +251,58 @@ __device__ __forceinline__ void split4(float4 v, float f, uint2& hi, uint2& lo) 
 __device__ __forceinline__ float finite_abs(float x) { return fabsf(x) <= 3.402823466e38f ? fabsf(x) : 0.0f; }
 __device__ __forceinline__ float finite_max(float4 v) { return fmaxf(fmaxf(finite_abs(v.x), finite_abs(v.y)), fmaxf(finite_abs(v.z), finite_abs(v.w))); }
 
-// Place idx of the list, by a whole warp; false: there is nothing there.  The last places come first, since a sequence's last blocks have the
-// most keys and the launch then ends with short ones.
+// The blocks of 2 * tile_tokens tokens, counted through the sequences, by a whole warp: how many there are (want < 0), or which sequence has number
+// `want` and which of its blocks that is (*seq -1: none).  With more sequences than a warp can walk through for every item, numbers are
+// places as of find_seq, not all of which have a block.
+constexpr int PR_WALK = 1024;
+__device__ __forceinline__ int count_blocks(const PromptArgs& a, int want, int* seq, int* at) {
+    const int block = 2 * a.tile_tokens, lane = threadIdx.x & 31;
+    *seq = -1, *at = 0;
+    if (a.p.n_seqs > PR_WALK) {
+        if (want < 0) return a.slots;
+        *seq = find_seq(a.p.starts, a.p.n_seqs, a.p.n_tokens, block, want);
+        if (*seq >= 0) *at = want - (max(0, min(a.p.starts[*seq], a.p.n_tokens)) / block + *seq);
+        return a.slots;
+    }
+    int before = 0;
+    for (int s0 = 0; s0 < a.p.n_seqs; s0 += 32) {
+        const int s = s0 + lane;
+        int n = 0;
+        if (s < a.p.n_seqs) {
+            const int q0 = max(0, min(a.p.starts[s], a.p.n_tokens)), q1 = max(q0, min(a.p.starts[s + 1], a.p.n_tokens));
+            n = (q1 - q0 + block - 1) / block;
+        }
+        int upto = n;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int v = __shfl_up_sync(0xffffffffu, upto, o);
+            if (lane >= o) upto += v;
+        }
+        const uint32_t past = __ballot_sync(0xffffffffu, want >= 0 && before + upto > want);
+        if (past) {
+            const int l = __ffs(past) - 1;
+            *seq = s0 + l;
+            *at = want - before - __shfl_sync(0xffffffffu, upto - n, l);
+            return 0;
+        }
+        before += __shfl_sync(0xffffffffu, upto, 31);
+    }
+    return before;
+}
+
+// A block of tokens with all its keys, by a whole warp; false: there is none of this number.
 template <int NK>
-__device__ __forceinline__ bool make_item(const PromptArgs& a, int idx, Item& it) {
-    const int block = 2 * a.tile_tokens, slot = a.slots - 1 - idx / a.p.n_kv;
-    const int seq = find_seq(a.p.starts, a.p.n_seqs, a.p.n_tokens, block, slot);
+__device__ __forceinline__ bool find_block(const PromptArgs& a, int number, Item& it) {
+    const int block = 2 * a.tile_tokens;
+    int seq, blk;
+    count_blocks(a, number, &seq, &blk);
     if (seq < 0) return false;
     const int32_t* ks = a.p.key_starts ? a.p.key_starts : a.p.starts;
     const int s0 = a.p.starts[seq], s1 = a.p.starts[seq + 1], t0 = ks[seq], t1 = ks[seq + 1];
     const int q0 = max(0, min(s0, a.p.n_tokens)), q1 = max(q0, min(s1, a.p.n_tokens));
     const int k0 = max(0, min(t0, a.p.n_keys)), k1 = max(k0, min(t1, a.p.n_keys));
-    const int at = (slot - (q0 / block + seq)) * block;
+    const int at = blk * block;
     if (at >= q1 - q0) return false;
-    it.kvh = idx % a.p.n_kv;
     it.token0 = q0 + at;
     it.tokens = min(block, q1 - it.token0);
     it.key0 = k0, it.keys = k1 - k0;
@@ -267,6 +312,24 @@ __device__ __forceinline__ bool make_item(const PromptArgs& a, int idx, Item& it
     for (int m = 0; m < 2; m++) {
         const int rows = min(a.tile_tokens, it.tokens - m * a.tile_tokens);
         it.n_tiles[m] = rows > 0 ? (it.visible(m * a.tile_tokens + rows - 1) + NK - 1) / NK : 0;
+    }
+    return true;
+}
+// Where part `part` of nt tiles begins: equal parts, and what has no tiles is the first one's.
+__device__ __forceinline__ int part_begin(int nt, int part, int splits) { return (int)((long long)nt * part / splits); }
+// Place idx of the list.  The last places come first, since a sequence's last blocks have the most keys and the launch then ends with short ones.
+template <int NK>
+__device__ __forceinline__ bool make_item(const PromptArgs& a, int blocks, int idx, Item& it) {
+    const int part = idx % a.splits, place = idx / a.splits;
+    if (!find_block<NK>(a, blocks - 1 - place / a.p.n_kv, it)) return false;
+    it.kvh = place % a.p.n_kv;
+    it.part = part;
+    if (a.splits > 1) {  // the sequence as this part sees it: its keys begin at the part's first tile
+        const int nt = it.nt(), t0 = part_begin(nt, part, a.splits), t1 = part_begin(nt, part + 1, a.splits);
+        if (t0 == t1 && (nt > 0 || part > 0)) return false;
+        it.key0 += t0 * NK, it.keys -= t0 * NK, it.first_visible -= t0 * NK, it.key_slot0 += t0;
+#pragma unroll
+        for (int m = 0; m < 2; m++) it.n_tiles[m] = max(0, min(it.n_tiles[m], t1) - t0);
     }
     return true;
 }
@@ -324,17 +387,18 @@ k_attention_prompts(const __grid_constant__ CUtensorMap map_q, const __grid_cons
         asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
         if (warp == 3) {
         // ── items ────────────────────────────────────────────────────────────
-        const int total = a.slots * a.p.n_kv;
+        int unused;
+        const int blocks = count_blocks(a, -1, &unused, &unused), total = blocks * a.p.n_kv * a.splits;
         uint32_t k = 0;
         for (int idx = blockIdx.x;; idx += gridDim.x) {
             Item it;
             it.kvh = -1;
-            if (idx < total && !make_item<NK>(a, idx, it)) continue;
+            if (idx < total && !make_item<NK>(a, blocks, idx, it)) continue;
             if (!__all_sync(0xffffffffu, bar_wait(sh, &sh->item_empty[k % PR_ITEMS], ((k / PR_ITEMS) & 1) ^ 1))) break;
             if (lane == 0) {
                 Item* to = &sh->item[k % PR_ITEMS];
                 to->token0 = it.token0, to->tokens = it.tokens, to->key0 = it.key0, to->keys = it.keys, to->first_visible = it.first_visible;
-                to->key_slot0 = it.key_slot0, to->kvh = it.kvh, to->n_tiles[0] = it.n_tiles[0], to->n_tiles[1] = it.n_tiles[1];
+                to->key_slot0 = it.key_slot0, to->kvh = it.kvh, to->part = it.part, to->n_tiles[0] = it.n_tiles[0], to->n_tiles[1] = it.n_tiles[1];
                 bar_arrive(&sh->item_full[k % PR_ITEMS]);
             }
             __syncwarp();
@@ -506,8 +570,11 @@ k_attention_prompts(const __grid_constant__ CUtensorMap map_q, const __grid_cons
             Item* notes = &sh->item[k % PR_ITEMS];
             const int nt = it->nt(), first_masked = it->template first_masked<NK>();
             for (int i = 0; i < nt; i++) {
+                // Every use of a slot is waited for, K's too: with an odd number of slots a slot has K and V in turn, and a wait for V that came
+                // before its K had landed would see the phase before that as its own.
                 const uint32_t g = g0 + 2 * i + 1, s = g % NS;
-                if (!(ok = __all_sync(0xffffffffu, bar_wait(sh, &sh->full[s], (g / NS) & 1)))) break;
+                ok = bar_wait(sh, &sh->full[(g - 1) % NS], ((g - 1) / NS) & 1) && bar_wait(sh, &sh->full[s], (g / NS) & 1);
+                if (!(ok = __all_sync(0xffffffffu, ok))) break;
                 if (i >= first_masked) {
                     uint8_t* tile = sm + 2 * PLANES * C::QBYTES + s * C::SLOT;
                     uint32_t found[4] = {0, 0, 0, 0};
@@ -798,8 +865,24 @@ k_attention_prompts(const __grid_constant__ CUtensorMap map_q, const __grid_cons
 
             // ── the rows: quotient, rounding, values that are not finite ─────
             const float inv = limit > 0 ? __fdiv_rn(1.0f, row_sum) : 0.0f;
-            T* out = reinterpret_cast<T*>(a.p.out) + ((size_t)(it->token0 + j) * a.p.n_heads + head) * hd;
+            const size_t out_row = (size_t)(it->token0 + j) * a.p.n_heads + head, part_row = (size_t)it->part * a.p.n_tokens * a.p.n_heads + out_row;
+            T* out = reinterpret_cast<T*>(a.p.out) + out_row * hd;
+            float* sums = a.part_o + part_row * hd;
+            const bool split = a.splits > 1;
+            if (split && real && ok) *reinterpret_cast<float2*>(a.part_ml + part_row * 2) = make_float2(limit > 0 ? row_max : NEG, limit > 0 ? row_sum : 0.0f);
             auto write_32 = [&](int c, float (&x)[32]) {
+                if (split) {
+#pragma unroll
+                    for (int d = 0; d < 32; d += 8)  // (head_dim is a multiple of 8: rows start on 32-byte boundaries)
+                        if (c + d < hd) {
+#pragma unroll
+                            for (int u = 0; u < 8; u++) x[d + u] = limit > 0 ? x[d + u] : 0.0f;
+                            asm volatile("st.global.v8.f32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(sums + c + d), "f"(x[d]), "f"(x[d + 1]), "f"(x[d + 2]),
+                                         "f"(x[d + 3]), "f"(x[d + 4]), "f"(x[d + 5]), "f"(x[d + 6]), "f"(x[d + 7])
+                                         : "memory");
+                        }
+                    return;
+                }
 #pragma unroll
                 for (int d = 0; d < 32; d++) x[d] = limit > 0 ? __fmul_rn(x[d], inv) : 0.0f;
                 constexpr int V = 16 / (int)sizeof(T);
@@ -853,7 +936,11 @@ k_attention_prompts(const __grid_constant__ CUtensorMap map_q, const __grid_cons
 #pragma unroll 1
                         for (int d = 0; d < hd; d++) {
                             const float y = to_f32(v[d]);
-                            if (!(fabsf(y) <= 3.402823466e38f)) out[d] = from_f32<T>(__fadd_rn(to_f32(out[d]), y));
+                            if (fabsf(y) <= 3.402823466e38f) continue;
+                            if (split)
+                                sums[d] = __fadd_rn(sums[d], y);
+                            else
+                                out[d] = from_f32<T>(__fadd_rn(to_f32(out[d]), y));
                         }
                     }
             tc_fence_before();  // (tensor memory has been read before the next P V, which waits for p_ready)
@@ -867,12 +954,18 @@ k_attention_prompts(const __grid_constant__ CUtensorMap map_q, const __grid_cons
     if (warp == 1) {
         if (sh->abort) {
             for (int i = 0; i < 64; i++) __nanosleep(1000);  // copies issued before the failure may still be landing
-            for (int idx = blockIdx.x; idx < a.slots * a.p.n_kv; idx += gridDim.x) {  // no row is left without a sign of it
+            int unused;
+            const int blocks = count_blocks(a, -1, &unused, &unused);
+            for (int idx = blockIdx.x; idx < blocks * a.p.n_kv * a.splits; idx += gridDim.x) {  // no row is left without a sign of it
                 Item it;
-                if (!make_item<NK>(a, idx, it)) continue;
-                for (int i = lane; i < it.tokens * a.group * hd; i += 32)
-                    reinterpret_cast<T*>(a.p.out)[((size_t)(it.token0 + i / (a.group * hd)) * a.p.n_heads + it.kvh * a.group) * hd + i % (a.group * hd)] =
-                        from_f32<T>(__int_as_float(0x7FC00000));
+                if (!make_item<NK>(a, blocks, idx, it)) continue;
+                for (int i = lane; i < it.tokens * a.group * hd; i += 32) {
+                    const size_t row = (size_t)(it.token0 + i / (a.group * hd)) * a.p.n_heads + it.kvh * a.group + i % (a.group * hd) / hd;
+                    if (a.splits > 1)
+                        a.part_ml[((size_t)it.part * a.p.n_tokens * a.p.n_heads + row) * 2 + 1] = __int_as_float(0x7FC00000);
+                    else
+                        reinterpret_cast<T*>(a.p.out)[row * hd + i % hd] = from_f32<T>(__int_as_float(0x7FC00000));
+                }
             }
         }
         tc_fence_after();
@@ -938,6 +1031,52 @@ __global__ void __launch_bounds__(SP_THREADS) k_split(const __grid_constant__ Sp
     if (threadIdx.x == 0) a.inv[val][(size_t)slot * a.p.n_kv + kvh] = __fdiv_rn(1.0f, f);
 }
 
+// The parts of a block's keys, added up in their order: four values of a row per thread, all parts' loads under way together.
+constexpr int JOIN_THREADS = 256, JOIN_CTAS = 8, MAX_SPLITS = 8;  // CTAs of a block
+template <class T, int NK>
+__global__ void __launch_bounds__(JOIN_THREADS) k_join(const __grid_constant__ PromptArgs a) {
+    pdl_trigger();
+    pdl_wait();
+    Item it;
+    if (!find_block<NK>(a, blockIdx.x / a.p.n_kv, it)) return;
+    const int kvh = blockIdx.x % a.p.n_kv, hd = a.p.head_dim, pieces = hd / 4, nt = it.nt();
+    const size_t rows = (size_t)a.p.n_tokens * a.p.n_heads;
+    uint32_t there = 0;  // the parts that have tiles
+    for (int s = 0; s < a.splits; s++) there |= part_begin(nt, s, a.splits) < part_begin(nt, s + 1, a.splits) ? 1u << s : 0u;
+    for (int i = blockIdx.y * JOIN_THREADS + threadIdx.x; i < it.tokens * a.group * pieces; i += JOIN_CTAS * JOIN_THREADS) {
+        const int r = i / pieces, d = i % pieces * 4;
+        const size_t row = (size_t)(it.token0 + r / a.group) * a.p.n_heads + kvh * a.group + r % a.group;
+        float2 ml[MAX_SPLITS];
+        float4 x[MAX_SPLITS];
+        float m = __int_as_float(0xFF800000);
+#pragma unroll
+        for (int s = 0; s < MAX_SPLITS; s++) {
+            ml[s] = make_float2(m, 0.0f), x[s] = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (there >> s & 1) {
+                ml[s] = *reinterpret_cast<const float2*>(a.part_ml + (s * rows + row) * 2);
+                x[s] = *reinterpret_cast<const float4*>(a.part_o + (s * rows + row) * hd + d);
+            }
+        }
+#pragma unroll
+        for (int s = 0; s < MAX_SPLITS; s++) m = fmaxf(m, ml[s].x);
+        float l = 0.0f;
+        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int s = 0; s < MAX_SPLITS; s++)
+            if (there >> s & 1) {
+                const float f = ml[s].x == m ? 1.0f : exp2_approx(ml[s].x - m);
+                l = fmaf(ml[s].y, f, l);
+                o.x = fmaf(x[s].x, f, o.x), o.y = fmaf(x[s].y, f, o.y), o.z = fmaf(x[s].z, f, o.z), o.w = fmaf(x[s].w, f, o.w);
+            }
+        const float inv = l == 0.0f ? 0.0f : __fdiv_rn(1.0f, l);
+        T* out = reinterpret_cast<T*>(a.p.out) + row * hd + d;
+        if constexpr (sizeof(T) == 4)
+            *reinterpret_cast<float4*>(out) = make_float4(__fmul_rn(o.x, inv), __fmul_rn(o.y, inv), __fmul_rn(o.z, inv), __fmul_rn(o.w, inv));
+        else
+            *reinterpret_cast<uint2*>(out) = make_uint2(pack16<T>(__fmul_rn(o.x, inv), __fmul_rn(o.y, inv)), pack16<T>(__fmul_rn(o.z, inv), __fmul_rn(o.w, inv)));
+    }
+}
+
 // ── host side ───────────────────────────────────────────────────────────────
 typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
                                   const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
@@ -969,9 +1108,25 @@ cudaError_t encode_heads(const void* base, int dtype, int hd, int heads, int row
 constexpr size_t up128(size_t n) { return (n + 127) & ~(size_t)127; }
 int keys_per_tile(const Prompts& p) { return p.dtype == DT_F32 && p.head_dim > 64 ? Cfg<2, 128>::NK : Cfg<1, 64>::NK; }
 int places(int rows, int seqs, int block) { return rows / block + seqs + 1; }
+int block_tokens(const Prompts& p) { return 2 * (PR_ROWS / (p.n_heads / p.n_kv)); }
+// Parts of a block's keys.  An item takes its tiles and about 2.5 more (its first scores, its rows), the launch as many items as come to the fullest
+// SM, a join three: the number for which that is least, by the mean number of keys of a sequence.  (Four chunks of up to 512 tokens behind 3500
+// keys, 184 blocks of 30 tiles: 1, 2, 3, 4 parts 134, 135, 123, 135 us.  The sizes decide alone, so that the workspace can be asked for.)
+int key_splits(const Prompts& p) {
+    const int sms = 148, block = block_tokens(p);
+    const double items = std::max(1.0, (double)p.n_tokens / block + 0.5 * p.n_seqs) * p.n_kv;
+    const double tiles = p.n_seqs ? (double)p.n_keys / p.n_seqs / keys_per_tile(p) : 0.0;
+    int best = 1;
+    double least = 0.0;
+    for (int s = 1; s <= MAX_SPLITS && (s == 1 || tiles / s >= 2.0); s++) {
+        const double cost = std::ceil(items * s / sms) * (tiles / s + 2.5) + (s > 1 ? 3.0 : 0.0);
+        if (s == 1 || cost < 0.95 * least) least = cost, best = s;
+    }
+    return best;
+}
 
 struct Workspace {
-    size_t k, v, k_inv, v_inv, bytes;
+    size_t k = 0, v = 0, k_inv = 0, v_inv = 0, part_o = 0, part_ml = 0, bytes;
     explicit Workspace(const Prompts& p) {
         const size_t key_slots = (size_t)places(p.n_keys, p.n_seqs, keys_per_tile(p));
         size_t at = 0;
@@ -980,10 +1135,17 @@ struct Workspace {
             at += up128(n);
             return here;
         };
-        k = take((size_t)p.n_keys * p.n_kv * p.head_dim * 4);
-        v = take((size_t)p.n_keys * p.n_kv * p.head_dim * 4);
-        k_inv = take(key_slots * p.n_kv * 4);
-        v_inv = take(key_slots * p.n_kv * 4);
+        if (p.dtype == DT_F32) {
+            k = take((size_t)p.n_keys * p.n_kv * p.head_dim * 4);
+            v = take((size_t)p.n_keys * p.n_kv * p.head_dim * 4);
+            k_inv = take(key_slots * p.n_kv * 4);
+            v_inv = take(key_slots * p.n_kv * 4);
+        }
+        const int splits = key_splits(p);
+        if (splits > 1) {
+            part_o = take((size_t)splits * p.n_tokens * p.n_heads * p.head_dim * 4);
+            part_ml = take((size_t)splits * p.n_tokens * p.n_heads * 8);
+        }
         bytes = at;
     }
 };
@@ -1005,9 +1167,11 @@ cudaError_t launch_typed(cudaStream_t st, const Prompts& p, void* workspace) {
     const int parts = PLANES == 2 ? DT_F16 : p.dtype;  // what K and V are in
     const void *k = p.k, *v = p.v;
     size_t ks = p.k_stride, vs = p.v_stride;
+    const Workspace w(p);
+    uint8_t* base = static_cast<uint8_t*>(workspace);
+    a.splits = key_splits(p);
+    a.part_o = (float*)(base + w.part_o), a.part_ml = (float*)(base + w.part_ml);
     if (PLANES == 2 && p.n_keys > 0) {
-        const Workspace w(p);
-        uint8_t* base = static_cast<uint8_t*>(workspace);
         SplitArgs s{p, {(__half*)(base + w.k), (__half*)(base + w.v)}, {(float*)(base + w.k_inv), (float*)(base + w.v_inv)}, 1};
         while (s.lanes * 4 < p.head_dim) s.lanes *= 2;
         const long long ctas = (long long)places(p.n_keys, p.n_seqs, C::NK) * p.n_kv * 2;
@@ -1028,15 +1192,18 @@ cudaError_t launch_typed(cudaStream_t st, const Prompts& p, void* workspace) {
     int dev = 0, sms = 0;
     if ((e = cudaGetDevice(&dev)) != cudaSuccess) return e;
     if ((e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev)) != cudaSuccess) return e;
-    const long long items = (long long)a.slots * p.n_kv;
+    const long long items = (long long)a.slots * p.n_kv * a.splits;
     if (items > 0x7FFFFFFFll - sms) return cudaErrorInvalidValue;
     g_kernel_launches++;
-    return launch_pdl(st, k_attention_prompts<T, PLANES, HDP>, dim3((unsigned)std::min<long long>(items, sms)), dim3(PR_THREADS), C::SMEM, mq, mk, mv, a);
+    e = launch_pdl(st, k_attention_prompts<T, PLANES, HDP>, dim3((unsigned)std::min<long long>(items, sms)), dim3(PR_THREADS), C::SMEM, mq, mk, mv, a);
+    if (e != cudaSuccess || a.splits == 1) return e;
+    g_kernel_launches++;
+    return launch_pdl(st, k_join<T, C::NK>, dim3((unsigned)(a.slots * p.n_kv), JOIN_CTAS), dim3(JOIN_THREADS), 0, a);
 }
 
 }  // namespace
 
-size_t attention_prompts_workspace(const Prompts& p) { return p.dtype == DT_F32 ? Workspace(p).bytes : 0; }
+size_t attention_prompts_workspace(const Prompts& p) { return Workspace(p).bytes; }
 
 cudaError_t launch_attention_prompts(cudaStream_t st, const Prompts& p, void* workspace) {
     const bool wide = p.head_dim > 64;

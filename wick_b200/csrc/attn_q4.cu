@@ -28,7 +28,7 @@ namespace wick {
 namespace {
 
 constexpr int A4_TILE = KV_Q4_TILE, A4_HEADS = 8;
-constexpr uint32_t A4_SPIN_LIMIT = 1u << 18;
+constexpr uint32_t A4_SPIN_LIMIT = 1u << 24;  // about half a second
 constexpr int A4_MIN_EXP = -24;  // of f16's smallest number
 
 template <int NB>  // 32-element blocks of a head
