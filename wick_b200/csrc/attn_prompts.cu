@@ -290,12 +290,10 @@ __device__ __forceinline__ int count_blocks(const PromptArgs& a, int want, int* 
     return before;
 }
 
-// A block of tokens with all its keys, by a whole warp; false: there is none of this number.
+// Block blk of a sequence, with all its keys; false: there is none.
 template <int NK>
-__device__ __forceinline__ bool find_block(const PromptArgs& a, int number, Item& it) {
+__device__ __forceinline__ bool block_of(const PromptArgs& a, int seq, int blk, Item& it) {
     const int block = 2 * a.tile_tokens;
-    int seq, blk;
-    count_blocks(a, number, &seq, &blk);
     if (seq < 0) return false;
     const int32_t* ks = a.p.key_starts ? a.p.key_starts : a.p.starts;
     const int s0 = a.p.starts[seq], s1 = a.p.starts[seq + 1], t0 = ks[seq], t1 = ks[seq + 1];
@@ -317,12 +315,10 @@ __device__ __forceinline__ bool find_block(const PromptArgs& a, int number, Item
 }
 // Where part `part` of nt tiles begins: equal parts, and what has no tiles is the first one's.
 __device__ __forceinline__ int part_begin(int nt, int part, int splits) { return (int)((long long)nt * part / splits); }
-// Place idx of the list.  The last places come first, since a sequence's last blocks have the most keys and the launch then ends with short ones.
+// A part of a block's keys as an item; false: it has no tiles.
 template <int NK>
-__device__ __forceinline__ bool make_item(const PromptArgs& a, int blocks, int idx, Item& it) {
-    const int part = idx % a.splits, place = idx / a.splits;
-    if (!find_block<NK>(a, blocks - 1 - place / a.p.n_kv, it)) return false;
-    it.kvh = place % a.p.n_kv;
+__device__ __forceinline__ bool part_of(const PromptArgs& a, int kvh, int part, Item& it) {
+    it.kvh = kvh;
     it.part = part;
     if (a.splits > 1) {  // the sequence as this part sees it: its keys begin at the part's first tile
         const int nt = it.nt(), t0 = part_begin(nt, part, a.splits), t1 = part_begin(nt, part + 1, a.splits);
@@ -333,6 +329,53 @@ __device__ __forceinline__ bool make_item(const PromptArgs& a, int blocks, int i
     }
     return true;
 }
+
+// A CTA's items one after the other, by a whole warp: the list is dealt to the CTAs forwards and backwards in turn, and begins with the
+// blocks that have the most keys, so that the CTAs end about together.  Up to 32 sequences (a lane each) their last blocks come first, then
+// their last but one ..; with more, one sequence's blocks after the other's, backwards.
+template <int NK>
+struct Deal {
+    int blocks, mine, turn, level, above;  // blocks in all; this lane's sequence's; rounds so far; blocks of higher number than `level`
+    bool by_level;
+    __device__ __forceinline__ explicit Deal(const PromptArgs& a) : mine(0), turn(0), level(0), above(0), by_level(a.p.n_seqs <= 32) {
+        int seq, blk;
+        blocks = count_blocks(a, -1, &seq, &blk);
+        if (by_level) {
+            const int s = threadIdx.x & 31, block = 2 * a.tile_tokens;
+            if (s < a.p.n_seqs) {
+                const int q0 = max(0, min(a.p.starts[s], a.p.n_tokens)), q1 = max(q0, min(a.p.starts[s + 1], a.p.n_tokens));
+                mine = (q1 - q0 + block - 1) / block;
+            }
+            level = __reduce_max_sync(0xffffffffu, mine) - 1;
+        }
+    }
+    // false: the CTA has had its items
+    __device__ __forceinline__ bool next(const PromptArgs& a, Item& it) {
+        const int total = blocks * a.p.n_kv * a.splits;
+        while (true) {
+            const long long idx = (long long)turn * gridDim.x + ((turn & 1) ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
+            if ((long long)turn * gridDim.x >= total) return false;
+            turn++;
+            if (idx >= total) continue;
+            const int part = (int)idx % a.splits, place = (int)idx / a.splits, kvh = place % a.p.n_kv, number = place / a.p.n_kv;
+            int seq = -1, blk = 0;
+            if (by_level) {
+                uint32_t have = __ballot_sync(0xffffffffu, mine > level);
+                while (level > 0 && above + __popc(have) <= number) {
+                    above += __popc(have);
+                    level--;
+                    have = __ballot_sync(0xffffffffu, mine > level);
+                }
+                const int lane = threadIdx.x & 31;
+                const bool it_is = (have >> lane & 1) && __popc(have & ((1u << lane) - 1)) == number - above;
+                seq = __ffs(__ballot_sync(0xffffffffu, it_is)) - 1, blk = level;
+            } else {
+                count_blocks(a, blocks - 1 - number, &seq, &blk);
+            }
+            if (block_of<NK>(a, seq, blk, it) && part_of<NK>(a, kvh, part, it)) return true;
+        }
+    }
+};
 
 template <class T, int PLANES, int HDP>
 __global__ void __launch_bounds__(PR_THREADS, 1)
@@ -387,13 +430,11 @@ k_attention_prompts(const __grid_constant__ CUtensorMap map_q, const __grid_cons
         asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
         if (warp == 3) {
         // ── items ────────────────────────────────────────────────────────────
-        int unused;
-        const int blocks = count_blocks(a, -1, &unused, &unused), total = blocks * a.p.n_kv * a.splits;
+        Deal<NK> deal(a);
         uint32_t k = 0;
-        for (int idx = blockIdx.x;; idx += gridDim.x) {
+        while (true) {
             Item it;
-            it.kvh = -1;
-            if (idx < total && !make_item<NK>(a, blocks, idx, it)) continue;
+            if (!deal.next(a, it)) it.kvh = -1;
             if (!__all_sync(0xffffffffu, bar_wait(sh, &sh->item_empty[k % PR_ITEMS], ((k / PR_ITEMS) & 1) ^ 1))) break;
             if (lane == 0) {
                 Item* to = &sh->item[k % PR_ITEMS];
@@ -954,11 +995,9 @@ k_attention_prompts(const __grid_constant__ CUtensorMap map_q, const __grid_cons
     if (warp == 1) {
         if (sh->abort) {
             for (int i = 0; i < 64; i++) __nanosleep(1000);  // copies issued before the failure may still be landing
-            int unused;
-            const int blocks = count_blocks(a, -1, &unused, &unused);
-            for (int idx = blockIdx.x; idx < blocks * a.p.n_kv * a.splits; idx += gridDim.x) {  // no row is left without a sign of it
-                Item it;
-                if (!make_item<NK>(a, blocks, idx, it)) continue;
+            Deal<NK> deal(a);
+            Item it;
+            while (deal.next(a, it)) {  // no row is left without a sign of it
                 for (int i = lane; i < it.tokens * a.group * hd; i += 32) {
                     const size_t row = (size_t)(it.token0 + i / (a.group * hd)) * a.p.n_heads + it.kvh * a.group + i % (a.group * hd) / hd;
                     if (a.splits > 1)
@@ -1038,7 +1077,9 @@ __global__ void __launch_bounds__(JOIN_THREADS) k_join(const __grid_constant__ P
     pdl_trigger();
     pdl_wait();
     Item it;
-    if (!find_block<NK>(a, blockIdx.x / a.p.n_kv, it)) return;
+    int seq, blk;
+    count_blocks(a, blockIdx.x / a.p.n_kv, &seq, &blk);
+    if (!block_of<NK>(a, seq, blk, it)) return;
     const int kvh = blockIdx.x % a.p.n_kv, hd = a.p.head_dim, pieces = hd / 4, nt = it.nt();
     const size_t rows = (size_t)a.p.n_tokens * a.p.n_heads;
     uint32_t there = 0;  // the parts that have tiles

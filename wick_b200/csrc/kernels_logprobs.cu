@@ -63,7 +63,7 @@ struct Running {
     float m = -LP_BOUND;
     f32x2 s = 0, t = 0;  // (two zeros)
     template <int N>
-    __device__ __forceinline__ void add(float (&x)[N]) {
+    __device__ __forceinline__ float add(float (&x)[N]) {  // the largest of them
         static_assert(N == 1 || N % 2 == 0, "pairs");
         float top = x[0], low = x[0];
 #pragma unroll
@@ -96,6 +96,7 @@ struct Running {
                 t = fma2(e, d, t);
             }
         }
+        return top;
     }
 };
 struct Joined {
@@ -141,7 +142,8 @@ struct Slice {  // the part of a row that a CTA reads: 16-byte pieces [v0, v1), 
 };
 
 // HELD: the CTA's part of the row stays in registers (at most LP_HELD elements per thread), and is not read a second time for the alternatives.
-constexpr int LP_HELD = 32;
+// Otherwise the largest of every 32 elements is noted (of the first LP_CHUNKS of a thread), and only those that can hold an alternative are.
+constexpr int LP_HELD = 32, LP_CHUNKS = 24;
 template <class T, bool HELD>
 __global__ void __launch_bounds__(LP_THREADS) k_token_logprobs(const T* __restrict__ logits, size_t row_stride, int vocab,
                                                                const int32_t* __restrict__ tokens, int top_n, float* __restrict__ logprob,
@@ -155,6 +157,7 @@ __global__ void __launch_bounds__(LP_THREADS) k_token_logprobs(const T* __restri
     __shared__ unsigned long long cand[LP_CAND];
     __shared__ int n_cand;
     __shared__ uint32_t sh_floor[LP_WARPS];
+    __shared__ float chunk_max[HELD ? 1 : LP_CHUNKS][LP_THREADS];
     cg::cluster_group cluster = cg::this_cluster();
     const int ctas = (int)cluster.num_blocks(), rank = (int)cluster.block_rank(), row = blockIdx.x / ctas;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -182,7 +185,7 @@ __global__ void __launch_bounds__(LP_THREADS) k_token_logprobs(const T* __restri
         }
         r.add(x);
     } else {
-        int v = sl.v0 + tid;
+        int v = sl.v0 + tid, chunk = 0;
         for (; v + (AT_ONCE - 1) * LP_THREADS < sl.v1; v += AT_ONCE * LP_THREADS) {
 #pragma unroll
             for (int u = 0; u < AT_ONCE; u++) {
@@ -191,13 +194,17 @@ __global__ void __launch_bounds__(LP_THREADS) k_token_logprobs(const T* __restri
 #pragma unroll
                 for (int i = 0; i < V; i++) x[u * V + i] = y[i];
             }
-            r.add(x);
+            const float top = r.add(x);
+            if (chunk < LP_CHUNKS) chunk_max[HELD ? 0 : chunk][tid] = top;
+            chunk++;
         }
+        float top = -LP_BOUND;
         for (; v < sl.v1; v += LP_THREADS) {
             float y[V];
             sl.load(v, y);
-            r.add(y);
+            top = fmaxf(top, r.add(y));
         }
+        if (chunk < LP_CHUNKS) chunk_max[HELD ? 0 : chunk][tid] = top;
     }
     const uint32_t mine = value_key(r.m);
     Joined j;
@@ -211,16 +218,17 @@ __global__ void __launch_bounds__(LP_THREADS) k_token_logprobs(const T* __restri
     if (lane == 0) sh_m[warp] = j.m, sh_s[warp] = j.s, sh_t[warp] = j.t;
     if (tid == 0) n_cand = 0;
     if (top_n > 0) {
-        // A value that top_n elements of the CTA reach: every warp has k = top_n / 8 (upwards) threads whose maxima do, if it is the smallest
-        // of the warps' k-th largest maxima.
+        // A value that top_n elements of the CTA reach: each of A warps has k = top_n / A (upwards) threads whose maxima do, if it is the smallest
+        // of those warps' k-th largest maxima.  (A: the warps whose threads all have elements.)
+        const int full = max(1, min(LP_WARPS, (sl.v1 - sl.v0) / 32));
         uint32_t left = mine;
         uint32_t kth = 0;
-        for (int k = 0; k < top_n; k += LP_WARPS) {
+        for (int k = 0; k < top_n; k += full) {
             kth = __reduce_max_sync(0xffffffffu, left);
             const uint32_t at = __ballot_sync(0xffffffffu, left == kth);
             if (lane == __ffs(at) - 1) left = 0;
         }
-        if (lane == 0) sh_floor[warp] = kth;
+        if (lane == 0) sh_floor[warp] = warp < full ? kth : 0xFFFFFFFFu;
     }
     __syncthreads();
     if (warp == 0) {
@@ -253,12 +261,14 @@ __global__ void __launch_bounds__(LP_THREADS) k_token_logprobs(const T* __restri
                     }
                 }
             } else {
-                for (int v = sl.v0 + tid; v < sl.v1; v += 4 * LP_THREADS) {
-                    float y[4][V];
+                int chunk = 0;
+                for (int v = sl.v0 + tid; v < sl.v1; v += AT_ONCE * LP_THREADS, chunk++) {
+                    if (chunk < LP_CHUNKS && !(chunk_max[HELD ? 0 : chunk][tid] >= floor_value)) continue;
+                    float y[AT_ONCE][V];
 #pragma unroll
-                    for (int u = 0; u < 4; u++) sl.load(min(v + u * LP_THREADS, sl.v1 - 1), y[u]);
+                    for (int u = 0; u < AT_ONCE; u++) sl.load(min(v + u * LP_THREADS, sl.v1 - 1), y[u]);
 #pragma unroll
-                    for (int u = 0; u < 4; u++)
+                    for (int u = 0; u < AT_ONCE; u++)
                         if (v + u * LP_THREADS < sl.v1) {
 #pragma unroll
                             for (int i = 0; i < V; i++) offer(held(y[u][i]), sl.index(v + u * LP_THREADS) + i);
@@ -272,6 +282,7 @@ __global__ void __launch_bounds__(LP_THREADS) k_token_logprobs(const T* __restri
             for (int c = tid; c < n; c += LP_THREADS) {
                 const unsigned long long k = cand[c];
                 int p = 0;
+#pragma unroll 8
                 for (int i = 0; i < n; i++) p += cand[i] > k;
                 if (p < top_n) best[p] = k;
             }
@@ -333,8 +344,22 @@ __global__ void __launch_bounds__(LP_THREADS) k_token_logprobs(const T* __restri
             const unsigned long long* keys = ctas > 1 ? cand : best;
             for (int c = tid; c < total; c += LP_THREADS) {
                 const unsigned long long k = keys[c];
-                int p = 0;
-                for (int i = 0; i < total; i++) p += keys[i] > k;
+                int p = c % top_n;  // the larger ones of its own list, and of each other: lists descend
+                if (total <= 64) {
+                    p = 0;
+#pragma unroll 8
+                    for (int i = 0; i < total; i++) p += keys[i] > k;
+                }
+                for (int l = 0; total > 64 && l < total; l += top_n) {
+                    if (l == c - c % top_n) continue;
+                    int lo = 0, hi = top_n;
+                    while (lo < hi) {
+                        const int mid = (lo + hi) >> 1;
+                        if (keys[l + mid] > k) lo = mid + 1;
+                        else hi = mid;
+                    }
+                    p += lo;
+                }
                 if (k != 0 && p < top_n) {
                     top_ids[(size_t)row * top_n + p] = (int32_t)(0xFFFFFFFFu - (uint32_t)k);
                     top_logprobs[(size_t)row * top_n + p] = log_p(key_value((uint32_t)(k >> 32)));
