@@ -315,19 +315,17 @@ __device__ __forceinline__ bool block_of(const PromptArgs& a, int seq, int blk, 
 }
 // Where part `part` of nt tiles begins: equal parts, and what has no tiles is the first one's.
 __device__ __forceinline__ int part_begin(int nt, int part, int splits) { return (int)((long long)nt * part / splits); }
-// A part of a block's keys as an item; false: it has no tiles.
+// A part of a block's keys as an item (one without tiles too: its rows' maxima of -inf tell the join).
 template <int NK>
-__device__ __forceinline__ bool part_of(const PromptArgs& a, int kvh, int part, Item& it) {
+__device__ __forceinline__ void part_of(const PromptArgs& a, int kvh, int part, Item& it) {
     it.kvh = kvh;
     it.part = part;
     if (a.splits > 1) {  // the sequence as this part sees it: its keys begin at the part's first tile
         const int nt = it.nt(), t0 = part_begin(nt, part, a.splits), t1 = part_begin(nt, part + 1, a.splits);
-        if (t0 == t1 && (nt > 0 || part > 0)) return false;
         it.key0 += t0 * NK, it.keys -= t0 * NK, it.first_visible -= t0 * NK, it.key_slot0 += t0;
 #pragma unroll
         for (int m = 0; m < 2; m++) it.n_tiles[m] = max(0, min(it.n_tiles[m], t1) - t0);
     }
-    return true;
 }
 
 // A CTA's items one after the other, by a whole warp: the list is dealt to the CTAs forwards and backwards in turn, and begins with the
@@ -372,7 +370,10 @@ struct Deal {
             } else {
                 count_blocks(a, blocks - 1 - number, &seq, &blk);
             }
-            if (block_of<NK>(a, seq, blk, it) && part_of<NK>(a, kvh, part, it)) return true;
+            if (block_of<NK>(a, seq, blk, it)) {
+                part_of<NK>(a, kvh, part, it);
+                return true;
+            }
         }
     }
 };
@@ -910,14 +911,14 @@ k_attention_prompts(const __grid_constant__ CUtensorMap map_q, const __grid_cons
             T* out = reinterpret_cast<T*>(a.p.out) + out_row * hd;
             float* sums = a.part_o + part_row * hd;
             const bool split = a.splits > 1;
-            if (split && real && ok) *reinterpret_cast<float2*>(a.part_ml + part_row * 2) = make_float2(limit > 0 ? row_max : NEG, limit > 0 ? row_sum : 0.0f);
+            if (split && real && ok) *reinterpret_cast<float2*>(a.part_ml + part_row * 2) = make_float2(limit > 0 && n > 0 ? row_max : NEG, limit > 0 && n > 0 ? row_sum : 0.0f);
             auto write_32 = [&](int c, float (&x)[32]) {
                 if (split) {
 #pragma unroll
                     for (int d = 0; d < 32; d += 8)  // (head_dim is a multiple of 8: rows start on 32-byte boundaries)
                         if (c + d < hd) {
 #pragma unroll
-                            for (int u = 0; u < 8; u++) x[d + u] = limit > 0 ? x[d + u] : 0.0f;
+                            for (int u = 0; u < 8; u++) x[d + u] = limit > 0 && n > 0 ? x[d + u] : 0.0f;
                             asm volatile("st.global.v8.f32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(sums + c + d), "f"(x[d]), "f"(x[d + 1]), "f"(x[d + 2]),
                                          "f"(x[d + 3]), "f"(x[d + 4]), "f"(x[d + 5]), "f"(x[d + 6]), "f"(x[d + 7])
                                          : "memory");
@@ -1070,52 +1071,45 @@ __global__ void __launch_bounds__(SP_THREADS) k_split(const __grid_constant__ Sp
     if (threadIdx.x == 0) a.inv[val][(size_t)slot * a.p.n_kv + kvh] = __fdiv_rn(1.0f, f);
 }
 
-// The parts of a block's keys, added up in their order: four values of a row per thread, all parts' loads under way together.
-constexpr int JOIN_THREADS = 256, JOIN_CTAS = 8, MAX_SPLITS = 8;  // CTAs of a block
-template <class T, int NK>
+// The parts of the rows' keys, added up in their order: four values of a row per thread (threadIdx.x), all parts' loads under way together.
+constexpr int JOIN_THREADS = 256, MAX_SPLITS = 8;
+template <class T>
 __global__ void __launch_bounds__(JOIN_THREADS) k_join(const __grid_constant__ PromptArgs a) {
     pdl_trigger();
     pdl_wait();
-    Item it;
-    int seq, blk;
-    count_blocks(a, blockIdx.x / a.p.n_kv, &seq, &blk);
-    if (!block_of<NK>(a, seq, blk, it)) return;
-    const int kvh = blockIdx.x % a.p.n_kv, hd = a.p.head_dim, pieces = hd / 4, nt = it.nt();
-    const size_t rows = (size_t)a.p.n_tokens * a.p.n_heads;
-    uint32_t there = 0;  // the parts that have tiles
-    for (int s = 0; s < a.splits; s++) there |= part_begin(nt, s, a.splits) < part_begin(nt, s + 1, a.splits) ? 1u << s : 0u;
-    for (int i = blockIdx.y * JOIN_THREADS + threadIdx.x; i < it.tokens * a.group * pieces; i += JOIN_CTAS * JOIN_THREADS) {
-        const int r = i / pieces, d = i % pieces * 4;
-        const size_t row = (size_t)(it.token0 + r / a.group) * a.p.n_heads + kvh * a.group + r % a.group;
-        float2 ml[MAX_SPLITS];
-        float4 x[MAX_SPLITS];
-        float m = __int_as_float(0xFF800000);
+    const int hd = a.p.head_dim, d = threadIdx.x * 4;
+    const size_t rows = (size_t)a.p.n_tokens * a.p.n_heads, first = (size_t)max(0, min(a.p.starts[0], a.p.n_tokens)) * a.p.n_heads;
+    const size_t last = (size_t)max(0, min(a.p.starts[a.p.n_seqs], a.p.n_tokens)) * a.p.n_heads;
+    const size_t row = (size_t)blockIdx.x * blockDim.y + threadIdx.y;
+    if (row < first || row >= last) return;  // (a row of no sequence)
+    float2 ml[MAX_SPLITS];
+    float4 x[MAX_SPLITS];
+    float m = __int_as_float(0xFF800000);
 #pragma unroll
-        for (int s = 0; s < MAX_SPLITS; s++) {
-            ml[s] = make_float2(m, 0.0f), x[s] = make_float4(0.f, 0.f, 0.f, 0.f);
-            if (there >> s & 1) {
-                ml[s] = *reinterpret_cast<const float2*>(a.part_ml + (s * rows + row) * 2);
-                x[s] = *reinterpret_cast<const float4*>(a.part_o + (s * rows + row) * hd + d);
-            }
+    for (int s = 0; s < MAX_SPLITS; s++) {
+        ml[s] = make_float2(m, 0.0f), x[s] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (s < a.splits) {
+            ml[s] = *reinterpret_cast<const float2*>(a.part_ml + (s * rows + row) * 2);
+            x[s] = *reinterpret_cast<const float4*>(a.part_o + (s * rows + row) * hd + d);
         }
-#pragma unroll
-        for (int s = 0; s < MAX_SPLITS; s++) m = fmaxf(m, ml[s].x);
-        float l = 0.0f;
-        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-        for (int s = 0; s < MAX_SPLITS; s++)
-            if (there >> s & 1) {
-                const float f = ml[s].x == m ? 1.0f : exp2_approx(ml[s].x - m);
-                l = fmaf(ml[s].y, f, l);
-                o.x = fmaf(x[s].x, f, o.x), o.y = fmaf(x[s].y, f, o.y), o.z = fmaf(x[s].z, f, o.z), o.w = fmaf(x[s].w, f, o.w);
-            }
-        const float inv = l == 0.0f ? 0.0f : __fdiv_rn(1.0f, l);
-        T* out = reinterpret_cast<T*>(a.p.out) + row * hd + d;
-        if constexpr (sizeof(T) == 4)
-            *reinterpret_cast<float4*>(out) = make_float4(__fmul_rn(o.x, inv), __fmul_rn(o.y, inv), __fmul_rn(o.z, inv), __fmul_rn(o.w, inv));
-        else
-            *reinterpret_cast<uint2*>(out) = make_uint2(pack16<T>(__fmul_rn(o.x, inv), __fmul_rn(o.y, inv)), pack16<T>(__fmul_rn(o.z, inv), __fmul_rn(o.w, inv)));
     }
+#pragma unroll
+    for (int s = 0; s < MAX_SPLITS; s++) m = fmaxf(m, ml[s].x);
+    float l = 0.0f;
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int s = 0; s < MAX_SPLITS; s++)
+        if (s < a.splits) {
+            const float f = ml[s].x == m ? 1.0f : exp2_approx(ml[s].x - m);
+            l = fmaf(ml[s].y, f, l);
+            o.x = fmaf(x[s].x, f, o.x), o.y = fmaf(x[s].y, f, o.y), o.z = fmaf(x[s].z, f, o.z), o.w = fmaf(x[s].w, f, o.w);
+        }
+    const float inv = l == 0.0f ? 0.0f : __fdiv_rn(1.0f, l);
+    T* out = reinterpret_cast<T*>(a.p.out) + row * hd + d;
+    if constexpr (sizeof(T) == 4)
+        *reinterpret_cast<float4*>(out) = make_float4(__fmul_rn(o.x, inv), __fmul_rn(o.y, inv), __fmul_rn(o.z, inv), __fmul_rn(o.w, inv));
+    else
+        *reinterpret_cast<uint2*>(out) = make_uint2(pack16<T>(__fmul_rn(o.x, inv), __fmul_rn(o.y, inv)), pack16<T>(__fmul_rn(o.z, inv), __fmul_rn(o.w, inv)));
 }
 
 // ── host side ───────────────────────────────────────────────────────────────
@@ -1155,13 +1149,13 @@ int block_tokens(const Prompts& p) { return 2 * (PR_ROWS / (p.n_heads / p.n_kv))
 // keys, 184 blocks of 30 tiles: 1, 2, 3, 4 parts 134, 135, 123, 135 us.  The sizes decide alone, so that the workspace can be asked for.)
 int key_splits(const Prompts& p) {
     const int sms = 148, block = block_tokens(p);
-    const double items = std::max(1.0, (double)p.n_tokens / block + 0.5 * p.n_seqs) * p.n_kv;
+    const double items = std::max(1.0, (double)p.n_tokens / block + 0.25 * p.n_seqs) * p.n_kv;
     const double tiles = p.n_seqs ? (double)p.n_keys / p.n_seqs / keys_per_tile(p) : 0.0;
     int best = 1;
     double least = 0.0;
     for (int s = 1; s <= MAX_SPLITS && (s == 1 || tiles / s >= 2.0); s++) {
         const double cost = std::ceil(items * s / sms) * (tiles / s + 2.5) + (s > 1 ? 3.0 : 0.0);
-        if (s == 1 || cost < 0.95 * least) least = cost, best = s;
+        if (s == 1 || cost < 0.97 * least) least = cost, best = s;
     }
     return best;
 }
@@ -1239,7 +1233,9 @@ cudaError_t launch_typed(cudaStream_t st, const Prompts& p, void* workspace) {
     e = launch_pdl(st, k_attention_prompts<T, PLANES, HDP>, dim3((unsigned)std::min<long long>(items, sms)), dim3(PR_THREADS), C::SMEM, mq, mk, mv, a);
     if (e != cudaSuccess || a.splits == 1) return e;
     g_kernel_launches++;
-    return launch_pdl(st, k_join<T, C::NK>, dim3((unsigned)(a.slots * p.n_kv), JOIN_CTAS), dim3(JOIN_THREADS), 0, a);
+    const unsigned pieces = (unsigned)p.head_dim / 4, per = JOIN_THREADS / pieces;
+    const size_t rows = (size_t)p.n_tokens * p.n_heads;
+    return launch_pdl(st, k_join<T>, dim3((unsigned)((rows + per - 1) / per)), dim3(pieces, per), 0, a);
 }
 
 }  // namespace

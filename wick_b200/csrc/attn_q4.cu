@@ -589,14 +589,17 @@ __global__ void __launch_bounds__(Q4Cfg<NB>::THREADS, 1) k_attention_q4(const __
     }
 }
 
-// What reaches over CTAs: CTA b joins what begins in CTA b of the kernel above and goes on, a warp per head.
+// What reaches over CTAs: CTA (b, g) joins head g of what begins in CTA b of the kernel above and goes on.  Its warps take the parts in turn, and
+// warp 0 adds up their sums in the warps' order.
+constexpr int JOIN_WARPS = 8;
 template <class T, int NB>
-__global__ void __launch_bounds__(32 * A4_HEADS) k_attention_q4_join(const __grid_constant__ Q4Args a) {
+__global__ void __launch_bounds__(32 * JOIN_WARPS) k_attention_q4_join(const __grid_constant__ Q4Args a) {
     using C = Q4Cfg<NB>;
+    __shared__ float sums[JOIN_WARPS][C::HD + 2];
     pdl_trigger();
     pdl_wait();
     const int4 d = a.descs[(size_t)blockIdx.x * 2 + 1];
-    const int g = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int g = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     if (!d.w || d.y % a.sub * A4_HEADS + g >= a.group) return;
     int last = blockIdx.x;  // the CTA that holds the end
     for (int b = blockIdx.x + 1;; b += 32) {
@@ -609,7 +612,61 @@ __global__ void __launch_bounds__(32 * A4_HEADS) k_attention_q4_join(const __gri
         if (b + 32 >= (int)gridDim.x) return;  // (cannot be)
     }
     const float* first = a.parts + ((size_t)blockIdx.x * 2 + 1) * C::PART;
-    join_head<T, NB>(a, d.x, d.y, g, last - (int)blockIdx.x + 1, [&](int k) { return first + (k == 0 ? 0 : (k * 2 - 1) * C::PART); }, nullptr);
+    const int n = last - (int)blockIdx.x + 1, mine = (n - warp + JOIN_WARPS - 1) / JOIN_WARPS;
+    auto part = [&](int k) { return first + (k == 0 ? 0 : (k * 2 - 1) * C::PART); };
+    if (n <= 4) {
+        if (warp == 0) join_head<T, NB>(a, d.x, d.y, g, n, part, nullptr);
+        return;
+    }
+    float m = __int_as_float(0xFF800000), l = 0.0f, o[NB] = {};
+    for (int k0 = 0; k0 < mine; k0 += 8) {  // eight parts' loads together; rescaled where a maximum grows
+        float x[8][NB], mi[8], li[8];
+#pragma unroll
+        for (int u = 0; u < 8; u++) {
+            const float* p = part(min(warp + (k0 + u) * JOIN_WARPS, n - 1));
+            const bool in = k0 + u < mine;
+            mi[u] = in ? p[A4_HEADS * C::HD + g] : __int_as_float(0xFF800000);
+            li[u] = p[A4_HEADS * C::HD + A4_HEADS + g];
+#pragma unroll
+            for (int b = 0; b < NB; b++) x[u][b] = p[g * C::HD + 32 * b + lane];
+        }
+        float top = m;
+#pragma unroll
+        for (int u = 0; u < 8; u++) top = fmaxf(top, mi[u]);
+        const float f0 = m == top ? 1.0f : exp2_approx(m - top);
+        l *= f0;
+#pragma unroll
+        for (int b = 0; b < NB; b++) o[b] *= f0;
+#pragma unroll
+        for (int u = 0; u < 8; u++)
+            if (k0 + u < mine) {
+                const float f = mi[u] == top ? 1.0f : exp2_approx(mi[u] - top);
+                l = fmaf(li[u], f, l);
+#pragma unroll
+                for (int b = 0; b < NB; b++) o[b] = fmaf(x[u][b], f, o[b]);
+            }
+        m = top;
+    }
+#pragma unroll
+    for (int b = 0; b < NB; b++) sums[warp][32 * b + lane] = o[b];
+    if (lane == 0) sums[warp][C::HD] = m, sums[warp][C::HD + 1] = l;
+    __syncthreads();
+    if (warp != 0) return;
+    m = __int_as_float(0xFF800000);
+    for (int w = 0; w < JOIN_WARPS; w++) m = fmaxf(m, sums[w][C::HD]);
+    l = 0.0f;
+#pragma unroll
+    for (int b = 0; b < NB; b++) o[b] = 0.0f;
+    for (int w = 0; w < JOIN_WARPS && w < n; w++) {
+        const float f = sums[w][C::HD] == m ? 1.0f : exp2_approx(sums[w][C::HD] - m);
+        l = fmaf(sums[w][C::HD + 1], f, l);
+#pragma unroll
+        for (int b = 0; b < NB; b++) o[b] = fmaf(sums[w][32 * b + lane], f, o[b]);
+    }
+    const float inv = __fdiv_rn(1.0f, l);
+    T* out = static_cast<T*>(a.out) + ((size_t)d.x * a.n_heads + d.y / a.sub * a.group + d.y % a.sub * A4_HEADS + g) * C::HD;
+#pragma unroll
+    for (int b = 0; b < NB; b++) out[32 * b + lane] = from_f32<T>(__fmul_rn(o[b], inv));
 }
 
 constexpr int A4_MAX_CTAS = 256;
@@ -627,7 +684,7 @@ cudaError_t launch_quads(cudaStream_t st, Q4Args& a) {
     const dim3 grid((unsigned)(sms < A4_MAX_CTAS ? sms : A4_MAX_CTAS));
     g_kernel_launches += 2;
     if ((e = launch_pdl(st, k_attention_q4<T, NB, HQ>, grid, dim3(C::THREADS), C::SMEM, a)) != cudaSuccess) return e;
-    return launch_pdl(st, k_attention_q4_join<T, NB>, grid, dim3(32 * A4_HEADS), 0, a);
+    return launch_pdl(st, k_attention_q4_join<T, NB>, dim3(grid.x, (unsigned)(a.group < A4_HEADS ? a.group : A4_HEADS)), dim3(32 * JOIN_WARPS), 0, a);
 }
 template <class T, int NB>
 cudaError_t launch_typed(cudaStream_t st, Q4Args& a) {
