@@ -289,6 +289,51 @@ def test_attention_prompts_many_short_sequences(ops):
             _check(out[a:b], ref, tol, v.abs().max().double())
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16], ids=str)
+@pytest.mark.parametrize("seqs", [32, 33, 100, 1024, 1025])
+def test_attention_prompts_every_way_of_counting_blocks(ops, dtype, seqs):
+    """Sequences are walked through by level, one after the other, or searched for, by how many they are; some are empty."""
+    heads, kv, hd = 4, 1, 32
+    lengths = [(i * 37) % 90 if seqs <= 100 else (i * 5) % 7 for i in range(seqs)]
+    lengths[seqs // 2] = 300
+    g = _gen(seqs)
+    n = sum(lengths)
+    q, k, v = (_randn(g, n, h * hd).to(dtype) for h in (heads, kv, kv))
+    out = torch.full_like(q, math.nan)
+    ops.attention_prompts(q, k, v, _starts(lengths), heads, kv, hd, out=out)
+    assert torch.isfinite(out).all()
+    at = np.concatenate([[0], np.cumsum(lengths)])
+    for s in {0, 1, seqs // 2 - 1, seqs // 2, seqs // 2 + 1, seqs - 1}:
+        a, b = int(at[s]), int(at[s + 1])
+        if a < b:
+            ref, tol = _prompts_ref(q[a:b], k[a:b], v[a:b], [b - a], [b - a], heads, kv, hd)
+            _check(out[a:b], ref, tol, v.abs().max().double())
+
+
+def test_attention_prompts_two_graphs_in_turn(ops):
+    """Two captured calls, one of them cut into parts, replayed in any order."""
+    heads, kv, hd = 8, 2, 64
+    g = _gen(15)
+    for dtype in TYPES:
+        calls = []
+        for nq, nk in (([60, 70], [3000, 4000]), ([500, 300], [500, 300])):
+            q, k, v = _randn(g, sum(nq), heads * hd).to(dtype), _randn(g, sum(nk), kv * hd).to(dtype), _randn(g, sum(nk), kv * hd).to(dtype)
+            calls.append((q, k, v, _starts(nq), heads, kv, hd, _starts(nk), torch.zeros_like(q)))
+        want = [ops.attention_prompts(*c[:8]) for c in calls]
+        side, graphs = torch.cuda.Stream(), []
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            for c in calls:
+                graphs.append(torch.cuda.CUDAGraph())
+                with torch.cuda.graph(graphs[-1], stream=side):
+                    ops.attention_prompts(*c)
+        torch.cuda.current_stream().wait_stream(side)
+        for i in (0, 1, 1, 0, 0, 1):
+            calls[i][8].fill_(3)
+            graphs[i].replay()
+            assert torch.equal(calls[i][8], want[i])
+
+
 def test_attention_prompts_two_streams_at_once(ops):
     heads, kv, hd, n = 8, 2, 64, 900
     g = _gen(14)
@@ -700,3 +745,12 @@ def test_a_serving_step(ops):
     torch.cuda.current_stream().wait_stream(side)
     graph.replay()
     assert all(torch.equal(a, b) for a, b in zip(captured, eager))
+
+
+def test_attention_prompts_without_sequences(ops):
+    x = torch.ones(3, 64, device="cuda")
+    out = torch.full_like(x, 2.0)
+    assert (ops.attention_prompts(x, x, x, _i32([0]), 1, 1, 64, out=out) == 2).all()
+    assert (ops.attention_prompts(x, x, x, _i32([0]), 1, 1, 64) == 0).all()
+    assert (ops.attention_prompts(x, x, x, _i32([1, 2]), 1, 1, 64, key_starts=_i32([0, 3]))[[0, 2]] == 0).all()
+    assert ops.attention_prompts(x[:0], x, x, _i32([0, 0]), 1, 1, 64).shape == (0, 64)

@@ -1131,7 +1131,8 @@ cudaError_t encode_heads(const void* base, int dtype, int hd, int heads, int row
     EncodeTiledFn fn = encode_tiled_fn();
     if (!fn) return cudaErrorNotSupported;
     const cuuint64_t size = (cuuint64_t)dtype_bytes(dtype), dims[4] = {(cuuint64_t)hd, (cuuint64_t)heads, (cuuint64_t)rows, (cuuint64_t)planes};
-    const cuuint64_t strides[3] = {(cuuint64_t)hd * size, (cuuint64_t)stride * size, (cuuint64_t)stride * size * (cuuint64_t)rows};
+    const cuuint64_t strides[3] = {(cuuint64_t)hd * size, (cuuint64_t)stride * size,
+                                   (cuuint64_t)stride * size * (planes > 1 ? (cuuint64_t)rows : 1)};  // (of one plane: any)
     const cuuint32_t box[4] = {(cuuint32_t)(128 / size), (cuuint32_t)box_heads, (cuuint32_t)box_rows, 1}, step[4] = {1, 1, 1, 1};
     const CUtensorMapDataType type = dtype == DT_F32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : dtype == DT_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
     const CUresult r = fn(out, type, 4, const_cast<void*>(base), dims, strides, box,

@@ -2590,7 +2590,12 @@ int32_t wick_cuda_attention_prompts(const void* q_dev, uint64_t q_stride, const 
     Prompts p{q_dev, k_dev, v_dev, q_stride, k_stride, v_stride, dtype, starts_dev, key_starts_dev, (int)n_seqs, (int)n_tokens, (int)n_keys,
               (int)n_heads, (int)n_kv_heads, (int)head_dim, out_dev, zero_rest};
     W_TRY(check_prompts(p, n_seqs, n_tokens, n_keys, n_heads, n_kv_heads, head_dim));
-    if (n_seqs == 0 || n_tokens == 0) return WICK_CUDA_OK;
+    if (n_tokens == 0 || (n_seqs == 0 && !zero_rest)) return WICK_CUDA_OK;
+    if (n_seqs == 0) {  // no row belongs to a sequence
+        if (!out_dev) return fail(WICK_CUDA_ERR_BAD_ARG, "NULL argument");
+        CU_TRY(cudaMemsetAsync(out_dev, 0, (size_t)n_tokens * n_heads * head_dim * dtype_bytes(dtype), (cudaStream_t)stream));
+        return WICK_CUDA_OK;
+    }
     if (!q_dev || (n_keys && (!k_dev || !v_dev)) || !starts_dev || !out_dev) return fail(WICK_CUDA_ERR_BAD_ARG, "NULL argument");
     const size_t b = dtype_bytes(dtype);
     if (q_stride < (uint64_t)n_heads * head_dim || k_stride < (uint64_t)n_kv_heads * head_dim || v_stride < (uint64_t)n_kv_heads * head_dim)

@@ -390,8 +390,6 @@ def attention_prompts(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, starts:
         out = torch.empty_like(q) if q.is_contiguous() else torch.empty((n, dim), dtype=q.dtype, device=q.device)
     else:
         _out(out, q, (n, dim), dev)
-    if n_seqs == 0:
-        return out.zero_() if fresh else out
     room = _workspace("wick_cuda_attention_prompts_workspace", dtype, n_seqs, n, n_keys, n_heads, n_kv_heads, head_dim)
     work = torch.empty(room, dtype=torch.uint8, device=q.device) if room else None
     _call(_lib.load().wick_cuda_attention_prompts, dev, q.data_ptr(), q_stride, k.data_ptr(), k_stride, v.data_ptr(), v_stride, dtype,
