@@ -384,7 +384,8 @@ int32_t wick_cuda_decode_batch_logits(wick_cuda_model* m, const uint32_t* tokens
  * Attention of packed prompts, a K / V cache in 4 bits with the attention of single tokens over it, and log probabilities.  They
  * agree with the formulas within rounding (f32 sums), they do not repeat the CPU path's order of operations.  Like the operators
  * above they take device pointers and are asynchronous on `stream`; none allocates, synchronises or keeps anything from one call for the
- * next, so that they can be captured.  The device of the buffers has to be the current one.  `dtype` is a ggml type id. */
+ * next, so that they can be captured.  The device of the buffers has to be the current one.  `dtype` is a ggml type id.
+ * Waits on the device are bounded (about half a second each): rows whose wait expires are NaN. */
 #define WICK_DTYPE_F32 0
 #define WICK_DTYPE_F16 1
 #define WICK_DTYPE_BF16 30

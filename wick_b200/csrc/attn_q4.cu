@@ -19,6 +19,9 @@
 // bulk copies per tile).  A (row, group) that lies within a warp's part is finished there, parts of one are joined within the CTA, and
 // what reaches over CTAs goes to the workspace, where k_attention_q4_join adds it up in order: results do not depend on timing.
 //
+// On a B200: 64 rows of 1025 to 4100 keys, 32 / 8 heads of 64: 35 us (issue slots 56 %, the integer pipe 43 %, tensor pipe 16 %; the bytes would take 14);
+// one row of 131,000 keys, 16 / 4 heads of 128: 28 us (issue 47 %, 8 warps fit the SM; bytes 12); one row of 517 keys, start, a tile and the join: 10 us.
+//
 // What lies behind a row's length is read (the tile is there) but not used: its scores are masked, its scales count as 0.
 // Waits are bounded: on expiry the warp's outputs become NaN.
 #include "serving.cuh"

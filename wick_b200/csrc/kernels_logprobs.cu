@@ -13,6 +13,10 @@
 // Where ties make too many candidates (a vocabulary that is masked but for a few tokens), top_n rounds of "largest key below the
 // last one" follow instead.
 //
+// On a B200: 2500 rows of 50021 in bf16 57 us (4.4 TB/s, 67 % of a copy's rate: per element an exponential, of which the special function unit
+// does 16 a cycle, 28 us here, and some ten operations), 64 rows of 65536 in f32 with twenty alternatives 14 us, one with five 7 us (the
+// cluster's barriers and the candidates).
+//
 // Sums: f32 within a thread's few hundred elements, f64 from there on (log S and T / S cancel for sharp rows).
 // NaN counts as -inf, as for the argmax (wick/src/sampler.rs:8-19); logits are held to +-1e30, so that +inf and -inf need no case of
 // their own: several +inf share the row, -inf has probability 0, a row of -inf alone has no probabilities (-inf, entropy 0).
