@@ -703,6 +703,16 @@ def test_wrappers_refuse(ops):
             f()
 
 
+def test_offsets_and_slots_without_a_dimension(ops):
+    from wick_b200 import _lib
+    x, one = torch.zeros(2, 64, device="cuda"), torch.zeros((), dtype=torch.int32, device="cuda")
+    cache = ops.KvCacheQ4.empty(1, 64, 1, 64)
+    for f in (lambda: ops.kv_read_q4(cache, one, one), lambda: ops.attention_prompts(x, x, x, one, 1, 1, 64),
+              lambda: ops.attention_prompts(x, x, x, _i32([[0, 1], [1, 2]]), 1, 1, 64)):
+        with pytest.raises(_lib.WickCudaError):
+            f()
+
+
 # ── together ───────────────────────────────────────────────────────────────────────────────────────
 def test_a_serving_step(ops):
     """Packed prompts, their keys and values into the cache, the next tokens' attention over it, log probabilities of the choice:

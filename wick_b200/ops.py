@@ -329,7 +329,7 @@ def kv_append_q4(cache: KvCacheQ4, k: torch.Tensor, v: torch.Tensor, slots: torc
 
 def kv_read_q4(cache: KvCacheQ4, slots: torch.Tensor, positions: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
     """The values of row positions[j] of slot slots[j]: k and v [n, kv_heads * head_dim] f32; zeros where the cache has no such row."""
-    dev, n = cache.dev, slots.shape[0]
+    dev, n = cache.dev, slots.numel()
     slots, positions = _ids(slots, n, "slots", dev), _ids(positions, n, "positions", dev)
     k = torch.empty((n, cache.n_kv_heads * cache.head_dim), dtype=torch.float32, device=slots.device)
     v = torch.empty_like(k)
@@ -372,7 +372,7 @@ def attention_prompts(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, starts:
         _bad("q, k and v must have the same type")
     if n_heads <= 0 or n_kv_heads <= 0 or head_dim <= 0 or dim != n_heads * head_dim or n_values != n_keys or dim_k != n_kv_heads * head_dim or dim_v != dim_k:
         _bad("q must have n_heads * head_dim columns, k and v n_kv_heads * head_dim columns and the same rows")
-    n_seqs = starts.shape[0] - 1
+    n_seqs = starts.numel() - 1
     if n_seqs < 0:
         _bad("starts must hold at least one offset")
     starts = _ids(starts, n_seqs + 1, "starts", dev)
