@@ -24,7 +24,8 @@
 // Bound, on a B200: the softmax and its MMAs in turn.  A pair of f32 tiles (heads of 64) takes 5300 cycles, 3072 of them MMAs: 2000 waiting for P V
 // and the next scores, 600 the maximum, 2150 the weights and their parts, 500 adding O.  A pair in 16 bits takes 3750 (heads of 64, 2750 the weights,
 // of which the special function unit needs 2048) or 4300 (heads of 128; 2048 MMA).  Eight prompts of 250 to 1001 tokens, 32 / 8 heads of 64, f32: 103 us
-// (tensor pipe 34 %); one of 8000, heads of 128, bf16: 473 to 533 us, 983 to 1108 TFLOP/s.  Loops that run once per item stay rolled: unrolled they
+// (tensor pipe 34 %); one of 8000, heads of 128, bf16: 473 us (1108 TFLOP/s), 533 under
+// the power cap.  Loops that run once per item stay rolled: unrolled they
 // took longer to fetch than to run (161 -> 116 us in the first case).
 //
 // Every wait is bounded: on expiry all roles leave their loops and all rows of the CTA's items become NaN.
@@ -1153,7 +1154,7 @@ int places(int rows, int seqs, int block) { return rows / block + seqs + 1; }
 int block_tokens(const Prompts& p) { return 2 * (PR_ROWS / (p.n_heads / p.n_kv)); }
 // Parts of a block's keys.  An item takes its tiles and about 2.5 more (its first scores, its rows), the launch as many items as come to the fullest
 // SM, a join three: the number for which that is least, by the mean number of keys of a sequence.  (Four chunks of up to 512 tokens behind 3500
-// keys, 184 blocks of 30 tiles: 1, 2, 3, 4 parts 129, 120, 115, 118 us.  The sizes decide alone, so that the workspace can be asked for.)
+// keys, 184 blocks of 30 tiles: 1, 2, 3, 4 parts 129, 120, 115, 118 us at 1965 MHz.  The sizes decide alone, so that the workspace can be asked for.)
 int key_splits(const Prompts& p) {
     const int sms = 148, block = block_tokens(p);
     const double items = std::max(1.0, (double)p.n_tokens / block + 0.25 * p.n_seqs) * p.n_kv;
