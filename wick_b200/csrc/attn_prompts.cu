@@ -21,7 +21,7 @@
 // Masked places may hold anything.  Scores are masked after the product; V is different, 0 * NaN is NaN: a warp looks at every V
 // tile that some row sees in part, zeroes what is not finite, and notes the keys; rows that attend such a key add its values at the end.
 //
-// Bound, on a B200: the softmax and its MMAs in turn.  A pair of f32 tiles (heads of 64) takes 5300 cycles, 3072 of them MMAs: 2000 waiting for P V
+// Bound, on a B200: the softmax and its MMAs in turn.  A pair of f32 tiles (heads of 64) takes 5300 cycles, 58 % of them MMAs: 2000 waiting for P V
 // and the next scores, 600 the maximum, 2150 the weights and their parts, 500 adding O.  A pair in 16 bits takes 3750 (heads of 64, 2750 the weights,
 // of which the special function unit needs 2048) or 4300 (heads of 128; 2048 MMA).  Eight prompts of 250 to 1001 tokens, 32 / 8 heads of 64, f32: 103 us
 // (tensor pipe 34 %); one of 8000, heads of 128, bf16: 473 us (1108 TFLOP/s), 533 under
