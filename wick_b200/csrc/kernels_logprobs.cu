@@ -225,9 +225,10 @@ __global__ void __launch_bounds__(LP_THREADS) k_token_logprobs(const T* __restri
         // A value that top_n elements of the CTA reach: each of A warps has k = top_n / A (upwards) threads whose maxima do, if it is the smallest
         // of those warps' k-th largest maxima.  (A: the warps whose threads all have elements.)
         const int full = max(1, min(LP_WARPS, (sl.v1 - sl.v0) / 32));
+        // (A warp has 32 maxima.  Where that is too few, full is 1 and the row has fewer than 64 pieces: everything is a candidate.)
         uint32_t left = mine;
-        uint32_t kth = 0;
-        for (int k = 0; k < top_n; k += full) {
+        uint32_t kth = value_key(-LP_BOUND);
+        for (int k = 0; k < top_n && top_n <= 32 * full; k += full) {
             kth = __reduce_max_sync(0xffffffffu, left);
             const uint32_t at = __ballot_sync(0xffffffffu, left == kth);
             if (lane == __ffs(at) - 1) left = 0;
