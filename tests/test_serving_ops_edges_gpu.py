@@ -1,9 +1,12 @@
-"""Operators of a serving step where they can go wrong: small vocabularies with many alternatives.  References and bounds are those of
-test_serving_ops_gpu."""
+"""Operators of a serving step where they can go wrong: small vocabularies with many alternatives, magnitudes that lie
+far apart.  References and bounds are those of test_serving_ops_gpu."""
+import math
+
 import pytest
 import torch
 
-from test_serving_ops_gpu import TYPES, _check_logprobs, _gen, _randn, ops  # noqa: F401
+from test_serving_ops_gpu import (TYPES, _attend, _check, _check_logprobs, _gen, _i32, _prompts_ref, _q4_ref, _randn, _random_cache,  # noqa: F401
+                                  _starts, ops)
 
 pytestmark = pytest.mark.gpu
 
@@ -28,3 +31,97 @@ def test_token_logprobs_small_masked_vocabularies(ops):
     x[3, :50] = float("nan")
     x[3, 50:] = _randn(_gen(1), 50)
     _check_logprobs(ops, x, [17, 0, 3, 70], 64)
+
+
+# ── packed prompts in f32: magnitudes that differ within a tile ────────────────────────────────────
+# (Rows of a tile that cannot share one power of two; heads up to 64 have tiles of 128 keys, wider ones of 64.)
+def _attend_all_but(q, k, v, seen, far):
+    """_attend with one key left out, whose weight is 0."""
+    seen = seen.clone()
+    seen[:, far] = False
+    return _attend(q, k, v, seen)
+
+
+SIZES = [(2, 1, 64), (3, 1, 128), (2, 2, 32)]
+PLACES = [1, 60, 64, 65, 127, 128, 200, 255, 256, 298]
+
+
+@pytest.mark.parametrize("factor", [1e6, 1e7, 1e10, 1e20, 1e30])
+@pytest.mark.parametrize("shape", SIZES, ids=str)
+def test_attention_prompts_later_keys_and_values_of_any_magnitude(ops, shape, factor):
+    """A finite key or value reaches the tokens that attend it and no others, wherever in its tile it lies."""
+    heads, kv, hd = shape
+    n = 300
+    g = _gen(n)
+    q, k, v = (_randn(g, n, h * hd) for h in (heads, kv, kv))
+    for at in PLACES:
+        ref, tol = _prompts_ref(q[:at], k[:at], v[:at], [at], [at], heads, kv, hd)
+        for far_k, far_v in ((1.0, factor), (factor, 1.0), (factor, factor)):
+            k2, v2 = k.clone(), v.clone()
+            k2[at] *= far_k
+            v2[at] *= far_v
+            out = ops.attention_prompts(q, k2, v2, _starts([n]), heads, kv, hd)
+            _check(out[:at], ref, tol, v[:at].abs().max().double())
+
+
+@pytest.mark.parametrize("prefix", [0, 3000])
+@pytest.mark.parametrize("shape", SIZES, ids=str)
+def test_attention_prompts_small_rows_before_large_ones(ops, shape, prefix):
+    """The first tokens of a sequence attend keys and values that are far smaller than the rest of their tile."""
+    heads, kv, hd = shape
+    n, small = 200, 70
+    g = _gen(n + prefix)
+    q, k, v = _randn(g, n, heads * hd), _randn(g, n + prefix, kv * hd), _randn(g, n + prefix, kv * hd)
+    for factor in (1e-5, 1e-9, 1e-25):
+        k2, v2, q2 = k.clone(), v.clone(), q.clone()
+        k2[:prefix + small] *= factor
+        v2[:prefix + small] *= factor
+        q2[:small] /= factor
+        out = ops.attention_prompts(q2, k2, v2, _starts([n]), heads, kv, hd, key_starts=_starts([n + prefix]))
+        ref, tol = _prompts_ref(q2[:small], k2[:prefix + small], v2[:prefix + small], [small], [prefix + small], heads, kv, hd)
+        _check(out[:small], ref, tol, v2[:prefix + small].abs().max().double())
+
+
+@pytest.mark.parametrize("prefix", [0, 3000])
+@pytest.mark.parametrize("shape", SIZES, ids=str)
+def test_attention_prompts_far_keys_that_are_attended(ops, shape, prefix):
+    """An attended key whose score is so low that its weight is 0, and whose value is huge: the scores, weights and values of the keys
+    beside it are as without it."""
+    heads, kv, hd = shape
+    n = 300
+    g = _gen(n + 1)
+    q, k, v = _randn(g, n, heads * hd), _randn(g, n + prefix, kv * hd), _randn(g, n + prefix, kv * hd)
+    q.view(n, heads, hd)[:, :, 0].abs_().add_(1.0)
+    seen = torch.arange(n + prefix, device="cuda")[None] <= torch.arange(n, device="cuda")[:, None] + prefix
+    for at, low, high in ((5, -1e4, 1e30), (64, -1e6, 1.0), (130, -1e10, 1e10), (250, -1e20, 1e37)):
+        k2, v2 = k.clone(), v.clone()
+        for c in range(kv):
+            k2[prefix + at, c * hd] = low
+        v2[prefix + at] = high
+        out = ops.attention_prompts(q, k2, v2, _starts([n]), heads, kv, hd, key_starts=_starts([n + prefix]))
+        for h in range(heads):
+            c = h * kv // heads
+            a, b = k2[:, c * hd:(c + 1) * hd].double(), v2[:, c * hd:(c + 1) * hd].double()
+            ref, tol = _attend_all_but(q[:, h * hd:(h + 1) * hd].double(), a, b, seen, prefix + at)
+            _check(out[:, h * hd:(h + 1) * hd], ref, tol.expand(-1, hd), 0)
+
+
+def test_attention_prompts_small_weights_of_huge_values(ops):
+    """Weights down to 2^-100 of values up to 2^110, beside ordinary ones: the sum of p |v| bounds the error, not the largest |v|."""
+    hd, n = 64, 260
+    g = _gen(3)
+    q, k, v = (_randn(g, n, hd) for _ in range(3))
+    q[:, 0] = 8.0
+    k[:, 0] = 0.0
+    for at, log2_weight, log2_value in ((3, -60, 70), (70, -100, 110), (140, -40, 36), (259, -20, 30)):
+        k2, v2 = k.clone(), v.clone()
+        k2[at, 0] = log2_weight * math.log(2.0)  # its score beside the others': 8 / sqrt(64) times it
+        v2[at] = _randn(g, hd) * 2.0 ** log2_value
+        out = ops.attention_prompts(q, k2, v2, _starts([n]), 1, 1, hd).double()
+        seen = torch.arange(n, device="cuda")[None] <= torch.arange(n, device="cuda")[:, None]
+        s = (q.double() @ k2.double().T / 8).masked_fill(~seen, -math.inf)
+        p = torch.softmax(s, 1)
+        e = ((q.double().abs() @ k2.double().abs().T) / 8).masked_fill(~seen, 0).amax(1, keepdim=True) * 2.0 ** -21
+        near = torch.where(seen.any(0)[:, None], v.double().abs(), 0).max()
+        bound = (2 * e + 2.0 ** -20) * (p @ v2.double().abs() + near)
+        assert torch.isfinite(out).all() and ((out - p @ v2.double()).abs() <= bound).all()

@@ -12,8 +12,14 @@
 // f16, bf16: one product each; O stays in tensor memory, and is rescaled only where a row's maximum has grown by more than 2^8 (a weight is at
 //   most 2^8 then; the last maximum that was used cancels in the quotient).
 // f32: every operand is split into two f16 parts, x = 2^e (hi + lo), 22 bits, with one power of two per row of Q and per tile of K and V
-//   (K and V by k_split; a row of Q where it lies in shared memory, by the thread that owns it), and a product is hi hi + hi lo + lo hi (lo lo is 2^-22 of it).  The tensor core adds with truncation, so that a sum over
-//   thousands of keys would drift by 1e-5: O is taken out after every tile and added up in registers.
+//   (K and V by k_split; a row of Q where it lies in shared memory, by the thread that owns it), and a product is hi hi + hi lo + lo hi (lo lo
+//   is 2^-22 of it).  An element is held to 2^-22 of itself or 2^-24 of its row's largest.  Rows of a K or V tile whose magnitudes are too far
+//   apart for one power of two (a row's largest element below 2^-14 of the others', or above them) are zeros in the parts: the threads
+//   that attend such a far key compute its score, and add its weighted value, in f32 from K and V themselves (eight prompts of 1000 tokens, 32 / 8
+//   heads of 64: 161 us without far keys, 323 with one in every tile, 1075 with one in 16).  What a token does not attend does not change
+//   its result beyond that rounding.
+//   The tensor core adds with truncation, so that a sum over thousands of keys would drift by 1e-5: O is taken out after every tile and added
+//   up in registers.
 //
 // Few items with many keys (a chunk of tokens behind a long prefix): the keys of an item are cut into `splits` parts, each an item of its own,
 // whose sums go to the workspace in f32 and are joined by k_join.
@@ -64,6 +70,8 @@ struct Cfg {
     static constexpr size_t SMEM = 1024 + (size_t)2 * PLANES * QBYTES + (size_t)NS * SLOT + 1024;
 };
 
+constexpr int FAR_WORDS = 4;  // of 32 rows; a tile has at most 128
+
 struct Item {
     int token0, tokens;   // first token (a row of q), tokens
     int key0, keys;       // first key (a row of k), keys of the sequence
@@ -89,7 +97,8 @@ static_assert(sizeof(Shared) <= 1024, "room behind the ring");
 // What the kernels read besides the tensor maps.
 struct PromptArgs {
     Prompts p;
-    const float *k_inv, *v_inv;          // f32: the powers of two taken out of K / V tiles
+    const float *k_inv, *v_inv;          // f32: the powers of two taken out of K / V tiles, negative where the tile has far rows,
+    const uint32_t *k_far, *v_far;       // and, for those tiles, which: bit per row, [slot][n_kv][FAR_WORDS]
     int group, tile_tokens;              // query heads per KV head, tokens of a row tile
     int slots;                           // places for (sequence, block of 2 * tile_tokens tokens)
     int splits;                          // parts of a block's keys, and where their rows' sums go: [splits][tokens][heads][head_dim], [..][2]
@@ -194,6 +203,14 @@ __device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t* r) {
         "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]),
         "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(addr)
         : "memory");
+}
+__device__ __forceinline__ float tmem_ld1(uint32_t addr) {
+    float r;
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x1.b32 {%0}, [%1];" : "=f"(r) : "r"(addr) : "memory");
+    return r;
+}
+__device__ __forceinline__ void tmem_st1(uint32_t addr, float v) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x1.b32 [%0], {%1};" ::"r"(addr), "f"(v) : "memory");
 }
 __device__ __forceinline__ void tmem_ld_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
@@ -333,6 +350,19 @@ __device__ __forceinline__ void part_of(const PromptArgs& a, int kvh, int part, 
 #pragma unroll
         for (int m = 0; m < 2; m++) it.n_tiles[m] = max(0, min(it.n_tiles[m], t1) - t0);
     }
+}
+
+// The same value, from which nothing is computed ahead: what only far keys need takes no registers of the loops around.
+template <class X>
+__device__ __forceinline__ X aside(X x) {
+    if constexpr (sizeof(X) == 8)
+        asm volatile("" : "+l"(x));
+    else
+        asm volatile("" : "+r"(x));
+    return x;
+}
+__device__ __forceinline__ size_t far_tile(const PromptArgs& a, const Item* it, int i) {
+    return ((size_t)(it->key_slot0 + i) * a.p.n_kv + it->kvh) * FAR_WORDS;
 }
 
 // A CTA's items one after the other, by a whole warp: the list is dealt to the CTAs forwards and backwards in turn, and begins with the
@@ -826,13 +856,51 @@ k_attention_prompts(const __grid_constant__ CUtensorMap map_q, const __grid_cons
                     }
                 };
                 for (int i = 0; i < n && ok; i++) {
-                    const float scale = __fmul_rn(row_scale, k_next), v_before = v_now;
+                    const float k_now = k_next, v_before = fabsf(v_now);
+                    const bool k_far = k_now < 0.0f, v_far = v_next < 0.0f;
+                    const float scale = k_far ? a.scale_log2 : __fmul_rn(row_scale, k_now);
                     v_now = v_next;
                     if (i + 1 < n) k_next = k_inv[(size_t)(i + 1) * a.p.n_kv], v_next = v_inv[(size_t)(i + 1) * a.p.n_kv];
                     if (!(ok = __all_sync(0xffffffffu, bar_wait(sh, &sh->s_full[m], (done + i) & 1)))) break;
                     tc_fence_after();
                     const int seen = limit - i * NK;
                     const bool masked = __any_sync(0xffffffffu, seen < NK);
+                    if (__builtin_expect(k_far, 0)) {  // S without its powers of two (products with which are exact), far keys' anew
+#pragma unroll 1
+                        for (int c = 0; c < NK / 32; c++) {
+                            float s[32];
+                            tmem_ld32(t_s + 32 * c, s);
+                            tmem_ld_wait();
+#pragma unroll
+                            for (int x = 0; x < 32; x++) s[x] = __fmul_rn(__fmul_rn(s[x], next_q), -k_now);
+                            tmem_st32(t_s + 32 * c, s);
+                        }
+                        tmem_st_wait();
+                        const Item* at = aside(it);
+                        const int row = aside(r), width = aside(hd);
+                        const uint32_t* far = a.k_far + far_tile(a, at, i);
+                        const float* q = reinterpret_cast<const float*>(a.p.q) + (size_t)(at->token0 + m * a.tile_tokens + row / a.group) * a.p.q_stride +
+                                         (size_t)(at->kvh * a.group + row % a.group) * width;
+                        const float* k0 = reinterpret_cast<const float*>(a.p.k) + (size_t)(at->key0 + i * NK) * a.p.k_stride + (size_t)at->kvh * width;
+#pragma unroll 1
+                        for (int w = 0; w < NK / 32; w++)
+#pragma unroll 1
+                            for (uint32_t bits = far[w]; bits; bits &= bits - 1) {
+                                const int t = 32 * w + __ffs(bits) - 1;
+                                float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+                                if (t < seen) {
+                                    const float* key = k0 + (size_t)t * a.p.k_stride;
+#pragma unroll 2
+                                    for (int d = 0; d < width; d += 4) {
+                                        const float4 x = *reinterpret_cast<const float4*>(q + d), y = *reinterpret_cast<const float4*>(key + d);
+                                        sum.x = fmaf(x.x, y.x, sum.x), sum.y = fmaf(x.y, y.y, sum.y), sum.z = fmaf(x.z, y.z, sum.z), sum.w = fmaf(x.w, y.w, sum.w);
+                                    }
+                                }
+                                __syncwarp();
+                                tmem_st1(t_s + t, (sum.x + sum.y) + (sum.z + sum.w));
+                            }
+                        tmem_st_wait();
+                    }
                     float tops[4] = {NEG, NEG, NEG, NEG};
 #pragma unroll 1
                     for (int c = 0; c < NK / 32; c++) {
@@ -854,6 +922,35 @@ k_attention_prompts(const __grid_constant__ CUtensorMap map_q, const __grid_cons
                     // weights up to 2^8, so that the low parts of small ones stay in f16's range
                     const float base = new_max == NEG ? 0.0f : PR_LAZY - new_max;
                     row_max = new_max;
+                    if (__builtin_expect(v_far, 0)) {  // the far keys' weighted values; the tensor core's product has zeros there
+                        if (C::O_BUFS == 2 && i > 0) take_o(i - 1, v_before);
+#pragma unroll
+                        for (int d = 0; d < HDP; d++) o[d] = __fmul_rn(o[d], f);
+                        const Item* at = aside(it);
+                        const int width = aside(hd);
+                        const uint32_t* far = a.v_far + far_tile(a, at, i);
+                        const float* v0 = reinterpret_cast<const float*>(a.p.v) + (size_t)(at->key0 + i * NK) * a.p.v_stride + (size_t)at->kvh * width;
+#pragma unroll 1
+                        for (int w = 0; w < NK / 32; w++)
+#pragma unroll 1
+                            for (uint32_t bits = far[w]; bits; bits &= bits - 1) {
+                                const int t = 32 * w + __ffs(bits) - 1;
+                                const float score = tmem_ld1(t_s + t);
+                                tmem_ld_wait();
+                                if (t < seen) {
+                                    const float weight = exp2_approx(fmaf(score, scale, base));
+                                    const float* value = v0 + (size_t)t * a.p.v_stride;
+#pragma unroll
+                                    for (int d = 0; d < HDP; d += 4)
+                                        if (d < width) {
+                                            const float4 y = *reinterpret_cast<const float4*>(value + d);
+                                            o[d] = fmaf(weight, y.x, o[d]), o[d + 1] = fmaf(weight, y.y, o[d + 1]);
+                                            o[d + 2] = fmaf(weight, y.z, o[d + 2]), o[d + 3] = fmaf(weight, y.w, o[d + 3]);
+                                        }
+                                }
+                                __syncwarp();
+                            }
+                    }
                     const f32x2 base2 = pack2(base, base), scale2 = pack2(scale, scale), minus = pack2(-1.0f, -1.0f);
                     f32x2 sum[2] = {pack2(0.f, 0.f), pack2(0.f, 0.f)};
 #pragma unroll 1
@@ -890,8 +987,8 @@ k_attention_prompts(const __grid_constant__ CUtensorMap map_q, const __grid_cons
                     tc_fence_before();
                     __syncwarp();
                     if (lane == 0) bar_arrive(&sh->p_ready[m]);
-                    if (C::O_BUFS == 2 && i > 0) take_o(i - 1, v_before);
-                    rescale = f;
+                    if (C::O_BUFS == 2 && i > 0 && !v_far) take_o(i - 1, v_before);
+                    rescale = v_far ? 1.0f : f;
                 }
                 if (n > 0 && ok) {
                     // the next item's Q while the last P V runs (all of this one's scores have been computed)
@@ -902,7 +999,7 @@ k_attention_prompts(const __grid_constant__ CUtensorMap map_q, const __grid_cons
                     }
                     if ((ok = __all_sync(0xffffffffu, bar_wait(sh, &sh->o_full[m], items & 1)))) {
                         tc_fence_after();
-                        take_o(n - 1, v_now);
+                        take_o(n - 1, fabsf(v_now));
                     }
                 }
             }
@@ -1024,17 +1121,22 @@ struct SplitArgs {
     Prompts p;
     __half* to[2];  // keys, values: [2][rows][heads * head_dim]
     float* inv[2];
+    uint32_t* far[2];
     int lanes;      // of a row: head_dim / 4 rounded up to a power of two
 };
 constexpr int SP_THREADS = 256;
 
-// A tile of K or V per CTA, held in registers between the search for its largest magnitude and its parts.  Bound: HBM (4 bytes in, 4 out
+// A tile of K or V per CTA, held in registers between the search for its rows' largest magnitudes and its parts.  Bound: HBM (4 bytes in, 4 out
 // per element), the launch for short prompts.
+// The tile's power of two is that of its largest row, if no row lies below 2^-14 of it (its largest element then has 24 bits or more above the
+// parts' 2^-25).  Otherwise it is the row's from which most rows lie within 2^-14, the larger of equals; the others are far.
 template <int NK>
 __global__ void __launch_bounds__(SP_THREADS) k_split(const __grid_constant__ SplitArgs a) {
     pdl_trigger();
     pdl_wait();
-    __shared__ float red[SP_THREADS / 32];
+    __shared__ uint2 red[SP_THREADS / 32];
+    __shared__ uint32_t row_top[NK];  // bits of the rows' largest magnitudes
+    __shared__ unsigned long long best[SP_THREADS / 32];
     const int hd = a.p.head_dim, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int val = blockIdx.x & 1, kvh = (blockIdx.x >> 1) % a.p.n_kv, slot = (blockIdx.x >> 1) / a.p.n_kv;
     const int32_t* ks = a.p.key_starts ? a.p.key_starts : a.p.starts;
@@ -1049,33 +1151,73 @@ __global__ void __launch_bounds__(SP_THREADS) k_split(const __grid_constant__ Sp
     const bool in = 4 * piece < hd;
     constexpr int MOST = NK * (NK == 128 ? 16 : 32) / SP_THREADS;  // rows of a thread, at most (heads of up to 64 have tiles of 128 keys)
     float4 x[MOST];
-    float top = 0.0f;
 #pragma unroll
     for (int i = 0; i < MOST; i++) {
         const int row = row0 + i * step;
         x[i] = in && row < rows ? *reinterpret_cast<const float4*>(src + row * stride) : make_float4(0.f, 0.f, 0.f, 0.f);
     }
+    // Bits of magnitudes: their difference counts powers of two.  First by the threads' pieces of rows, zeros left out: where none of them lies below
+    // the window, no row does.
+    constexpr uint32_t WINDOW = 14u << 23;
+    uint32_t most = 0, least = 0xFFFFFFFFu;
 #pragma unroll
-    for (int i = 0; i < MOST; i++) top = fmaxf(top, finite_max(x[i]));
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-    if (lane == 0) red[warp] = top;
+    for (int i = 0; i < MOST; i++) {
+        const uint32_t top = __float_as_uint(finite_max(x[i]));
+        most = max(most, top), least = min(least, top - 1);
+    }
+    most = __reduce_max_sync(0xffffffffu, most), least = __reduce_min_sync(0xffffffffu, least);
+    if (lane == 0) red[warp] = make_uint2(most, least);
     __syncthreads();
 #pragma unroll
-    for (int w = 0; w < SP_THREADS / 32; w++) top = fmaxf(top, red[w]);
-    const float f = to_range(top);
+    for (int w = 0; w < SP_THREADS / 32; w++) most = max(most, red[w].x), least = min(least, red[w].y);
+    bool far_rows = most != 0 && most - (least + 1) > WINDOW;
+    if (far_rows) {  // by whole rows
+        for (int i = 0; i < MOST; i++) {
+            float top = finite_max(x[i]);
+            for (int o = a.lanes / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+            if (piece == 0 && row0 + i * step < NK) row_top[row0 + i * step] = __float_as_uint(top);
+        }
+        __syncthreads();
+        least = 0xFFFFFFFFu;
+        for (int r = lane; r < NK; r += 32) least = min(least, row_top[r] - 1);
+        far_rows = most - (__reduce_min_sync(0xffffffffu, least) + 1) > WINDOW;
+    }
+    if (far_rows) {
+        unsigned long long mine = 0;
+        if (threadIdx.x < NK) {
+            const uint32_t top = row_top[threadIdx.x];
+            uint32_t count = 0;
+            for (int r = 0; r < NK; r++) count += row_top[r] != 0 && top - row_top[r] <= WINDOW;
+            mine = top ? (unsigned long long)count << 32 | top : 0;
+        }
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) mine = max(mine, __shfl_xor_sync(0xffffffffu, mine, o));
+        if (lane == 0) best[warp] = mine;
+        __syncthreads();
+#pragma unroll
+        for (int w = 0; w < SP_THREADS / 32; w++) mine = max(mine, best[w]);
+        most = (uint32_t)mine;
+    }
+    const float f = to_range(__uint_as_float(most));
+    auto far_row = [&](int row) { return row_top[row] != 0 && most - row_top[row] > WINDOW; };  // (above: the difference wraps)
+    const size_t tile = (size_t)slot * a.p.n_kv + kvh;
+    if (far_rows && threadIdx.x < NK) {
+        const uint32_t word = __ballot_sync(0xffffffffu, far_row(threadIdx.x));
+        if (lane == 0) a.far[val][tile * FAR_WORDS + warp] = word;
+    }
     __half* dst = a.to[val] + (size_t)first * dim + (size_t)kvh * hd + 4 * piece;
 #pragma unroll
     for (int i = 0; i < MOST; i++) {
         const int row = row0 + i * step;
         if (in && row < rows) {
             uint2 hi, lo;
+            if (far_rows && far_row(row)) x[i] = make_float4(0.f, 0.f, 0.f, 0.f);
             split4(x[i], f, hi, lo);
             *reinterpret_cast<uint2*>(dst + row * dim) = hi;
             *reinterpret_cast<uint2*>(dst + row * dim + plane) = lo;
         }
     }
-    if (threadIdx.x == 0) a.inv[val][(size_t)slot * a.p.n_kv + kvh] = __fdiv_rn(1.0f, f);
+    if (threadIdx.x == 0) a.inv[val][tile] = far_rows ? -__fdiv_rn(1.0f, f) : __fdiv_rn(1.0f, f);
 }
 
 // The parts of the rows' keys, added up in their order: four values of a row per thread (threadIdx.x), all parts' loads under way together.
@@ -1169,7 +1311,7 @@ int key_splits(const Prompts& p) {
 }
 
 struct Workspace {
-    size_t k = 0, v = 0, k_inv = 0, v_inv = 0, part_o = 0, part_ml = 0, bytes;
+    size_t k = 0, v = 0, k_inv = 0, v_inv = 0, k_far = 0, v_far = 0, part_o = 0, part_ml = 0, bytes;
     explicit Workspace(const Prompts& p) {
         const size_t key_slots = (size_t)places(p.n_keys, p.n_seqs, keys_per_tile(p));
         size_t at = 0;
@@ -1183,6 +1325,8 @@ struct Workspace {
             v = take((size_t)p.n_keys * p.n_kv * p.head_dim * 4);
             k_inv = take(key_slots * p.n_kv * 4);
             v_inv = take(key_slots * p.n_kv * 4);
+            k_far = take(key_slots * p.n_kv * FAR_WORDS * 4);
+            v_far = take(key_slots * p.n_kv * FAR_WORDS * 4);
         }
         const int splits = key_splits(p);
         if (splits > 1) {
@@ -1215,7 +1359,8 @@ cudaError_t launch_typed(cudaStream_t st, const Prompts& p, void* workspace) {
     a.splits = key_splits(p);
     a.part_o = (float*)(base + w.part_o), a.part_ml = (float*)(base + w.part_ml);
     if (PLANES == 2 && p.n_keys > 0) {
-        SplitArgs s{p, {(__half*)(base + w.k), (__half*)(base + w.v)}, {(float*)(base + w.k_inv), (float*)(base + w.v_inv)}, 1};
+        SplitArgs s{p, {(__half*)(base + w.k), (__half*)(base + w.v)}, {(float*)(base + w.k_inv), (float*)(base + w.v_inv)},
+                    {(uint32_t*)(base + w.k_far), (uint32_t*)(base + w.v_far)}, 1};
         while (s.lanes * 4 < p.head_dim) s.lanes *= 2;
         const long long ctas = (long long)places(p.n_keys, p.n_seqs, C::NK) * p.n_kv * 2;
         if (ctas > 0x7FFFFFFFll) return cudaErrorInvalidValue;
@@ -1224,6 +1369,7 @@ cudaError_t launch_typed(cudaStream_t st, const Prompts& p, void* workspace) {
         k = s.to[0], v = s.to[1];
         ks = vs = (size_t)p.n_kv * p.head_dim;
         a.k_inv = s.inv[0], a.v_inv = s.inv[1];
+        a.k_far = s.far[0], a.v_far = s.far[1];
     }
     CUtensorMap mq, mk, mv;  // (without any keys none is read)
     if ((e = encode_heads(p.q, p.dtype, p.head_dim, p.n_heads, p.n_tokens, 1, p.q_stride, a.group, a.tile_tokens, &mq)) != cudaSuccess) return e;
