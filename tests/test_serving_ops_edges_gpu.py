@@ -125,3 +125,14 @@ def test_attention_prompts_small_weights_of_huge_values(ops):
         near = torch.where(seen.any(0)[:, None], v.double().abs(), 0).max()
         bound = (2 * e + 2.0 ** -20) * (p @ v2.double().abs() + near)
         assert torch.isfinite(out).all() and ((out - p @ v2.double()).abs() <= bound).all()
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+def test_attention_prompts_values_near_the_end_of_f32(ops, hd):
+    """A weighted mean of values of up to 1e37 is no larger than they are."""
+    n = 20
+    g = _gen(hd)
+    q, k, v = _randn(g, n, hd), _randn(g, n, hd), _randn(g, n, hd).abs() * 1e36 + 8e36
+    out = ops.attention_prompts(q, k, v, _starts([n]), 1, 1, hd)
+    ref, tol = _prompts_ref(q, k, v, [n], [n], 1, 1, hd)
+    _check(out, ref, tol, v.abs().max().double())

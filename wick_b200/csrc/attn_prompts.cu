@@ -51,7 +51,7 @@ constexpr int PR_THREADS = 384;   // TMA, MMA, V check, items; 2 x 4 softmax war
 constexpr int PR_ITEMS = 3;       // items that are known ahead
 constexpr int PR_MASKED = 8;      // tiles that some row of a CTA sees in part: at most 256 / 64 + 2
 constexpr uint32_t PR_SPIN_LIMIT = 1u << 24;  // about half a second (2^18: 8 ms)
-constexpr float PR_LAZY = 8.0f;
+constexpr float PR_LAZY = 8.0f, PR_DOWN = 0x1p-8f;  // 2^-PR_LAZY
 
 template <int PLANES, int HDP>
 struct Cfg {
@@ -856,7 +856,7 @@ k_attention_prompts(const __grid_constant__ CUtensorMap map_q, const __grid_cons
                     }
                 };
                 for (int i = 0; i < n && ok; i++) {
-                    const float k_now = k_next, v_before = fabsf(v_now);
+                    const float k_now = k_next, v_before = __fmul_rn(fabsf(v_now), PR_DOWN);
                     const bool k_far = k_now < 0.0f, v_far = v_next < 0.0f;
                     const float scale = k_far ? a.scale_log2 : __fmul_rn(row_scale, k_now);
                     v_now = v_next;
@@ -919,7 +919,8 @@ k_attention_prompts(const __grid_constant__ CUtensorMap map_q, const __grid_cons
                     if (C::O_BUFS == 1 && i > 0) take_o(i - 1, v_before);
                     const float new_max = fmaxf(row_max, __fmul_rn(top, scale));
                     const float f = row_max == NEG ? 0.0f : exp2_approx(row_max - new_max);
-                    // weights up to 2^8, so that the low parts of small ones stay in f16's range
+                    // weights up to 2^8 in the products, so that the low parts of small ones stay in f16's range; in the sums up to 1 again, so that
+                    // values near the end of f32 stay in its range
                     const float base = new_max == NEG ? 0.0f : PR_LAZY - new_max;
                     row_max = new_max;
                     if (__builtin_expect(v_far, 0)) {  // the far keys' weighted values; the tensor core's product has zeros there
@@ -938,7 +939,7 @@ k_attention_prompts(const __grid_constant__ CUtensorMap map_q, const __grid_cons
                                 const float score = tmem_ld1(t_s + t);
                                 tmem_ld_wait();
                                 if (t < seen) {
-                                    const float weight = exp2_approx(fmaf(score, scale, base));
+                                    const float weight = __fmul_rn(exp2_approx(fmaf(score, scale, base)), PR_DOWN);
                                     const float* value = v0 + (size_t)t * a.p.v_stride;
 #pragma unroll
                                     for (int d = 0; d < HDP; d += 4)
@@ -981,7 +982,7 @@ k_attention_prompts(const __grid_constant__ CUtensorMap map_q, const __grid_cons
                     {
                         float s0, s1;
                         unpack2(add2(sum[0], sum[1]), s0, s1);
-                        row_sum = fmaf(row_sum, f, s0 + s1);
+                        row_sum = fmaf(row_sum, f, __fmul_rn(s0 + s1, PR_DOWN));
                     }
                     tmem_st_wait();
                     tc_fence_before();
@@ -999,7 +1000,7 @@ k_attention_prompts(const __grid_constant__ CUtensorMap map_q, const __grid_cons
                     }
                     if ((ok = __all_sync(0xffffffffu, bar_wait(sh, &sh->o_full[m], items & 1)))) {
                         tc_fence_after();
-                        take_o(n - 1, fabsf(v_now));
+                        take_o(n - 1, __fmul_rn(fabsf(v_now), PR_DOWN));
                     }
                 }
             }
