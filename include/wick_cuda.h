@@ -439,7 +439,8 @@ int32_t wick_cuda_attention_q4(const wick_cuda_kv_q4* cache, const void* q_dev, 
  * v are q_stride / k_stride / v_stride elements apart; out rows are dense.  head_dim is a multiple of 8 and at most 128;
  * pointers and row strides are multiples of 16 bytes.  f32 elements are held to 2^-22 of themselves or 2^-24 of their row's (token's
  * and head's) largest, whatever the other rows hold; in 16 bits the weights are rounded to that type.  A key or value that is infinite or NaN
- * reaches the tokens that attend it and no others.  workspace_dev: 128-byte aligned, as many bytes as
+ * reaches the tokens that attend it and no others: a score of -inf has no weight, an infinite value makes its column infinite (in 16 bits
+ * NaN where the weight rounds to 0), values of both infinities make it NaN.  workspace_dev: 128-byte aligned, as many bytes as
  * wick_cuda_attention_prompts_workspace says, with any content; of this call alone until it has finished. */
 int32_t wick_cuda_attention_prompts_workspace(int32_t dtype, uint32_t n_seqs, uint32_t n_tokens, uint32_t n_keys, uint32_t n_heads,
                                               uint32_t n_kv_heads, uint32_t head_dim, uint64_t* bytes);

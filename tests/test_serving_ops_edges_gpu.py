@@ -136,3 +136,47 @@ def test_attention_prompts_values_near_the_end_of_f32(ops, hd):
     out = ops.attention_prompts(q, k, v, _starts([n]), 1, 1, hd)
     ref, tol = _prompts_ref(q, k, v, [n], [n], 1, 1, hd)
     _check(out, ref, tol, v.abs().max().double())
+
+
+# ── packed prompts: infinities ─────────────────────────────────────────────────────────────────────
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("shape", SIZES, ids=str)
+def test_attention_prompts_keys_of_minus_infinity(ops, dtype, shape):
+    """A key whose score is -inf has no weight, also where q has no more bits than 16-bit types."""
+    heads, kv, hd = shape
+    n = 300
+    g = _gen(hd)
+    q, k, v = (_randn(g, n, h * hd).half().to(dtype) for h in (heads, kv, kv))
+    q.view(n, heads, hd)[:, :, 3].abs_().add_(0.5)
+    seen = torch.arange(n, device="cuda")[None] <= torch.arange(n, device="cuda")[:, None]
+    for at in (1, 10, 64, 140, 299):
+        k2 = k.clone()
+        k2.view(n, kv, hd)[at, :, 3] = -math.inf
+        out = ops.attention_prompts(q, k2, v, _starts([n]), heads, kv, hd)
+        for h in range(heads):
+            c = h * kv // heads
+            ref, tol = _attend_all_but(q[:, h * hd:(h + 1) * hd].double(), k[:, c * hd:(c + 1) * hd].double(), v[:, c * hd:(c + 1) * hd].double(), seen, at)
+            _check(out[:, h * hd:(h + 1) * hd], ref, tol.expand(-1, hd), v.abs().max().double())
+
+
+@pytest.mark.parametrize("shape", SIZES, ids=str)
+def test_attention_prompts_infinite_values_in_f32(ops, shape):
+    """An infinite value makes its column of the tokens that attend it infinite, whatever its weight and wherever in a tile it lies; two of
+    different signs make it NaN; nothing else changes."""
+    heads, kv, hd = shape
+    n, inf = 700, math.inf
+    g = _gen(hd + 1)
+    q, k, v = (_randn(g, n, h * hd) for h in (heads, kv, kv))
+    q *= 30  # (weights down to nothing)
+    clean = ops.attention_prompts(q, k, v, _starts([n]), heads, kv, hd).view(n, heads, hd)
+    for at, value, then in ((10, inf, 400), (64, -inf, 650), (127, inf, 128), (300, -inf, 301), (0, math.nan, 1)):
+        v2 = v.clone()
+        v2.view(n, kv, hd)[at, :, 5] = value
+        v2.view(n, kv, hd)[then, :, 6] = value
+        v2.view(n, kv, hd)[then, :, 5] = -value
+        out = ops.attention_prompts(q, k, v2, _starts([n]), heads, kv, hd).view(n, heads, hd)
+        want = clean.clone()
+        want[at:then, :, 5] = value
+        want[then:, :, 5] = math.nan
+        want[then:, :, 6] = value
+        assert torch.equal(out.nan_to_num(7e30, 8e30, 9e30), want.nan_to_num(7e30, 8e30, 9e30))

@@ -17,7 +17,8 @@
 //   apart for one power of two (a row's largest element below 2^-14 of the others', or above them) are zeros in the parts: the threads
 //   that attend such a far key compute its score, and add its weighted value, in f32 from K and V themselves (eight prompts of 1000 tokens, 32 / 8
 //   heads of 64: 161 us without far keys, 323 with one in every tile, 1075 with one in 16).  What a token does not attend does not change
-//   its result beyond that rounding.
+//   its result beyond that rounding.  Keys with infinities or NaN are far, too; values that are not finite are zeros in the parts and are added
+//   to the rows that attend them at the end.
 //   The tensor core adds with truncation, so that a sum over thousands of keys would drift by 1e-5: O is taken out after every tile and added
 //   up in registers.
 //
@@ -25,7 +26,8 @@
 // whose sums go to the workspace in f32 and are joined by k_join.
 //
 // Masked places may hold anything.  Scores are masked after the product; V is different, 0 * NaN is NaN: a warp looks at every V
-// tile that some row sees in part, zeroes what is not finite, and notes the keys; rows that attend such a key add its values at the end.
+// tile that some row sees in part, zeroes what is not finite (in f32: left behind the sequences in the workspace), and notes the keys; rows that
+// attend such a key add its values at the end.
 //
 // Bound, on a B200: the softmax and its MMAs in turn.  A pair of f32 tiles (heads of 64) takes 5300 cycles, 58 % of them MMAs: 2000 waiting for P V
 // and the next scores, 600 the maximum, 2150 the weights and their parts, 500 adding O.  A pair in 16 bits takes 3750 (heads of 64, 2750 the weights,
@@ -97,8 +99,9 @@ static_assert(sizeof(Shared) <= 1024, "room behind the ring");
 // What the kernels read besides the tensor maps.
 struct PromptArgs {
     Prompts p;
-    const float *k_inv, *v_inv;          // f32: the powers of two taken out of K / V tiles, negative where the tile has far rows,
-    const uint32_t *k_far, *v_far;       // and, for those tiles, which: bit per row, [slot][n_kv][FAR_WORDS]
+    const float *k_inv, *v_inv;          // f32: the powers of two taken out of K / V tiles, negative where the tile has far or bad rows,
+    const uint32_t *k_far, *v_far;       // and, for those tiles, which: bit per row, [slot][n_kv][FAR_WORDS];
+    const uint32_t* v_bad;               // rows of V with elements that are not finite, likewise
     int group, tile_tokens;              // query heads per KV head, tokens of a row tile
     int slots;                           // places for (sequence, block of 2 * tile_tokens tokens)
     int splits;                          // parts of a block's keys, and where their rows' sums go: [splits][tokens][heads][head_dim], [..][2]
@@ -260,20 +263,24 @@ __device__ __forceinline__ float to_range(float top) {
     if (e == 0) return top > 0.0f ? 0x1p126f : 1.0f;  // (subnormal: as far as one factor goes)
     return __uint_as_float((uint32_t)min(253, 127 + 13 + 127 - e) << 23);
 }
-__device__ __forceinline__ void split4(float4 v, float f, uint2& hi, uint2& lo) {
+__device__ __forceinline__ void split4(float4 v, float f, uint2& hi, uint2& lo) {  // (finite, and below 2^14 with the factor)
     const float x[4] = {v.x, v.y, v.z, v.w};
     float h[4], l[4];
 #pragma unroll
     for (int i = 0; i < 4; i++) {
         const float y = __fmul_rn(x[i], f);
         h[i] = __uint_as_float(__float_as_uint(y) & 0xFFFFE000u);  // 11 bits: exact in f16
-        l[i] = fabsf(y) <= 65504.0f ? __fsub_rn(y, h[i]) : 0.0f;   // (an infinity's or NaN's high part says it)
+        l[i] = __fsub_rn(y, h[i]);
     }
     hi = make_uint2(pack16<__half>(h[0], h[1]), pack16<__half>(h[2], h[3]));
     lo = make_uint2(pack16<__half>(l[0], l[1]), pack16<__half>(l[2], l[3]));
 }
-__device__ __forceinline__ float finite_abs(float x) { return fabsf(x) <= 3.402823466e38f ? fabsf(x) : 0.0f; }
-__device__ __forceinline__ float finite_max(float4 v) { return fmaxf(fmaxf(finite_abs(v.x), finite_abs(v.y)), fmaxf(finite_abs(v.z), finite_abs(v.w))); }
+constexpr float MAX_F32 = 3.402823466e38f;
+__device__ __forceinline__ float finite(float x) { return fabsf(x) <= MAX_F32 ? x : 0.0f; }
+__device__ __forceinline__ float4 finite(float4 v) { return make_float4(finite(v.x), finite(v.y), finite(v.z), finite(v.w)); }
+__device__ __forceinline__ uint32_t magnitude(float4 v) {  // the largest one's bits
+    return max(max(__float_as_uint(v.x) & 0x7FFFFFFFu, __float_as_uint(v.y) & 0x7FFFFFFFu), max(__float_as_uint(v.z) & 0x7FFFFFFFu, __float_as_uint(v.w) & 0x7FFFFFFFu));
+}
 
 // The blocks of 2 * tile_tokens tokens, counted through the sequences, by a whole warp: how many there are (want < 0), or which sequence has number
 // `want` and which of its blocks that is (*seq -1: none).  With more sequences than a warp can walk through for every item, numbers are
@@ -688,7 +695,7 @@ k_attention_prompts(const __grid_constant__ CUtensorMap map_q, const __grid_cons
                                 if (r / 32 == x) found[x] |= rows << (r % 32);
                         }
                     }
-                    if (lane < 4) notes->mask[i - first_masked][lane] = lane == 0 ? found[0] : lane == 1 ? found[1] : lane == 2 ? found[2] : found[3];
+                    if (PLANES == 1 && lane < 4) notes->mask[i - first_masked][lane] = lane == 0 ? found[0] : lane == 1 ? found[1] : lane == 2 ? found[2] : found[3];
                     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 }
                 __syncwarp();
@@ -761,6 +768,7 @@ k_attention_prompts(const __grid_constant__ CUtensorMap map_q, const __grid_cons
             const bool real = r < a.tile_tokens * a.group && j < it->tokens;
             const int limit = real ? it->visible(j) : 0;
             float row_max = NEG, row_sum = 0.0f;
+            bool bad = false;  // f32: some tile has values that are not finite
             float o[C::O_IN_TMEM ? 1 : HDP];
             if constexpr (C::O_IN_TMEM) {
                 for (int i = 0; i < n && ok; i++) {
@@ -929,12 +937,12 @@ k_attention_prompts(const __grid_constant__ CUtensorMap map_q, const __grid_cons
                         for (int d = 0; d < HDP; d++) o[d] = __fmul_rn(o[d], f);
                         const Item* at = aside(it);
                         const int width = aside(hd);
-                        const uint32_t* far = a.v_far + far_tile(a, at, i);
+                        const uint32_t *far = a.v_far + far_tile(a, at, i), *not_finite = a.v_bad + far_tile(a, at, i);
                         const float* v0 = reinterpret_cast<const float*>(a.p.v) + (size_t)(at->key0 + i * NK) * a.p.v_stride + (size_t)at->kvh * width;
 #pragma unroll 1
                         for (int w = 0; w < NK / 32; w++)
 #pragma unroll 1
-                            for (uint32_t bits = far[w]; bits; bits &= bits - 1) {
+                            for (uint32_t bits = (bad |= not_finite[w] != 0, far[w]); bits; bits &= bits - 1) {
                                 const int t = 32 * w + __ffs(bits) - 1;
                                 const float score = tmem_ld1(t_s + t);
                                 tmem_ld_wait();
@@ -944,7 +952,7 @@ k_attention_prompts(const __grid_constant__ CUtensorMap map_q, const __grid_cons
 #pragma unroll
                                     for (int d = 0; d < HDP; d += 4)
                                         if (d < width) {
-                                            const float4 y = *reinterpret_cast<const float4*>(value + d);
+                                            const float4 y = finite(*reinterpret_cast<const float4*>(value + d));
                                             o[d] = fmaf(weight, y.x, o[d]), o[d + 1] = fmaf(weight, y.y, o[d + 1]);
                                             o[d + 2] = fmaf(weight, y.z, o[d + 2]), o[d + 3] = fmaf(weight, y.w, o[d + 3]);
                                         }
@@ -1073,23 +1081,35 @@ k_attention_prompts(const __grid_constant__ CUtensorMap map_q, const __grid_cons
                     write_32(c, x);
                 }
             }
-            for (int i = first_masked; i < nt; i++)
+            auto add_not_finite = [&](int first, uint32_t bits) {  // of the keys from `first` on that have a bit
+                for (; bits; bits &= bits - 1) {
+                    const int t = first + __ffs(bits) - 1;
+                    if (t >= limit || !ok) continue;
+                    const T* v = reinterpret_cast<const T*>(a.p.v) + (size_t)(it->key0 + t) * a.p.v_stride + (size_t)it->kvh * hd;
 #pragma unroll 1
-                for (int w = 0; w < NK / 32; w++)
-                    for (uint32_t bits = it->mask[i - first_masked][w]; bits; bits &= bits - 1) {
-                        const int t = i * NK + w * 32 + __ffs(bits) - 1;
-                        if (t >= limit || !ok) continue;
-                        const T* v = reinterpret_cast<const T*>(a.p.v) + (size_t)(it->key0 + t) * a.p.v_stride + (size_t)it->kvh * hd;
-#pragma unroll 1
-                        for (int d = 0; d < hd; d++) {
-                            const float y = to_f32(v[d]);
-                            if (fabsf(y) <= 3.402823466e38f) continue;
-                            if (split)
-                                sums[d] = __fadd_rn(sums[d], y);
-                            else
-                                out[d] = from_f32<T>(__fadd_rn(to_f32(out[d]), y));
-                        }
+                    for (int d = 0; d < hd; d++) {
+                        const float y = to_f32(v[d]);
+                        if (fabsf(y) <= MAX_F32) continue;
+                        if (split)
+                            sums[d] = __fadd_rn(sums[d], y);
+                        else
+                            out[d] = from_f32<T>(__fadd_rn(to_f32(out[d]), y));
                     }
+                }
+            };
+            if constexpr (PLANES == 1) {
+                for (int i = first_masked; i < nt; i++)
+#pragma unroll 1
+                    for (int w = 0; w < NK / 32; w++) add_not_finite(i * NK + w * 32, it->mask[i - first_masked][w]);
+            } else if (bad) {
+#pragma unroll 1
+                for (int i = 0; i < n; i++) {
+                    const size_t tile = far_tile(a, it, i);
+                    if (a.v_inv[tile / FAR_WORDS] >= 0.0f) continue;
+#pragma unroll 1
+                    for (int w = 0; w < NK / 32; w++) add_not_finite(i * NK + w * 32, a.v_bad[tile + w]);
+                }
+            }
             tc_fence_before();  // (tensor memory has been read before the next P V, which waits for p_ready)
             done += n, items += n > 0 ? 1 : 0;
             leave_item(k);
@@ -1122,7 +1142,7 @@ struct SplitArgs {
     Prompts p;
     __half* to[2];  // keys, values: [2][rows][heads * head_dim]
     float* inv[2];
-    uint32_t* far[2];
+    uint32_t *far[2], *v_bad;
     int lanes;      // of a row: head_dim / 4 rounded up to a power of two
 };
 constexpr int SP_THREADS = 256;
@@ -1130,13 +1150,13 @@ constexpr int SP_THREADS = 256;
 // A tile of K or V per CTA, held in registers between the search for its rows' largest magnitudes and its parts.  Bound: HBM (4 bytes in, 4 out
 // per element), the launch for short prompts.
 // The tile's power of two is that of its largest row, if no row lies below 2^-14 of it (its largest element then has 24 bits or more above the
-// parts' 2^-25).  Otherwise it is the row's from which most rows lie within 2^-14, the larger of equals; the others are far.
+// parts' 2^-25); elements that are not finite do not count.  Otherwise it is the row's from which most rows lie within 2^-14, the larger of equals; the others are far.
 template <int NK>
 __global__ void __launch_bounds__(SP_THREADS) k_split(const __grid_constant__ SplitArgs a) {
     pdl_trigger();
     pdl_wait();
     __shared__ uint2 red[SP_THREADS / 32];
-    __shared__ uint32_t row_top[NK];  // bits of the rows' largest magnitudes
+    __shared__ uint32_t row_top[NK], row_bad[NK];  // bits of the rows' largest finite magnitudes; whether they have others
     __shared__ unsigned long long best[SP_THREADS / 32];
     const int hd = a.p.head_dim, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int val = blockIdx.x & 1, kvh = (blockIdx.x >> 1) % a.p.n_kv, slot = (blockIdx.x >> 1) / a.p.n_kv;
@@ -1159,11 +1179,11 @@ __global__ void __launch_bounds__(SP_THREADS) k_split(const __grid_constant__ Sp
     }
     // Bits of magnitudes: their difference counts powers of two.  First by the threads' pieces of rows, zeros left out: where none of them lies below
     // the window, no row does.
-    constexpr uint32_t WINDOW = 14u << 23;
+    constexpr uint32_t WINDOW = 14u << 23, INF = 0x7F800000u;
     uint32_t most = 0, least = 0xFFFFFFFFu;
 #pragma unroll
     for (int i = 0; i < MOST; i++) {
-        const uint32_t top = __float_as_uint(finite_max(x[i]));
+        const uint32_t top = magnitude(x[i]);
         most = max(most, top), least = min(least, top - 1);
     }
     most = __reduce_max_sync(0xffffffffu, most), least = __reduce_min_sync(0xffffffffu, least);
@@ -1171,17 +1191,22 @@ __global__ void __launch_bounds__(SP_THREADS) k_split(const __grid_constant__ Sp
     __syncthreads();
 #pragma unroll
     for (int w = 0; w < SP_THREADS / 32; w++) most = max(most, red[w].x), least = min(least, red[w].y);
-    bool far_rows = most != 0 && most - (least + 1) > WINDOW;
-    if (far_rows) {  // by whole rows
+    const bool bad_rows = most >= INF;  // rows with elements that are not finite
+    bool far_rows = bad_rows || (most != 0 && most - (least + 1) > WINDOW);
+    if (far_rows) {  // by whole rows, their finite elements
+#pragma unroll
         for (int i = 0; i < MOST; i++) {
-            float top = finite_max(x[i]);
-            for (int o = a.lanes / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-            if (piece == 0 && row0 + i * step < NK) row_top[row0 + i * step] = __float_as_uint(top);
+            uint32_t bad = magnitude(x[i]) >= INF;
+            x[i] = finite(x[i]);
+            uint32_t top = magnitude(x[i]);
+            for (int o = a.lanes / 2; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o)), bad |= __shfl_xor_sync(0xffffffffu, bad, o);
+            if (piece == 0 && row0 + i * step < NK) row_top[row0 + i * step] = top, row_bad[row0 + i * step] = bad;
         }
         __syncthreads();
-        least = 0xFFFFFFFFu;
-        for (int r = lane; r < NK; r += 32) least = min(least, row_top[r] - 1);
-        far_rows = most - (__reduce_min_sync(0xffffffffu, least) + 1) > WINDOW;
+        most = 0, least = 0xFFFFFFFFu;
+        for (int r = lane; r < NK; r += 32) most = max(most, row_top[r]), least = min(least, row_top[r] - 1);
+        most = __reduce_max_sync(0xffffffffu, most), least = __reduce_min_sync(0xffffffffu, least);
+        far_rows = most != 0 && most - (least + 1) > WINDOW;
     }
     if (far_rows) {
         unsigned long long mine = 0;
@@ -1200,11 +1225,17 @@ __global__ void __launch_bounds__(SP_THREADS) k_split(const __grid_constant__ Sp
         most = (uint32_t)mine;
     }
     const float f = to_range(__uint_as_float(most));
-    auto far_row = [&](int row) { return row_top[row] != 0 && most - row_top[row] > WINDOW; };  // (above: the difference wraps)
+    auto far_row = [&](int row) {  // (above the window: the difference wraps)
+        return (far_rows && row_top[row] != 0 && most - row_top[row] > WINDOW) || (bad_rows && !val && row_bad[row]);
+    };
     const size_t tile = (size_t)slot * a.p.n_kv + kvh;
-    if (far_rows && threadIdx.x < NK) {
-        const uint32_t word = __ballot_sync(0xffffffffu, far_row(threadIdx.x));
-        if (lane == 0) a.far[val][tile * FAR_WORDS + warp] = word;
+    const bool marked = far_rows || bad_rows;
+    if (marked && threadIdx.x < NK) {
+        const uint32_t far = __ballot_sync(0xffffffffu, far_row(threadIdx.x)), bad = __ballot_sync(0xffffffffu, bad_rows && row_bad[threadIdx.x]);
+        if (lane == 0) {
+            a.far[val][tile * FAR_WORDS + warp] = far;
+            if (val) a.v_bad[tile * FAR_WORDS + warp] = bad;
+        }
     }
     __half* dst = a.to[val] + (size_t)first * dim + (size_t)kvh * hd + 4 * piece;
 #pragma unroll
@@ -1212,13 +1243,13 @@ __global__ void __launch_bounds__(SP_THREADS) k_split(const __grid_constant__ Sp
         const int row = row0 + i * step;
         if (in && row < rows) {
             uint2 hi, lo;
-            if (far_rows && far_row(row)) x[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (marked && far_row(row)) x[i] = make_float4(0.f, 0.f, 0.f, 0.f);
             split4(x[i], f, hi, lo);
             *reinterpret_cast<uint2*>(dst + row * dim) = hi;
             *reinterpret_cast<uint2*>(dst + row * dim + plane) = lo;
         }
     }
-    if (threadIdx.x == 0) a.inv[val][tile] = far_rows ? -__fdiv_rn(1.0f, f) : __fdiv_rn(1.0f, f);
+    if (threadIdx.x == 0) a.inv[val][tile] = marked ? -__fdiv_rn(1.0f, f) : __fdiv_rn(1.0f, f);
 }
 
 // The parts of the rows' keys, added up in their order: four values of a row per thread (threadIdx.x), all parts' loads under way together.
@@ -1252,7 +1283,8 @@ __global__ void __launch_bounds__(JOIN_THREADS) k_join(const __grid_constant__ P
         if (s < a.splits) {
             const float f = ml[s].x == m ? 1.0f : exp2_approx(ml[s].x - m);
             l = fmaf(ml[s].y, f, l);
-            o.x = fmaf(x[s].x, f, o.x), o.y = fmaf(x[s].y, f, o.y), o.z = fmaf(x[s].z, f, o.z), o.w = fmaf(x[s].w, f, o.w);
+            auto add = [f](float y, float to) { return fmaf(y, fabsf(y) <= MAX_F32 ? f : 1.0f, to); };  // (an infinite value has no factor)
+            o = make_float4(add(x[s].x, o.x), add(x[s].y, o.y), add(x[s].z, o.z), add(x[s].w, o.w));
         }
     const float inv = l == 0.0f ? 0.0f : __fdiv_rn(1.0f, l);
     T* out = reinterpret_cast<T*>(a.p.out) + row * hd + d;
@@ -1312,7 +1344,7 @@ int key_splits(const Prompts& p) {
 }
 
 struct Workspace {
-    size_t k = 0, v = 0, k_inv = 0, v_inv = 0, k_far = 0, v_far = 0, part_o = 0, part_ml = 0, bytes;
+    size_t k = 0, v = 0, k_inv = 0, v_inv = 0, k_far = 0, v_far = 0, v_bad = 0, part_o = 0, part_ml = 0, bytes;
     explicit Workspace(const Prompts& p) {
         const size_t key_slots = (size_t)places(p.n_keys, p.n_seqs, keys_per_tile(p));
         size_t at = 0;
@@ -1328,6 +1360,7 @@ struct Workspace {
             v_inv = take(key_slots * p.n_kv * 4);
             k_far = take(key_slots * p.n_kv * FAR_WORDS * 4);
             v_far = take(key_slots * p.n_kv * FAR_WORDS * 4);
+            v_bad = take(key_slots * p.n_kv * FAR_WORDS * 4);
         }
         const int splits = key_splits(p);
         if (splits > 1) {
@@ -1361,7 +1394,7 @@ cudaError_t launch_typed(cudaStream_t st, const Prompts& p, void* workspace) {
     a.part_o = (float*)(base + w.part_o), a.part_ml = (float*)(base + w.part_ml);
     if (PLANES == 2 && p.n_keys > 0) {
         SplitArgs s{p, {(__half*)(base + w.k), (__half*)(base + w.v)}, {(float*)(base + w.k_inv), (float*)(base + w.v_inv)},
-                    {(uint32_t*)(base + w.k_far), (uint32_t*)(base + w.v_far)}, 1};
+                    {(uint32_t*)(base + w.k_far), (uint32_t*)(base + w.v_far)}, (uint32_t*)(base + w.v_bad), 1};
         while (s.lanes * 4 < p.head_dim) s.lanes *= 2;
         const long long ctas = (long long)places(p.n_keys, p.n_seqs, C::NK) * p.n_kv * 2;
         if (ctas > 0x7FFFFFFFll) return cudaErrorInvalidValue;
@@ -1370,7 +1403,7 @@ cudaError_t launch_typed(cudaStream_t st, const Prompts& p, void* workspace) {
         k = s.to[0], v = s.to[1];
         ks = vs = (size_t)p.n_kv * p.head_dim;
         a.k_inv = s.inv[0], a.v_inv = s.inv[1];
-        a.k_far = s.far[0], a.v_far = s.far[1];
+        a.k_far = s.far[0], a.v_far = s.far[1], a.v_bad = s.v_bad;
     }
     CUtensorMap mq, mk, mv;  // (without any keys none is read)
     if ((e = encode_heads(p.q, p.dtype, p.head_dim, p.n_heads, p.n_tokens, 1, p.q_stride, a.group, a.tile_tokens, &mq)) != cudaSuccess) return e;
