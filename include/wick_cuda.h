@@ -434,7 +434,7 @@ int32_t wick_cuda_attention_q4(const wick_cuda_kv_q4* cache, const void* q_dev, 
 /* Causal attention of packed prompts: sequence s has the tokens [starts[s], starts[s+1]) of q [n_tokens][n_heads*head_dim] and the keys
  * [key_starts[s], key_starts[s+1]) of k and v [n_keys][n_kv_heads*head_dim]; its last key belongs to its last token, so that token j of
  * nq attends its keys t <= j + nk - nq.  starts_dev / key_starts_dev hold n_seqs + 1 ascending offsets; key_starts_dev NULL: the same as
- * starts_dev.  A token without keys gets zeros.  Rows of q, k and v that belong to no sequence (behind the last one) are not used, those of
+ * starts_dev.  A token without keys, or all of whose scores are -inf, gets zeros.  Rows of q, k and v that belong to no sequence (behind the last one) are not used, those of
  * out are set to zero with zero_rest != 0 and left as they were otherwise.  Scores are scaled by 1 / sqrt(head_dim).  All of q, k, v, out have the type `dtype`; rows of q, k,
  * v are q_stride / k_stride / v_stride elements apart; out rows are dense.  head_dim is a multiple of 8 and at most 128;
  * pointers and row strides are multiples of 16 bytes.  f32 elements are held to 2^-22 of themselves or 2^-24 of their row's (token's

@@ -180,3 +180,30 @@ def test_attention_prompts_infinite_values_in_f32(ops, shape):
         want[then:, :, 5] = math.nan
         want[then:, :, 6] = value
         assert torch.equal(out.nan_to_num(7e30, 8e30, 9e30), want.nan_to_num(7e30, 8e30, 9e30))
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("tokens,prefix", [(50, 0), (200, 100), (3, 6000)])
+def test_attention_prompts_tokens_whose_scores_are_all_minus_infinity(ops, dtype, tokens, prefix):
+    """No weight at all: zeros, as without a key, also where the keys are cut into parts."""
+    heads, kv, hd = 2, 1, 64
+    g = _gen(tokens)
+    q, k, v = _randn(g, tokens, heads * hd).to(dtype), _randn(g, tokens + prefix, kv * hd).to(dtype), _randn(g, tokens + prefix, kv * hd).to(dtype)
+    q.view(tokens, heads, hd)[:, :, 3] = 1.0
+    k[:, 3] = -math.inf
+    out = ops.attention_prompts(q, k, v, _starts([tokens]), heads, kv, hd, key_starts=_starts([tokens + prefix]))
+    assert (out == 0).all()
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+def test_attention_prompts_first_key_of_minus_infinity(ops, dtype):
+    """The first token has no weight, the others those of the remaining keys."""
+    n, hd = 200, 64
+    g = _gen(4)
+    q, k, v = (_randn(g, n, hd).half().to(dtype) for _ in range(3))
+    q[:, 3], k[0, 3] = 0.5, -math.inf
+    out = ops.attention_prompts(q, k, v, _starts([n]), 1, 1, hd)
+    k[0, 3] = 0.0
+    ref, tol = _attend_all_but(q.double(), k.double(), v.double(), torch.arange(n, device="cuda")[None] <= torch.arange(n, device="cuda")[:, None], 0)
+    assert (out[0] == 0).all()
+    _check(out, ref, tol, v.abs().max().double())

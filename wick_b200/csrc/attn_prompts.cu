@@ -1019,7 +1019,7 @@ k_attention_prompts(const __grid_constant__ CUtensorMap map_q, const __grid_cons
             ok = ok && __all_sync(0xffffffffu, bar_wait(sh, &sh->checked[k % PR_ITEMS], (k / PR_ITEMS) & 1));
 
             // ── the rows: quotient, rounding, values that are not finite ─────
-            const float inv = limit > 0 ? __fdiv_rn(1.0f, row_sum) : 0.0f;
+            const float inv = limit > 0 && row_sum != 0.0f ? __fdiv_rn(1.0f, row_sum) : 0.0f;  // (no weight at all: zeros, as without a key)
             const size_t out_row = (size_t)(it->token0 + j) * a.p.n_heads + head, part_row = (size_t)it->part * a.p.n_tokens * a.p.n_heads + out_row;
             T* out = reinterpret_cast<T*>(a.p.out) + out_row * hd;
             float* sums = a.part_o + part_row * hd;
