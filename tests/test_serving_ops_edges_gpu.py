@@ -207,3 +207,19 @@ def test_attention_prompts_first_key_of_minus_infinity(ops, dtype):
     ref, tol = _attend_all_but(q.double(), k.double(), v.double(), torch.arange(n, device="cuda")[None] <= torch.arange(n, device="cuda")[:, None], 0)
     assert (out[0] == 0).all()
     _check(out, ref, tol, v.abs().max().double())
+
+
+# ── packed prompts in 16 bits: small weights, long sums ────────────────────────────────────────────
+# 147 blocks of 256 tokens: every SM has one, so that the keys are not cut into parts.
+def test_attention_prompts_many_small_weights_in_f16(ops):
+    """40000 weights of 2^-25.1 beside one of 1: they are 1e-3 of the sum, of values that are all theirs.  Weights are held to 2^-32 of
+    the largest (half of f16's smallest number, 2^7 lifted)."""
+    hd, tokens, n = 8, 147 * 256, 40000 + 147 * 256
+    q, k, v = torch.zeros(tokens, hd, device="cuda"), torch.zeros(n, hd, device="cuda"), torch.ones(n, hd, device="cuda")
+    q[:, 0], k[0, 0], v[0] = 1.0, 25.1 * math.log(2.0) * math.sqrt(hd), 0.0
+    q, k, v = (t.half() for t in (q, k, v))
+    out = ops.attention_prompts(q, k, v, _starts([tokens]), 1, 1, hd, key_starts=_starts([n]))
+    w = math.exp(-float(k[0, 0]) / math.sqrt(hd))
+    seen = torch.arange(n - tokens, n, device="cuda", dtype=torch.float64)[:, None]
+    ref = (seen * w / (1 + seen * w)).expand(-1, hd)
+    assert ((out.double() - ref).abs() <= seen * 2.0 ** -32 + 2.0 ** -11 * ref + 2.0 ** -25).all()

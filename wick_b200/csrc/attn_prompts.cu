@@ -10,7 +10,8 @@
 // in the tensor core the other is in its softmax; and an item's last rows are written while the next one's first scores are computed.
 //
 // f16, bf16: one product each; O stays in tensor memory, and is rescaled only where a row's maximum has grown by more than 2^8 (a weight is at
-//   most 2^8 then; the last maximum that was used cancels in the quotient).
+//   most 2^8 then, times 2^7 in f16; the last maximum that was used cancels in the quotient).  Weights are rounded to the operands' type, half a step each, as the
+//   tensor core takes them; their sum is of the unrounded ones.
 // f32: every operand is split into two f16 parts, x = 2^e (hi + lo), 22 bits, with one power of two per row of Q and per tile of K and V
 //   (K and V by k_split; a row of Q where it lies in shared memory, by the thread that owns it), and a product is hi hi + hi lo + lo hi (lo lo
 //   is 2^-22 of it).  An element is held to 2^-22 of itself or 2^-24 of its row's largest.  Rows of a K or V tile whose magnitudes are too far
@@ -815,7 +816,8 @@ k_attention_prompts(const __grid_constant__ CUtensorMap map_q, const __grid_cons
                             }
                         }
                     }
-                    const float base = row_max == NEG ? 0.0f : -row_max;
+                    // f16: 2^7 times the weights, at most 2^15 then: those down to 2^-32 of the maximum stay in its range (bf16 has f32's)
+                    const float base = (row_max == NEG ? 0.0f : -row_max) + (std::is_same<T16, __half>::value ? 7.0f : 0.0f);
                     const f32x2 base2 = pack2(base, base), scale2 = pack2(a.scale_log2, a.scale_log2);
                     f32x2 sum[2] = {pack2(0.f, 0.f), pack2(0.f, 0.f)};
 #pragma unroll
