@@ -223,3 +223,17 @@ def test_attention_prompts_many_small_weights_in_f16(ops):
     seen = torch.arange(n - tokens, n, device="cuda", dtype=torch.float64)[:, None]
     ref = (seen * w / (1 + seen * w)).expand(-1, hd)
     assert ((out.double() - ref).abs() <= seen * 2.0 ** -32 + 2.0 ** -11 * ref + 2.0 ** -25).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16], ids=str)
+def test_attention_prompts_of_a_million_keys(ops, dtype):
+    """Sums over a million keys stay within the types' roundings: a half step of the weights, one of the result."""
+    heads, kv, hd, tokens, n = 1, 1, 64, 147 * 256, 1 << 20
+    g = _gen(21)
+    q, k, v = _randn(g, tokens, hd).to(dtype), _randn(g, n, hd).to(dtype), (_randn(g, n, hd) * 0.25 + 1).to(dtype)
+    out = ops.attention_prompts(q, k, v, _starts([tokens]), heads, kv, hd, key_starts=_starts([n]))
+    some = torch.tensor([0, 1, 100, 20000, tokens - 1], device="cuda")
+    seen = torch.arange(n, device="cuda")[None] <= (some + n - tokens)[:, None]
+    ref, tol = _attend(q[some].double(), k.double(), v.double(), seen)
+    # rounded weights err at random: beside the result's half step, a quarter of one is left for them and the sums
+    assert ((out[some].double() - ref).abs() <= tol + torch.finfo(dtype).eps / 2 * 1.25 * ref.abs()).all()

@@ -11,7 +11,8 @@
 //
 // f16, bf16: one product each; O stays in tensor memory, and is rescaled only where a row's maximum has grown by more than 2^8 (a weight is at
 //   most 2^8 then, times 2^7 in f16; the last maximum that was used cancels in the quotient).  Weights are rounded to the operands' type, half a step each, as the
-//   tensor core takes them; their sum is of the unrounded ones.
+//   tensor core takes them; their sum is of the unrounded ones.  The tensor core adds with truncation: O is
+//   taken out and added up in f32 every 64 tiles (8192 keys: 5e-5 of the sum; 131072 without this were 7e-4, 1.5 half steps of f16).
 // f32: every operand is split into two f16 parts, x = 2^e (hi + lo), 22 bits, with one power of two per row of Q and per tile of K and V
 //   (K and V by k_split; a row of Q where it lies in shared memory, by the thread that owns it), and a product is hi hi + hi lo + lo hi (lo lo
 //   is 2^-22 of it).  An element is held to 2^-22 of itself or 2^-24 of its row's largest.  Rows of a K or V tile whose magnitudes are too far
@@ -54,6 +55,7 @@ constexpr int PR_THREADS = 384;   // TMA, MMA, V check, items; 2 x 4 softmax war
 constexpr int PR_ITEMS = 3;       // items that are known ahead
 constexpr int PR_MASKED = 8;      // tiles that some row of a CTA sees in part: at most 256 / 64 + 2
 constexpr uint32_t PR_SPIN_LIMIT = 1u << 24;  // about half a second (2^18: 8 ms)
+constexpr int PR_CARRY = 64;     // tiles
 constexpr float PR_LAZY = 8.0f, PR_DOWN = 0x1p-8f;  // 2^-PR_LAZY
 
 template <int PLANES, int HDP>
@@ -771,77 +773,102 @@ k_attention_prompts(const __grid_constant__ CUtensorMap map_q, const __grid_cons
             float row_max = NEG, row_sum = 0.0f;
             bool bad = false;  // f32: some tile has values that are not finite
             float o[C::O_IN_TMEM ? 1 : HDP];
+            // 16 bits: O of PR_CARRY tiles at a time, added up outside the tensor core, behind it the maximum that the sum goes by (local memory: few
+            // calls come here, and it takes no registers from the others)
+            float carry[C::O_IN_TMEM ? HDP + 1 : 1];
+            auto with_carry = [&](int c, float (&x)[32]) {
+                const float was = carry[C::O_IN_TMEM ? HDP : 0], f = was == row_max ? 1.0f : exp2_approx(was - row_max);
+#pragma unroll
+                for (int d = 0; d < 32; d++) x[d] = fmaf(carry[C::O_IN_TMEM ? c + d : 0], f, x[d]);
+            };
             if constexpr (C::O_IN_TMEM) {
-                for (int i = 0; i < n && ok; i++) {
-                    if (!(ok = __all_sync(0xffffffffu, bar_wait(sh, &sh->s_full[m], (done + i) & 1)))) break;
-                    tc_fence_after();
-                    float s[NK];
-#pragma unroll
-                    for (int c = 0; c < NK / 32; c++) tmem_ld32(t_s + 32 * c, s + 32 * c);
-                    tmem_ld_wait();
-                    if (C::P_APART) {
-                        tc_fence_before();
-                        __syncwarp();
-                        if (lane == 0) bar_arrive(&sh->s_read[m]);
-                    }
-                    const int seen = limit - i * NK;
-                    if (__any_sync(0xffffffffu, seen < NK)) {
-#pragma unroll
-                        for (int c = 0; c < NK; c++)
-                            if (c >= seen) s[c] = NEG;
-                    }
-                    float top[4] = {s[0], s[1], s[2], s[3]};
-#pragma unroll
-                    for (int c = 4; c < NK; c++) top[c & 3] = fmaxf(top[c & 3], s[c]);
-                    const float tile_max = __fmul_rn(fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])), a.scale_log2);
-                    const bool grown = tile_max > row_max + PR_LAZY || (row_max == NEG && tile_max > NEG);
-                    // P V of the tile before is done: with P over S by the order of the tensor core's work, with P apart by this wait
-                    if (C::P_APART && i > 0 && !(ok = __all_sync(0xffffffffu, bar_wait(sh, &sh->o_full[m], (done + i - 1) & 1)))) break;
-                    if (__any_sync(0xffffffffu, grown)) {
-                        float f = 1.0f;
-                        if (grown) {
-                            f = exp2_approx(row_max - tile_max);
-                            row_max = tile_max;
-                            row_sum = __fmul_rn(row_sum, f);
-                        }
-                        if (i > 0) {
+                for (int first = 0; first < n && ok; first += PR_CARRY) {
+                    if (first > 0) {  // (behind the P V of the tile before: with P over S by this tile's S, with P apart by its own sign)
+                        if (!(ok = __all_sync(0xffffffffu, C::P_APART ? bar_wait(sh, &sh->o_full[m], (done + first - 1) & 1) : bar_wait(sh, &sh->s_full[m], (done + first) & 1)))) break;
+                        tc_fence_after();
 #pragma unroll 1
-                            for (int c = 0; c < HDP; c += 32) {
-                                float x[32];
-                                tmem_ld32(t_o + c, x);
-                                tmem_ld_wait();
+                        for (int c = 0; c < HDP; c += 32) {
+                            float x[32];
+                            tmem_ld32(t_o + c, x);
+                            tmem_ld_wait();
+                            if (first > PR_CARRY) with_carry(c, x);
 #pragma unroll
-                                for (int d = 0; d < 32; d++) x[d] = __fmul_rn(x[d], f);
-                                tmem_st32(t_o + c, x);
+                            for (int d = 0; d < 32; d++) carry[C::O_IN_TMEM ? c + d : 0] = x[d], x[d] = 0.0f;
+                            tmem_st32(t_o + c, x);
+                        }
+                        carry[C::O_IN_TMEM ? HDP : 0] = row_max;
+                    }
+                    for (int i = first; i < min(n, first + PR_CARRY) && ok; i++) {
+                        if (!(ok = __all_sync(0xffffffffu, bar_wait(sh, &sh->s_full[m], (done + i) & 1)))) break;
+                        tc_fence_after();
+                        float s[NK];
+#pragma unroll
+                        for (int c = 0; c < NK / 32; c++) tmem_ld32(t_s + 32 * c, s + 32 * c);
+                        tmem_ld_wait();
+                        if (C::P_APART) {
+                            tc_fence_before();
+                            __syncwarp();
+                            if (lane == 0) bar_arrive(&sh->s_read[m]);
+                        }
+                        const int seen = limit - i * NK;
+                        if (__any_sync(0xffffffffu, seen < NK)) {
+#pragma unroll
+                            for (int c = 0; c < NK; c++)
+                                if (c >= seen) s[c] = NEG;
+                        }
+                        float top[4] = {s[0], s[1], s[2], s[3]};
+#pragma unroll
+                        for (int c = 4; c < NK; c++) top[c & 3] = fmaxf(top[c & 3], s[c]);
+                        const float tile_max = __fmul_rn(fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])), a.scale_log2);
+                        const bool grown = tile_max > row_max + PR_LAZY || (row_max == NEG && tile_max > NEG);
+                        // P V of the tile before is done: with P over S by the order of the tensor core's work, with P apart by this wait
+                        if (C::P_APART && i > 0 && !(ok = __all_sync(0xffffffffu, bar_wait(sh, &sh->o_full[m], (done + i - 1) & 1)))) break;
+                        if (__any_sync(0xffffffffu, grown)) {
+                            float f = 1.0f;
+                            if (grown) {
+                                f = exp2_approx(row_max - tile_max);
+                                row_max = tile_max;
+                                row_sum = __fmul_rn(row_sum, f);
+                            }
+                            if (i > 0) {
+#pragma unroll 1
+                                for (int c = 0; c < HDP; c += 32) {
+                                    float x[32];
+                                    tmem_ld32(t_o + c, x);
+                                    tmem_ld_wait();
+#pragma unroll
+                                    for (int d = 0; d < 32; d++) x[d] = __fmul_rn(x[d], f);
+                                    tmem_st32(t_o + c, x);
+                                }
                             }
                         }
-                    }
-                    // f16: 2^7 times the weights, at most 2^15 then: those down to 2^-32 of the maximum stay in its range (bf16 has f32's)
-                    const float base = (row_max == NEG ? 0.0f : -row_max) + (std::is_same<T16, __half>::value ? 7.0f : 0.0f);
-                    const f32x2 base2 = pack2(base, base), scale2 = pack2(a.scale_log2, a.scale_log2);
-                    f32x2 sum[2] = {pack2(0.f, 0.f), pack2(0.f, 0.f)};
+                        // f16: 2^7 times the weights, at most 2^15 then: those down to 2^-32 of the maximum stay in its range (bf16 has f32's)
+                        const float base = (row_max == NEG ? 0.0f : -row_max) + (std::is_same<T16, __half>::value ? 7.0f : 0.0f);
+                        const f32x2 base2 = pack2(base, base), scale2 = pack2(a.scale_log2, a.scale_log2);
+                        f32x2 sum[2] = {pack2(0.f, 0.f), pack2(0.f, 0.f)};
 #pragma unroll
-                    for (int c = 0; c < NK / 32; c++) {
-                        uint32_t p[16];
+                        for (int c = 0; c < NK / 32; c++) {
+                            uint32_t p[16];
 #pragma unroll
-                        for (int x = 0; x < 16; x++) {
-                            float p0, p1;
-                            unpack2(fma2(pack2(s[32 * c + 2 * x], s[32 * c + 2 * x + 1]), scale2, base2), p0, p1);
-                            p0 = exp2_approx(p0), p1 = exp2_approx(p1);
-                            sum[x & 1] = add2(sum[x & 1], pack2(p0, p1));
-                            p[x] = pack16<T16>(p0, p1);
+                            for (int x = 0; x < 16; x++) {
+                                float p0, p1;
+                                unpack2(fma2(pack2(s[32 * c + 2 * x], s[32 * c + 2 * x + 1]), scale2, base2), p0, p1);
+                                p0 = exp2_approx(p0), p1 = exp2_approx(p1);
+                                sum[x & 1] = add2(sum[x & 1], pack2(p0, p1));
+                                p[x] = pack16<T16>(p0, p1);
+                            }
+                            tmem_st16(t_p + 16 * c, p);
                         }
-                        tmem_st16(t_p + 16 * c, p);
+                        {
+                            float s0, s1;
+                            unpack2(add2(sum[0], sum[1]), s0, s1);
+                            row_sum += s0 + s1;
+                        }
+                        tmem_st_wait();
+                        tc_fence_before();
+                        __syncwarp();
+                        if (lane == 0) bar_arrive(&sh->p_ready[m]);
                     }
-                    {
-                        float s0, s1;
-                        unpack2(add2(sum[0], sum[1]), s0, s1);
-                        row_sum += s0 + s1;
-                    }
-                    tmem_st_wait();
-                    tc_fence_before();
-                    __syncwarp();
-                    if (lane == 0) bar_arrive(&sh->p_ready[m]);
                 }
             } else {
                 if (n > 0 && !written) next_q = write_q();
@@ -1071,6 +1098,7 @@ k_attention_prompts(const __grid_constant__ CUtensorMap map_q, const __grid_cons
                     if (n > 0) {  // (uniform in the warp)
                         tmem_ld32(t_o + c, x);
                         tmem_ld_wait();
+                        if (n > PR_CARRY) with_carry(c, x);
                     }
                     if (real && ok) write_32(c, x);
                 }
