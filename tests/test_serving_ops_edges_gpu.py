@@ -237,3 +237,15 @@ def test_attention_prompts_of_a_million_keys(ops, dtype):
     ref, tol = _attend(q[some].double(), k.double(), v.double(), seen)
     # rounded weights err at random: beside the result's half step, a quarter of one is left for them and the sums
     assert ((out[some].double() - ref).abs() <= tol + torch.finfo(dtype).eps / 2 * 1.25 * ref.abs()).all()
+
+
+# ── attention over the 4-bit cache ─────────────────────────────────────────────────────────────────
+def test_attention_q4_of_huge_queries(ops):
+    """Queries up to f32's largest: the key of the largest score has all the weight."""
+    heads, kv, hd, n = 4, 2, 64, 200
+    g = _gen(22)
+    cache = _random_cache(ops, g, 1, 256, kv, hd)
+    for factor in (1e20, 2.0 ** 100, 1e31, 1e36):
+        q = _randn(g, 1, heads * hd) * factor
+        ref, _, vmax = _q4_ref(q, cache, [0], [n], heads)
+        _check(ops.attention_q4(q, cache, _i32([0]), _i32([n]), heads), ref, 2.0 ** -20 * vmax, vmax)

@@ -371,7 +371,7 @@ __global__ void __launch_bounds__(Q4Cfg<NB>::THREADS, 1) k_attention_q4(const __
                             }
                     top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
                     top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-                    const int e = max(-100, min(100, (int)((__float_as_uint(top) >> 23) & 255u) - 127));
+                    const int e = max(-100, min(127, (int)((__float_as_uint(top) >> 23) & 255u) - 127));
                     const float f = pow2(12 - e);
                     q_inv[u] = __shfl_sync(0xffffffffu, pow2(e - 12), 8 * t4);  // (from the lanes of column 2 t4)
 #pragma unroll
