@@ -249,3 +249,22 @@ def test_attention_q4_of_huge_queries(ops):
         q = _randn(g, 1, heads * hd) * factor
         ref, _, vmax = _q4_ref(q, cache, [0], [n], heads)
         _check(ops.attention_q4(q, cache, _i32([0]), _i32([n]), heads), ref, 2.0 ** -20 * vmax, vmax)
+
+
+# ── packed prompts: the ring of K and V tiles ──────────────────────────────────────────────────────
+@pytest.mark.parametrize("dtype,hd", [(torch.float32, 64), (torch.float32, 128), (torch.float16, 64), (torch.bfloat16, 128)], ids=str)
+def test_attention_prompts_items_of_any_length_in_a_row(ops, dtype, hd):
+    """Many items per SM whose tiles end anywhere in the ring (3, 5 and 6 slots): no wait takes another use of a slot for its own."""
+    heads = kv = 4
+    lengths = [(i * 67) % 400 + 1 for i in range(150)]
+    n, g = sum(lengths), _gen(hd)
+    q, k, v = (_randn(g, n, h * hd).to(dtype) for h in (heads, kv, kv))
+    starts = _starts(lengths)
+    want = ops.attention_prompts(q, k, v, starts, heads, kv, hd)
+    for _ in range(20):
+        assert torch.equal(ops.attention_prompts(q, k, v, starts, heads, kv, hd), want)
+    at = starts.tolist()
+    for s in (0, 1, 74, 148, 149):
+        a, b = at[s], at[s + 1]
+        ref, tol = _prompts_ref(q[a:b], k[a:b], v[a:b], [b - a], [b - a], heads, kv, hd)
+        _check(want[a:b], ref, tol, v.abs().max().double())

@@ -91,7 +91,7 @@ struct Item {
     __device__ __forceinline__ int first_masked() const { return max(0, first_visible) / NK; }  // tiles from here on are seen in part by some row
 };
 struct Shared {
-    unsigned long long q_full[2], q_raw[2], q_empty, full[6], empty[6], ready[6], s_full[2], s_read[2], p_ready[2], o_full[2];
+    unsigned long long q_full[2], q_raw[2], q_empty, k_full[6], v_full[6], empty[6], ready[6], s_full[2], s_read[2], p_ready[2], o_full[2];
     unsigned long long item_full[PR_ITEMS], item_empty[PR_ITEMS], checked[PR_ITEMS];
     Item item[PR_ITEMS];
     uint32_t tmem_base;
@@ -444,7 +444,7 @@ k_attention_prompts(const __grid_constant__ CUtensorMap map_q, const __grid_cons
             bar_init(&sh->s_full[m], 1), bar_init(&sh->s_read[m], 4), bar_init(&sh->p_ready[m], 4), bar_init(&sh->o_full[m], 1);
         }
         bar_init(&sh->q_empty, 1);
-        for (int s = 0; s < NS; s++) bar_init(&sh->full[s], 1), bar_init(&sh->empty[s], 1), bar_init(&sh->ready[s], 1);
+        for (int s = 0; s < NS; s++) bar_init(&sh->k_full[s], 1), bar_init(&sh->v_full[s], 1), bar_init(&sh->empty[s], 1), bar_init(&sh->ready[s], 1);
         for (int i = 0; i < PR_ITEMS; i++) bar_init(&sh->item_full[i], 1), bar_init(&sh->item_empty[i], 11), bar_init(&sh->checked[i], 1);
         sh->abort = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -463,6 +463,9 @@ k_attention_prompts(const __grid_constant__ CUtensorMap map_q, const __grid_cons
 
     // Registers: the launch has 12 warps of 168; four give up 80 each, eight take 40 more (4 x 88 + 8 x 208 = 12 x 168).  One instruction for the
     // four, in front of their branches: a warpgroup executes it together.
+    // Ring positions g = 0, 1, .. hold K0 V0 K1 V1 ..; K and V have barriers of their own, so that who waits for V needs nothing of the K's that share
+    // its slot: an odd number of slots has them in turn, and a use's number among those of its kind is half its number then.
+    auto use_parity = [](uint32_t g) { return ((NS & 1) ? g / NS >> 1 : g / NS) & 1; };
     // An item of the list, for a role: waits until it is known.  false: no more items (or a wait ran out).
     auto next_item = [&](uint32_t k) -> const Item* {
         if (!__all_sync(0xffffffffu, bar_wait(sh, &sh->item_full[k % PR_ITEMS], (k / PR_ITEMS) & 1))) return nullptr;
@@ -525,10 +528,11 @@ k_attention_prompts(const __grid_constant__ CUtensorMap map_q, const __grid_cons
                         const uint32_t s = (g + i) % NS, u = (g + i) / NS;
                         ok = bar_wait(sh, &sh->empty[s], (u & 1) ^ 1);
                         if (!ok) break;
-                        bar_expect(&sh->full[s], C::SLOT);
+                        unsigned long long* bar = (i & 1) ? &sh->v_full[s] : &sh->k_full[s];
+                        bar_expect(bar, C::SLOT);
                         for (int p = 0; p < PLANES; p++)
                             for (int c = 0; c < C::CH; c++)
-                                tma_4d(ring + s * C::SLOT + p * C::KBYTES + c * NK * 128, (i & 1) ? &map_v : &map_k, &sh->full[s], c * 64, it->kvh,
+                                tma_4d(ring + s * C::SLOT + p * C::KBYTES + c * NK * 128, (i & 1) ? &map_v : &map_k, bar, c * 64, it->kvh,
                                        it->key0 + (i >> 1) * NK, p);
                     }
                 }
@@ -591,7 +595,7 @@ k_attention_prompts(const __grid_constant__ CUtensorMap map_q, const __grid_cons
                 return true;
             };
             if (nt > 0) {
-                ok = __all_sync(0xffffffffu, bar_wait(sh, &sh->full[g % NS], (g / NS) & 1));
+                ok = __all_sync(0xffffffffu, bar_wait(sh, &sh->k_full[g % NS], use_parity(g)));
                 for (int m = 0; m < 2 && ok; m++)
                     if (it->n_tiles[m] > 0) {
                         ok = __all_sync(0xffffffffu, bar_wait(sh, &sh->q_full[m], qn[m] & 1));
@@ -605,10 +609,10 @@ k_attention_prompts(const __grid_constant__ CUtensorMap map_q, const __grid_cons
                 __syncwarp();
             }
             for (int i = 0; i < nt && ok; i++) {
-                const uint32_t gv = g + 2 * i + 1, gk = gv + 1, sv = gv % NS, uv = gv / NS, sk = gk % NS, uk = gk / NS;
+                const uint32_t gv = g + 2 * i + 1, gk = gv + 1, sv = gv % NS, sk = gk % NS;
                 const bool more = i + 1 < nt;
                 if (C::P_APART && more) {  // the next scores first
-                    ok = __all_sync(0xffffffffu, bar_wait(sh, &sh->full[sk], uk & 1));
+                    ok = __all_sync(0xffffffffu, bar_wait(sh, &sh->k_full[sk], use_parity(gk)));
                     for (int m = 0; m < 2 && ok; m++)
                         if (i + 1 < it->n_tiles[m]) ok = issue_scores(m, sk, i + 1);
                     if (!ok) break;
@@ -618,7 +622,7 @@ k_attention_prompts(const __grid_constant__ CUtensorMap map_q, const __grid_cons
                     }
                     __syncwarp();
                 }
-                ok = __all_sync(0xffffffffu, bar_wait(sh, &sh->ready[sv], ((NS & 1) ? uv >> 1 : uv) & 1));
+                ok = __all_sync(0xffffffffu, bar_wait(sh, &sh->ready[sv], use_parity(gv)));
                 for (int m = 0; m < 2 && ok; m++) {
                     const int n = m ? n1 : n0;
                     if (i >= n) continue;
@@ -631,7 +635,7 @@ k_attention_prompts(const __grid_constant__ CUtensorMap map_q, const __grid_cons
                     }
                     __syncwarp();
                     if (!C::P_APART && i + 1 < n) {
-                        ok = __all_sync(0xffffffffu, bar_wait(sh, &sh->full[sk], uk & 1));
+                        ok = __all_sync(0xffffffffu, bar_wait(sh, &sh->k_full[sk], use_parity(gk)));
                         if (ok) ok = issue_scores(m, sk, i + 1);
                     }
                 }
@@ -659,11 +663,8 @@ k_attention_prompts(const __grid_constant__ CUtensorMap map_q, const __grid_cons
             Item* notes = &sh->item[k % PR_ITEMS];
             const int nt = it->nt(), first_masked = it->template first_masked<NK>();
             for (int i = 0; i < nt; i++) {
-                // Every use of a slot is waited for, K's too: with an odd number of slots a slot has K and V in turn, and a wait for V that came
-                // before its K had landed would see the phase before that as its own.
                 const uint32_t g = g0 + 2 * i + 1, s = g % NS;
-                ok = bar_wait(sh, &sh->full[(g - 1) % NS], ((g - 1) / NS) & 1) && bar_wait(sh, &sh->full[s], (g / NS) & 1);
-                if (!(ok = __all_sync(0xffffffffu, ok))) break;
+                if (!(ok = __all_sync(0xffffffffu, bar_wait(sh, &sh->v_full[s], use_parity(g))))) break;
                 if (i >= first_masked) {
                     uint8_t* tile = sm + 2 * PLANES * C::QBYTES + s * C::SLOT;
                     uint32_t found[4] = {0, 0, 0, 0};
