@@ -21,6 +21,7 @@ struct KvQ4 {
 };
 constexpr int KV_Q4_TILE = 64;  // max_seq is a multiple of it: a tile of rows never leaves its (slot, KV head)
 constexpr int KV_Q4_MAX_HEAD = 128;
+constexpr uint32_t KV_Q4_MAX_ROWS = 0x7FFFFF00u;  // of an append or a reading: a row's number, and the numbers up to the end of its block, are ints
 cudaError_t launch_kv_append_q4(cudaStream_t st, const KvQ4& c, const void* k, size_t k_stride, const void* v, size_t v_stride, int dtype, int n,
                                 const int32_t* slots, const int32_t* positions);
 cudaError_t launch_kv_read_q4(cudaStream_t st, const KvQ4& c, int n, const int32_t* slots, const int32_t* positions, float* k, float* v);

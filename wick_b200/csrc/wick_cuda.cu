@@ -2515,7 +2515,7 @@ int32_t wick_cuda_kv_append_q4(const wick_cuda_kv_q4* cache, const void* k_dev, 
     if (!k_dev || !v_dev || !slots_dev || !positions_dev) return fail(WICK_CUDA_ERR_BAD_ARG, "NULL argument");
     const uint64_t dim = (uint64_t)c.n_kv * c.head_dim;
     if (k_stride < dim || v_stride < dim) return fail(WICK_CUDA_ERR_BAD_ARG, "kv_append_q4: rows overlap");
-    if (n * dim > (1ull << 38)) return fail(WICK_CUDA_ERR_BAD_ARG, "kv_append_q4: too many rows");
+    if (n > KV_Q4_MAX_ROWS || n * dim > (1ull << 38)) return fail(WICK_CUDA_ERR_BAD_ARG, "kv_append_q4: too many rows");
     if (misaligned(k_dev, dtype_bytes(dtype)) || misaligned(v_dev, dtype_bytes(dtype))) return fail(WICK_CUDA_ERR_BAD_ARG, "kv_append_q4: misaligned rows");
     CU_TRY(launch_kv_append_q4((cudaStream_t)stream, c, k_dev, k_stride, v_dev, v_stride, dtype, (int)n, slots_dev, positions_dev));
     OP_END();
@@ -2528,7 +2528,7 @@ int32_t wick_cuda_kv_read_q4(const wick_cuda_kv_q4* cache, uint32_t n, const int
     if (n == 0) return WICK_CUDA_OK;
     if (!k_dev || !v_dev || !slots_dev || !positions_dev) return fail(WICK_CUDA_ERR_BAD_ARG, "NULL argument");
     if (misaligned(k_dev, 16) || misaligned(v_dev, 16)) return fail(WICK_CUDA_ERR_BAD_ARG, "kv_read_q4: k and v must be 16-byte aligned");
-    if (n * ((uint64_t)c.n_kv * c.head_dim) > (1ull << 38)) return fail(WICK_CUDA_ERR_BAD_ARG, "kv_read_q4: too many rows");
+    if (n > KV_Q4_MAX_ROWS || n * ((uint64_t)c.n_kv * c.head_dim) > (1ull << 38)) return fail(WICK_CUDA_ERR_BAD_ARG, "kv_read_q4: too many rows");
     CU_TRY(launch_kv_read_q4((cudaStream_t)stream, c, (int)n, slots_dev, positions_dev, k_dev, v_dev));
     OP_END();
 }
