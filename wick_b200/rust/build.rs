@@ -2,8 +2,8 @@
 // statically into the wick crate.  Not compiled where it was written (no Rust toolchain there); the nvcc command
 // line is the one wick_b200/build.py uses.
 //
-// Expects the sources under $WICK_CUDA_SRC (default: ../wick_b200/csrc relative to the crate) and the public header
-// under $WICK_CUDA_INCLUDE (default: ../include).
+// Expects the sources under $WICK_CUDA_SRC (default: ../wick_b200/csrc relative to the crate); they include the public header as
+// ../../include/wick_cuda.h.
 use std::{env, path::PathBuf, process::Command};
 
 const SOURCES: &[&str] = &[
@@ -12,10 +12,15 @@ const SOURCES: &[&str] = &[
     "kernels_attn.cu",
     "kernels_q6k.cu",
     "kernels_batch.cu",
-    "kernels_sample.cu", "kernels_logprobs.cu", "kernels_kv_q4.cu", "attn_q4.cu", "attn_prompts.cu",
+    "kernels_sample.cu",
+    "kernels_logprobs.cu",
+    "kernels_kv_q4.cu",
+    "attn_q4.cu",
+    "attn_prompts.cu",
     "tp_comm.cu",
     "decode_mega.cu",
     "gemm_tc.cu",
+    "gemm_mma.cu",
     "argmax_noalloc.cu",
     "wick_cuda.cu",
 ];
@@ -26,12 +31,13 @@ fn main() {
     }
     let manifest = PathBuf::from(env::var("CARGO_MANIFEST_DIR").unwrap());
     let src_dir = env::var("WICK_CUDA_SRC").map(PathBuf::from).unwrap_or_else(|_| manifest.join("../wick_b200/csrc"));
+    println!("cargo:rerun-if-changed={}", src_dir.display()); // (the headers, too)
+    println!("cargo:rerun-if-changed={}", src_dir.join("../../include/wick_cuda.h").display());
     let out = PathBuf::from(env::var("OUT_DIR").unwrap());
     let nvcc = env::var("NVCC").unwrap_or_else(|_| "nvcc".into());
     let mut objects = Vec::new();
     for s in SOURCES {
         let src = src_dir.join(s);
-        println!("cargo:rerun-if-changed={}", src.display());
         let obj = out.join(s.replace(".cu", ".o"));
         let status = Command::new(&nvcc)
             .args(["-gencode", "arch=compute_100a,code=sm_100a", "-O3", "-std=c++17", "-lineinfo"])
