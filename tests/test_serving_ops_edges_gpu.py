@@ -268,3 +268,44 @@ def test_attention_prompts_items_of_any_length_in_a_row(ops, dtype, hd):
         a, b = at[s], at[s + 1]
         ref, tol = _prompts_ref(q[a:b], k[a:b], v[a:b], [b - a], [b - a], heads, kv, hd)
         _check(want[a:b], ref, tol, v.abs().max().double())
+
+
+# ── out that is q itself, or lies over another input ───────────────────────────────────────────────
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("prefix", [0, 4000])
+def test_attention_prompts_in_place(ops, dtype, prefix):
+    """Undivided and in parts; in f32 with a far key, which is scored from q itself."""
+    heads, kv, hd, n = 8, 2, 64, 300
+    g = _gen(prefix)
+    q, k, v = _randn(g, n, heads * hd).to(dtype), _randn(g, n + prefix, kv * hd), _randn(g, n + prefix, kv * hd).to(dtype)
+    k[prefix + 20] *= 1e7 if dtype == torch.float32 else 1
+    k, starts, keys = k.to(dtype), _starts([200, 100]), _starts([200 + prefix, 100])
+    want = ops.attention_prompts(q, k, v, starts, heads, kv, hd, key_starts=keys)
+    for _ in range(5):
+        at = q.clone()
+        assert ops.attention_prompts(at, k, v, starts, heads, kv, hd, key_starts=keys, out=at) is at and torch.equal(at, want)
+
+
+def test_attention_q4_in_place(ops):
+    heads, kv, hd = 16, 2, 64
+    g = _gen(30)
+    cache = _random_cache(ops, g, 3, 4096, kv, hd)
+    slots, lengths, q = _i32([0, 1, 2]), _i32([4000, 1, 300]), _randn(g, 3, heads * hd)
+    want = ops.attention_q4(q, cache, slots, lengths, heads)
+    for _ in range(5):
+        at = q.clone()
+        assert ops.attention_q4(at, cache, slots, lengths, heads, out=at) is at and torch.equal(at, want)
+
+
+def test_out_over_another_input(ops):
+    from wick_b200 import _lib
+    x, i = torch.zeros(40, 64, device="cuda"), _i32([0, 9])
+    q, k = x[:9], x[9:18]
+    cache = ops.KvCacheQ4(*(torch.zeros(1, 1, 64, w, dtype=t, device="cuda") for w, t in ((32, torch.uint8), (2, torch.float16)) * 2))
+    for f in (lambda: ops.attention_prompts(q, k, k, i, 1, 1, 64, out=k), lambda: ops.attention_prompts(q, k, k, i, 1, 1, 64, out=x[4:13]),
+              lambda: ops.attention_prompts(q, x[:27:3], k, i, 1, 1, 64, out=x[20:29]),
+              lambda: ops.attention_q4(q, cache, i.new_zeros(9), i.new_zeros(9), 1, out=x[1:10]),
+              lambda: ops.attention_q4(q[:1], cache, i[:1], i[:1], 1, out=cache.k_quants.view(-1)[:256].view(torch.float32).view(1, 64))):
+        with pytest.raises(_lib.WickCudaError, match="overlaps"):
+            f()
+    ops.attention_prompts(q, k, k, i, 1, 1, 64, out=x[18:27])  # beside them

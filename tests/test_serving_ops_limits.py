@@ -11,3 +11,38 @@ def test_more_rows_than_a_row_number_holds(cuda_lib):
     for n in (0x7FFFFF01, 0x7FFFFFFF, 0x80000000, 0xFFFFFFFF):
         assert cuda_lib.wick_cuda_kv_append_q4(c, A, 32, A, 32, 1, n, A, A, None) == _lib.ERR_BAD_ARG
         assert cuda_lib.wick_cuda_kv_read_q4(c, n, A, A, A, A, None) == _lib.ERR_BAD_ARG
+
+
+def _refused_for_overlap(lib, code):
+    from wick_b200 import _lib
+    return code == _lib.ERR_BAD_ARG and b"overlaps" in lib.wick_cuda_last_error()
+
+
+# Addresses that are never followed; what does not overlap fails at its workspace, which is checked behind it.
+def test_attention_prompts_refuses_an_out_over_its_inputs(cuda_lib):
+    def call(out, q=A, qs=256, k=4 * A, ks=128, v=8 * A, vs=128, starts=16 * A, keys=32 * A):
+        return _refused_for_overlap(cuda_lib, cuda_lib.wick_cuda_attention_prompts(q, qs, k, ks, v, vs, 0, starts, keys, 2, 9, 20, 4, 2, 64, out, 0, None, 0, None))
+
+    size = 9 * 256 * 4
+    assert not call(2 * A) and not call(A)  # (q itself)
+    for at, length in ((A, size), (4 * A, 20 * 512), (8 * A, 20 * 512), (16 * A, 12), (32 * A, 12)):
+        assert not call(at - size) and not call(at + (length + 15) // 16 * 16)
+        assert call(at - size + 16) and call(at + (length - 1) // 16 * 16)
+    # rows apart from one another: q itself only where they are dense; between the columns of a single row
+    assert call(A, qs=260) and call(A + 256 * 4, qs=260)
+    assert not call(4 * A + 512, ks=128 + 256 * 9)
+    assert call(4 * A + 496, ks=128 + 256 * 9) and call(4 * A + 528, ks=128 + 256 * 9)
+
+
+def test_attention_q4_refuses_an_out_over_its_inputs(cuda_lib):
+    cache = C.byref(_cache(k_quants=4 * A, k_scales=8 * A, v_quants=12 * A, v_scales=16 * A))
+
+    def call(out, q=A, qs=256):
+        return _refused_for_overlap(cuda_lib, cuda_lib.wick_cuda_attention_q4(cache, q, qs, 0, 3, 4, 20 * A, 24 * A, out, 0, None, 0, None))
+
+    size, rows = 3 * 256 * 4, 2 * 2 * 128
+    assert not call(2 * A) and not call(A)
+    for at, length in ((A, size), (4 * A, rows * 32), (8 * A, rows * 4), (12 * A, rows * 32), (16 * A, rows * 4), (20 * A, 12), (24 * A, 12)):
+        assert not call(at - size) and not call(at + length)
+        assert call(at - size + 4) and call(at + length - 4)
+    assert call(A, qs=257)

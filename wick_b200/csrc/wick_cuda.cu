@@ -2476,6 +2476,12 @@ static int32_t check_dtype(int32_t dtype) {
     return dtype_bytes(dtype) ? WICK_CUDA_OK : fail(WICK_CUDA_ERR_UNSUPPORTED_DTYPE, "dtype must be f32, f16 or bf16");
 }
 static bool misaligned(const void* p, size_t bytes) { return ((uintptr_t)p & (bytes - 1)) != 0; }
+// Whether `bytes` at p meet one of n rows of row_bytes at q, stride bytes apart.
+static bool meets(const void* p, uint64_t bytes, const void* q, uint64_t n, uint64_t stride, uint64_t row_bytes) {
+    if (!bytes || !n || !row_bytes) return false;
+    const uint64_t a = (uintptr_t)p, b = (uintptr_t)q, first = a < b + row_bytes ? 0 : (a - b - row_bytes) / stride + 1;  // row that ends behind p
+    return first < n && b + first * stride < a + bytes;
+}
 
 int32_t wick_cuda_token_logprobs(const void* logits_dev, int32_t dtype, uint64_t row_stride, uint32_t n, uint32_t vocab, const int32_t* tokens_dev,
                                  uint32_t top_n, float* logprob_dev, float* entropy_dev, int32_t* top_ids_dev, float* top_logprobs_dev,
@@ -2557,6 +2563,12 @@ int32_t wick_cuda_attention_q4(const wick_cuda_kv_q4* cache, const void* q_dev, 
     if (!q_dev || !slots_dev || !lengths_dev || !out_dev) return fail(WICK_CUDA_ERR_BAD_ARG, "NULL argument");
     if (q_stride < (uint64_t)n_heads * c.head_dim) return fail(WICK_CUDA_ERR_BAD_ARG, "attention_q4: rows of q overlap");
     if (misaligned(q_dev, dtype_bytes(dtype)) || misaligned(out_dev, dtype_bytes(dtype))) return fail(WICK_CUDA_ERR_BAD_ARG, "attention_q4: misaligned rows");
+    const uint64_t b = dtype_bytes(dtype), dim = (uint64_t)n_heads * c.head_dim, rows = (uint64_t)c.n_slots * c.n_kv * c.max_seq;
+    bool over = meets(out_dev, n * dim * b, q_dev, n, q_stride * b, dim * b) && !(out_dev == q_dev && q_stride == dim);
+    for (int side = 0; side < 2; side++)
+        over = over || meets(out_dev, n * dim * b, c.q[side], 1, 1, rows * (c.head_dim / 2)) || meets(out_dev, n * dim * b, c.d[side], 1, 1, rows * (c.head_dim / QK) * 2);
+    if (over || meets(out_dev, n * dim * b, slots_dev, 1, 1, n * 4ull) || meets(out_dev, n * dim * b, lengths_dev, 1, 1, n * 4ull))
+        return fail(WICK_CUDA_ERR_BAD_ARG, "attention_q4: out overlaps an input (it may be q itself, with dense rows)");
     const uint64_t need = attention_q4_workspace(c.head_dim);
     if (workspace_bytes < need || (need && (!workspace_dev || misaligned(workspace_dev, 16))))
         return fail(WICK_CUDA_ERR_BAD_ARG, "attention_q4: workspace missing, misaligned or too small");
@@ -2604,6 +2616,11 @@ int32_t wick_cuda_attention_prompts(const void* q_dev, uint64_t q_stride, const 
         return fail(WICK_CUDA_ERR_BAD_ARG, "attention_prompts: q, k, v, out and the row strides must be multiples of 16 bytes");
     if (q_stride * b >= (1ull << 40) || k_stride * b >= (1ull << 40) || v_stride * b >= (1ull << 40))
         return fail(WICK_CUDA_ERR_BAD_ARG, "attention_prompts: row strides too large");
+    const uint64_t dim = (uint64_t)n_heads * head_dim, kv_dim = (uint64_t)n_kv_heads * head_dim, out_bytes = n_tokens * dim * b, offsets = (n_seqs + 1ull) * 4;
+    if ((meets(out_dev, out_bytes, q_dev, n_tokens, q_stride * b, dim * b) && !(out_dev == q_dev && q_stride == dim)) ||
+        meets(out_dev, out_bytes, k_dev, n_keys, k_stride * b, kv_dim * b) || meets(out_dev, out_bytes, v_dev, n_keys, v_stride * b, kv_dim * b) ||
+        meets(out_dev, out_bytes, starts_dev, 1, 1, offsets) || (key_starts_dev && meets(out_dev, out_bytes, key_starts_dev, 1, 1, offsets)))
+        return fail(WICK_CUDA_ERR_BAD_ARG, "attention_prompts: out overlaps an input (it may be q itself, with dense rows)");
     const uint64_t need = attention_prompts_workspace(p);
     if (workspace_bytes < need || (need && (!workspace_dev || misaligned(workspace_dev, 128))))
         return fail(WICK_CUDA_ERR_BAD_ARG, "attention_prompts: workspace missing, misaligned or too small");

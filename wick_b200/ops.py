@@ -341,7 +341,7 @@ def attention_q4(q: torch.Tensor, cache: KvCacheQ4, slots: torch.Tensor, lengths
                  out: torch.Tensor | None = None) -> torch.Tensor:
     """Attention of single tokens over the cache: row j of q [n, n_heads * head_dim] attends the first lengths[j] rows of slot
     slots[j]; several rows may name one slot.  Length 0 gives zeros; rows whose slot the cache does not have (padding: -1) are left as
-    they are in `out` (a new one has zeros there)."""
+    they are in `out` (a new one has zeros there).  `out` overlaps no input, but may be q itself."""
     dev = cache.dev
     q, n, dim, stride = _rows(q, "q", dev)
     if dim != n_heads * cache.head_dim:
@@ -363,7 +363,8 @@ def attention_prompts(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, starts:
                       key_starts: torch.Tensor | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
     """Causal attention of packed prompts: sequence s has the tokens starts[s] .. starts[s + 1] of q [tokens, n_heads * head_dim] and the
     keys key_starts[s] .. key_starts[s + 1] (default: the same) of k and v [keys, n_kv_heads * head_dim]; its last key belongs to its last
-    token.  Tokens without a key get zeros; rows behind the last sequence are left as they are in `out` (a new one has zeros there)."""
+    token.  Tokens without a key get zeros; rows behind the last sequence are left as they are in `out` (a new one has zeros there).
+    `out` overlaps no input, but may be q itself."""
     dev = q.get_device()
     q, n, dim, q_stride = _rows(q, "q", dev)
     k, n_keys, dim_k, k_stride = _rows(k, "k", dev)
