@@ -386,7 +386,7 @@ __global__ void __launch_bounds__(Q4Cfg<NB>::THREADS, 1) k_attention_q4(const __
                 }
             }
             const unsigned st = i % C::STAGES;
-            ok = ok && bar_wait(bars_at + st * 8, (i / C::STAGES) & 1);
+            if (ok) ok = __all_sync(0xffffffffu, bar_wait(bars_at + st * 8, (i / C::STAGES) & 1));  // (the warp's answer: all its outputs or none)
             const uint8_t* stage = ring + st * C::STAGE;
             const uint32_t* kw = reinterpret_cast<const uint32_t*>(stage);
             const uint32_t* vw = reinterpret_cast<const uint32_t*>(stage + C::QUANTS);
