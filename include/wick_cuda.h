@@ -385,7 +385,7 @@ int32_t wick_cuda_decode_batch_logits(wick_cuda_model* m, const uint32_t* tokens
  * agree with the formulas within rounding (f32 sums), they do not repeat the CPU path's order of operations.  Like the operators
  * above they take device pointers and are asynchronous on `stream`; none allocates, synchronises or keeps anything from one call for the
  * next, so that they can be captured.  The device of the buffers has to be the current one.  `dtype` is a ggml type id.
- * Waits on the device are bounded (about half a second each): rows whose wait expires are NaN. */
+ * Waits on the device are bounded (0.4 s each): rows whose wait expires are NaN, the context stays usable. */
 #define WICK_DTYPE_F32 0
 #define WICK_DTYPE_F16 1
 #define WICK_DTYPE_BF16 30
@@ -431,6 +431,10 @@ int32_t wick_cuda_attention_q4_workspace(uint32_t head_dim, uint64_t* bytes);
 int32_t wick_cuda_attention_q4(const wick_cuda_kv_q4* cache, const void* q_dev, uint64_t q_stride, int32_t dtype, uint32_t n, uint32_t n_heads,
                                const int32_t* slots_dev, const int32_t* lengths_dev, void* out_dev, int32_t zero_rest, void* workspace_dev,
                                uint64_t workspace_bytes, void* stream);
+
+/* Test hook for the bounded waits of the two attentions, for later calls of this thread: after how many rounds (a multiple of 256, of about 1.5 us
+ * each; 0: the usual 2^18) they expire, and whether (missing = 1) the copies' barriers want an arrival that nobody makes. */
+int32_t wick_cuda_debug_serving_waits(uint32_t rounds, uint32_t missing);
 
 /* Causal attention of packed prompts: sequence s has the tokens [starts[s], starts[s+1]) of q [n_tokens][n_heads*head_dim] and the keys
  * [key_starts[s], key_starts[s+1]) of k and v [n_keys][n_kv_heads*head_dim]; its last key belongs to its last token, so that token j of

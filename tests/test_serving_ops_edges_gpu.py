@@ -309,3 +309,48 @@ def test_out_over_another_input(ops):
         with pytest.raises(_lib.WickCudaError, match="overlaps"):
             f()
     ops.attention_prompts(q, k, k, i, 1, 1, 64, out=x[18:27])  # beside them
+
+
+# ── waits that run out ─────────────────────────────────────────────────────────────────────────────
+@pytest.fixture
+def expiring(cuda_lib):
+    """Copies whose barriers want one arrival more than anybody makes, and waits of 1.5 ms."""
+    assert cuda_lib.wick_cuda_debug_serving_waits(1024, 1) == 0
+    yield
+    assert cuda_lib.wick_cuda_debug_serving_waits(0, 0) == 0
+
+
+@pytest.mark.parametrize("dtype,hd", [(torch.float32, 64), (torch.float32, 128), (torch.float16, 64), (torch.bfloat16, 128)], ids=str)
+@pytest.mark.parametrize("nq,prefix", [([300, 0, 45], 0), ([60, 7], 3000)], ids=str)
+def test_attention_prompts_whose_waits_run_out(ops, cuda_lib, expiring, dtype, hd, nq, prefix):
+    """Every row with a key is NaN, rows of no sequence are as they were, and the next call is right."""
+    heads, kv = 4, 2
+    n, nk, g = sum(nq), [m + prefix for m in nq], _gen(hd)
+    q, k, v = _randn(g, n + 5, heads * hd).to(dtype), _randn(g, sum(nk), kv * hd).to(dtype), _randn(g, sum(nk), kv * hd).to(dtype)
+    out = torch.full_like(q, 3.0)
+    args = (q, k, v, _starts(nq), heads, kv, hd, _starts(nk), out)
+    ops.attention_prompts(*args)
+    torch.cuda.synchronize()
+    assert torch.isnan(out[:n]).all() and (out[n:] == 3).all()
+    assert cuda_lib.wick_cuda_debug_serving_waits(0, 0) == 0
+    ops.attention_prompts(*args)
+    ref, tol = _prompts_ref(q[:n], k, v, nq, nk, heads, kv, hd)
+    _check(out[:n], ref, tol, v.abs().max().double())
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("heads,kv,hd", [(8, 2, 64), (12, 2, 96), (16, 4, 128)])
+def test_attention_q4_whose_waits_run_out(ops, cuda_lib, expiring, dtype, heads, kv, hd):
+    """The same, for rows of one tile, of several CTAs, of no key and of no slot."""
+    g = _gen(heads)
+    cache = _random_cache(ops, g, 4, 8192, kv, hd)
+    slots, lengths = [0, 1, 2, -1, 3], [1, 8000, 0, 5, 700]
+    q = _randn(g, 5, heads * hd).to(dtype)
+    out = torch.full_like(q, 3.0)
+    ops.attention_q4(q, cache, _i32(slots), _i32(lengths), heads, out=out)
+    torch.cuda.synchronize()
+    assert torch.isnan(out[[0, 1, 4]]).all() and (out[2] == 0).all() and (out[3] == 3).all()
+    assert cuda_lib.wick_cuda_debug_serving_waits(0, 0) == 0
+    ops.attention_q4(q, cache, _i32(slots), _i32(lengths), heads, out=out)
+    ref, tol, vmax = _q4_ref(q[[0, 1, 4]], cache, [0, 1, 3], [1, 8000, 700], heads)
+    _check(out[[0, 1, 4]], ref, tol, vmax)

@@ -46,3 +46,10 @@ def test_attention_q4_refuses_an_out_over_its_inputs(cuda_lib):
         assert not call(at - size) and not call(at + length)
         assert call(at - size + 4) and call(at + length - 4)
     assert call(A, qs=257)
+
+
+def test_limits_of_the_hook_for_waits(cuda_lib):
+    from wick_b200 import _lib
+    for rounds, missing in ((100, 0), ((1 << 18) + 256, 0), (0, 2)):
+        assert cuda_lib.wick_cuda_debug_serving_waits(rounds, missing) == _lib.ERR_BAD_ARG
+    assert cuda_lib.wick_cuda_debug_serving_waits(0, 0) == _lib.OK

@@ -118,6 +118,7 @@ SIGNATURES = {
     "wick_cuda_token_logprobs": [_vp, _i32, _u64, _u32, _u32, _vp, _u32, _vp, _vp, _vp, _vp, _vp],
     "wick_cuda_kv_append_q4": [C.POINTER(KvQ4), _vp, _u64, _vp, _u64, _i32, _u32, _vp, _vp, _vp],
     "wick_cuda_kv_read_q4": [C.POINTER(KvQ4), _u32, _vp, _vp, _vp, _vp, _vp],
+    "wick_cuda_debug_serving_waits": [_u32, _u32],
     "wick_cuda_attention_q4_workspace": [_u32, C.POINTER(_u64)],
     "wick_cuda_attention_q4": [C.POINTER(KvQ4), _vp, _u64, _i32, _u32, _u32, _vp, _vp, _vp, _i32, _vp, _u64, _vp],
     "wick_cuda_attention_prompts_workspace": [_i32, _u32, _u32, _u32, _u32, _u32, _u32, C.POINTER(_u64)],

@@ -54,7 +54,6 @@ constexpr int PR_ROWS = 128;      // rows of a tile == lanes of tensor memory
 constexpr int PR_THREADS = 384;   // TMA, MMA, V check, items; 2 x 4 softmax warps
 constexpr int PR_ITEMS = 3;       // items that are known ahead
 constexpr int PR_MASKED = 8;      // tiles that some row of a CTA sees in part: at most 256 / 64 + 2
-constexpr uint32_t PR_SPIN_LIMIT = 1u << 24;  // about half a second (2^18: 8 ms)
 constexpr int PR_CARRY = 64;     // tiles
 constexpr float PR_LAZY = 8.0f, PR_DOWN = 0x1p-8f;  // 2^-PR_LAZY
 
@@ -94,7 +93,7 @@ struct Shared {
     unsigned long long q_full[2], q_raw[2], q_empty, k_full[6], v_full[6], empty[6], ready[6], s_full[2], s_read[2], p_ready[2], o_full[2];
     unsigned long long item_full[PR_ITEMS], item_empty[PR_ITEMS], checked[PR_ITEMS];
     Item item[PR_ITEMS];
-    uint32_t tmem_base;
+    uint32_t tmem_base, wait_rounds;
     volatile uint32_t abort;
 };
 static_assert(sizeof(Shared) <= 1024, "room behind the ring");
@@ -112,6 +111,7 @@ struct PromptArgs {
     int zero_rest;
     int wide_rows;                       // rows of out start on 32-byte boundaries
     float scale_log2;
+    ServingWaits waits;
 };
 
 __device__ __forceinline__ uint32_t smem_u32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
@@ -137,9 +137,12 @@ __device__ __forceinline__ bool bar_try(void* bar, uint32_t parity) {
 }
 // false: the limit, or another role has given up
 __device__ __forceinline__ bool bar_wait(Shared* b, void* bar, uint32_t parity) {
-    for (uint32_t i = 0; i < PR_SPIN_LIMIT; i++) {
+    for (uint32_t i = 1;; i++) {
         if (bar_try(bar, parity)) return true;
-        if ((i & 255u) == 255u && b->abort) return false;
+        if ((i & 255u) == 0) {
+            if (b->abort) return false;
+            if (i >= b->wait_rounds) break;
+        }
     }
     b->abort = 1;
     return false;
@@ -444,9 +447,9 @@ k_attention_prompts(const __grid_constant__ CUtensorMap map_q, const __grid_cons
             bar_init(&sh->s_full[m], 1), bar_init(&sh->s_read[m], 4), bar_init(&sh->p_ready[m], 4), bar_init(&sh->o_full[m], 1);
         }
         bar_init(&sh->q_empty, 1);
-        for (int s = 0; s < NS; s++) bar_init(&sh->k_full[s], 1), bar_init(&sh->v_full[s], 1), bar_init(&sh->empty[s], 1), bar_init(&sh->ready[s], 1);
+        for (int s = 0; s < NS; s++) bar_init(&sh->k_full[s], 1), bar_init(&sh->v_full[s], 1 + a.waits.missing), bar_init(&sh->empty[s], 1), bar_init(&sh->ready[s], 1);
         for (int i = 0; i < PR_ITEMS; i++) bar_init(&sh->item_full[i], 1), bar_init(&sh->item_empty[i], 11), bar_init(&sh->checked[i], 1);
-        sh->abort = 0;
+        sh->abort = 0, sh->wait_rounds = a.waits.rounds;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     }
@@ -777,10 +780,13 @@ k_attention_prompts(const __grid_constant__ CUtensorMap map_q, const __grid_cons
             // 16 bits: O of PR_CARRY tiles at a time, added up outside the tensor core, behind it the maximum that the sum goes by (local memory: few
             // calls come here, and it takes no registers from the others)
             float carry[C::O_IN_TMEM ? HDP + 1 : 1];
+            carry[0] = 0.0f;
             auto with_carry = [&](int c, float (&x)[32]) {
-                const float was = carry[C::O_IN_TMEM ? HDP : 0], f = was == row_max ? 1.0f : exp2_approx(was - row_max);
+                if constexpr (C::O_IN_TMEM) {
+                    const float was = carry[HDP], f = was == row_max ? 1.0f : exp2_approx(was - row_max);
 #pragma unroll
-                for (int d = 0; d < 32; d++) x[d] = fmaf(carry[C::O_IN_TMEM ? c + d : 0], f, x[d]);
+                    for (int d = 0; d < 32; d++) x[d] = fmaf(carry[c + d], f, x[d]);
+                }
             };
             if constexpr (C::O_IN_TMEM) {
                 for (int first = 0; first < n && ok; first += PR_CARRY) {
@@ -794,10 +800,10 @@ k_attention_prompts(const __grid_constant__ CUtensorMap map_q, const __grid_cons
                             tmem_ld_wait();
                             if (first > PR_CARRY) with_carry(c, x);
 #pragma unroll
-                            for (int d = 0; d < 32; d++) carry[C::O_IN_TMEM ? c + d : 0] = x[d], x[d] = 0.0f;
+                            for (int d = 0; d < 32; d++) carry[c + d] = x[d], x[d] = 0.0f;
                             tmem_st32(t_o + c, x);
                         }
-                        carry[C::O_IN_TMEM ? HDP : 0] = row_max;
+                        carry[HDP] = row_max;
                     }
                     for (int i = first; i < min(n, first + PR_CARRY) && ok; i++) {
                         if (!(ok = __all_sync(0xffffffffu, bar_wait(sh, &sh->s_full[m], (done + i) & 1)))) break;
@@ -1151,7 +1157,7 @@ k_attention_prompts(const __grid_constant__ CUtensorMap map_q, const __grid_cons
     __syncthreads();
     if (warp == 1) {
         if (sh->abort) {
-            for (int i = 0; i < 64; i++) __nanosleep(1000);  // copies issued before the failure may still be landing
+            settle();
             Deal<NK> deal(a);
             Item it;
             while (deal.next(a, it)) {  // no row is left without a sign of it
@@ -1414,6 +1420,7 @@ cudaError_t launch_typed(cudaStream_t st, const Prompts& p, void* workspace) {
     a.tile_tokens = PR_ROWS / a.group;
     a.slots = places(p.n_tokens, p.n_seqs, 2 * a.tile_tokens);
     a.zero_rest = p.zero_rest;
+    a.waits = serving_waits();
     a.wide_rows = (((uintptr_t)p.out | (size_t)p.head_dim * sizeof(T)) & 31) == 0;
     a.scale_log2 = 1.4426950408889634f / sqrtf((float)p.head_dim);
     const int parts = PLANES == 2 ? DT_F16 : p.dtype;  // what K and V are in
@@ -1458,6 +1465,11 @@ cudaError_t launch_typed(cudaStream_t st, const Prompts& p, void* workspace) {
 }
 
 }  // namespace
+
+ServingWaits& serving_waits() {
+    static thread_local ServingWaits waits;
+    return waits;
+}
 
 size_t attention_prompts_workspace(const Prompts& p) { return Workspace(p).bytes; }
 

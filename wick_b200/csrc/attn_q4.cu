@@ -31,7 +31,6 @@ namespace wick {
 namespace {
 
 constexpr int A4_TILE = KV_Q4_TILE, A4_HEADS = 8;
-constexpr uint32_t A4_SPIN_LIMIT = 1u << 24;  // about half a second
 constexpr int A4_MIN_EXP = -24;  // of f16's smallest number
 
 template <int NB>  // 32-element blocks of a head
@@ -55,6 +54,7 @@ struct Q4Args {
     int n, n_heads, group, sub, n_hg;  // query heads per KV head, head groups per KV head and in all
     int zero_rest;
     float scale_log2;
+    ServingWaits waits;
     float* parts;   // [ctas][2][PART]: a CTA's part of what began before it, and of what goes on behind it
     int4* descs;    // [ctas][2]: row, head group, whether it holds its begin (1) and its end (2), whether there is one
 };
@@ -64,8 +64,8 @@ __device__ __forceinline__ void bulk_copy(uint32_t dst, const void* src, uint32_
     asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src), "r"(bytes), "r"(bar)
                  : "memory");
 }
-__device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity) {
-    for (uint32_t i = 0; i < A4_SPIN_LIMIT; i++) {
+__device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity, uint32_t rounds) {
+    for (uint32_t i = 0; i < rounds; i++) {
         uint32_t ok;
         asm volatile(
             "{\n\t.reg .pred p;\n\t"
@@ -267,7 +267,7 @@ __global__ void __launch_bounds__(Q4Cfg<NB>::THREADS, 1) k_attention_q4(const __
     __shared__ unsigned long long warp_sum[C::WARPS];
     __shared__ int4 desc[C::WARPS][2];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t4 = lane & 3;
-    if (lane < C::STAGES) asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(s_u32(&bars[warp][lane])) : "memory");
+    if (lane < C::STAGES) asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(s_u32(&bars[warp][lane])), "r"(1 + a.waits.missing) : "memory");
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     if (lane < 2) desc[warp][lane] = make_int4(0, 0, 0, 0);
@@ -386,7 +386,7 @@ __global__ void __launch_bounds__(Q4Cfg<NB>::THREADS, 1) k_attention_q4(const __
                 }
             }
             const unsigned st = i % C::STAGES;
-            if (ok) ok = __all_sync(0xffffffffu, bar_wait(bars_at + st * 8, (i / C::STAGES) & 1));  // (the warp's answer: all its outputs or none)
+            if (ok) ok = __all_sync(0xffffffffu, bar_wait(bars_at + st * 8, (i / C::STAGES) & 1, a.waits.rounds));  // (the warp's answer: all its outputs or none)
             const uint8_t* stage = ring + st * C::STAGE;
             const uint32_t* kw = reinterpret_cast<const uint32_t*>(stage);
             const uint32_t* vw = reinterpret_cast<const uint32_t*>(stage + C::QUANTS);
@@ -565,8 +565,7 @@ __global__ void __launch_bounds__(Q4Cfg<NB>::THREADS, 1) k_attention_q4(const __
         if (row_tiles(a, j) == 0 && (a.zero_rest || (a.slots[j] >= 0 && a.slots[j] < a.c.n_slots)))
             for (int i = tid; i < a.n_heads * C::HD; i += C::THREADS) static_cast<T*>(a.out)[(size_t)j * a.n_heads * C::HD + i] = from_f32<T>(0.0f);
     if (tid < 2) a.descs[(size_t)blockIdx.x * 2 + tid] = make_int4(0, 0, 0, 0);
-    if (!ok)
-        for (int i = 0; i < 64; i++) __nanosleep(1000);  // copies may still be landing
+    if (!ok) settle();  // (copies may still be landing)
     __syncthreads();
 
     // ── parts within the CTA.  A chain starts with the part that begins in a warp (place 1) or with the first part of all, if that began
@@ -716,6 +715,7 @@ cudaError_t launch_attention_q4(cudaStream_t st, const KvQ4& c, const void* q, s
     a.out = out;
     a.n = n, a.n_heads = n_heads, a.group = n_heads / c.n_kv, a.sub = (a.group + A4_HEADS - 1) / A4_HEADS, a.n_hg = c.n_kv * a.sub;
     a.zero_rest = zero_rest;
+    a.waits = serving_waits();
     a.scale_log2 = 1.4426950408889634f / sqrtf((float)c.head_dim);
     a.parts = static_cast<float*>(workspace);
     a.descs = reinterpret_cast<int4*>(static_cast<uint8_t*>(workspace) + part_bytes(c.head_dim));

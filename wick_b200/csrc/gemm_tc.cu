@@ -50,7 +50,7 @@ __host__ __device__ constexpr int tc_units() { return 512 / (BN * TC_KB_PER_STAG
 constexpr int TC_COL_GROUPS = 2;    // epilogue warps per TMEM lane quarter; each takes half of a tile's columns
 constexpr int TC_EPI_WARPS = 4 * TC_COL_GROUPS;
 constexpr int TC_THREADS = 32 * (4 + TC_EPI_WARPS);
-constexpr uint32_t TC_SPIN_LIMIT = 1u << 18;  // try_wait itself suspends for a while, so this is of the order of a second
+constexpr uint32_t TC_SPIN_LIMIT = 1u << 18;  // rounds of try_wait, 1.48 us each on a phase that does not end: 0.39 s
 
 template <int BN>
 struct alignas(1024) TcStage {

@@ -7,6 +7,25 @@
 
 namespace wick {
 
+// The device-side waits of the two attentions, for the calling thread's launches: rounds of try_wait after which one gives up (a round on a phase that does
+// not end takes 1.48 us, 2^18 of them 0.39 s), and, for tests, arrivals that a copy's barrier wants and nobody makes.
+struct ServingWaits {
+    uint32_t rounds = 1u << 18, missing = 0;
+};
+ServingWaits& serving_waits();
+#ifdef __CUDACC__
+// Behind a wait that ran out: copies and matrix instructions that are under way end within this time.
+__device__ __forceinline__ void settle() {
+    unsigned long long t0, t;
+    asm volatile("mov.u64 %0, %globaltimer;" : "=l"(t0));
+    for (int i = 0; i < 1000; i++) {
+        __nanosleep(1000);
+        asm volatile("mov.u64 %0, %globaltimer;" : "=l"(t));
+        if (t - t0 > 100000) break;
+    }
+}
+#endif
+
 constexpr int LOGPROBS_MAX_TOP = 64;
 cudaError_t launch_token_logprobs(cudaStream_t st, const void* logits, int dtype, size_t row_stride, int n, int vocab, const int32_t* tokens,
                                   int top_n, float* logprob, float* entropy, int32_t* top_ids, float* top_logprobs);

@@ -2472,6 +2472,14 @@ int32_t wick_cuda_argmax(const float* logits_dev, uint32_t count, uint32_t* out_
 }
 
 // ── operators of a serving step ─────────────────────────────────────────────
+int32_t wick_cuda_debug_serving_waits(uint32_t rounds, uint32_t missing) {
+    if (rounds % 256 || rounds > (1u << 18) || missing > 1)
+        return fail(WICK_CUDA_ERR_BAD_ARG, "debug_serving_waits: a multiple of 256 rounds, at most 2^18, and at most one missing arrival");
+    serving_waits() = ServingWaits{};
+    if (rounds) serving_waits().rounds = rounds;
+    serving_waits().missing = missing;
+    return WICK_CUDA_OK;
+}
 static int32_t check_dtype(int32_t dtype) {
     return dtype_bytes(dtype) ? WICK_CUDA_OK : fail(WICK_CUDA_ERR_UNSUPPORTED_DTYPE, "dtype must be f32, f16 or bf16");
 }
