@@ -413,7 +413,8 @@ typedef struct wick_cuda_kv_q4 {
 } wick_cuda_kv_q4;
 /* Rounds row j of k and v [n][n_kv_heads*head_dim] (rows k_stride / v_stride elements apart) to Q4_0 and writes them to row
  * positions_dev[j] of slot slots_dev[j].  A row whose slot or position the cache does not have (a padding row: -1) is skipped.  The
- * pairs (slot, position) of a call differ from one another: of two rows with the same pair every block is one row's or the other's.
+ * pairs (slot, position) of a call differ from one another: what a row holds that two of them name is not defined (numbers of one may stand
+ * beside scales of the other).
  * Values are finite and below 524032 in magnitude (the f16 scale).  At most 2^31 - 256 rows and 2^38 elements a call, here and below. */
 int32_t wick_cuda_kv_append_q4(const wick_cuda_kv_q4* cache, const void* k_dev, uint64_t k_stride, const void* v_dev, uint64_t v_stride,
                                int32_t dtype, uint32_t n, const int32_t* slots_dev, const int32_t* positions_dev, void* stream);

@@ -53,3 +53,40 @@ def test_limits_of_the_hook_for_waits(cuda_lib):
     for rounds, missing in ((100, 0), ((1 << 18) + 256, 0), (0, 2)):
         assert cuda_lib.wick_cuda_debug_serving_waits(rounds, missing) == _lib.ERR_BAD_ARG
     assert cuda_lib.wick_cuda_debug_serving_waits(0, 0) == _lib.OK
+
+
+def test_calls_for_another_device_than_the_current_one(monkeypatch):
+    """They are made with the tensors' device as the current one and on its stream; the old one comes back, after a failure too."""
+    import pytest
+    import torch
+    from wick_b200 import _lib, ops
+    current, calls = [0], []
+
+    class Device:
+        def __init__(self, index):
+            self.index = index
+
+        def __enter__(self):
+            self.before, current[0] = current[0], self.index
+
+        def __exit__(self, *error):
+            current[0] = self.before
+
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: current[0])
+    monkeypatch.setattr(torch.cuda, "device", Device)
+    monkeypatch.setattr(ops, "_raw_stream", lambda dev: 1000 + dev)
+    code = _lib.OK
+    monkeypatch.setattr(ops, "check", lambda c: (_ for _ in ()).throw(_lib.WickCudaError(c, "refused")))
+
+    def fn(*args):
+        calls.append((current[0], *args))
+        return code
+
+    ops._call(fn, 0, 7)
+    ops._call(fn, 3, 7, 8)
+    assert calls == [(0, 7, 1000), (3, 7, 8, 1003)] and current == [0]
+    code = _lib.ERR_BAD_ARG
+    for dev in (0, 2):
+        with pytest.raises(_lib.WickCudaError):
+            ops._call(fn, dev)
+    assert calls[2:] == [(0, 1000), (2, 1002)] and current == [0]
