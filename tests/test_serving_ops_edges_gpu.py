@@ -354,3 +354,22 @@ def test_attention_q4_whose_waits_run_out(ops, cuda_lib, expiring, dtype, heads,
     ops.attention_q4(q, cache, _i32(slots), _i32(lengths), heads, out=out)
     ref, tol, vmax = _q4_ref(q[[0, 1, 4]], cache, [0, 1, 3], [1, 8000, 700], heads)
     _check(out[[0, 1, 4]], ref, tol, vmax)
+
+
+@pytest.mark.parametrize("seqs", [255, 256, 257, 600])
+def test_attention_prompts_around_the_walk_over_sequences(ops, seqs):
+    """Up to 256 sequences are walked through for every item, more are searched for; some are empty."""
+    heads, kv, hd = 4, 2, 64
+    lengths = [(i * 37) % 90 for i in range(seqs)]
+    lengths[-1] = 400
+    g, n = _gen(seqs), sum(lengths)
+    q, k, v = (_randn(g, n, h * hd).half() for h in (heads, kv, kv))
+    starts = _starts(lengths)
+    out = ops.attention_prompts(q, k, v, starts, heads, kv, hd, out=torch.full_like(q, math.nan))
+    assert torch.isfinite(out).all()
+    at = starts.tolist()
+    for s in {0, 1, 31, 32, 100, seqs // 2, seqs - 2, seqs - 1}:
+        a, b = at[s], at[s + 1]
+        if a < b:
+            ref, tol = _prompts_ref(q[a:b], k[a:b], v[a:b], [b - a], [b - a], heads, kv, hd)
+            _check(out[a:b], ref, tol, v.abs().max().double())

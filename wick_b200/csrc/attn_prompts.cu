@@ -289,9 +289,11 @@ __device__ __forceinline__ uint32_t magnitude(float4 v) {  // the largest one's 
 }
 
 // The blocks of 2 * tile_tokens tokens, counted through the sequences, by a whole warp: how many there are (want < 0), or which sequence has number
-// `want` and which of its blocks that is (*seq -1: none).  With more sequences than a warp can walk through for every item, numbers are
-// places as of find_seq, not all of which have a block.
-constexpr int PR_WALK = 1024;
+// `want` and which of its blocks that is (*seq -1: none).  From PR_WALK sequences on, numbers are places as of find_seq, not all of which
+// have a block: two or three steps in place of a walk over 32 sequences at a time, but items dealt less evenly.  (Prompts of 64 tokens, 16 / 8 heads of 64, f16: 33,
+// 128, 256, 512, 1024 sequences walked through 15, 40, 75, 156, 421 us, searched for 19, 42, 70, 132, 257; of 200 tokens 31, 100, 192, 378, 936 and 37,
+// 103, 190, 366, 705.)
+constexpr int PR_WALK = 256;
 __device__ __forceinline__ int count_blocks(const PromptArgs& a, int want, int* seq, int* at) {
     const int block = 2 * a.tile_tokens, lane = threadIdx.x & 31;
     *seq = -1, *at = 0;

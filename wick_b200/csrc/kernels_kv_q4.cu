@@ -29,7 +29,8 @@ dim3 row_threads(const KvQ4& c, int per_block) {
     return dim3((unsigned)x, (unsigned)(KV_THREADS / x));
 }
 // Rows that a thread has under way together: a row is two or three dependent trips to memory, and at prompts the SMs' threads are too few
-// to hide them one by one (4093 rows of 512, append and read back: 18.3 us one at a time, 15.4 us so).
+// to hide them one by one; below, more blocks do.  (Rows of 512, one at a time / four, append: 512 rows 3.3 / 3.7 us, 1024 4.3 / 4.4, 2048 6.5 / 6.1, 4093 11.0 / 9.4;
+// reading: 2.2 / 3.1, 3.0 / 3.3, 4.3 / 4.5, 6.8 / 6.6.  Rows of 1024 alike, rows of 64 gain from 4000 on: 0.7 us at most either way.)
 constexpr int KV_MANY = 4, KV_MANY_FROM = 1024;
 
 // Four values per lane, a block on 8 lanes.  4093 rows of 512 with their reading back: 15.4 us where the bytes take 5.8; it waits for memory (a row is two or
