@@ -425,9 +425,9 @@ int32_t wick_cuda_kv_read_q4(const wick_cuda_kv_q4* cache, uint32_t n, const int
 /* Attention of single tokens over the cache: row j of q [n][n_heads*head_dim] (rows q_stride elements apart) attends the first
  * lengths_dev[j] rows (at most max_seq) of slot slots_dev[j], scores scaled by 1 / sqrt(head_dim); several rows may name the same slot.
  * out [n][n_heads*head_dim] has q's type.  Length 0 (or less) gives zeros; a row whose slot the cache does not have (a padding row: -1)
- * is set to zero with zero_rest != 0 and left as it was otherwise.  What the cache holds behind a row's length is never used, whatever it is.  out overlaps no input,
- * but may be q itself where q's rows are dense.  At most 65535 rows and heads.  workspace_dev: 16-byte aligned, as many
- * bytes as wick_cuda_attention_q4_workspace says, with any content; of this call alone until it has finished. */
+ * is set to zero with zero_rest != 0 and left as it was otherwise.  What the cache holds behind a row's length is never used, whatever it is.
+ * out overlaps no input, but may be q itself where q's rows are dense.  At most 65535 rows and heads.  workspace_dev: 16-byte aligned,
+ * as many bytes as wick_cuda_attention_q4_workspace says, with any content; of this call alone until it has finished. */
 int32_t wick_cuda_attention_q4_workspace(uint32_t head_dim, uint64_t* bytes);
 int32_t wick_cuda_attention_q4(const wick_cuda_kv_q4* cache, const void* q_dev, uint64_t q_stride, int32_t dtype, uint32_t n, uint32_t n_heads,
                                const int32_t* slots_dev, const int32_t* lengths_dev, void* out_dev, int32_t zero_rest, void* workspace_dev,
@@ -440,14 +440,15 @@ int32_t wick_cuda_debug_serving_waits(uint32_t rounds, uint32_t missing);
 /* Causal attention of packed prompts: sequence s has the tokens [starts[s], starts[s+1]) of q [n_tokens][n_heads*head_dim] and the keys
  * [key_starts[s], key_starts[s+1]) of k and v [n_keys][n_kv_heads*head_dim]; its last key belongs to its last token, so that token j of
  * nq attends its keys t <= j + nk - nq.  starts_dev / key_starts_dev hold n_seqs + 1 ascending offsets; key_starts_dev NULL: the same as
- * starts_dev.  A token without keys, or all of whose scores are -inf, gets zeros.  Rows of q, k and v that belong to no sequence (behind the last one) are not used, those of
- * out are set to zero with zero_rest != 0 and left as they were otherwise.  Scores are scaled by 1 / sqrt(head_dim).  All of q, k, v, out have the type `dtype`; rows of q, k,
- * v are q_stride / k_stride / v_stride elements apart; out rows are dense.  head_dim is a multiple of 8 and at most 128;
- * pointers and row strides are multiples of 16 bytes.  f32 elements are held to 2^-22 of themselves or 2^-24 of their row's (token's
- * and head's) largest, whatever the other rows hold; in 16 bits the weights are rounded to that type.  A key or value that is infinite or NaN
- * reaches the tokens that attend it and no others: a score of -inf has no weight, an infinite value makes its column infinite (in 16 bits
- * NaN where the weight rounds to 0), values of both infinities make it NaN.  out overlaps no input, but may be q itself where q's rows are dense.
- * workspace_dev: 128-byte aligned, as many bytes as
+ * starts_dev.  A token without keys, or all of whose scores are -inf, gets zeros.  Rows of q, k and v that belong to no sequence (behind the last
+ * one) are not used, those of out are set to zero with zero_rest != 0 and left as they were otherwise.  Scores are scaled by 1 / sqrt(head_dim).
+ * All of q, k, v, out have the type `dtype`; rows of q, k, v are q_stride / k_stride / v_stride elements apart; out rows are dense.  head_dim
+ * is a multiple of 8 and at most 128; pointers and row strides are multiples of 16 bytes.
+ * f32 elements are held to 2^-22 of themselves or 2^-24 of their row's (token's and head's) largest, whatever the other rows hold; in 16 bits
+ * the weights are rounded to that type.  A key or value that is infinite or NaN reaches the tokens that attend it and no others: a score of
+ * -inf has no weight, an infinite value makes its column infinite (in 16 bits infinite or NaN where the weight rounds to 0), values of both
+ * infinities make it NaN.
+ * out overlaps no input, but may be q itself where q's rows are dense.  workspace_dev: 128-byte aligned, as many bytes as
  * wick_cuda_attention_prompts_workspace says, with any content; of this call alone until it has finished. */
 int32_t wick_cuda_attention_prompts_workspace(int32_t dtype, uint32_t n_seqs, uint32_t n_tokens, uint32_t n_keys, uint32_t n_heads,
                                               uint32_t n_kv_heads, uint32_t head_dim, uint64_t* bytes);

@@ -9,20 +9,18 @@
 // softmax warps, one row per thread -> P in tensor memory -> P V with P as the A operand from there.  The two row tiles alternate: while one is
 // in the tensor core the other is in its softmax; and an item's last rows are written while the next one's first scores are computed.
 //
-// f16, bf16: one product each; O stays in tensor memory, and is rescaled only where a row's maximum has grown by more than 2^8 (a weight is at
-//   most 2^8 then, times 2^7 in f16; the last maximum that was used cancels in the quotient).  Weights are rounded to the operands' type, half a step each, as the
-//   tensor core takes them; their sum is of the unrounded ones.  The tensor core adds with truncation: O is
-//   taken out and added up in f32 every 64 tiles (8192 keys: 5e-5 of the sum; 131072 without this were 7e-4, 1.5 half steps of f16).
-// f32: every operand is split into two f16 parts, x = 2^e (hi + lo), 22 bits, with one power of two per row of Q and per tile of K and V
-//   (K and V by k_split; a row of Q where it lies in shared memory, by the thread that owns it), and a product is hi hi + hi lo + lo hi (lo lo
-//   is 2^-22 of it).  An element is held to 2^-22 of itself or 2^-24 of its row's largest.  Rows of a K or V tile whose magnitudes are too far
-//   apart for one power of two (a row's largest element below 2^-14 of the others', or above them) are zeros in the parts: the threads
-//   that attend such a far key compute its score, and add its weighted value, in f32 from K and V themselves (eight prompts of 1000 tokens, 32 / 8
-//   heads of 64: 161 us without far keys, 323 with one in every tile, 1075 with one in 16).  What a token does not attend does not change
-//   its result beyond that rounding.  Keys with infinities or NaN are far, too; values that are not finite are zeros in the parts and are added
-//   to the rows that attend them at the end.
-//   The tensor core adds with truncation, so that a sum over thousands of keys would drift by 1e-5: O is taken out after every tile and added
-//   up in registers.
+// f16, bf16: one product each; O stays in tensor memory, and is rescaled only where a row's maximum has grown by more than 2^8 (a weight is at most
+//   2^8 then, times 2^7 in f16; the last maximum that was used cancels in the quotient).  Weights are rounded to the operands' type, half a step
+//   each, as the tensor core takes them; their sum is of the unrounded ones.  The tensor core adds with truncation: O is taken out and added up in
+//   f32 every 64 tiles (8192 keys: 5e-5 of the sum; 131072 without this were 7e-4, 1.5 half steps of f16).
+// f32: every operand is split into two f16 parts, x = 2^e (hi + lo), 22 bits, with one power of two per row of Q and per tile of K and V (K and V by
+//   k_split; a row of Q where it lies in shared memory, by the thread that owns it), and a product is hi hi + hi lo + lo hi (lo lo is 2^-22 of it).
+//   O is taken out after every tile and added up in registers, as with truncated additions a sum over thousands of keys would drift by 1e-5.
+//   An element is held to 2^-22 of itself or 2^-24 of its row's largest.  Rows of a K or V tile that are too far apart for one power of two (a row's
+//   largest element below 2^-14 of the others', or above them) are zeros in the parts: the threads that attend such a far key compute its score, and
+//   add its weighted value, in f32 from K and V themselves (eight prompts of 1000 tokens, 32 / 8 heads of 64: 161 us without far keys, 323 with one in
+//   every tile, 1075 with one in 16).  What a token does not attend does not change its result beyond that rounding.  Keys with infinities or NaN are
+//   far, too; values that are not finite are zeros in the parts and are added to the rows that attend them at the end.
 //
 // Few items with many keys (a chunk of tokens behind a long prefix): the keys of an item are cut into `splits` parts, each an item of its own,
 // whose sums go to the workspace in f32 and are joined by k_join.
@@ -31,12 +29,12 @@
 // tile that some row sees in part, zeroes what is not finite (in f32: left behind the sequences in the workspace), and notes the keys; rows that
 // attend such a key add its values at the end.
 //
-// Bound, on a B200: the softmax and its MMAs in turn.  A pair of f32 tiles (heads of 64) takes 5300 cycles, 58 % of them MMAs: 2000 waiting for P V
-// and the next scores, 600 the maximum, 2150 the weights and their parts, 500 adding O.  A pair in 16 bits takes 3750 (heads of 64, 2750 the weights,
-// of which the special function unit needs 2048) or 4300 (heads of 128; 2048 MMA).  Eight prompts of 250 to 1001 tokens, 32 / 8 heads of 64, f32: 103 us
-// (tensor pipe 34 %); one of 8000, heads of 128, bf16: 473 us (1108 TFLOP/s), 533 under
-// the power cap.  Loops that run once per item stay rolled: unrolled they
-// took longer to fetch than to run (161 -> 116 us in the first case).
+// Bound, on a B200: the softmax and its MMAs in turn, two softmax warps to a scheduler, which wait for one another's results more than they issue (issue
+// slots 40 % in f32, 33 % in 16 bits).  A pair of tiles, one of each row tile, takes (slope of the time over the keys, 1965 MHz) in f32 5500 cycles (heads
+// of 64, 128 keys; 3072 of them MMAs by count) or 5700 (heads of 128, 64 keys), in 16 bits 3600 to 3700 (the special function unit needs 2048 for its
+// exponentials, the MMAs 1024 with heads of 64 and 2048 with 128).  Eight prompts of 250 to 1001 tokens, 32 / 8 heads of 64, f32: 97 us (tensor pipe
+// 35 %); one of 8000, heads of 128, bf16: 456 us (1150 TFLOP/s; tensor pipe 54 %, special function unit 54 %), 515 under the power cap.  Loops that run once per item stay rolled:
+// unrolled they took longer to fetch than to run (161 -> 116 us in the first case, before other steps).
 //
 // Every wait is bounded: on expiry all roles leave their loops and all rows of the CTA's items become NaN.
 #include <cuda.h>
@@ -124,21 +122,10 @@ __device__ __forceinline__ void bar_arrive(void* bar) {
 __device__ __forceinline__ void bar_expect(void* bar, uint32_t bytes) {
     asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(smem_u32(bar)), "r"(bytes) : "memory");
 }
-__device__ __forceinline__ bool bar_try(void* bar, uint32_t parity) {
-    uint32_t ok;
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
-        "selp.u32 %0, 1, 0, p;\n\t}"
-        : "=r"(ok)
-        : "r"(smem_u32(bar)), "r"(parity)
-        : "memory");
-    return ok != 0;
-}
 // false: the limit, or another role has given up
 __device__ __forceinline__ bool bar_wait(Shared* b, void* bar, uint32_t parity) {
     for (uint32_t i = 1;; i++) {
-        if (bar_try(bar, parity)) return true;
+        if (mbar_try_wait(smem_u32(bar), parity)) return true;
         if ((i & 255u) == 0) {
             if (b->abort) return false;
             if (i >= b->wait_rounds) break;
@@ -229,11 +216,6 @@ __device__ __forceinline__ void lds_4(uint32_t at, float* v) {
 }
 __device__ __forceinline__ void sts_4(uint32_t at, const uint32_t* v) {
     asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]) : "memory");
-}
-__device__ __forceinline__ float exp2_approx(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
 }
 template <class T>
 __device__ __forceinline__ uint32_t pack16(float a, float b) {  // a in the low half
@@ -466,8 +448,6 @@ k_attention_prompts(const __grid_constant__ CUtensorMap map_q, const __grid_cons
     tc_fence_after();
     const uint32_t tmem = sh->tmem_base;
 
-    // Registers: the launch has 12 warps of 168; four give up 80 each, eight take 40 more (4 x 88 + 8 x 208 = 12 x 168).  One instruction for the
-    // four, in front of their branches: a warpgroup executes it together.
     // Ring positions g = 0, 1, .. hold K0 V0 K1 V1 ..; K and V have barriers of their own, so that who waits for V needs nothing of the K's that share
     // its slot: an odd number of slots has them in turn, and a use's number among those of its kind is half its number then.
     auto use_parity = [](uint32_t g) { return ((NS & 1) ? g / NS >> 1 : g / NS) & 1; };
@@ -482,240 +462,242 @@ k_attention_prompts(const __grid_constant__ CUtensorMap map_q, const __grid_cons
         if (lane == 0) bar_arrive(&sh->item_empty[k % PR_ITEMS]);
     };
 
+    // Registers: the launch has 12 warps of 168; four give up 80 each, eight take 40 more (4 x 88 + 8 x 208 = 12 x 168).  One instruction for the
+    // four, in front of their branches: a warpgroup executes it together.
     if (warp < 4) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
         if (warp == 3) {
-        // ── items ────────────────────────────────────────────────────────────
-        Deal<NK> deal(a);
-        uint32_t k = 0;
-        while (true) {
-            Item it;
-            if (!deal.next(a, it)) it.kvh = -1;
-            if (!__all_sync(0xffffffffu, bar_wait(sh, &sh->item_empty[k % PR_ITEMS], ((k / PR_ITEMS) & 1) ^ 1))) break;
-            if (lane == 0) {
-                Item* to = &sh->item[k % PR_ITEMS];
-                to->token0 = it.token0, to->tokens = it.tokens, to->key0 = it.key0, to->keys = it.keys, to->first_visible = it.first_visible;
-                to->key_slot0 = it.key_slot0, to->kvh = it.kvh, to->part = it.part, to->n_tiles[0] = it.n_tiles[0], to->n_tiles[1] = it.n_tiles[1];
-                bar_arrive(&sh->item_full[k % PR_ITEMS]);
-            }
-            __syncwarp();
-            k++;
-            if (it.kvh < 0) break;
-        }
-        if (a.zero_rest) {  // rows of no sequence
-            const int first = max(0, min(a.p.starts[0], a.p.n_tokens)), last = max(first, min(a.p.starts[a.p.n_seqs], a.p.n_tokens));
-            const size_t row = (size_t)a.p.n_heads * hd * sizeof(T) / 16, n = (size_t)(a.p.n_tokens - last + first) * row;
-            for (size_t i = (size_t)blockIdx.x * 32 + lane; i < n; i += (size_t)gridDim.x * 32)
-                reinterpret_cast<uint4*>(a.p.out)[i < first * row ? i : i + (size_t)(last - first) * row] = make_uint4(0, 0, 0, 0);
-        }
-    } else if (warp == 0) {
-        // ── TMA ──────────────────────────────────────────────────────────────
-        uint32_t g = 0, qn = 0;  // ring positions; items with keys
-        bool ok = true;
-        for (uint32_t k = 0; ok; k++) {
-            const Item* it = next_item(k);
-            if (!it) break;
-            const int nt = it->nt();
-            if (nt > 0) {
+            // ── items ────────────────────────────────────────────────────────────
+            Deal<NK> deal(a);
+            uint32_t k = 0;
+            while (true) {
+                Item it;
+                if (!deal.next(a, it)) it.kvh = -1;
+                if (!__all_sync(0xffffffffu, bar_wait(sh, &sh->item_empty[k % PR_ITEMS], ((k / PR_ITEMS) & 1) ^ 1))) break;
                 if (lane == 0) {
-                    // Q: 128-byte columns, 64 elements of 16 bits or 32 of f32 (which its owners turn into two parts where they lie)
-                    constexpr int COLS = PLANES * C::CH, WIDTH = 64 / PLANES;
-                    ok = bar_wait(sh, &sh->q_empty, (qn & 1) ^ 1);
-                    for (int m = 0; m < 2 && ok; m++) {
-                        if (it->n_tiles[m] == 0) continue;
-                        unsigned long long* bar = PLANES == 2 ? &sh->q_raw[m] : &sh->q_full[m];
-                        bar_expect(bar, (uint32_t)(COLS * a.group * a.tile_tokens * 128));
-                        for (int c = 0; c < COLS; c++)
-                            tma_4d(q_smem + m * PLANES * C::QBYTES + c * PR_ROWS * 128, &map_q, bar, c * WIDTH, it->kvh * a.group,
-                                   it->token0 + m * a.tile_tokens, 0);
-                    }
-                    for (int i = 0; i < 2 * nt && ok; i++) {
-                        const uint32_t s = (g + i) % NS, u = (g + i) / NS;
-                        ok = bar_wait(sh, &sh->empty[s], (u & 1) ^ 1);
-                        if (!ok) break;
-                        unsigned long long* bar = (i & 1) ? &sh->v_full[s] : &sh->k_full[s];
-                        bar_expect(bar, C::SLOT);
-                        for (int p = 0; p < PLANES; p++)
-                            for (int c = 0; c < C::CH; c++)
-                                tma_4d(ring + s * C::SLOT + p * C::KBYTES + c * NK * 128, (i & 1) ? &map_v : &map_k, bar, c * 64, it->kvh,
-                                       it->key0 + (i >> 1) * NK, p);
-                    }
-                }
-                ok = __all_sync(0xffffffffu, ok);
-                g += 2 * nt, qn++;
-            }
-            leave_item(k);
-        }
-    } else if (warp == 1) {
-        // ── MMA ──────────────────────────────────────────────────────────────
-        const uint32_t leader = elect_one();
-        constexpr uint32_t type = std::is_same<T16, __nv_bfloat16>::value ? 1u : 0u;
-        constexpr uint32_t idesc_s = (1u << 4) | (type << 7) | (type << 10) | ((uint32_t)(NK >> 3) << 17) | ((uint32_t)(PR_ROWS >> 4) << 24);
-        constexpr uint32_t idesc_o = (1u << 4) | (type << 7) | (type << 10) | (1u << 16) | ((uint32_t)(HDP >> 3) << 17) | ((uint32_t)(PR_ROWS >> 4) << 24);
-        auto scores = [&](int m, uint32_t k_tile) {  // the small products first
-            const uint32_t d = tmem + m * 256 + C::S_COL, q = q_smem + m * PLANES * C::QBYTES;
-            uint32_t add = 0;
-#pragma unroll
-            for (int part = PLANES == 2 ? 0 : 2; part < 3; part++) {
-                const uint32_t ka = k_tile + (part == 0 ? C::KBYTES : 0);
-#pragma unroll
-                for (int ks = 0; ks < HDP / 16; ks++) {
-                    // Q: 64 elements to a 128-byte column; of f32 32, the low parts behind the high ones
-                    const uint32_t qa = PLANES == 1 ? q + (ks / 4) * PR_ROWS * 128 + (ks % 4) * 32
-                                                    : q + (ks / 2) * PR_ROWS * 128 + (part == 1 ? 64 : 0) + (ks % 2) * 32;
-                    umma_ss(d, umma_desc(qa, 16), umma_desc(ka + (ks / 4) * NK * 128 + (ks % 4) * 32, 16), idesc_s, add);
-                    add = 1;
-                }
-            }
-        };
-        auto weighted = [&](int m, int i, uint32_t buf, uint32_t v_tile) {
-            const uint32_t d = tmem + m * 256 + C::O_COL + (C::O_BUFS == 2 ? buf * HDP : 0), p = tmem + m * 256 + C::P_COL;
-            uint32_t add = C::O_IN_TMEM && i > 0;
-#pragma unroll
-            for (int part = PLANES == 2 ? 0 : 2; part < 3; part++) {
-#pragma unroll
-                for (int ks = 0; ks < NK / 16; ks++) {
-                    // P of 32 keys: 16 columns, of f32 followed by the 16 of its low parts
-                    const uint32_t pa = PLANES == 1 ? p + ks * 8 : p + (ks / 2) * 32 + (ks % 2) * 8 + (part == 1 ? 16 : 0);
-                    umma_ts(d, pa, umma_desc(v_tile + (part == 0 ? C::KBYTES : 0) + ks * 2048, NK * 128), idesc_o, add);
-                    add = 1;
-                }
-            }
-        };
-        uint32_t g = 0, done[2] = {0, 0}, qn[2] = {0, 0};  // ring positions; tiles and items of each row tile so far
-        bool ok = true;
-        for (uint32_t k = 0; ok; k++) {
-            const Item* it = next_item(k);
-            if (!it) break;
-            const int n0 = it->n_tiles[0], n1 = it->n_tiles[1], nt = max(n0, n1);
-            // S of tile i of a row tile, in whose place (P_APART: behind whose reading) the one before has been
-            auto issue_scores = [&](int m, uint32_t slot, int i) -> bool {
-                if (C::P_APART && done[m] + i > 0 && !__all_sync(0xffffffffu, bar_wait(sh, &sh->s_read[m], (done[m] + i - 1) & 1))) return false;
-                tc_fence_after();
-                if (leader) {
-                    scores(m, ring + slot * C::SLOT);
-                    umma_commit(&sh->s_full[m]);
+                    Item* to = &sh->item[k % PR_ITEMS];
+                    to->token0 = it.token0, to->tokens = it.tokens, to->key0 = it.key0, to->keys = it.keys, to->first_visible = it.first_visible;
+                    to->key_slot0 = it.key_slot0, to->kvh = it.kvh, to->part = it.part, to->n_tiles[0] = it.n_tiles[0], to->n_tiles[1] = it.n_tiles[1];
+                    bar_arrive(&sh->item_full[k % PR_ITEMS]);
                 }
                 __syncwarp();
-                return true;
+                k++;
+                if (it.kvh < 0) break;
+            }
+            if (a.zero_rest) {  // rows of no sequence
+                const int first = max(0, min(a.p.starts[0], a.p.n_tokens)), last = max(first, min(a.p.starts[a.p.n_seqs], a.p.n_tokens));
+                const size_t row = (size_t)a.p.n_heads * hd * sizeof(T) / 16, n = (size_t)(a.p.n_tokens - last + first) * row;
+                for (size_t i = (size_t)blockIdx.x * 32 + lane; i < n; i += (size_t)gridDim.x * 32)
+                    reinterpret_cast<uint4*>(a.p.out)[i < first * row ? i : i + (size_t)(last - first) * row] = make_uint4(0, 0, 0, 0);
+            }
+        } else if (warp == 0) {
+            // ── TMA ──────────────────────────────────────────────────────────────
+            uint32_t g = 0, qn = 0;  // ring positions; items with keys
+            bool ok = true;
+            for (uint32_t k = 0; ok; k++) {
+                const Item* it = next_item(k);
+                if (!it) break;
+                const int nt = it->nt();
+                if (nt > 0) {
+                    if (lane == 0) {
+                        // Q: 128-byte columns, 64 elements of 16 bits or 32 of f32 (which its owners turn into two parts where they lie)
+                        constexpr int COLS = PLANES * C::CH, WIDTH = 64 / PLANES;
+                        ok = bar_wait(sh, &sh->q_empty, (qn & 1) ^ 1);
+                        for (int m = 0; m < 2 && ok; m++) {
+                            if (it->n_tiles[m] == 0) continue;
+                            unsigned long long* bar = PLANES == 2 ? &sh->q_raw[m] : &sh->q_full[m];
+                            bar_expect(bar, (uint32_t)(COLS * a.group * a.tile_tokens * 128));
+                            for (int c = 0; c < COLS; c++)
+                                tma_4d(q_smem + m * PLANES * C::QBYTES + c * PR_ROWS * 128, &map_q, bar, c * WIDTH, it->kvh * a.group,
+                                       it->token0 + m * a.tile_tokens, 0);
+                        }
+                        for (int i = 0; i < 2 * nt && ok; i++) {
+                            const uint32_t s = (g + i) % NS, u = (g + i) / NS;
+                            ok = bar_wait(sh, &sh->empty[s], (u & 1) ^ 1);
+                            if (!ok) break;
+                            unsigned long long* bar = (i & 1) ? &sh->v_full[s] : &sh->k_full[s];
+                            bar_expect(bar, C::SLOT);
+                            for (int p = 0; p < PLANES; p++)
+                                for (int c = 0; c < C::CH; c++)
+                                    tma_4d(ring + s * C::SLOT + p * C::KBYTES + c * NK * 128, (i & 1) ? &map_v : &map_k, bar, c * 64, it->kvh,
+                                           it->key0 + (i >> 1) * NK, p);
+                        }
+                    }
+                    ok = __all_sync(0xffffffffu, ok);
+                    g += 2 * nt, qn++;
+                }
+                leave_item(k);
+            }
+        } else if (warp == 1) {
+            // ── MMA ──────────────────────────────────────────────────────────────
+            const uint32_t leader = elect_one();
+            constexpr uint32_t type = std::is_same<T16, __nv_bfloat16>::value ? 1u : 0u;
+            constexpr uint32_t idesc_s = (1u << 4) | (type << 7) | (type << 10) | ((uint32_t)(NK >> 3) << 17) | ((uint32_t)(PR_ROWS >> 4) << 24);
+            constexpr uint32_t idesc_o = (1u << 4) | (type << 7) | (type << 10) | (1u << 16) | ((uint32_t)(HDP >> 3) << 17) | ((uint32_t)(PR_ROWS >> 4) << 24);
+            auto scores = [&](int m, uint32_t k_tile) {  // the small products first
+                const uint32_t d = tmem + m * 256 + C::S_COL, q = q_smem + m * PLANES * C::QBYTES;
+                uint32_t add = 0;
+#pragma unroll
+                for (int part = PLANES == 2 ? 0 : 2; part < 3; part++) {
+                    const uint32_t ka = k_tile + (part == 0 ? C::KBYTES : 0);
+#pragma unroll
+                    for (int ks = 0; ks < HDP / 16; ks++) {
+                        // Q: 64 elements to a 128-byte column; of f32 32, the low parts behind the high ones
+                        const uint32_t qa = PLANES == 1 ? q + (ks / 4) * PR_ROWS * 128 + (ks % 4) * 32
+                                                        : q + (ks / 2) * PR_ROWS * 128 + (part == 1 ? 64 : 0) + (ks % 2) * 32;
+                        umma_ss(d, umma_desc(qa, 16), umma_desc(ka + (ks / 4) * NK * 128 + (ks % 4) * 32, 16), idesc_s, add);
+                        add = 1;
+                    }
+                }
             };
-            if (nt > 0) {
-                ok = __all_sync(0xffffffffu, bar_wait(sh, &sh->k_full[g % NS], use_parity(g)));
-                for (int m = 0; m < 2 && ok; m++)
-                    if (it->n_tiles[m] > 0) {
-                        ok = __all_sync(0xffffffffu, bar_wait(sh, &sh->q_full[m], qn[m] & 1));
-                        if (ok) ok = issue_scores(m, g % NS, 0);
-                        qn[m]++;
+            auto weighted = [&](int m, int i, uint32_t buf, uint32_t v_tile) {
+                const uint32_t d = tmem + m * 256 + C::O_COL + (C::O_BUFS == 2 ? buf * HDP : 0), p = tmem + m * 256 + C::P_COL;
+                uint32_t add = C::O_IN_TMEM && i > 0;
+#pragma unroll
+                for (int part = PLANES == 2 ? 0 : 2; part < 3; part++) {
+#pragma unroll
+                    for (int ks = 0; ks < NK / 16; ks++) {
+                        // P of 32 keys: 16 columns, of f32 followed by the 16 of its low parts
+                        const uint32_t pa = PLANES == 1 ? p + ks * 8 : p + (ks / 2) * 32 + (ks % 2) * 8 + (part == 1 ? 16 : 0);
+                        umma_ts(d, pa, umma_desc(v_tile + (part == 0 ? C::KBYTES : 0) + ks * 2048, NK * 128), idesc_o, add);
+                        add = 1;
                     }
-                if (ok && leader) {
-                    umma_commit(&sh->empty[g % NS]);
-                    if (nt == 1) umma_commit(&sh->q_empty);
                 }
-                __syncwarp();
-            }
-            for (int i = 0; i < nt && ok; i++) {
-                const uint32_t gv = g + 2 * i + 1, gk = gv + 1, sv = gv % NS, sk = gk % NS;
-                const bool more = i + 1 < nt;
-                if (C::P_APART && more) {  // the next scores first
-                    ok = __all_sync(0xffffffffu, bar_wait(sh, &sh->k_full[sk], use_parity(gk)));
-                    for (int m = 0; m < 2 && ok; m++)
-                        if (i + 1 < it->n_tiles[m]) ok = issue_scores(m, sk, i + 1);
-                    if (!ok) break;
-                    if (leader) {
-                        umma_commit(&sh->empty[sk]);
-                        if (i + 2 == nt) umma_commit(&sh->q_empty);
-                    }
-                    __syncwarp();
-                }
-                ok = __all_sync(0xffffffffu, bar_wait(sh, &sh->ready[sv], use_parity(gv)));
-                for (int m = 0; m < 2 && ok; m++) {
-                    const int n = m ? n1 : n0;
-                    if (i >= n) continue;
-                    ok = __all_sync(0xffffffffu, bar_wait(sh, &sh->p_ready[m], (done[m] + i) & 1));
-                    if (!ok) break;
+            };
+            uint32_t g = 0, done[2] = {0, 0}, qn[2] = {0, 0};  // ring positions; tiles and items of each row tile so far
+            bool ok = true;
+            for (uint32_t k = 0; ok; k++) {
+                const Item* it = next_item(k);
+                if (!it) break;
+                const int n0 = it->n_tiles[0], n1 = it->n_tiles[1], nt = max(n0, n1);
+                // S of tile i of a row tile, in whose place (P_APART: behind whose reading) the one before has been
+                auto issue_scores = [&](int m, uint32_t slot, int i) -> bool {
+                    if (C::P_APART && done[m] + i > 0 && !__all_sync(0xffffffffu, bar_wait(sh, &sh->s_read[m], (done[m] + i - 1) & 1))) return false;
                     tc_fence_after();
                     if (leader) {
-                        weighted(m, i, (done[m] + i) & 1, ring + sv * C::SLOT);
-                        if (C::P_APART || i + 1 == n) umma_commit(&sh->o_full[m]);
+                        scores(m, ring + slot * C::SLOT);
+                        umma_commit(&sh->s_full[m]);
                     }
                     __syncwarp();
-                    if (!C::P_APART && i + 1 < n) {
+                    return true;
+                };
+                if (nt > 0) {
+                    ok = __all_sync(0xffffffffu, bar_wait(sh, &sh->k_full[g % NS], use_parity(g)));
+                    for (int m = 0; m < 2 && ok; m++)
+                        if (it->n_tiles[m] > 0) {
+                            ok = __all_sync(0xffffffffu, bar_wait(sh, &sh->q_full[m], qn[m] & 1));
+                            if (ok) ok = issue_scores(m, g % NS, 0);
+                            qn[m]++;
+                        }
+                    if (ok && leader) {
+                        umma_commit(&sh->empty[g % NS]);
+                        if (nt == 1) umma_commit(&sh->q_empty);
+                    }
+                    __syncwarp();
+                }
+                for (int i = 0; i < nt && ok; i++) {
+                    const uint32_t gv = g + 2 * i + 1, gk = gv + 1, sv = gv % NS, sk = gk % NS;
+                    const bool more = i + 1 < nt;
+                    if (C::P_APART && more) {  // the next scores first
                         ok = __all_sync(0xffffffffu, bar_wait(sh, &sh->k_full[sk], use_parity(gk)));
-                        if (ok) ok = issue_scores(m, sk, i + 1);
+                        for (int m = 0; m < 2 && ok; m++)
+                            if (i + 1 < it->n_tiles[m]) ok = issue_scores(m, sk, i + 1);
+                        if (!ok) break;
+                        if (leader) {
+                            umma_commit(&sh->empty[sk]);
+                            if (i + 2 == nt) umma_commit(&sh->q_empty);
+                        }
+                        __syncwarp();
                     }
-                }
-                if (ok && leader) {
-                    umma_commit(&sh->empty[sv]);
-                    if (!C::P_APART && more) {
-                        umma_commit(&sh->empty[sk]);
-                        if (i + 2 == nt) umma_commit(&sh->q_empty);
+                    ok = __all_sync(0xffffffffu, bar_wait(sh, &sh->ready[sv], use_parity(gv)));
+                    for (int m = 0; m < 2 && ok; m++) {
+                        const int n = m ? n1 : n0;
+                        if (i >= n) continue;
+                        ok = __all_sync(0xffffffffu, bar_wait(sh, &sh->p_ready[m], (done[m] + i) & 1));
+                        if (!ok) break;
+                        tc_fence_after();
+                        if (leader) {
+                            weighted(m, i, (done[m] + i) & 1, ring + sv * C::SLOT);
+                            if (C::P_APART || i + 1 == n) umma_commit(&sh->o_full[m]);
+                        }
+                        __syncwarp();
+                        if (!C::P_APART && i + 1 < n) {
+                            ok = __all_sync(0xffffffffu, bar_wait(sh, &sh->k_full[sk], use_parity(gk)));
+                            if (ok) ok = issue_scores(m, sk, i + 1);
+                        }
                     }
+                    if (ok && leader) {
+                        umma_commit(&sh->empty[sv]);
+                        if (!C::P_APART && more) {
+                            umma_commit(&sh->empty[sk]);
+                            if (i + 2 == nt) umma_commit(&sh->q_empty);
+                        }
+                    }
+                    __syncwarp();
                 }
-                __syncwarp();
+                g += 2 * nt, done[0] += n0, done[1] += n1;
+                leave_item(k);
             }
-            g += 2 * nt, done[0] += n0, done[1] += n1;
-            leave_item(k);
-        }
-    } else if (warp == 2) {
-        // ── V check ──────────────────────────────────────────────────────────
-        constexpr uint32_t EXP = std::is_same<T16, __nv_bfloat16>::value ? 0x7F807F80u : 0x7C007C00u;  // exponent bits, and
-        constexpr uint32_t ONE = std::is_same<T16, __nv_bfloat16>::value ? 0x00800080u : 0x04000400u;  // their lowest one
-        uint32_t g0 = 0;
-        bool ok = true;
-        for (uint32_t k = 0; ok; k++) {
-            const Item* it = next_item(k);
-            if (!it) break;
-            Item* notes = &sh->item[k % PR_ITEMS];
-            const int nt = it->nt(), first_masked = it->template first_masked<NK>();
-            for (int i = 0; i < nt; i++) {
-                const uint32_t g = g0 + 2 * i + 1, s = g % NS;
-                if (!(ok = __all_sync(0xffffffffu, bar_wait(sh, &sh->v_full[s], use_parity(g))))) break;
-                if (i >= first_masked) {
-                    uint8_t* tile = sm + 2 * PLANES * C::QBYTES + s * C::SLOT;
-                    uint32_t found[4] = {0, 0, 0, 0};
-                    for (int r = 0; r < NK; r += 4) {  // 8 lanes to a row of 128 bytes
-                        bool odd = false;
+        } else if (warp == 2) {
+            // ── V check ──────────────────────────────────────────────────────────
+            constexpr uint32_t EXP = std::is_same<T16, __nv_bfloat16>::value ? 0x7F807F80u : 0x7C007C00u;  // exponent bits, and
+            constexpr uint32_t ONE = std::is_same<T16, __nv_bfloat16>::value ? 0x00800080u : 0x04000400u;  // their lowest one
+            uint32_t g0 = 0;
+            bool ok = true;
+            for (uint32_t k = 0; ok; k++) {
+                const Item* it = next_item(k);
+                if (!it) break;
+                Item* notes = &sh->item[k % PR_ITEMS];
+                const int nt = it->nt(), first_masked = it->template first_masked<NK>();
+                for (int i = 0; i < nt; i++) {
+                    const uint32_t g = g0 + 2 * i + 1, s = g % NS;
+                    if (!(ok = __all_sync(0xffffffffu, bar_wait(sh, &sh->v_full[s], use_parity(g))))) break;
+                    if (i >= first_masked) {
+                        uint8_t* tile = sm + 2 * PLANES * C::QBYTES + s * C::SLOT;
+                        uint32_t found[4] = {0, 0, 0, 0};
+                        for (int r = 0; r < NK; r += 4) {  // 8 lanes to a row of 128 bytes
+                            bool odd = false;
 #pragma unroll
-                        for (int c = 0; c < PLANES * C::CH; c++) {
-                            uint4* at = reinterpret_cast<uint4*>(tile + c * NK * 128 + (r + lane / 8) * 128) + lane % 8;
-                            uint4 w = *at;
-                            uint32_t* u = reinterpret_cast<uint32_t*>(&w);
-                            uint32_t hit = 0;
+                            for (int c = 0; c < PLANES * C::CH; c++) {
+                                uint4* at = reinterpret_cast<uint4*>(tile + c * NK * 128 + (r + lane / 8) * 128) + lane % 8;
+                                uint4 w = *at;
+                                uint32_t* u = reinterpret_cast<uint32_t*>(&w);
+                                uint32_t hit = 0;
 #pragma unroll
-                            for (int x = 0; x < 4; x++) hit |= (u[x] & EXP) + ONE;
-                            if (hit & 0x80008000u) {
-                                odd = true;
+                                for (int x = 0; x < 4; x++) hit |= (u[x] & EXP) + ONE;
+                                if (hit & 0x80008000u) {
+                                    odd = true;
 #pragma unroll
-                                for (int x = 0; x < 4; x++) {
-                                    const uint32_t h = (u[x] & EXP) + ONE;
-                                    if (h & 0x8000u) u[x] &= 0xFFFF0000u;
-                                    if (h & 0x80000000u) u[x] &= 0x0000FFFFu;
+                                    for (int x = 0; x < 4; x++) {
+                                        const uint32_t h = (u[x] & EXP) + ONE;
+                                        if (h & 0x8000u) u[x] &= 0xFFFF0000u;
+                                        if (h & 0x80000000u) u[x] &= 0x0000FFFFu;
+                                    }
+                                    *at = w;
                                 }
-                                *at = w;
+                            }
+                            const uint32_t votes = __ballot_sync(0xffffffffu, odd);
+                            if (votes) {
+                                uint32_t rows = 0;
+#pragma unroll
+                                for (int x = 0; x < 4; x++) rows |= ((votes >> (8 * x)) & 255u) ? 1u << x : 0u;
+#pragma unroll
+                                for (int x = 0; x < 4; x++)
+                                    if (r / 32 == x) found[x] |= rows << (r % 32);
                             }
                         }
-                        const uint32_t votes = __ballot_sync(0xffffffffu, odd);
-                        if (votes) {
-                            uint32_t rows = 0;
-#pragma unroll
-                            for (int x = 0; x < 4; x++) rows |= ((votes >> (8 * x)) & 255u) ? 1u << x : 0u;
-#pragma unroll
-                            for (int x = 0; x < 4; x++)
-                                if (r / 32 == x) found[x] |= rows << (r % 32);
-                        }
+                        if (PLANES == 1 && lane < 4) notes->mask[i - first_masked][lane] = lane == 0 ? found[0] : lane == 1 ? found[1] : lane == 2 ? found[2] : found[3];
+                        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                     }
-                    if (PLANES == 1 && lane < 4) notes->mask[i - first_masked][lane] = lane == 0 ? found[0] : lane == 1 ? found[1] : lane == 2 ? found[2] : found[3];
-                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                    __syncwarp();
+                    if (lane == 0) bar_arrive(&sh->ready[s]);
                 }
+                g0 += 2 * nt;
                 __syncwarp();
-                if (lane == 0) bar_arrive(&sh->ready[s]);
+                if (lane == 0 && ok) bar_arrive(&sh->checked[k % PR_ITEMS]);
+                leave_item(k);
             }
-            g0 += 2 * nt;
-            __syncwarp();
-            if (lane == 0 && ok) bar_arrive(&sh->checked[k % PR_ITEMS]);
-            leave_item(k);
         }
-    }
     } else {
         // ── softmax: one row per thread ──────────────────────────────────────
         asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");

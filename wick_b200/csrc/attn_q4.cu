@@ -1,8 +1,10 @@
 // Attention of single tokens over the 4-bit cache:  o = sum_t p_t V_t / sum_t p_t,  p_t = 2^(x_t - m),
 // x_t = log2(e) / sqrt(d) q . K_t, with K_t and V_t blocks d (n - 8) of four-bit numbers n.
 //
-// Bound by HBM it would be 18 bytes per 32 elements of keys or values; it is bound by instructions, most of them the unpacking (per 8 numbers one
-// shift, four bit operations and four f16 ones), and mma.sync holds the issue port for 8 cycles.  f32 arithmetic on the CUDA cores would need 14
+// Bound by HBM it would be 18 bytes per 32 elements of keys or values, 40 % of its time.  Most instructions are the unpacking (per 8 numbers one shift, four
+// bit operations and four f16 ones); issue slots are 55 % busy (47 % with heads of 128): three warps to a scheduler (two), whose K part, softmax and V part
+// follow one another, wait for their own results (of 4.2 cycles per instruction 1.1 for a fixed latency, 0.5 each for memory and for a busy pipe).
+// f32 arithmetic on the CUDA cores would need 14
 // operations per byte for 4 query heads, and an M = 128 tile of tcgen05 operands in shared memory that the CUDA cores would have to write.  So the
 // products are mma.sync m16n8k16 with the numbers n - 8, exact in f16, as the 16-row operand.  The 8 columns of the other are 4 query
 // heads: q, or the weights, is f32 and is held as two f16 parts (22 bits), the high one in an even column, the low one in the odd column behind it,
@@ -19,8 +21,8 @@
 // bulk copies per tile).  A (row, group) that lies within a warp's part is finished there, parts of one are joined within the CTA, and
 // what reaches over CTAs goes to the workspace, where k_attention_q4_join adds it up in order: results do not depend on timing.
 //
-// On a B200: 64 rows of 1025 to 4100 keys, 32 / 8 heads of 64: 35 us (issue slots 56 %, the integer pipe 43 %, tensor pipe 16 %; the bytes would take 14);
-// one row of 131,000 keys, 16 / 4 heads of 128: 28 us (issue 47 %, 8 warps fit the SM; bytes 12); one row of 517 keys, start, a tile and the join: 10 us.
+// On a B200: 64 rows of 1025 to 4100 keys, 32 / 8 heads of 64: 35 us (tensor pipe 15 %; the bytes would take 14); one row of 131,000 keys, 16 / 4 heads of 128:
+// 28 us (8 warps fit the SM; bytes 12); one row of 517 keys, start, a tile and the join: 10 us.
 //
 // What lies behind a row's length is read (the tile is there) but not used: its scores are masked, its scales count as 0.
 // Waits are bounded: on expiry the warp's outputs become NaN.
@@ -40,7 +42,8 @@ struct Q4Cfg {
     static constexpr int STAGE = 2 * (QUANTS + SCALES);
     static constexpr int PART = A4_HEADS * HD + 2 * A4_HEADS;                    // floats of a partial result: o, m, l
     static constexpr int STAGES = 2;
-    static constexpr int FIT = (218 * 1024) / (STAGES * STAGE + 2 * PART * 4), WARPS = FIT < 12 ? FIT : 12;  // (10, 13, 14: 40, 40, 37 us where 12 and 16 take 36: whole warps per scheduler)
+    static constexpr int FIT = (218 * 1024) / (STAGES * STAGE + 2 * PART * 4), WARPS = FIT < 12 ? FIT : 12;
+    // (Heads of 64: 10, 13, 14 warps took 40, 40, 37 us where 12 and 16 took 36: whole warps per scheduler.)
     static constexpr int THREADS = 32 * WARPS;
     static constexpr size_t SMEM = (size_t)WARPS * (STAGES * STAGE + 2 * PART * 4);
 };
@@ -65,17 +68,8 @@ __device__ __forceinline__ void bulk_copy(uint32_t dst, const void* src, uint32_
                  : "memory");
 }
 __device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity, uint32_t rounds) {
-    for (uint32_t i = 0; i < rounds; i++) {
-        uint32_t ok;
-        asm volatile(
-            "{\n\t.reg .pred p;\n\t"
-            "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
-            "selp.u32 %0, 1, 0, p;\n\t}"
-            : "=r"(ok)
-            : "r"(bar), "r"(parity)
-            : "memory");
-        if (ok) return true;
-    }
+    for (uint32_t i = 0; i < rounds; i++)
+        if (mbar_try_wait(bar, parity)) return true;
     return false;
 }
 __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
@@ -92,11 +86,6 @@ __device__ __forceinline__ uint32_t pack_f16(float a, float b) {  // a in the lo
     uint32_t r;
     asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(b), "f"(a));
     return r;
-}
-__device__ __forceinline__ float exp2_approx(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
 }
 // Four-bit numbers at bits 0 and 16, or 4 and 20, of w as n - 8 in f16: 1024 + n is a number's bits behind f16's 1024.
 __device__ __forceinline__ uint32_t behind_1024(uint32_t w, uint32_t mask) {

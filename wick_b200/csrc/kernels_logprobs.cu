@@ -5,7 +5,7 @@
 // T' = (T + S (m - m')) e with e = exp(m - m')); threads, then the CTAs of a row, are joined by the same rule.
 //
 // A cluster of 1 to 8 CTAs takes a row: as many as give every SM work (the rule in launch_token_logprobs), joined through
-// distributed shared memory, so that the call is one launch and needs no workspace.  Bound: the read of the logits.
+// distributed shared memory, so that the call is one launch and needs no workspace.
 //
 // Alternatives: from the threads' maxima follows a value that top_n elements reach and few others do.  What reaches it is collected, from
 // registers where the CTA's part of the row fits them and by a second read otherwise (L2 has it by then); candidates are ordered by counting, the
@@ -13,9 +13,9 @@
 // Where ties make too many candidates (a vocabulary that is masked but for a few tokens), top_n rounds of "largest key below the
 // last one" follow instead.
 //
-// On a B200: 2500 rows of 50021 in bf16 57 us (4.4 TB/s, 67 % of a copy's rate: per element an exponential, of which the special function unit
-// does 16 a cycle, 28 us here, and some ten operations), 64 rows of 65536 in f32 with twenty alternatives 14 us, one with five 7 us (the
-// cluster's barriers and the candidates).
+// On a B200: 2500 rows of 50021 in bf16 57 us (4.4 TB/s, 67 % of a copy's rate; special function unit 58 %, issue slots 52 %: a thread's loads and its
+// arithmetic alternate), 64 rows of 65536 in f32 with twenty alternatives 14 us, one with five 7 us (the cluster's barriers and the candidates, one step
+// after the other).
 //
 // Sums: f32 within a thread's few hundred elements, f64 from there on (log S and T / S cancel for sharp rows).
 // NaN counts as -inf, as for the argmax (wick/src/sampler.rs:8-19); logits are held to +-1e30, so that +inf and -inf need no case of
@@ -45,11 +45,6 @@ __device__ __forceinline__ float key_value(uint32_t k) { return __uint_as_float(
 __device__ __forceinline__ unsigned long long full_key(float x, uint32_t i) { return ((unsigned long long)value_key(x) << 32) | (0xFFFFFFFFu - i); }
 
 constexpr float LOG2E = 1.44269504088896341f;
-__device__ __forceinline__ float exp2_approx(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
 __device__ __forceinline__ float max_nan(float a, float b, float c) {  // (NaN if one is)
     float r;
     asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
