@@ -373,3 +373,34 @@ def test_attention_prompts_around_the_walk_over_sequences(ops, seqs):
         if a < b:
             ref, tol = _prompts_ref(q[a:b], k[a:b], v[a:b], [b - a], [b - a], heads, kv, hd)
             _check(out[a:b], ref, tol, v.abs().max().double())
+
+
+# ── scores whose own rounding is more than a power of two ──────────────────────────────────────────
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("shape", SIZES, ids=str)
+@pytest.mark.parametrize("log2", [24, 27, 30, 33, 40, 60, 100])
+@pytest.mark.parametrize("prefix", [0, 3000])
+def test_attention_prompts_huge_scores(ops, dtype, shape, log2, prefix):
+    """Scores of 2^log2, of both signs: all the weight is that of the largest, whose like the others are far from."""
+    heads, kv, hd = shape
+    if dtype == torch.float16 and log2 // 2 + 1 > 15:
+        pytest.skip("beyond f16")  # (2^16 > 65504)
+    n, size, g = 200, 2.0 ** (log2 // 2 + 1), _gen(log2)
+    q = torch.where(torch.rand(n, heads, 1, generator=g, device="cuda") < 0.5, -size, size).expand(-1, -1, hd).flatten(1).to(dtype)
+    v = _randn(g, n + prefix, kv * hd).to(dtype)
+    if dtype == torch.float32:  # every score another, at least 2^-12 of the largest apart
+        height = (torch.randperm(n + prefix, generator=g, device="cuda") + 1.0) / (n + prefix)
+    else:  # a few that stand out: the first tokens' scores are all 0
+        height = torch.zeros(n + prefix, device="cuda")
+        height[[3, 70, 150, prefix + 130, prefix + 199]] = torch.tensor([0.5, -0.25, -0.5, 0.75, -1.0], device="cuda")
+    k = (height * size)[:, None].expand(-1, kv * hd).to(dtype)
+    out = ops.attention_prompts(q, k, v, _starts([n]), heads, kv, hd, key_starts=_starts([n + prefix]))
+    for h in range(heads):
+        rows, c = slice(h * hd, (h + 1) * hd), h * kv // heads
+        s = (q[:, rows].double() @ k[:, c * hd:(c + 1) * hd].double().T).masked_fill(torch.arange(n + prefix, device="cuda")[None] > torch.arange(n, device="cuda")[:, None] + prefix, -math.inf)
+        p = torch.softmax(s / math.sqrt(hd), 1)
+        alone = p.amax(1) == 1.0
+        assert alone.sum() > 100
+        ref = p @ v[:, c * hd:(c + 1) * hd].double()
+        _check(out[alone][:, rows], ref[alone], 2.0 ** -20 * v.abs().max().double(), 0)
+    assert torch.isfinite(out).all()

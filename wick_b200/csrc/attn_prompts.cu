@@ -362,6 +362,10 @@ __device__ __forceinline__ size_t far_tile(const PromptArgs& a, const Item* it, 
     return ((size_t)(it->key_slot0 + i) * a.p.n_kv + it->kvh) * FAR_WORDS;
 }
 
+// Scores so large that their distance from the maximum, as one product and sum that is rounded once, would see the rounding of the maximum itself: half a
+// unit of it must stay well below 1.  From there on a score is rounded before the maximum is taken off.
+__device__ __forceinline__ bool coarse(float top) { return fabsf(top) > 0x1p22f && top > __int_as_float(0xFF800000); }
+
 // A CTA's items one after the other, by a whole warp: the list is dealt to the CTAs forwards and backwards in turn, and begins with the
 // blocks that have the most keys, so that the CTAs end about together.  Up to 32 sequences (a lane each) their last blocks come first, then
 // their last but one ..; with more, one sequence's blocks after the other's, backwards.
@@ -834,8 +838,16 @@ k_attention_prompts(const __grid_constant__ CUtensorMap map_q, const __grid_cons
                             }
                         }
                         // f16: 2^7 times the weights, at most 2^15 then: those down to 2^-32 of the maximum stay in its range (bf16 has f32's)
-                        const float base = (row_max == NEG ? 0.0f : -row_max) + (std::is_same<T16, __half>::value ? 7.0f : 0.0f);
-                        const f32x2 base2 = pack2(base, base), scale2 = pack2(a.scale_log2, a.scale_log2);
+                        constexpr float LIFT = std::is_same<T16, __half>::value ? 7.0f : 0.0f;
+                        float scale = a.scale_log2, base = (row_max == NEG ? 0.0f : -row_max) + LIFT;
+                        if (__builtin_expect(__any_sync(0xffffffffu, coarse(row_max)), 0)) {  // (rarely: one look for the warp)
+                            if (coarse(row_max)) {
+#pragma unroll
+                                for (int c = 0; c < NK; c++) s[c] = __fsub_rn(__fmul_rn(s[c], scale), row_max);
+                                scale = 1.0f, base = LIFT;
+                            }
+                        }
+                        const f32x2 base2 = pack2(base, base), scale2 = pack2(scale, scale);
                         f32x2 sum[2] = {pack2(0.f, 0.f), pack2(0.f, 0.f)};
 #pragma unroll
                         for (int c = 0; c < NK / 32; c++) {
@@ -886,7 +898,7 @@ k_attention_prompts(const __grid_constant__ CUtensorMap map_q, const __grid_cons
                 for (int i = 0; i < n && ok; i++) {
                     const float k_now = k_next, v_before = __fmul_rn(fabsf(v_now), PR_DOWN);
                     const bool k_far = k_now < 0.0f, v_far = v_next < 0.0f;
-                    const float scale = k_far ? a.scale_log2 : __fmul_rn(row_scale, k_now);
+                    float scale = k_far ? a.scale_log2 : __fmul_rn(row_scale, k_now);
                     v_now = v_next;
                     if (i + 1 < n) k_next = k_inv[(size_t)(i + 1) * a.p.n_kv], v_next = v_inv[(size_t)(i + 1) * a.p.n_kv];
                     if (!(ok = __all_sync(0xffffffffu, bar_wait(sh, &sh->s_full[m], (done + i) & 1)))) break;
@@ -949,8 +961,22 @@ k_attention_prompts(const __grid_constant__ CUtensorMap map_q, const __grid_cons
                     const float f = row_max == NEG ? 0.0f : exp2_approx(row_max - new_max);
                     // weights up to 2^8 in the products, so that the low parts of small ones stay in f16's range; in the sums up to 1 again, so that
                     // values near the end of f32 stay in its range
-                    const float base = new_max == NEG ? 0.0f : PR_LAZY - new_max;
+                    float base = new_max == NEG ? 0.0f : PR_LAZY - new_max;
                     row_max = new_max;
+                    if (__builtin_expect(__any_sync(0xffffffffu, coarse(row_max)), 0)) {
+                        const bool mine = coarse(row_max);
+#pragma unroll 1
+                        for (int c = 0; c < NK / 32; c++) {
+                            float s[32];
+                            tmem_ld32(t_s + 32 * c, s);
+                            tmem_ld_wait();
+#pragma unroll
+                            for (int x = 0; x < 32; x++) s[x] = mine ? __fsub_rn(__fmul_rn(s[x], scale), row_max) : s[x];
+                            tmem_st32(t_s + 32 * c, s);
+                        }
+                        tmem_st_wait();
+                        if (mine) scale = 1.0f, base = PR_LAZY;
+                    }
                     if (__builtin_expect(v_far, 0)) {  // the far keys' weighted values; the tensor core's product has zeros there
                         if (C::O_BUFS == 2 && i > 0) take_o(i - 1, v_before);
 #pragma unroll
