@@ -404,3 +404,17 @@ def test_attention_prompts_huge_scores(ops, dtype, shape, log2, prefix):
         ref = p @ v[:, c * hd:(c + 1) * hd].double()
         _check(out[alone][:, rows], ref[alone], 2.0 ** -20 * v.abs().max().double(), 0)
     assert torch.isfinite(out).all()
+
+
+@pytest.mark.parametrize("log2", [24, 25, 26, 27, 28, 29, 30, 31, 32, 40])
+def test_attention_q4_huge_scores(ops, log2):
+    """Scores of about 2^(log2 - 2): the power of two that lifts the weights, which goes by the values' scales, must not meet their rounding."""
+    heads, kv, hd, n = 8, 2, 64, 700
+    g = _gen(log2)
+    cache = _random_cache(ops, g, 1, 704, kv, hd)
+    scales = cache.v_scales.float()
+    for scale in (1.0, 0.4, 0.2, 0.1, 0.05, 0.02, 0.01, 1e-3, 1e-5):
+        cache.v_scales.copy_(scales * scale)
+        q = _randn(g, 1, heads * hd) * 2.0 ** log2 / 20
+        ref, _, vmax = _q4_ref(q, cache, [0], [n], heads)
+        _check(ops.attention_q4(q, cache, _i32([0]), _i32([n]), heads), ref, 2.0 ** -20 * vmax, vmax)

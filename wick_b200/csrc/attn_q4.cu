@@ -451,13 +451,14 @@ __global__ void __launch_bounds__(Q4Cfg<NB>::THREADS, 1) k_attention_q4(const __
                 top = fmaxf(m[u], __fmul_rn(top, q_inv[u]));
                 keep[u] = __fmul_rn(m[u] == top ? 1.0f : exp2_approx(m[u] - top), moved);
                 m[u] = top;
-                const float base = (top == __int_as_float(0xFF800000) ? 0.0f : -top) + (float)(12 - vexp);
+                // (two additions: a large maximum would swallow the power of two; the product with q_inv is exact)
+                const float from = top == __int_as_float(0xFF800000) ? 0.0f : -top, lift = (float)(12 - vexp);
                 float sum = 0.0f;
 #pragma unroll
                 for (int b16 = 0; b16 < 4; b16++)
 #pragma unroll
                     for (int e = 0; e < 2; e++) {
-                        s[u][b16][e] = exp2_approx(fmaf(s[u][b16][e], q_inv[u], base));
+                        s[u][b16][e] = exp2_approx(__fadd_rn(fmaf(s[u][b16][e], q_inv[u], from), lift));
                         sum = __fadd_rn(sum, s[u][b16][e]);
                     }
                 l[u] = fmaf(l[u], keep[u], sum);
