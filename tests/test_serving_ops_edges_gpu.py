@@ -418,3 +418,19 @@ def test_attention_q4_huge_scores(ops, log2):
         q = _randn(g, 1, heads * hd) * 2.0 ** log2 / 20
         ref, _, vmax = _q4_ref(q, cache, [0], [n], heads)
         _check(ops.attention_q4(q, cache, _i32([0]), _i32([n]), heads), ref, 2.0 ** -20 * vmax, vmax)
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+def test_attention_prompts_values_near_the_end_of_bf16(ops, hd):
+    """Weights that grow by less than what O is rescaled for: 300 keys, then one of 2^7.5 times their weight."""
+    n = 400
+    g = _gen(hd + 7)
+    q, k, v = torch.zeros(n, hd, device="cuda"), torch.zeros(n, hd, device="cuda"), _randn(g, n, hd).abs() * 1e35 + 3e36
+    q[:, 0] = math.sqrt(hd)
+    k[350:, 0] = 7.5 * math.log(2.0)
+    q, k, v = q.bfloat16(), k.bfloat16(), v.bfloat16()
+    out = ops.attention_prompts(q, k, v, _starts([n]), 1, 1, hd)
+    some = torch.tensor([0, 10, 20, 350, 360], device="cuda")  # (more of equal weight have sums beyond f32, here and in plain f32)
+    seen = torch.arange(n, device="cuda")[None] <= some[:, None]
+    ref, tol = _attend(q[some].double(), k.double(), v.double(), seen)
+    _check(out[some], ref, tol, v.abs().max().double())

@@ -10,7 +10,7 @@
 // in the tensor core the other is in its softmax; and an item's last rows are written while the next one's first scores are computed.
 //
 // f16, bf16: one product each; O stays in tensor memory, and is rescaled only where a row's maximum has grown by more than 2^8 (a weight is at most
-//   2^8 then, times 2^7 in f16; the last maximum that was used cancels in the quotient).  Weights are rounded to the operands' type, half a step
+//   2^8 then, times 2^7 in f16 and 2^-8 in bf16; the last maximum that was used cancels in the quotient).  Weights are rounded to the operands' type, half a step
 //   each, as the tensor core takes them; their sum is of the unrounded ones.  The tensor core adds with truncation: O is taken out and added up in
 //   f32 every 64 tiles (8192 keys: 5e-5 of the sum; 131072 without this were 7e-4, 1.5 half steps of f16).
 // f32: every operand is split into two f16 parts, x = 2^e (hi + lo), 22 bits, with one power of two per row of Q and per tile of K and V (K and V by
@@ -837,8 +837,9 @@ k_attention_prompts(const __grid_constant__ CUtensorMap map_q, const __grid_cons
                                 }
                             }
                         }
-                        // f16: 2^7 times the weights, at most 2^15 then: those down to 2^-32 of the maximum stay in its range (bf16 has f32's)
-                        constexpr float LIFT = std::is_same<T16, __half>::value ? 7.0f : 0.0f;
+                        // f16: 2^7 times the weights, at most 2^15 then: those down to 2^-32 of the maximum stay in its range.  bf16, which has f32's: 2^-8
+                        // of them, at most 1, so that values near its end stay in range.
+                        constexpr float LIFT = std::is_same<T16, __half>::value ? 7.0f : -PR_LAZY;
                         float scale = a.scale_log2, base = (row_max == NEG ? 0.0f : -row_max) + LIFT;
                         if (__builtin_expect(__any_sync(0xffffffffu, coarse(row_max)), 0)) {  // (rarely: one look for the warp)
                             if (coarse(row_max)) {
