@@ -30,11 +30,11 @@
 // attend such a key add its values at the end.
 //
 // Bound, on a B200: the softmax and its MMAs in turn, two softmax warps to a scheduler, which wait for one another's results more than they issue (issue
-// slots 40 % in f32, 33 % in 16 bits).  A pair of tiles, one of each row tile, takes (slope of the time over the keys, 1965 MHz) in f32 5500 cycles (heads
-// of 64, 128 keys; 3072 of them MMAs by count) or 5700 (heads of 128, 64 keys), in 16 bits 3600 to 3700 (the special function unit needs 2048 for its
+// slots 40 % in f32, 33 % in 16 bits).  A pair of tiles, one of each row tile, takes (slope of the time over the keys, 1965 MHz) in f32 5600 cycles (heads
+// of 64, 128 keys; 54 % of them MMAs by count) or 5700 (heads of 128, 64 keys), in 16 bits 3600 to 3900 (the special function unit needs 2048 for its
 // exponentials, the MMAs 1024 with heads of 64 and 2048 with 128).  Eight prompts of 250 to 1001 tokens, 32 / 8 heads of 64, f32: 97 us (tensor pipe
-// 35 %); one of 8000, heads of 128, bf16: 456 us (1150 TFLOP/s; tensor pipe 54 %, special function unit 54 %), 515 under the power cap.  Loops that run once per item stay rolled:
-// unrolled they took longer to fetch than to run (161 -> 116 us in the first case, before other steps).
+// 35 %); one of 8000, heads of 128, bf16: 451 us (1160 TFLOP/s; tensor pipe 54 %, special function unit 54 %), 521 under the power cap.  Loops that
+// run once per item stay rolled: unrolled they took longer to fetch than to run (161 -> 116 us in the first case, before other steps).
 //
 // Every wait is bounded: on expiry all roles leave their loops and all rows of the CTA's items become NaN.
 #include <cuda.h>
